@@ -234,6 +234,128 @@ const char* reef_ops_conv2d_kernel(const reef_conv2d_desc* c, int* split_k);
 /* Frees the idle workspaces of reef_ops_conv2d. */
 int reef_ops_release(void);
 
+/* ---- generating text: a paged key-value cache and beam search, on plain device pointers ----
+ * One step of a decoder beside its matrix products, in the order of its calls: reef_ops_block_plan
+ * gives the step's tokens their places in the cache, reef_ops_cache_append puts their keys and values
+ * there, reef_ops_paged_attention attends over them, reef_ops_beam_select chooses the next tokens and
+ * reef_ops_beam_reorder lets the block tables follow the chosen beams.  No counterpart in the reference,
+ * whose models see whole sequences (resource/bert/bert.cu:22-271).
+ *
+ * All pointers but the descriptors are device memory of the current device, and `stream` is a
+ * hipStream_t of that device (NULL: the default stream).  The calls check what the host can see, enqueue
+ * kernels and return; they allocate nothing, keep nothing and may be captured into a graph (kernel
+ * nodes only).  Operands that overlap outputs are not supported unless said.  A call without rows
+ * (requests, tokens or rows 0) succeeds.  Anything refused is Status::Fail with a message, and nothing is launched.
+ * The workspace of a call is the caller's: uninitialised memory, 16-byte aligned, that no other call uses at the
+ * same time (two graphs that may run at once need one each).  Its size depends on the descriptor alone.
+ * Results depend neither on what else runs nor on earlier calls, bit for bit. */
+
+/* Types of values. */
+enum { REEF_TYPE_F32 = 0, REEF_TYPE_F16 = 1, REEF_TYPE_BF16 = 2 };
+
+/* A cache is two pools of one layout, keys and values.  Block b, token s of the block, head h starts
+ * at element b * block_stride + s * slot_stride + h * head_stride and holds head_dim consecutive
+ * values; heads may lie inside tokens or tokens inside heads.  head_dim: a multiple of 8 up to 256.
+ * Strides: no two rows overlap, multiples of 16 bytes; pools: 16-byte aligned. blocks * block_size < 2^31. */
+typedef struct {
+    int32_t type;                              /* REEF_TYPE_* */
+    int32_t blocks, block_size, kv_heads, head_dim;
+    int64_t block_stride, slot_stride, head_stride;   /* elements */
+} reef_cache_layout;
+
+/* Where token `token` of the request with this row of the block table (host memory, max_blocks entries) lies: 1 and the
+ * element offset of its first head, or 0 where the kernels take it as absent (behind the row's
+ * entries, or a block number outside the pool).  The device code's own arithmetic; needs no device. */
+int reef_ops_paged_row(const reef_cache_layout* cache, const int32_t* table_row, int max_blocks, int64_t token, int64_t* offset);
+
+/* Block tables and slot maps.  Request i holds cached[i] tokens and brings added[i] more (negative: 0); the
+ * new tokens of all requests lie one behind the other, in the order of the requests.  It needs
+ *     ceil((cached + added) / block_size) - ceil(cached / block_size)
+ * more blocks and gets the next ones of free_list, which are written to its row of `table` behind those that it has.
+ * A request is refused where its row of max_blocks entries is too short, where its tokens end behind
+ * max_tokens, or where it needs blocks and the list ends before it has them, counting the needs of all
+ * requests before it that fit their row and max_tokens, refused for blocks or not: it takes nothing.
+ *   table   [requests][table_stride], updated in place; entries that no new block gets stay as they are
+ *   lengths [requests]: cached + added, or cached for a refused request
+ *   starts  [requests + 1]: the first new token of each request, and the end (at most max_tokens)
+ *   slots   [max_tokens]: block * block_size + place in the block of each new token; -1 for tokens of refused
+ *           requests, where the block is not one of the pool's, and behind the last token
+ *   counts  [3]: entries of free_list used up, tokens (as the end of starts), requests refused
+ * free_list may be NULL where free_blocks is 0, slots where max_tokens is 0. */
+typedef struct {
+    int32_t requests;
+    int32_t blocks, block_size;                /* of the pool */
+    int32_t max_blocks, table_stride;          /* entries of a row that may be used; from row to row */
+    int32_t free_blocks, max_tokens;           /* entries of free_list and slots */
+} reef_block_plan_desc;
+int reef_ops_block_plan(const reef_block_plan_desc* d, const int32_t* cached, const int32_t* added, const int32_t* free_list,
+                        int32_t* table, int32_t* lengths, int32_t* starts, int32_t* slots, int32_t* counts, void* stream);
+
+/* Puts token t's key and value rows ([tokens][kv_heads][head_dim], strides in elements, multiples of 16 bytes, rows 16-byte
+ * aligned) at slots[t] of the pools, rounded to the cache's type (to nearest, ties to even).  A slot that is not one of the pool's is skipped.
+ * Two tokens with one slot: one of the two, not said which.  type: the cache's, or REEF_TYPE_F32. */
+typedef struct {
+    reef_cache_layout cache;
+    int32_t type, tokens;
+    int64_t key_stride, key_head_stride, value_stride, value_head_stride;
+} reef_cache_append_desc;
+int reef_ops_cache_append(const reef_cache_append_desc* d, const void* key, const void* value, const int32_t* slots,
+                          void* key_cache, void* value_cache, void* stream);
+
+/* Attention of one new token a request over its cached ones:
+ *     s_t = scale * query . key_t,   out = sum_t exp(s_t) value_t / sum_t exp(s_t),   lse = log sum_t exp(s_t)
+ * over the tokens t in [max(0, n - window), n) (window 0: [0, n)), n = lengths[i] held to [0, max_blocks * block_size], that
+ * are in blocks of the pool.  Query head h reads cache head h / (heads / kv_heads).  Without such a token, or where all
+ * s_t are -infinity, out is 0 and lse -infinity.  Values in places that are not read (behind a sequence, in front of the window)
+ * may be anything.  type (of query and out): the cache's, or REEF_TYPE_F32; products and sums in 32 bits.
+ * query, out: [requests][heads][head_dim], strides in elements, multiples of 16 bytes, 16-byte aligned.
+ * lse: [requests][heads], may be NULL.  `longest`: the largest length to expect, which sets into how many
+ * shares long sequences are split (0: what a row of the table can hold); other lengths are right too.
+ * reef_ops_paged_attention_workspace: bytes of workspace, which may be 0 (NULL then); -1: refused. */
+typedef struct {
+    reef_cache_layout cache;
+    int32_t type, requests, heads;
+    int32_t max_blocks, table_stride;
+    int32_t longest, window;
+    float scale;
+    int64_t query_stride, query_head_stride, out_stride, out_head_stride;
+} reef_paged_attention_desc;
+int64_t reef_ops_paged_attention_workspace(const reef_paged_attention_desc* d);
+int reef_ops_paged_attention(const reef_paged_attention_desc* d, const void* query, const void* key_cache, const void* value_cache,
+                             const int32_t* table, const int32_t* lengths, void* out, float* lse, void* workspace,
+                             int64_t workspace_bytes, void* stream);
+
+/* Beam search's choice.  Beam b of a request (row r = request * beams + b) offers token v at
+ *     scores[r] + logits[r][v] - log sum_u exp(logits[r][u]),
+ * a beam with ended[r] != 0 (ended may be NULL) only end_token, at scores[r].  What is not a finite number or lies below all
+ * (NaN, infinities of either sign) counts as -infinity.  Of the beams * vocab offers of a request the first
+ * `select` in descending order are given: best (the score), parents (the row r) and tokens, [requests][select].  They are
+ * compared in 64 bits; equal ones (those at -infinity among them) go by beam, then token, the lower first.
+ * logits: [rows][logits_stride] of `type`, aligned to their own size.  select: up to 128 and beams * vocab; beams: up to 128;
+ * vocab: below 2^24. */
+typedef struct {
+    int32_t type, requests, beams, vocab, select, end_token;
+    int64_t logits_stride;
+} reef_beam_select_desc;
+int64_t reef_ops_beam_select_workspace(const reef_beam_select_desc* d);
+int reef_ops_beam_select(const reef_beam_select_desc* d, const void* logits, const float* scores, const uint8_t* ended, float* best,
+                         int32_t* parents, int32_t* tokens, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Row i of the next step continues row p = parents[i] of this one, n = lengths[p] tokens long (held to [0, max_blocks * block_size]):
+ * its first ceil(n / block_size) table entries are those of p, with full blocks shared.  A last block that is not full is
+ * shared only by row p itself; for p != i its n % block_size tokens are copied, in all layers of both pools, to the block
+ * spare[i], which takes its place (a block number outside the pool, either one: entry -1 and nothing is copied).  lengths_out[i] = n.
+ * Entries behind stay as they are, and so does a row whose parent is not a row.
+ * table [table_rows][table_stride], table_out [rows][out_stride]: not the same memory.  spare: `rows` blocks that no row of `table`
+ * uses, no two alike.  The pools hold `layers` caches of the layout, layer_stride elements from one to the next. */
+typedef struct {
+    reef_cache_layout cache;
+    int32_t rows, table_rows, max_blocks, table_stride, out_stride, layers;
+    int64_t layer_stride;
+} reef_beam_reorder_desc;
+int reef_ops_beam_reorder(const reef_beam_reorder_desc* d, const int32_t* parents, const int32_t* lengths, const int32_t* table,
+                          const int32_t* spare, int32_t* table_out, int32_t* lengths_out, void* key_cache, void* value_cache, void* stream);
+
 /* GPUConfig (src/reef/executor/hip/hip_impl.cpp:9-74) */
 int reef_gpuconfig_num_cus(void);
 int reef_gpuconfig_num_xcds(void);

@@ -5,6 +5,7 @@ the library has not been built -- there is no fallback path.
 """
 import ctypes
 import os
+import sys
 
 import numpy as np
 
@@ -15,6 +16,7 @@ BASE, TRANS, HYBRID = 0, 1, 2
 RUN_DEFAULT, RUN_PREEMPTIBLE = 0, 1
 
 _lib = None
+_torch_first = False    # torch was there before the library was loaded: both then run on torch's HIP runtime
 
 
 class ReefError(RuntimeError):
@@ -24,7 +26,7 @@ class ReefError(RuntimeError):
 
 
 def lib():
-    global _lib
+    global _lib, _torch_first
     if _lib is None:
         if not os.path.exists(LIB_PATH):
             raise RuntimeError("libreef_amd.so is not built: run __graft_entry__.build() "
@@ -33,6 +35,7 @@ def lib():
         # the runtime's default of 4 hardware queues per process they share queues.  The runtime
         # reads this when it is loaded, so it has to be in the environment before the CDLL call.
         os.environ.setdefault("GPU_MAX_HW_QUEUES", "8")
+        _torch_first = "torch" in sys.modules
         _lib = ctypes.CDLL(LIB_PATH)
         _lib.reef_hal_last_error.restype = ctypes.c_char_p
     return _lib
@@ -461,3 +464,122 @@ def ops_conv2d_kernel(desc):
     split = ctypes.c_int()
     name = f(ctypes.byref(desc), ctypes.byref(split))
     return (name.decode(), split.value) if name else None
+
+
+# ---- generating text: paged key-value cache and beam search ---------------------------------
+TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+def _fields(ints, longs=(), floats=()):
+    return [(n, ctypes.c_int32) for n in ints] + [(n, ctypes.c_float) for n in floats] + [(n, ctypes.c_int64) for n in longs]
+
+
+class CacheLayout(ctypes.Structure):
+    _fields_ = _fields(("type", "blocks", "block_size", "kv_heads", "head_dim"), ("block_stride", "slot_stride", "head_stride"))
+
+
+class BlockPlanDesc(ctypes.Structure):
+    _fields_ = _fields(("requests", "blocks", "block_size", "max_blocks", "table_stride", "free_blocks", "max_tokens"))
+
+
+class CacheAppendDesc(ctypes.Structure):
+    _fields_ = [("cache", CacheLayout)] + _fields(("type", "tokens"), ("key_stride", "key_head_stride", "value_stride", "value_head_stride"))
+
+
+class PagedAttentionDesc(ctypes.Structure):
+    _fields_ = [("cache", CacheLayout)] + _fields(("type", "requests", "heads", "max_blocks", "table_stride", "longest", "window"),
+                                                  ("query_stride", "query_head_stride", "out_stride", "out_head_stride"), ("scale",))
+
+
+class BeamSelectDesc(ctypes.Structure):
+    _fields_ = _fields(("type", "requests", "beams", "vocab", "select", "end_token"), ("logits_stride",))
+
+
+class BeamReorderDesc(ctypes.Structure):
+    _fields_ = [("cache", CacheLayout)] + _fields(("rows", "table_rows", "max_blocks", "table_stride", "out_stride", "layers"), ("layer_stride",))
+
+
+# pointers behind the descriptor (workspaces go with their size)
+_OPS_POINTERS = {"block_plan": 8, "cache_append": 5, "paged_attention": 7, "beam_select": 6, "beam_reorder": 8}
+_OPS_WORKSPACE = ("paged_attention", "beam_select")
+_ops = {}
+
+
+def _op(name):
+    f = _ops.get(name)
+    if f is None:
+        f = getattr(lib(), "reef_ops_" + name)
+        p = ctypes.c_void_p
+        f.argtypes = [p] * (1 + _OPS_POINTERS[name]) + ([p, ctypes.c_int64] if name in _OPS_WORKSPACE else []) + [p]
+        _ops[name] = f
+    return f
+
+
+def _at(x):
+    """Address of a DeviceBuffer, of anything with data_ptr() (a torch tensor), or an address as it is."""
+    if x is None or isinstance(x, int):
+        return x
+    if isinstance(x, DeviceBuffer):
+        return x.ptr
+    # Loaded before torch, the library has a HIP runtime of its own, whose streams do not wait for torch's.
+    if not _torch_first:
+        raise RuntimeError("tensors of torch: import torch before the library is first used")
+    return x.data_ptr()
+
+
+def _nbytes(x):
+    return 0 if x is None else x.nbytes
+
+
+def ops_block_plan(desc, cached, added, free_list, table, lengths, starts, slots, counts, stream=None):
+    """reef_ops_block_plan; operands are DeviceBuffers, torch tensors or addresses.  Like the calls below it enqueues,
+    does not wait and returns the status."""
+    return _op("block_plan")(ctypes.addressof(desc), _at(cached), _at(added), _at(free_list), _at(table), _at(lengths), _at(starts),
+                             _at(slots), _at(counts), stream)
+
+
+def ops_cache_append(desc, key, value, slots, key_cache, value_cache, stream=None):
+    return _op("cache_append")(ctypes.addressof(desc), _at(key), _at(value), _at(slots), _at(key_cache), _at(value_cache), stream)
+
+
+def _workspace(name, desc):
+    f = getattr(lib(), "reef_ops_%s_workspace" % name)
+    f.argtypes, f.restype = [ctypes.c_void_p], ctypes.c_int64
+    n = f(ctypes.addressof(desc))
+    if n < 0:
+        raise ReefError("reef_ops_%s_workspace" % name, 1)
+    return n
+
+
+def ops_paged_attention_workspace(desc):
+    """Bytes of workspace that reef_ops_paged_attention wants for this descriptor."""
+    return _workspace("paged_attention", desc)
+
+
+def ops_paged_attention(desc, query, key_cache, value_cache, table, lengths, out, lse=None, workspace=None, stream=None):
+    return _op("paged_attention")(ctypes.addressof(desc), _at(query), _at(key_cache), _at(value_cache), _at(table), _at(lengths), _at(out),
+                                  _at(lse), _at(workspace), _nbytes(workspace), stream)
+
+
+def ops_beam_select_workspace(desc):
+    """Bytes of workspace that reef_ops_beam_select wants for this descriptor."""
+    return _workspace("beam_select", desc)
+
+
+def ops_beam_select(desc, logits, scores, ended, best, parents, tokens, workspace=None, stream=None):
+    return _op("beam_select")(ctypes.addressof(desc), _at(logits), _at(scores), _at(ended), _at(best), _at(parents), _at(tokens),
+                              _at(workspace), _nbytes(workspace), stream)
+
+
+def ops_beam_reorder(desc, parents, lengths, table, spare, table_out, lengths_out, key_cache, value_cache, stream=None):
+    return _op("beam_reorder")(ctypes.addressof(desc), _at(parents), _at(lengths), _at(table), _at(spare), _at(table_out), _at(lengths_out),
+                               _at(key_cache), _at(value_cache), stream)
+
+
+def ops_paged_row(cache, table_row, token):
+    """Element offset of a token's first head in the pools by one row of a block table, or None where it counts as absent.
+    The kernels' own arithmetic, on the host."""
+    row = np.ascontiguousarray(table_row, np.int32)
+    at = ctypes.c_int64()
+    ok = lib().reef_ops_paged_row(ctypes.byref(cache), row.ctypes.data_as(ctypes.c_void_p), len(row), ctypes.c_int64(token), ctypes.byref(at))
+    return at.value if ok else None

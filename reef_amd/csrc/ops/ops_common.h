@@ -1,0 +1,88 @@
+// What the operators on plain device pointers share: refusals, launches, the layout of a paged cache.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+
+#include "reef_c.h"
+#include "reef_hal.h"
+
+namespace reef_ops {
+
+inline int refuse(const char* what, const char* format, ...) {
+    char msg[256];
+    const int n = std::snprintf(msg, sizeof(msg), "%s: ", what);
+    va_list args;
+    va_start(args, format);
+    std::vsnprintf(msg + n, sizeof(msg) - n, format, args);
+    va_end(args);
+    reef_hal_set_error(msg);
+    return 1;   // Status::Fail
+}
+
+template <class Args>
+int launch(const char* what, void (*kernel)(Args), dim3 grid, dim3 block, Args args, void* stream) {
+    void* p[] = {&args};
+    const hipError_t e = hipLaunchKernel((const void*)kernel, grid, block, p, 0, (hipStream_t)stream);
+    return e == hipSuccess ? 0 : refuse(what, "%s", hipGetErrorString(e));
+}
+
+inline int type_bytes(int type) { return type == REEF_TYPE_F32 ? 4 : type == REEF_TYPE_F16 || type == REEF_TYPE_BF16 ? 2 : 0; }
+inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+// Two int32 arrays and the like: a pointer that is there and aligned.
+inline bool words(const void* p) { return p && aligned(p, 4); }
+inline bool rows16(const void* p) { return p && aligned(p, 16); }
+
+// Whether `count` steps of `stride` elements keep to 16 bytes.
+inline bool stride16(int64_t count, int64_t stride, int bytes) { return count <= 1 || (stride >= 0 && stride * bytes % 16 == 0); }
+
+// A layout that the kernels take: rows of 16-byte pieces, none over another, offsets that fit 60 bits.
+inline int check_layout(const char* what, const reef_cache_layout& c, int64_t layers = 1, int64_t layer_stride = 0) {
+    const int bytes = type_bytes(c.type);
+    if (!bytes) return refuse(what, "unknown cache type %d", c.type);
+    if (c.blocks < 1 || c.block_size < 1 || c.kv_heads < 1 || (int64_t)c.blocks * c.block_size >= (1ll << 31))
+        return refuse(what, "bad cache: %d blocks of %d tokens, %d heads", c.blocks, c.block_size, c.kv_heads);
+    if (c.head_dim < 8 || c.head_dim > 256 || c.head_dim % 8) return refuse(what, "head_dim %d is not a multiple of 8 up to 256", c.head_dim);
+    int64_t count[4] = {c.kv_heads, c.block_size, c.blocks, layers}, stride[4] = {c.head_stride, c.slot_stride, c.block_stride, layer_stride};
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j + 1 < 4 - i; ++j)
+            if (count[j] > 1 && (count[j + 1] <= 1 || stride[j] > stride[j + 1])) {   // (steps of one place go first)
+                const int64_t n = count[j], s = stride[j];
+                count[j] = count[j + 1], stride[j] = stride[j + 1], count[j + 1] = n, stride[j + 1] = s;
+            }
+    __int128 extent = c.head_dim;
+    for (int i = 0; i < 4; ++i) {
+        if (count[i] <= 1) continue;
+        if (!stride16(count[i], stride[i], bytes)) return refuse(what, "a cache stride of %lld elements is not a multiple of 16 bytes", (long long)stride[i]);
+        if (stride[i] < extent) return refuse(what, "a cache stride of %lld elements lets rows overlap", (long long)stride[i]);
+        extent += (__int128)stride[i] * (count[i] - 1);
+        if (extent >= (__int128)1 << 60) return refuse(what, "cache too large");
+    }
+    return 0;
+}
+
+// ---- places in a paged cache, the same on both sides ----------------------------------------------
+// Element offset of a token's first head, or -1: behind the entries, or a block number outside the pool.
+struct PagedView {
+    int32_t blocks, block_size, max_blocks;
+    int64_t block_stride, slot_stride;
+};
+__host__ __device__ inline int64_t paged_row(const PagedView& v, int32_t entry, int32_t place) {
+    return (uint32_t)entry < (uint32_t)v.blocks ? (int64_t)entry * v.block_stride + (int64_t)place * v.slot_stride : -1;
+}
+// What a request's length counts for: [0, what a row of the table holds].
+__host__ __device__ inline int32_t held_length(int32_t n, int32_t max_blocks, int32_t block_size) {
+    const int64_t room = (int64_t)max_blocks * block_size;
+    return n < 0 ? 0 : (int64_t)n > room ? (int32_t)room : n;
+}
+
+// ---- values in their types --------------------------------------------------------------------------
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+}  // namespace reef_ops

@@ -1,0 +1,194 @@
+"""The operators of text generation, what needs no device: places in a paged cache, and refused calls.  A refusal comes before
+anything is launched, so the addresses here are never followed."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from reef_amd import binding as B
+
+P = 4096        # an aligned address
+F32, F16, BF16 = 0, 1, 2
+
+
+def layout(**kw):
+    v = dict(type=BF16, blocks=10, block_size=16, kv_heads=2, head_dim=64, block_stride=2048, slot_stride=128, head_stride=64)
+    v.update(kw)
+    return B.CacheLayout(**v)
+
+
+def test_places_of_tokens():
+    c = layout()
+    row = [3, 9, -1, 10, 0, 2 ** 31 - 1]
+    assert B.ops_paged_row(c, row, 0) == 3 * 2048
+    assert B.ops_paged_row(c, row, 31) == 9 * 2048 + 15 * 128
+    assert B.ops_paged_row(c, row, 64) == 0
+    for token in (32, 47, 48, 63, 80, 96, 2 ** 40, -1):     # block -1, block 10 of 10, a wild one, behind the row
+        assert B.ops_paged_row(c, row, token) is None
+
+
+def test_places_past_32_bits():
+    c = layout(blocks=2 ** 20, block_size=1024, block_stride=1024 * 2048, slot_stride=2048, head_stride=64)
+    assert B.ops_paged_row(c, [2 ** 20 - 1], 1023) == (2 ** 20 - 1) * 1024 * 2048 + 1023 * 2048
+    c = layout(block_size=3)
+    assert B.ops_paged_row(c, [1, 2], 5) == 2 * 2048 + 2 * 128
+
+
+BAD_LAYOUTS = [(dict(type=3), "type"), (dict(type=-1), "type"), (dict(blocks=0), "bad cache"), (dict(block_size=0), "bad cache"),
+               (dict(kv_heads=0), "bad cache"), (dict(blocks=2 ** 20, block_size=2 ** 11), "bad cache"), (dict(head_dim=60), "head_dim"),
+               (dict(head_dim=264), "head_dim"), (dict(head_dim=0), "head_dim"), (dict(head_stride=63), "16 bytes"),
+               (dict(head_stride=32), "overlap"), (dict(slot_stride=64), "overlap"), (dict(slot_stride=0), "overlap"),
+               (dict(block_stride=1024), "overlap"), (dict(block_stride=-2048), "16 bytes"), (dict(block_stride=2 ** 61), "too large")]
+
+
+def refused(status, text):
+    assert status == 1
+    assert text in B.last_error(), B.last_error()
+
+
+def call(name, desc, *args):
+    return B._op(name)(ctypes.addressof(desc), *args, None)
+
+
+def attention(cache, **kw):
+    v = dict(type=BF16, requests=2, heads=8, max_blocks=4, table_stride=4, longest=0, window=0, scale=0.125, query_stride=512,
+             query_head_stride=64, out_stride=512, out_head_stride=64)
+    v.update(kw)
+    return B.PagedAttentionDesc(cache=cache, **v)
+
+
+def append(cache, **kw):
+    v = dict(type=BF16, tokens=3, key_stride=128, key_head_stride=64, value_stride=128, value_head_stride=64)
+    v.update(kw)
+    return B.CacheAppendDesc(cache=cache, **v)
+
+
+def reorder(cache, **kw):
+    v = dict(rows=4, table_rows=4, max_blocks=4, table_stride=4, out_stride=4, layers=1, layer_stride=0)
+    v.update(kw)
+    return B.BeamReorderDesc(cache=cache, **v)
+
+
+def test_layouts_that_are_refused():
+    for change, text in BAD_LAYOUTS:
+        c = layout(**change)
+        refused(B.ops_cache_append(append(c, type=c.type), P, P, P, P, P), text)
+        refused(call("paged_attention", attention(c, type=c.type), *[P] * 8, 1 << 40), text)
+        refused(B.ops_beam_reorder(reorder(c), P, P, P, P, 2 * P, P, P, P), text)
+        with pytest.raises(B.ReefError):
+            B.ops_paged_attention_workspace(attention(c, type=c.type))
+
+
+def test_steps_of_one_place_may_be_anything():
+    c = layout(kv_heads=1, head_stride=1, blocks=1, block_stride=0)
+    assert B.ops_paged_attention_workspace(attention(c)) >= 0
+    c = layout(type=F32, head_dim=8, kv_heads=1, head_stride=0, slot_stride=8, block_stride=128)
+    assert B.ops_paged_attention_workspace(attention(c, type=F32)) >= 0
+
+
+@pytest.mark.parametrize("change,text", [(dict(type=F16), "type"), (dict(type=7), "type"), (dict(tokens=-1), "negative"),
+                                         (dict(key_stride=100), "16 bytes"), (dict(value_head_stride=-64), "16 bytes")])
+def test_append_refusals(change, text):
+    refused(B.ops_cache_append(append(layout(), **change), P, P, P, P, P), text)
+
+
+def test_append_pointers():
+    for i in range(5):
+        for bad in (None, P + (2 if i == 2 else 8)):
+            args = [P] * 5
+            args[i] = bad
+            refused(B.ops_cache_append(append(layout()), *args), "unaligned")
+    assert B.ops_cache_append(append(layout(), tokens=0), None, None, None, None, None) == 0
+    refused(B._op("cache_append")(None, P, P, P, P, P, None), "null")
+
+
+@pytest.mark.parametrize("change,text", [(dict(type=F16), "type"), (dict(heads=7), "heads"), (dict(heads=0), "heads"), (dict(requests=-1), "requests"),
+                                         (dict(requests=1 << 23, heads=8), "too many"), (dict(max_blocks=0), "table"), (dict(table_stride=3), "table"),
+                                         (dict(max_blocks=1 << 28, table_stride=1 << 28), "table"), (dict(window=-1), "window"),
+                                         (dict(longest=-5), "length"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+                                         (dict(query_stride=500), "16 bytes"), (dict(out_head_stride=60), "16 bytes")])
+def test_attention_refusals(change, text):
+    d = attention(layout(), **change)
+    refused(call("paged_attention", d, *[P] * 8, 1 << 40), text)
+    with pytest.raises(B.ReefError):
+        B.ops_paged_attention_workspace(d)
+
+
+def test_attention_pointers_and_workspace():
+    d = attention(layout())
+    for i in range(7):
+        for bad in ((None, P + 2) if i != 6 else (P + 2,)):
+            args = [P] * 7
+            args[i] = bad
+            refused(call("paged_attention", d, *args, P, 1 << 40), "unaligned")
+    assert call("paged_attention", attention(layout(), requests=0), *[None] * 8, 0) == 0
+
+
+@pytest.mark.parametrize("change,text", [(dict(requests=-1), "negative"), (dict(free_blocks=-1), "negative"), (dict(max_tokens=-1), "negative"),
+                                         (dict(blocks=0), "pool"), (dict(block_size=0), "pool"), (dict(blocks=1 << 20, block_size=1 << 11), "pool"),
+                                         (dict(max_blocks=0), "table"), (dict(table_stride=7), "table"), (dict(max_blocks=1 << 28, table_stride=1 << 28), "table")])
+def test_plan_refusals(change, text):
+    v = dict(requests=2, blocks=10, block_size=16, max_blocks=8, table_stride=8, free_blocks=4, max_tokens=8)
+    v.update(change)
+    refused(B.ops_block_plan(B.BlockPlanDesc(**v), *[P] * 8), text)
+
+
+def test_plan_pointers():
+    d = B.BlockPlanDesc(2, 10, 16, 8, 8, 4, 8)
+    for i in range(8):
+        for bad in (None, P + 1):
+            args = [P] * 8
+            args[i] = bad
+            refused(B.ops_block_plan(d, *args), "unaligned")
+
+
+@pytest.mark.parametrize("change,text", [(dict(type=5), "type"), (dict(requests=-1), "sizes"), (dict(beams=0), "sizes"), (dict(beams=129), "sizes"),
+                                         (dict(vocab=0), "sizes"), (dict(vocab=1 << 24), "sizes"), (dict(requests=1 << 22), "sizes"), (dict(select=0), "select"),
+                                         (dict(select=129), "select"), (dict(vocab=2, logits_stride=2, select=9), "select"), (dict(logits_stride=99), "overlap")])
+def test_select_refusals(change, text):
+    v = dict(type=F32, requests=2, beams=4, vocab=100, select=8, end_token=2, logits_stride=100)
+    v.update(change)
+    d = B.BeamSelectDesc(**v)
+    refused(call("beam_select", d, *[P] * 7, 1 << 40), text)
+    with pytest.raises(B.ReefError):
+        B.ops_beam_select_workspace(d)
+
+
+def test_select_pointers():
+    d = B.BeamSelectDesc(BF16, 2, 4, 100, 8, 2, 100)
+    for i in (0, 1, 3, 4, 5):
+        for bad in (None, P + 1):
+            args = [P] * 6
+            args[i] = bad
+            refused(call("beam_select", d, *args, P, 1 << 40), "unaligned")
+
+
+@pytest.mark.parametrize("change,text", [(dict(rows=-1), "rows"), (dict(table_rows=0), "rows"), (dict(layers=0), "layers"), (dict(max_blocks=0), "table"),
+                                         (dict(out_stride=3), "table"), (dict(table_stride=3), "table"), (dict(layers=2, layer_stride=2048), "overlap"),
+                                         (dict(layers=2, layer_stride=20484), "16 bytes")])
+def test_reorder_refusals(change, text):
+    refused(B.ops_beam_reorder(reorder(layout(), **change), P, P, P, P, 2 * P, P, P, P), text)
+
+
+def test_reorder_pointers():
+    d = reorder(layout(), layers=2, layer_stride=20480)
+    good = [P, P, P, P, 2 * P, P, P, P]
+    for i in range(8):
+        for bad in (None, good[i] + 2):
+            args = list(good)
+            args[i] = bad
+            refused(B.ops_beam_reorder(d, *args), "unaligned")
+    refused(B.ops_beam_reorder(d, P, P, P, P, P, P, P, P), "overlap")
+    refused(B.ops_beam_reorder(d, P, P, P, P, P + 60, P, P, P), "overlap")
+
+
+def test_tensors_of_a_torch_that_came_later_are_refused():
+    """Loaded first, the library has a HIP runtime of its own; in a process of its own, since the order is the test."""
+    import subprocess
+    import sys
+    code = ("from reef_amd import binding as B\nB.lib()\nimport torch\n"
+            "try:\n    B._at(torch.zeros(4))\nexcept RuntimeError as e:\n    assert 'import torch before' in str(e)\nelse:\n    raise SystemExit(3)\n")
+    import os
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stderr
