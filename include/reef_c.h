@@ -280,7 +280,8 @@ int reef_ops_paged_row(const reef_cache_layout* cache, const int32_t* table_row,
  *   starts  [requests + 1]: the first new token of each request, and the end (at most max_tokens)
  *   slots   [max_tokens]: block * block_size + place in the block of each new token; -1 for tokens of refused
  *           requests, where the block is not one of the pool's, and behind the last token
- *   counts  [3]: entries of free_list used up, tokens (as the end of starts), requests refused
+ *   counts  [3]: blocks that the requests up to the last granted one need, those refused for blocks among them (the entries of
+ *           free_list used up, where none is refused for blocks); tokens (as the end of starts); requests refused
  * free_list may be NULL where free_blocks is 0, slots where max_tokens is 0. */
 typedef struct {
     int32_t requests;

@@ -84,8 +84,8 @@ __global__ void __launch_bounds__(kThreads) block_plan(Args a) {
                 a.lengths[i] = granted ? (int32_t)(c[k] + n[k]) : c[k];
                 a.starts[i] = (int32_t)min(t_end[k] - n[k], (int64_t)d.max_tokens);
                 if (!granted) atomicAdd(&refused, 1);
-                if (granted && need[k] > 0) {
-                    atomicMax(&used, (int32_t)b_at);
+                if (granted) {
+                    atomicMax(&used, (int32_t)min(b_at, (int64_t)INT32_MAX));
                     for (int j = 0; j < need[k]; ++j) a.table[i * d.table_stride + have_[r] + j] = a.free_list[b_at - need[k] + j];
                 }
             }

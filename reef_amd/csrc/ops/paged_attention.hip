@@ -1,4 +1,5 @@
 // Attention of one new token a request over a paged key-value cache (reef_ops_paged_attention).
+#include <algorithm>
 #include <cmath>
 
 #include "ops_common.h"
@@ -7,6 +8,9 @@ namespace {
 using namespace reef_ops;
 
 constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMaxShares = 512;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Args {
     reef_paged_attention_desc d;
@@ -14,56 +18,400 @@ struct Args {
     const int32_t *table, *lengths;
     void* out;
     float* lse;
+    float* parts;           // [request][head][share][head_dim], sums that are not divided yet
+    float2* stats;          // [request][head][share]: maximum (of scores * log2 e) and sum
+    int32_t group, tiles;   // query heads a cache head; tiles of 16 of them
+    int32_t shares, least;  // a sequence's shares at most, tokens a share at least
 };
 
-// One workgroup a query head: 256 scores at a time, a token a thread, then the sum over them, an element a thread.
-template <class Q, class C>
-__global__ void __launch_bounds__(kThreads) paged_attention(Args a) {
+// Shares of a sequence of n tokens, and tokens of a share (the last one may be shorter).
+struct Shares {
+    int32_t n, tokens;
+};
+__host__ __device__ inline Shares shares_of(int32_t n, int32_t most, int32_t least) {
+    const int32_t by_size = (int32_t)(((int64_t)n + least - 1) / least), k = by_size < most ? by_size : most;
+    if (k <= 1) return {k, n};
+    const int32_t tokens = (int32_t)((((int64_t)n + k - 1) / k + 31) / 32 * 32);
+    return {(int32_t)(((int64_t)n + tokens - 1) / tokens), tokens};
+}
+
+// Four values of an output row: divided by the sum of the weights and rounded once, 0 where there are none.
+template <class Q>
+__device__ inline void put4(Q* to, f32x4 v, float sum) {
+    const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+    typedef Q Q4 __attribute__((ext_vector_type(4)));
+    const Q4 x = {(Q)(v[0] * f), (Q)(v[1] * f), (Q)(v[2] * f), (Q)(v[3] * f)};
+    *(Q4*)to = x;
+}
+
+// The maximum or sum over the four rows of 16 lanes.
+__device__ inline float over_rows_max(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ inline float over_rows_sum(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+template <class C>
+__device__ inline float to_float(uint32_t word, int odd) {
+    if constexpr (sizeof(C) == 4) return __uint_as_float(word);
+    else if constexpr (__is_same(C, __bf16)) return __uint_as_float(odd ? word & 0xFFFF0000u : word << 16);
+    else return (float)__builtin_bit_cast(_Float16, (uint16_t)(odd ? word >> 16 : word));
+}
+
+__device__ inline f32x4 product(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ inline f32x4 product(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ inline f32x4 product(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// Two weights as two terms of the type: the first cut, the second what is left of it.
+__device__ inline void two_terms(float a, float b, uint32_t* first, uint32_t* second, __bf16) {
+    *first = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 rest = {(__bf16)(a - __uint_as_float(__float_as_uint(a) & 0xFFFF0000u)), (__bf16)(b - __uint_as_float(__float_as_uint(b) & 0xFFFF0000u))};
+    *second = __builtin_bit_cast(uint32_t, rest);
+}
+__device__ inline void two_terms(float a, float b, uint32_t* first, uint32_t* second, _Float16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 cut = {(_Float16)a, (_Float16)b}, rest = {(_Float16)(a - (float)cut[0]), (_Float16)(b - (float)cut[1])};
+    *first = __builtin_bit_cast(uint32_t, cut);
+    *second = __builtin_bit_cast(uint32_t, rest);
+}
+
+// One share of a sequence, one cache head, up to 16 of its query heads: a workgroup whose wavefronts take tiles of 32 tokens (16
+// of a 32-bit cache) in turn, each with a running maximum, sum and output, and join at the end.
+//
+// Both products are 16x16 MFMAs whose operands come from memory as they lie there, 16 bytes a lane, with no way
+// through LDS:  S^T[token][head] = K Q^T, then O^T[dim][head] = V^T P^T.  A product does not care in which order its k runs:
+//   K Q^T: lane (row r, quarter g) loads pieces 4s + g of token r; the same pieces of Q are the other operand.
+//   V^T P^T: S^T leaves lane (head, g) the tokens 4g..4g+3 of a tile, so these are its k; lane (m, g) loads of each
+//   of them the m-th piece, whose e-th values are row m of the e-th product (dim = pieces * m + e).
+// So weights stay in the lane that made them, and a head's maximum, sum and rescaling are one value a lane.
+// 16-bit types use 16x16x32 products with weights in two terms of the type (a single one would put 2^-9 on bf16 outputs that
+// are off by 2^-9 at most from their own rounding); 32-bit queries use 16x16x4 products on 32-bit values, exact for 16-bit
+// caches.
+template <class Q, class C, int DP, bool WHOLE>
+__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attention(Args a) {
+    constexpr bool kNarrow = sizeof(Q) == 2;                  // products in the 16-bit type
+    constexpr int kPiece = 16 / sizeof(C);                    // values of 16 bytes
+    constexpr int kTile = sizeof(C) == 2 ? 32 : 16, kSub = kTile / 16;
+    constexpr int kSteps = DP / (4 * kPiece);                 // pieces of a key row a lane
+    constexpr int kV = DP / 16 < kPiece ? DP / 16 : kPiece;   // values of a value row a lane and slab
+    constexpr int kSlabs = DP / (16 * kV), kVWords = kV * sizeof(C) / 4;
+    constexpr int kQ = kNarrow ? kSteps * 4 : kSteps * kPiece;   // words of the query a lane
+    constexpr int kRow = DP + 4;                              // of the join, against bank conflicts
+
     const reef_paged_attention_desc& d = a.d;
-    const int r = blockIdx.x / d.heads, h = blockIdx.x % d.heads, kvh = h / (d.heads / d.cache.kv_heads), D = d.cache.head_dim;
+    int64_t id = blockIdx.x;
+    const int kvh = (int)(id % d.cache.kv_heads);
+    id /= d.cache.kv_heads;
+    const int tile16 = (int)(id % a.tiles);
+    id /= a.tiles;
+    const int share = (int)(id % a.shares), r = (int)(id / a.shares);
+    const int32_t held = held_length(a.lengths[r], d.max_blocks, d.cache.block_size);
+    const int32_t first = d.window && held > d.window ? held - d.window : 0;
+    const Shares of = shares_of(held - first, a.shares, a.least);
+    if (share >= of.n && !(share == 0)) return;
+    const int32_t begin = first + share * of.tokens, end = (int32_t)min((int64_t)held, (int64_t)begin + of.tokens);
+
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
+    const int D = d.cache.head_dim;
+    const int heads = min(16, a.group - tile16 * 16), head0 = kvh * a.group + tile16 * 16;
     const PagedView view{d.cache.blocks, d.cache.block_size, d.max_blocks, d.cache.block_stride, d.cache.slot_stride};
-    const int32_t n = held_length(a.lengths[r], d.max_blocks, d.cache.block_size);
-    const int32_t first = d.window && n > d.window ? n - d.window : 0;
-    __shared__ float q[256], p[kThreads], red[kThreads];
-    __shared__ int64_t rows[kThreads];
-    const Q* query = (const Q*)a.query + r * d.query_stride + h * d.query_head_stride;
     const C* keys = (const C*)a.key_cache + kvh * d.cache.head_stride;
     const C* values = (const C*)a.value_cache + kvh * d.cache.head_stride;
-    const int tid = threadIdx.x;
-    if (tid < D) q[tid] = (float)query[tid] * d.scale;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    for (int64_t t0 = first; t0 < n; t0 += kThreads) {
-        __syncthreads();
-        const int64_t t = t0 + tid;
-        float s = -INFINITY;
-        rows[tid] = -1;
-        if (t < n) {
-            const int64_t row = paged_row(view, a.table[(int64_t)r * d.table_stride + t / view.block_size], (int32_t)(t % view.block_size));
-            rows[tid] = row;
-            if (row >= 0) {
-                s = 0.0f;
-                for (int i = 0; i < D; ++i) s = fmaf(q[i], (float)keys[row + i], s);
+    const int32_t* table = a.table + (int64_t)r * d.table_stride;
+
+    __shared__ int64_t offsets[kWaves][2][kTile];
+    __shared__ float o_part[kWaves][16][kRow];
+    __shared__ float m_part[kWaves][16], l_part[kWaves][16];
+
+    // the queries: head n, the pieces that this lane's keys have
+    uint32_t q[kQ];
+    {
+        const Q* query = (const Q*)a.query + r * d.query_stride + (head0 + n) * d.query_head_stride;
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int at = (s * 4 + g) * kPiece;
+            const bool there = n < heads && at < D;
+#pragma unroll
+            for (int w = 0; w < kQ / kSteps; w += 4) {
+                u32x4 v = {0, 0, 0, 0};
+                if (there) v = *(const u32x4*)(query + at + w * 4 / sizeof(Q));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) q[s * (kQ / kSteps) + w + i] = v[i];
             }
         }
-        red[tid] = s;
-        __syncthreads();
-        float top = m;
-        for (int i = 0; i < kThreads; ++i) top = fmaxf(top, red[i]);
-        const float base = top == -INFINITY ? 0.0f : top;
-        p[tid] = rows[tid] >= 0 ? expf(s - base) : 0.0f;
-        __syncthreads();
-        const float f = expf(m - base);
-        l *= f;
-        o *= f;
-        for (int i = 0; i < kThreads; ++i) l += p[i];
-        if (tid < D)
-            for (int i = 0; i < kThreads; ++i)
-                if (rows[i] >= 0) o = fmaf(p[i], (float)values[rows[i] + tid], o);
-        m = top;
     }
-    Q* out = (Q*)a.out + r * d.out_stride + h * d.out_head_stride;
-    if (tid < D) out[tid] = (Q)(l == 0.0f ? 0.0f : o / l);
-    if (tid == 0 && a.lse) a.lse[(int64_t)r * d.heads + h] = l == 0.0f ? -INFINITY : m + logf(l);
+
+    const float scale = d.scale * kLog2e;
+    float m = -INFINITY, l = 0.0f;
+    f32x4 o[kSlabs][kV];
+#pragma unroll
+    for (int s = 0; s < kSlabs; ++s)
+#pragma unroll
+        for (int e = 0; e < kV; ++e) o[s][e] = {0.0f, 0.0f, 0.0f, 0.0f};
+
+    // the table's entry of one token of a tile a lane; -1: no token
+    auto entry_of = [&](int32_t t0) -> int32_t {
+        const int64_t t = (int64_t)t0 + lane;
+        return lane < kTile && t < end ? table[(int32_t)t / view.block_size] : -1;
+    };
+    // that token's place, for all lanes to read; which of the tile's tokens there are
+    auto place = [&](int32_t t0, int32_t entry, int buffer) -> uint32_t {
+        int64_t at = -1;
+        if (lane < kTile) {
+            at = paged_row(view, entry, (int32_t)(((int64_t)t0 + lane) % view.block_size));
+            offsets[wave][buffer][lane] = at < 0 ? 0 : at;
+        }
+        return (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0);
+    };
+    u32x4 k[kSub][kSteps];
+    uint32_t v[kSub][4][kSlabs][kVWords];
+    auto load_k = [&](int buffer) {
+#pragma unroll
+        for (int t = 0; t < kSub; ++t) {
+            const C* row = keys + offsets[wave][buffer][t * 16 + n];
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const int at = (s * 4 + g) * kPiece;
+                k[t][s] = *(const u32x4*)(row + (WHOLE || at < D ? at : 0));
+            }
+        }
+    };
+    auto load_v = [&](int buffer) {
+#pragma unroll
+        for (int t = 0; t < kSub; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const C* row = values + offsets[wave][buffer][t * 16 + g * 4 + i];
+#pragma unroll
+                for (int s = 0; s < kSlabs; ++s) {
+                    const int at = (s * 16 + n) * kV;
+                    const C* p = row + (WHOLE || at < D ? at : 0);
+                    if constexpr (kVWords == 4) {
+                        const u32x4 x = *(const u32x4*)p;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) v[t][i][s][w] = x[w];
+                    } else {
+                        const u32x2 x = *(const u32x2*)p;
+                        v[t][i][s][0] = x[0];
+                        v[t][i][s][1] = x[1];
+                    }
+                }
+            }
+    };
+
+    constexpr int32_t kStride = kWaves * kTile;
+    int32_t t0 = begin + wave * kTile;
+    uint32_t there = 0, there_next = 0;
+    int32_t entry = -1;
+    int buffer = 0;
+    if (t0 < end) {
+        there = place(t0, entry_of(t0), 0);
+        entry = t0 < end - kStride ? entry_of(t0 + kStride) : -1;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        load_k(0);
+        load_v(0);
+    }
+    while (t0 < end) {
+        const bool more = t0 < end - kStride;
+        if (more) {
+            there_next = place(t0 + kStride, entry, buffer ^ 1);
+            entry = t0 < end - 2 * kStride ? entry_of(t0 + 2 * kStride) : -1;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        // scores
+        f32x4 s[kSub];
+#pragma unroll
+        for (int t = 0; t < kSub; ++t) s[t] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+            for (int t = 0; t < kSub; ++t) {
+                u32x4 kk = k[t][c];
+                if constexpr (!WHOLE)
+                    if ((c * 4 + g) * kPiece >= D) kk = {0, 0, 0, 0};
+                if constexpr (kNarrow) {
+                    typedef C C8 __attribute__((ext_vector_type(8)));
+                    const u32x4 qq = {q[c * 4], q[c * 4 + 1], q[c * 4 + 2], q[c * 4 + 3]};
+                    s[t] = product(__builtin_bit_cast(C8, kk), __builtin_bit_cast(C8, qq), s[t]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < kPiece; ++e)
+                        s[t] = product(to_float<C>(kk[sizeof(C) == 2 ? e / 2 : e], e & 1), __uint_as_float(q[c * kPiece + e]), s[t]);
+                }
+            }
+        if (more) load_k(buffer ^ 1);
+        // weights
+        const bool all = there == (kTile == 32 ? 0xFFFFFFFFu : 0xFFFFu);
+        float top = m;
+#pragma unroll
+        for (int t = 0; t < kSub; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[t][i] *= scale;
+                if (!all && !(there >> (t * 16 + g * 4 + i) & 1)) s[t][i] = -INFINITY;
+                top = fmaxf(top, s[t][i]);
+            }
+        top = over_rows_max(top);
+        const float base = top == -INFINITY ? 0.0f : top;
+        if (__builtin_amdgcn_ballot_w64(top != m)) {
+            const float f = __builtin_amdgcn_exp2f(m - base);
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+                for (int e = 0; e < kV; ++e) o[c][e] *= f;
+        }
+        m = top;
+#pragma unroll
+        for (int t = 0; t < kSub; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - base);
+                l += s[t][i];
+            }
+        // values of places that are no tokens may be anything, and 0 times that too
+        if (!all) {
+#pragma unroll
+            for (int t = 0; t < kSub; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (!(there >> (t * 16 + g * 4 + i) & 1)) {
+#pragma unroll
+                        for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+                            for (int w = 0; w < kVWords; ++w) v[t][i][c][w] = 0;
+                    }
+        }
+        if constexpr (kNarrow) {
+            typedef C C8 __attribute__((ext_vector_type(8)));
+            u32x4 p1, p2;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t x, y;
+                two_terms(s[w >> 1][(w & 1) * 2], s[w >> 1][(w & 1) * 2 + 1], &x, &y, C());
+                p1[w] = x;
+                p2[w] = y;
+            }
+#pragma unroll
+            for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+                for (int e = 0; e < kV; ++e) {
+                    u32x4 x;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w)
+                        x[w] = __builtin_amdgcn_perm(v[w >> 1][(w & 1) * 2 + 1][c][e / 2], v[w >> 1][(w & 1) * 2][c][e / 2], e & 1 ? 0x07060302 : 0x05040100);
+                    o[c][e] = product(__builtin_bit_cast(C8, x), __builtin_bit_cast(C8, p1), o[c][e]);
+                    o[c][e] = product(__builtin_bit_cast(C8, x), __builtin_bit_cast(C8, p2), o[c][e]);
+                }
+        } else {
+#pragma unroll
+            for (int t = 0; t < kSub; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+                        for (int e = 0; e < kV; ++e)
+                            o[c][e] = product(to_float<C>(v[t][i][c][sizeof(C) == 2 ? e / 2 : e], e & 1), s[t][i], o[c][e]);
+        }
+        if (more) load_v(buffer ^ 1);
+        there = there_next;
+        buffer ^= 1;
+        if (!more) break;
+        t0 += kStride;
+    }
+
+    // the wavefronts' parts
+    l = over_rows_sum(l);
+    if (n < heads) {
+#pragma unroll
+        for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < kV; e += 4) {
+                    f32x4 x = {o[c][e][i], o[c][e + 1][i], o[c][e + 2][i], o[c][e + 3][i]};
+                    *(f32x4*)&o_part[wave][n][(c * 16 + g * 4 + i) * kV + e] = x;
+                }
+        if (g == 0) {
+            m_part[wave][n] = m;
+            l_part[wave][n] = l;
+        }
+    }
+    __syncthreads();
+    const int quads = D / 4;
+    for (int x = threadIdx.x; x < heads * quads; x += kThreads) {
+        const int h = x / quads, at = (x - h * quads) * 4;
+        float top = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, m_part[w][h]);
+        const float base = top == -INFINITY ? 0.0f : top;
+        f32x4 all = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            const float f = __builtin_amdgcn_exp2f(m_part[w][h] - base);
+            sum += f * l_part[w][h];
+            all += f * *(const f32x4*)&o_part[w][h][at];
+        }
+        const int64_t row = (int64_t)r * d.heads + head0 + h;
+        if (of.n > 1) {
+            *(f32x4*)(a.parts + (row * a.shares + share) * D + at) = all;
+            if (at == 0) a.stats[row * a.shares + share] = make_float2(top, sum);
+        } else {
+            put4((Q*)a.out + r * d.out_stride + (head0 + h) * d.out_head_stride + at, all, sum);
+            if (at == 0 && a.lse) a.lse[row] = sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
+        }
+    }
+}
+
+// The shares of a sequence of one query head: a workgroup, lanes over quads of the head, groups of them over the shares.
+template <class Q>
+__global__ void __launch_bounds__(kThreads) join_shares(Args a) {
+    const reef_paged_attention_desc& d = a.d;
+    const int64_t row = blockIdx.x;
+    const int r = (int)(row / d.heads), h = (int)(row - (int64_t)r * d.heads), D = d.cache.head_dim;
+    const int32_t held = held_length(a.lengths[r], d.max_blocks, d.cache.block_size);
+    const Shares of = shares_of(d.window && held > d.window ? d.window : held, a.shares, a.least);
+    if (of.n <= 1) return;
+    __shared__ float weight[kMaxShares];
+    __shared__ float red[2][kWaves];
+    __shared__ f32x4 sums[kThreads];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    float m = -INFINITY, l = 0.0f;
+    for (int s = tid; s < of.n; s += kThreads) m = fmaxf(m, a.stats[row * a.shares + s].x);
+    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, red[0][w]);
+    const float base = m == -INFINITY ? 0.0f : m;
+    for (int s = tid; s < of.n; s += kThreads) {
+        const float2 x = a.stats[row * a.shares + s];
+        weight[s] = __builtin_amdgcn_exp2f(x.x - base);
+        l += weight[s] * x.y;
+    }
+    for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x);
+    if (lane == 0) red[1][wave] = l;
+    __syncthreads();
+    l = 0.0f;
+    for (int w = 0; w < kWaves; ++w) l += red[1][w];
+    const int quads = D / 4, groups = kThreads / quads, mine = tid / quads, at = (tid - mine * quads) * 4;
+    f32x4 all = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (mine < groups)
+        for (int s = mine; s < of.n; s += groups) all += weight[s] * *(const f32x4*)(a.parts + (row * a.shares + s) * D + at);
+    sums[tid] = all;
+    __syncthreads();
+    if (mine) return;
+    for (int x = 1; x < groups; ++x) all += sums[x * quads + tid];
+    put4((Q*)a.out + r * d.out_stride + h * d.out_head_stride + at, all, l);
+    if (tid == 0 && a.lse) a.lse[row] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
 int check(const char* what, const reef_paged_attention_desc* d) {
@@ -83,11 +431,49 @@ int check(const char* what, const reef_paged_attention_desc* d) {
     return 0;
 }
 
+// Into how many shares sequences are split.
+struct Split {
+    int32_t tiles, shares, least;
+    size_t stats_bytes, bytes;
+};
+Split split_of(const reef_paged_attention_desc& d) {
+    const int32_t group = d.heads / d.cache.kv_heads, tiles = (group + 15) / 16;
+    int64_t longest = (int64_t)d.max_blocks * d.cache.block_size;
+    if (d.longest && d.longest < longest) longest = d.longest;
+    if (d.window && d.window < longest) longest = d.window;
+    const int64_t rows = (int64_t)d.requests * d.cache.kv_heads * tiles;
+    int32_t least = 512;
+    int64_t shares = std::min<int64_t>((longest + least - 1) / least, kMaxShares);
+    shares = std::max<int64_t>(1, std::min<int64_t>(shares, (int64_t)(1ll << 30) / std::max<int64_t>(rows, 1)));
+    Split s{tiles, (int32_t)shares, least, 0, 0};
+    if (shares > 1) {
+        const int64_t n = (int64_t)d.requests * d.heads * shares;
+        s.stats_bytes = (size_t)(n * 8 + 15) / 16 * 16;
+        s.bytes = s.stats_bytes + (size_t)n * d.cache.head_dim * 4;
+    }
+    return s;
+}
+
+template <class Q, class C>
+int run(const char* what, const Args& a, const Split& s, void* stream) {
+    const reef_paged_attention_desc& d = a.d;
+    const dim3 grid((unsigned)((int64_t)d.requests * d.cache.kv_heads * s.tiles * s.shares)), block(kThreads);
+    const int D = d.cache.head_dim;
+    const int rc = D == 64    ? launch(what, paged_attention<Q, C, 64, true>, grid, block, a, stream)
+                   : D < 64   ? launch(what, paged_attention<Q, C, 64, false>, grid, block, a, stream)
+                   : D == 128 ? launch(what, paged_attention<Q, C, 128, true>, grid, block, a, stream)
+                   : D < 128  ? launch(what, paged_attention<Q, C, 128, false>, grid, block, a, stream)
+                   : D == 256 ? launch(what, paged_attention<Q, C, 256, true>, grid, block, a, stream)
+                              : launch(what, paged_attention<Q, C, 256, false>, grid, block, a, stream);
+    if (rc || s.shares == 1) return rc;
+    return launch(what, join_shares<Q>, dim3((unsigned)(d.requests * d.heads)), block, a, stream);
+}
+
 }  // namespace
 
 extern "C" int64_t reef_ops_paged_attention_workspace(const reef_paged_attention_desc* d) {
     if (check("reef_ops_paged_attention_workspace", d)) return -1;
-    return 0;
+    return (int64_t)split_of(*d).bytes;
 }
 
 extern "C" int reef_ops_paged_attention(const reef_paged_attention_desc* d, const void* query, const void* key_cache, const void* value_cache,
@@ -98,13 +484,16 @@ extern "C" int reef_ops_paged_attention(const reef_paged_attention_desc* d, cons
     if (!d->requests) return 0;
     if (!rows16(query) || !rows16(key_cache) || !rows16(value_cache) || !rows16(out) || !words(table) || !words(lengths) || !aligned(lse, 4))
         return refuse(what, "null or unaligned argument");
-    const Args a{*d, query, key_cache, value_cache, table, lengths, out, lse};
-    const dim3 grid((unsigned)(d->requests * d->heads)), block(kThreads);
+    const Split s = split_of(*d);
+    if (s.bytes && (!rows16(workspace) || workspace_bytes < (int64_t)s.bytes))
+        return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", s.bytes, (long long)workspace_bytes);
+    const Args a{*d, query, key_cache, value_cache, table, lengths, out, lse, (float*)((char*)workspace + s.stats_bytes), (float2*)workspace,
+                 d->heads / d->cache.kv_heads, s.tiles, s.shares, s.least};
     switch (d->type * 4 + d->cache.type) {
-        case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return launch(what, paged_attention<float, float>, grid, block, a, stream);
-        case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return launch(what, paged_attention<float, _Float16>, grid, block, a, stream);
-        case REEF_TYPE_F32 * 4 + REEF_TYPE_BF16: return launch(what, paged_attention<float, __bf16>, grid, block, a, stream);
-        case REEF_TYPE_F16 * 4 + REEF_TYPE_F16: return launch(what, paged_attention<_Float16, _Float16>, grid, block, a, stream);
-        default: return launch(what, paged_attention<__bf16, __bf16>, grid, block, a, stream);
+        case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, s, stream);
+        case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return run<float, _Float16>(what, a, s, stream);
+        case REEF_TYPE_F32 * 4 + REEF_TYPE_BF16: return run<float, __bf16>(what, a, s, stream);
+        case REEF_TYPE_F16 * 4 + REEF_TYPE_F16: return run<_Float16, _Float16>(what, a, s, stream);
+        default: return run<__bf16, __bf16>(what, a, s, stream);
     }
 }

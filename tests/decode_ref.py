@@ -42,8 +42,9 @@ def plan(cached, added, free, table, blocks, bs, max_blocks, max_tokens):
         if ok:
             needs += need
             ok = need == 0 or needs <= len(free)
-        if ok and need:
+        if ok:
             used = needs
+        if ok and need:
             table[i, have:have + need] = free[needs - need:needs]
         if ok:
             for k in range(a):
