@@ -15,7 +15,13 @@ struct SelectArgs {
     const uint8_t* ended;
     float* best;
     int32_t *parents, *tokens;
+    float2* pieces;         // [row][piece]: maximum and sum of exp(x - maximum)
+    int32_t n_pieces;       // of a row
 };
+
+// A piece: 1 KiB of a row.
+template <class T>
+constexpr int kPiece = 1024 / sizeof(T);
 
 // A candidate: its score, its place beam * vocab + token.  Whether one goes before another.
 struct Offer {
@@ -28,60 +34,238 @@ __device__ inline bool before(const Offer& a, const Offer& b) {
 // Anything that is not a finite number counts as -infinity.
 __device__ inline double offered(double s) { return s < INFINITY && s > -INFINITY ? s : -INFINITY; }
 
+__device__ inline bool lives(const SelectArgs& a, int64_t row) { return !(a.ended && a.ended[row]); }
+
+// Everything that a choice needs of a row beside single values: of each piece the maximum and the sum over it.  Eight lanes a piece, 16
+// bytes a load, 128 bytes of one line a load and piece; a lane keeps its 64 (32) values, so the row is read once, and
+// the sum needs no rescaling.  Bound by memory: some ten operations a value are 60 % of the time that its bytes take.
 template <class T>
-__global__ void __launch_bounds__(kThreads) beam_select(SelectArgs a) {
+__global__ void __launch_bounds__(kThreads) row_pieces(SelectArgs a) {
+    constexpr int kE = 16 / sizeof(T);
     const reef_beam_select_desc& d = a.d;
-    const int tid = threadIdx.x;
-    __shared__ double red[kThreads];
-    __shared__ double lse[kMaxBeams];
-    __shared__ Offer top[kThreads];
+    const int lane = threadIdx.x & 63;
+    const int32_t rounds = (a.n_pieces + 7) / 8;
+    const int64_t id = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), row = id / rounds;
+    if (row >= (int64_t)d.requests * d.beams || !lives(a, row)) return;
+    const int32_t piece = (int32_t)(id - row * rounds) * 8 + (lane >> 3);
+    const int32_t at = piece * kPiece<T> + (lane & 7) * kE;
+    const T* x = (const T*)a.logits + row * d.logits_stride;
+    float v[8 * kE];
+    if ((piece + 1) * kPiece<T> <= d.vocab) {
+        T raw[8][kE];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) __builtin_memcpy(raw[u], x + at + u * 8 * kE, 16);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int e = 0; e < kE; ++e) v[u * kE + e] = (float)raw[u][e];
+    } else {
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int e = 0; e < kE; ++e) {
+                const int32_t i = at + u * 8 * kE + e;
+                v[u * kE + e] = i < d.vocab ? (float)x[i] : -INFINITY;
+            }
+    }
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < 8 * kE; ++i) m = fmaxf(m, v[i]);
+    m = fmaxf(m, -INFINITY);                  // (a NaN alone)
+    for (int i = 1; i < 8; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
+    const float base = m == -INFINITY ? 0.0f : m;
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8 * kE; ++i) s += __builtin_amdgcn_exp2f((v[i] - base) * 1.4426950408889634f);
+    for (int i = 1; i < 8; i <<= 1) s += __shfl_xor(s, i);
+    if ((lane & 7) == 0 && piece < a.n_pieces) a.pieces[row * a.n_pieces + piece] = make_float2(m, s);
+}
+
+constexpr int kChoose = 1024, kChooseWaves = kChoose / 64;
+constexpr int kBuffer = 2048;                 // candidates held; at least kMaxSelect and a piece
+
+// The choice of one request.  The maxima of the pieces, as scores, bound what a piece can hold: the select-th best of 256 groups'
+// best maxima lies below or at the select-th best offer, and only pieces that reach it are read again, some `select` of
+// them.  Their offers that pass the bound go to a buffer; where it would run over (many equal values) it is cut to its
+// best `select`, whose last one is the bound from then on.
+template <class T>
+__global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
+    constexpr int kE = kPiece<T> / 64;        // values of a piece a lane
+    const reef_beam_select_desc& d = a.d;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row0 = (int64_t)blockIdx.x * d.beams;
-    for (int b = 0; b < d.beams; ++b) {
-        const T* x = (const T*)a.logits + (row0 + b) * d.logits_stride;
+    __shared__ double lse[kMaxBeams], score[kMaxBeams];
+    __shared__ bool alive[kMaxBeams];
+    __shared__ double tops[256];
+    __shared__ Offer buffer[kBuffer], kept[kMaxSelect], bound;
+    __shared__ int32_t list[kChoose];
+    __shared__ int held, listed, wave_count[kChooseWaves];
+
+    for (int b = wave; b < d.beams; b += kChooseWaves) {
+        const bool live = lives(a, row0 + b);
+        double sum = 0.0;
         float m = -INFINITY;
-        for (int v = tid; v < d.vocab; v += kThreads) m = fmaxf(m, (float)x[v]);
-        red[tid] = m;
+        if (live) {
+            const float2* p = a.pieces + (row0 + b) * a.n_pieces;
+            for (int i = lane; i < a.n_pieces; i += 64) m = fmaxf(m, p[i].x);
+            for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+            const float base = m == -INFINITY ? 0.0f : m;
+            for (int i = lane; i < a.n_pieces; i += 64) sum += (double)p[i].y * exp((double)p[i].x - (double)base);
+            for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+        }
+        if (lane == 0) {
+            lse[b] = (double)m + log(sum);
+            score[b] = offered((double)a.scores[row0 + b]);
+            alive[b] = live;
+        }
+    }
+    if (tid == 0) held = listed = 0;
+    __syncthreads();
+    // what beam b offers for a logit; the best that a piece of it offers
+    auto offer = [&](int b, float x) { return offered(score[b] + ((double)x - lse[b])); };
+    const int32_t pieces = d.beams * a.n_pieces;
+    auto best_of = [&](int32_t i) -> double {
+        const int b = i / a.n_pieces, p = i - b * a.n_pieces;
+        if (alive[b]) return offer(b, a.pieces[(row0 + b) * a.n_pieces + p].x);
+        return d.end_token >= 0 && d.end_token < d.vocab && d.end_token / kPiece<T> == p ? score[b] : -INFINITY;
+    };
+    double top = -INFINITY;
+    for (int64_t i = tid; i < pieces; i += kChoose) top = fmax(top, best_of((int32_t)i));
+    top = fmax(top, __shfl_xor(top, 1));
+    top = fmax(top, __shfl_xor(top, 2));
+    if ((tid & 3) == 0) tops[tid >> 2] = top;
+    __syncthreads();
+    if (tid < 256) {
+        const double mine = tops[tid];
+        int rank = 0;
+        for (int i = 0; i < 256; ++i) rank += tops[i] > mine || (tops[i] == mine && i < tid);
+        if (rank == d.select - 1) bound = {mine, d.beams, 0};
+    }
+    __syncthreads();
+
+    // The best `select` of the buffer, in order; the last of them bounds what follows.
+    auto cut = [&]() {
+        const int n = held;
         __syncthreads();
-        double top_m = -INFINITY;
-        for (int i = 0; i < kThreads; ++i) top_m = fmax(top_m, red[i]);
-        double s = 0.0;
-        for (int v = tid; v < d.vocab; v += kThreads) s += exp((double)(float)x[v] - top_m);
-        __syncthreads();
-        red[tid] = s;
-        __syncthreads();
-        if (tid == 0) {
-            double all = 0.0;
-            for (int i = 0; i < kThreads; ++i) all += red[i];
-            lse[b] = top_m + log(all);
+        for (int i = tid; i < n; i += kChoose) {
+            const Offer mine = buffer[i];
+            int rank = 0;
+            for (int j = 0; j < n; ++j) rank += before(buffer[j], mine);
+            if (rank < d.select) kept[rank] = mine;
         }
         __syncthreads();
-    }
-    Offer last = {INFINITY, -1, 0};
-    for (int k = 0; k < d.select; ++k) {
-        Offer mine = {-INFINITY, d.beams, 0};
-        for (int b = 0; b < d.beams; ++b) {
-            const T* x = (const T*)a.logits + (row0 + b) * d.logits_stride;
-            const double score = offered((double)a.scores[row0 + b]);
-            const bool over = a.ended && a.ended[row0 + b];
-            for (int v = tid; v < d.vocab; v += kThreads) {
-                const Offer o = {over ? (v == d.end_token ? score : -INFINITY) : offered(score + ((double)(float)x[v] - lse[b])), b, v};
-                if (before(last, o) && before(o, mine)) mine = o;
+        const int m = min(n, d.select);
+        if (tid < m) buffer[tid] = kept[tid];
+        if (tid == 0) {
+            held = m;
+            if (m == d.select) bound = kept[m - 1];
+        }
+        __syncthreads();
+    };
+    for (int64_t i0 = 0; i0 < pieces; i0 += kChoose) {
+        const int64_t i = i0 + tid;
+        if (i < pieces) {
+            const double s = best_of((int32_t)i);
+            if (s > -INFINITY && s >= bound.score) list[atomicAdd(&listed, 1)] = (int32_t)i;
+        }
+        __syncthreads();
+        const int n = listed;
+        for (int j0 = 0; j0 < n; j0 += kChooseWaves) {
+            Offer mine[kE];
+            int count = 0;
+            auto passing = [&]() {
+                count = 0;
+#pragma unroll
+                for (int e = 0; e < kE; ++e) count += mine[e].score > -INFINITY && before(mine[e], bound);
+                for (int x = 1; x < 64; x <<= 1) count += __shfl_xor(count, x);
+            };
+            const bool busy = j0 + wave < n;
+            if (busy) {
+                const int32_t i = list[j0 + wave];
+                const int b = i / a.n_pieces;
+                const int32_t v0 = (i - b * a.n_pieces) * kPiece<T>;
+                const T* x = (const T*)a.logits + (row0 + b) * d.logits_stride;
+#pragma unroll
+                for (int e = 0; e < kE; ++e) {
+                    const int32_t v = v0 + e * 64 + lane;
+                    double s = -INFINITY;
+                    if (v < d.vocab) s = alive[b] ? offer(b, (float)x[v]) : v == d.end_token ? score[b] : -INFINITY;
+                    mine[e] = {s, b, v};
+                }
+                passing();
+            }
+            if (lane == 0) wave_count[wave] = count;
+            __syncthreads();
+            int all = held;
+            for (int w = 0; w < kChooseWaves; ++w) all += wave_count[w];
+            __syncthreads();
+            auto push = [&]() {
+#pragma unroll
+                for (int e = 0; e < kE; ++e) {
+                    const bool go = mine[e].score > -INFINITY && before(mine[e], bound);
+                    const uint64_t who = __builtin_amdgcn_ballot_w64(go);
+                    if (!who) continue;
+                    int at = 0;
+                    if (lane == 0) at = atomicAdd(&held, __popcll(who));
+                    at = __shfl(at, 0) + __popcll(who & ((1ull << lane) - 1));
+                    if (go) buffer[at] = mine[e];
+                }
+            };
+            if (all <= kBuffer) {
+                if (busy) push();
+                __syncthreads();
+            } else {
+                for (int w = 0; w < kChooseWaves; ++w) {      // one wavefront after another, cut in between
+                    if (held + kPiece<T> > kBuffer) cut();
+                    if (wave == w && busy) push();
+                    __syncthreads();
+                }
             }
         }
-        top[tid] = mine;
         __syncthreads();
-        for (int i = 0; i < kThreads; ++i)
-            if (before(top[i], mine)) mine = top[i];
-        last = mine;
-        if (tid == 0) {
-            const int64_t at = (int64_t)blockIdx.x * d.select + k;
-            a.best[at] = (float)mine.score;
-            a.parents[at] = (int32_t)(row0 + mine.beam);
-            a.tokens[at] = mine.token;
-        }
+        if (tid == 0) listed = 0;
         __syncthreads();
     }
+    cut();
+    const int found = held;
+    const int64_t out = (int64_t)blockIdx.x * d.select;
+    if (tid < found) {
+        a.best[out + tid] = (float)buffer[tid].score;
+        a.parents[out + tid] = (int32_t)(row0 + buffer[tid].beam);
+        a.tokens[out + tid] = buffer[tid].token;
+    }
+    if (found == d.select) return;
+    // Fewer offers than places: the rest at -infinity, in order.  All offers above it are in the buffer, fewer than
+    // select, so the first 2 * select places hold enough of the others.
+    int rank = 0;
+    const int64_t p = tid;
+    bool none = false;
+    if (p < 2 * d.select && p < (int64_t)d.beams * d.vocab) {
+        const int b = (int)(p / d.vocab);
+        const int32_t v = (int32_t)(p - (int64_t)b * d.vocab);
+        none = true;
+        for (int j = 0; j < found; ++j) none = none && !(buffer[j].beam == b && buffer[j].token == v);
+    }
+    const uint64_t who = __builtin_amdgcn_ballot_w64(none);
+    if (lane == 0) wave_count[wave] = __popcll(who);
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) rank += wave_count[w];
+    rank += __popcll(who & ((1ull << lane) - 1)) + found;
+    if (none && rank < d.select) {
+        a.best[out + rank] = -INFINITY;
+        a.parents[out + rank] = (int32_t)(row0 + p / d.vocab);
+        a.tokens[out + rank] = (int32_t)(p % d.vocab);
+    }
 }
+
+template <class T>
+int run_select(const char* what, SelectArgs a, void* stream) {
+    const int64_t waves = (int64_t)a.d.requests * a.d.beams * ((a.n_pieces + 7) / 8);
+    if (int rc = launch(what, row_pieces<T>, dim3((unsigned)((waves + 3) / 4)), dim3(kThreads), a, stream)) return rc;
+    return launch(what, beam_choose<T>, dim3((unsigned)a.d.requests), dim3(kChoose), a, stream);
+}
+
+int32_t pieces_of(const reef_beam_select_desc& d) { return (int32_t)(((int64_t)d.vocab * type_bytes(d.type) + 1023) / 1024); }
 
 int check_select(const char* what, const reef_beam_select_desc* d) {
     if (!d) return refuse(what, "null argument");
@@ -143,7 +327,7 @@ __global__ void __launch_bounds__(kThreads) beam_reorder(ReorderArgs a) {
 
 extern "C" int64_t reef_ops_beam_select_workspace(const reef_beam_select_desc* d) {
     if (check_select("reef_ops_beam_select_workspace", d)) return -1;
-    return 0;
+    return (int64_t)d->requests * d->beams * pieces_of(*d) * (int64_t)sizeof(float2);
 }
 
 extern "C" int reef_ops_beam_select(const reef_beam_select_desc* d, const void* logits, const float* scores, const uint8_t* ended, float* best,
@@ -153,12 +337,14 @@ extern "C" int reef_ops_beam_select(const reef_beam_select_desc* d, const void* 
     if (!d->requests) return 0;
     if (!logits || !aligned(logits, type_bytes(d->type)) || !words(scores) || !words(best) || !words(parents) || !words(tokens))
         return refuse(what, "null or unaligned argument");
-    const SelectArgs a{*d, logits, scores, ended, best, parents, tokens};
-    const dim3 grid((unsigned)d->requests), block(kThreads);
+    const SelectArgs a{*d, logits, scores, ended, best, parents, tokens, (float2*)workspace, pieces_of(*d)};
+    const int64_t need = reef_ops_beam_select_workspace(d);
+    if (!rows16(workspace) || workspace_bytes < need)
+        return refuse(what, "a workspace of %lld bytes on 16 is needed, %lld are given", (long long)need, (long long)workspace_bytes);
     switch (d->type) {
-        case REEF_TYPE_F32: return launch(what, beam_select<float>, grid, block, a, stream);
-        case REEF_TYPE_F16: return launch(what, beam_select<_Float16>, grid, block, a, stream);
-        default: return launch(what, beam_select<__bf16>, grid, block, a, stream);
+        case REEF_TYPE_F32: return run_select<float>(what, a, stream);
+        case REEF_TYPE_F16: return run_select<_Float16>(what, a, stream);
+        default: return run_select<__bf16>(what, a, stream);
     }
 }
 
