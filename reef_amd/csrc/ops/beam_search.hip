@@ -337,6 +337,10 @@ extern "C" int reef_ops_beam_select(const reef_beam_select_desc* d, const void* 
     if (!d->requests) return 0;
     if (!logits || !aligned(logits, type_bytes(d->type)) || !words(scores) || !words(best) || !words(parents) || !words(tokens))
         return refuse(what, "null or unaligned argument");
+    const int64_t n = (int64_t)d->requests * d->beams, picks = 4ll * d->requests * d->select;
+    const Span out[] = {{best, picks}, {parents, picks}, {tokens, picks}, {workspace, reef_ops_beam_select_workspace(d)}};
+    const Span in[] = {{logits, ((n - 1) * d->logits_stride + d->vocab) * type_bytes(d->type)}, {scores, 4 * n}, {ended, ended ? n : 0}};
+    if (overlap(out, in)) return refuse(what, "an output overlaps an input");
     const SelectArgs a{*d, logits, scores, ended, best, parents, tokens, (float2*)workspace, pieces_of(*d)};
     const int64_t need = reef_ops_beam_select_workspace(d);
     if (!rows16(workspace) || workspace_bytes < need)
@@ -361,9 +365,9 @@ extern "C" int reef_ops_beam_reorder(const reef_beam_reorder_desc* d, const int3
     if (!words(parents) || !words(lengths) || !words(table) || !words(spare) || !words(table_out) || !words(lengths_out) || !rows16(key_cache) ||
         !rows16(value_cache))
         return refuse(what, "null or unaligned argument");
-    const int32_t *t0 = table, *t1 = t0 + ((int64_t)d->table_rows - 1) * d->table_stride + d->max_blocks;
-    const int32_t *o0 = table_out, *o1 = o0 + ((int64_t)d->rows - 1) * d->out_stride + d->max_blocks;
-    if (t0 < o1 && o0 < t1) return refuse(what, "table and table_out overlap");
+    const Span out[] = {{table_out, 4 * ((d->rows - 1ll) * d->out_stride + d->max_blocks)}, {lengths_out, 4ll * d->rows}};
+    const Span in[] = {{table, 4 * ((d->table_rows - 1ll) * d->table_stride + d->max_blocks)}, {lengths, 4ll * d->table_rows}, {parents, 4ll * d->rows}, {spare, 4ll * d->rows}};
+    if (overlap(out, in)) return refuse(what, "an output overlaps an input");
     const ReorderArgs a{*d, parents, lengths, table, spare, table_out, lengths_out, key_cache, value_cache};
     return launch(what, beam_reorder, dim3((unsigned)d->rows, 1 + 2 * d->layers), dim3(kThreads), a, stream);
 }

@@ -35,6 +35,19 @@ inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) =
 inline bool words(const void* p) { return p && aligned(p, 4); }
 inline bool rows16(const void* p) { return p && aligned(p, 16); }
 
+// Whether an output shares memory with an input.
+struct Span {
+    const void* p;
+    int64_t bytes;
+};
+template <int N, int M>
+bool overlap(const Span (&out)[N], const Span (&in)[M]) {
+    for (const Span& o : out)
+        for (const Span& i : in)
+            if (o.bytes > 0 && i.bytes > 0 && (const char*)o.p < (const char*)i.p + i.bytes && (const char*)i.p < (const char*)o.p + o.bytes) return true;
+    return false;
+}
+
 // Whether `count` steps of `stride` elements keep to 16 bytes.
 inline bool stride16(int64_t count, int64_t stride, int bytes) { return count <= 1 || (stride >= 0 && stride * bytes % 16 == 0); }
 

@@ -133,6 +133,23 @@ def test_plan_refusals(change, text):
     refused(B.ops_block_plan(B.BlockPlanDesc(**v), *[P] * 8), text)
 
 
+def test_outputs_over_inputs():
+    d = B.BlockPlanDesc(2, 10, 16, 8, 8, 4, 8)
+    good = [i * P for i in range(1, 9)]
+    for out in range(3, 8):
+        for i in range(3):
+            args = list(good)
+            args[out] = good[i] + 4
+            refused(B.ops_block_plan(d, *args), "overlap")
+    d = B.BeamSelectDesc(BF16, 2, 4, 100, 8, 2, 100)
+    good = [i * P for i in range(1, 8)]
+    for out in range(3, 7):
+        for i in range(3):
+            args = list(good)
+            args[out] = good[i] & ~15
+            refused(call("beam_select", d, *args, 1 << 40), "overlap")
+
+
 def test_plan_pointers():
     d = B.BlockPlanDesc(2, 10, 16, 8, 8, 4, 8)
     for i in range(8):
@@ -172,14 +189,15 @@ def test_reorder_refusals(change, text):
 
 def test_reorder_pointers():
     d = reorder(layout(), layers=2, layer_stride=20480)
-    good = [P, P, P, P, 2 * P, P, P, P]
+    good = [P, P, P, P, 2 * P, 3 * P, P, P]
     for i in range(8):
         for bad in (None, good[i] + 2):
             args = list(good)
             args[i] = bad
             refused(B.ops_beam_reorder(d, *args), "unaligned")
-    refused(B.ops_beam_reorder(d, P, P, P, P, P, P, P, P), "overlap")
-    refused(B.ops_beam_reorder(d, P, P, P, P, P + 60, P, P, P), "overlap")
+    refused(B.ops_beam_reorder(d, P, P, P, P, P, 3 * P, P, P), "overlap")
+    refused(B.ops_beam_reorder(d, P, P, P, P, P + 60, 3 * P, P, P), "overlap")
+    refused(B.ops_beam_reorder(d, P, P, P, P, 2 * P, P + 12, P, P), "overlap")
 
 
 def test_tensors_of_a_torch_that_came_later_are_refused():
