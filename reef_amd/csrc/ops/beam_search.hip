@@ -19,9 +19,12 @@ struct SelectArgs {
     int32_t n_pieces;       // of a row
 };
 
-// A piece: 1 KiB of a row.
+// A piece: 1 KiB of a row, from a line of 128 bytes on.  The first one starts with the line that the row starts in, `lead` values
+// in front of it (rows of an odd length start anywhere).
 template <class T>
 constexpr int kPiece = 1024 / sizeof(T);
+template <class T>
+__device__ inline int lead_of(const T* row) { return (int)((uintptr_t)row & 127) / (int)sizeof(T); }
 
 // A candidate: its score, its place beam * vocab + token.  Whether one goes before another.
 struct Offer {
@@ -48,25 +51,34 @@ __global__ void __launch_bounds__(kThreads) row_pieces(SelectArgs a) {
     const int64_t id = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), row = id / rounds;
     if (row >= (int64_t)d.requests * d.beams || !lives(a, row)) return;
     const int32_t piece = (int32_t)(id - row * rounds) * 8 + (lane >> 3);
-    const int32_t at = piece * kPiece<T> + (lane & 7) * kE;
     const T* x = (const T*)a.logits + row * d.logits_stride;
+    const int32_t p0 = piece * kPiece<T> - lead_of(x), at = p0 + (lane & 7) * kE;
     float v[8 * kE];
-    if ((piece + 1) * kPiece<T> <= d.vocab) {
-        T raw[8][kE];
+    if (p0 >= 0 && p0 + kPiece<T> <= d.vocab) {
+        typedef T Raw __attribute__((ext_vector_type(kE)));
+        Raw raw[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) __builtin_memcpy(raw[u], x + at + u * 8 * kE, 16);
+        for (int u = 0; u < 8; ++u) raw[u] = *(const Raw*)(x + at + u * 8 * kE);
 #pragma unroll
         for (int u = 0; u < 8; ++u)
 #pragma unroll
             for (int e = 0; e < kE; ++e) v[u * kE + e] = (float)raw[u][e];
-    } else {
+    } else {                                  // the row begins or ends in here
+        typedef T Raw __attribute__((ext_vector_type(kE)));
+        Raw raw[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const int32_t i = at + u * 8 * kE;
+            if (i >= 0 && i + kE <= d.vocab) raw[u] = *(const Raw*)(x + i);
+            else {
+#pragma unroll
+                for (int e = 0; e < kE; ++e) raw[u][e] = (uint32_t)(i + e) < (uint32_t)d.vocab ? x[i + e] : (T)-INFINITY;
+            }
+        }
 #pragma unroll
         for (int u = 0; u < 8; ++u)
 #pragma unroll
-            for (int e = 0; e < kE; ++e) {
-                const int32_t i = at + u * 8 * kE + e;
-                v[u * kE + e] = i < d.vocab ? (float)x[i] : -INFINITY;
-            }
+            for (int e = 0; e < kE; ++e) v[u * kE + e] = (float)raw[u][e];
     }
     float m = v[0];
 #pragma unroll
@@ -83,143 +95,238 @@ __global__ void __launch_bounds__(kThreads) row_pieces(SelectArgs a) {
 
 constexpr int kChoose = 1024, kChooseWaves = kChoose / 64;
 constexpr int kBuffer = 2048;                 // candidates held; at least kMaxSelect and a piece
+constexpr int kNear = 4096;                   // pieces that are held near; more are read from memory again
 
 // The choice of one request.  The maxima of the pieces, as scores, bound what a piece can hold: the select-th best of 256 groups'
 // best maxima lies below or at the select-th best offer, and only pieces that reach it are read again, some `select` of
 // them.  Their offers that pass the bound go to a buffer; where it would run over (many equal values) it is cut to its
-// best `select`, whose last one is the bound from then on.
+// best `select`, whose last one is the bound from then on.  Bound by latency: two trips to memory and some 15 barriers.
 template <class T>
 __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
-    constexpr int kE = kPiece<T> / 64;        // values of a piece a lane
+    constexpr int kE = kPiece<T> / 64, kTwo = 2;   // values of a piece a lane; pieces a wavefront and step
     const reef_beam_select_desc& d = a.d;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row0 = (int64_t)blockIdx.x * d.beams;
     __shared__ double lse[kMaxBeams], score[kMaxBeams];
     __shared__ bool alive[kMaxBeams];
-    __shared__ double tops[256];
+    __shared__ float tops[256];
+    __shared__ int ranks[256];
     __shared__ Offer buffer[kBuffer], kept[kMaxSelect], bound;
-    __shared__ int32_t list[kChoose];
+    __shared__ int32_t list[kNear];
+    __shared__ float2 near[kNear];
     __shared__ int held, listed, wave_count[kChooseWaves];
 
-    for (int b = wave; b < d.beams; b += kChooseWaves) {
-        const bool live = lives(a, row0 + b);
-        double sum = 0.0;
-        float m = -INFINITY;
-        if (live) {
-            const float2* p = a.pieces + (row0 + b) * a.n_pieces;
-            for (int i = lane; i < a.n_pieces; i += 64) m = fmaxf(m, p[i].x);
-            for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-            const float base = m == -INFINITY ? 0.0f : m;
-            for (int i = lane; i < a.n_pieces; i += 64) sum += (double)p[i].y * exp((double)p[i].x - (double)base);
-            for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-        }
-        if (lane == 0) {
-            lse[b] = (double)m + log(sum);
-            score[b] = offered((double)a.scores[row0 + b]);
-            alive[b] = live;
-        }
+    const int32_t pieces = d.beams * a.n_pieces;
+    const float2* far = a.pieces + row0 * a.n_pieces;
+#pragma unroll
+    for (int k = 0; k < kNear / kChoose; ++k) {
+        const int32_t i = k * kChoose + tid;
+        if (i < pieces) near[i] = far[i];     // (of an ended beam: never used)
     }
-    if (tid == 0) held = listed = 0;
+    for (int b = tid; b < d.beams; b += kChoose) {
+        alive[b] = lives(a, row0 + b);
+        score[b] = offered((double)a.scores[row0 + b]);
+    }
+    if (tid == 0) {
+        held = listed = 0;
+        bound = {-INFINITY, d.beams, 0};
+    }
+    __syncthreads();
+    auto row_of = [&](int b) { return (const T*)a.logits + (row0 + b) * d.logits_stride; };
+    auto piece = [&](int32_t i) { return i < kNear ? near[i] : far[i]; };
+    for (int b = wave; b < d.beams; b += kChooseWaves) {
+        if (!alive[b]) continue;
+        const int32_t p0 = b * a.n_pieces;
+        float m = -INFINITY;
+        for (int i = lane; i < a.n_pieces; i += 64) m = fmaxf(m, piece(p0 + i).x);
+        for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+        const float base = m == -INFINITY ? 0.0f : m;
+        double sum = 0.0;
+        for (int i = lane; i < a.n_pieces; i += 64) {
+            const float2 p = piece(p0 + i);
+            sum += (double)(p.y * __builtin_amdgcn_exp2f((p.x - base) * 1.4426950408889634f));
+        }
+        for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+        if (lane == 0) lse[b] = (double)m + log(sum);
+    }
     __syncthreads();
     // what beam b offers for a logit; the best that a piece of it offers
     auto offer = [&](int b, float x) { return offered(score[b] + ((double)x - lse[b])); };
-    const int32_t pieces = d.beams * a.n_pieces;
     auto best_of = [&](int32_t i) -> double {
         const int b = i / a.n_pieces, p = i - b * a.n_pieces;
-        if (alive[b]) return offer(b, a.pieces[(row0 + b) * a.n_pieces + p].x);
-        return d.end_token >= 0 && d.end_token < d.vocab && d.end_token / kPiece<T> == p ? score[b] : -INFINITY;
+        if (alive[b]) return offer(b, piece(i).x);
+        return d.end_token >= 0 && d.end_token < d.vocab && (d.end_token + lead_of(row_of(b))) / kPiece<T> == p ? score[b] : -INFINITY;
     };
     double top = -INFINITY;
     for (int64_t i = tid; i < pieces; i += kChoose) top = fmax(top, best_of((int32_t)i));
-    top = fmax(top, __shfl_xor(top, 1));
-    top = fmax(top, __shfl_xor(top, 2));
-    if ((tid & 3) == 0) tops[tid >> 2] = top;
-    __syncthreads();
-    if (tid < 256) {
-        const double mine = tops[tid];
+    // Raises the bound by one offer a thread (or -infinity): of groups of `per` threads, at least `select` of them, the maxima in
+    // 32 bits, rounded down, ranked by all threads together.
+    auto raise = [&](double top, int per) {
+        const int groups = kChoose / per;
+        float low = (float)top;
+        low -= fabsf(low) * 0x1p-23f + 1e-37f;
+        if (top == -INFINITY) low = -INFINITY;
+        for (int x = 1; x < per; x <<= 1) low = fmaxf(low, __shfl_xor(low, x));
+        if ((tid & (per - 1)) == 0) {
+            tops[tid / per] = low;
+            ranks[tid / per] = 0;
+        }
+        __syncthreads();
+        const int mine = tid & (groups - 1), others = groups / per, o0 = tid / groups * others;
+        const float value = tops[mine];
         int rank = 0;
-        for (int i = 0; i < 256; ++i) rank += tops[i] > mine || (tops[i] == mine && i < tid);
-        if (rank == d.select - 1) bound = {mine, d.beams, 0};
-    }
-    __syncthreads();
+#pragma unroll 4
+        for (int o = o0; o < o0 + others; ++o) rank += tops[o] > value || (tops[o] == value && o < mine);
+        atomicAdd(&ranks[mine], rank);
+        __syncthreads();
+        if (tid < groups && ranks[tid] == d.select - 1 && (double)value > bound.score) bound = {(double)value, d.beams, 0};
+        __syncthreads();
+    };
+    raise(top, d.select <= 32 ? 16 : 4);
 
     // The best `select` of the buffer, in order; the last of them bounds what follows.
     auto cut = [&]() {
-        const int n = held;
+        const int n = held, m = min(n, d.select);
         __syncthreads();
-        for (int i = tid; i < n; i += kChoose) {
-            const Offer mine = buffer[i];
-            int rank = 0;
-            for (int j = 0; j < n; ++j) rank += before(buffer[j], mine);
-            if (rank < d.select) kept[rank] = mine;
+        if (n <= 256) {                                       // ranked, eight lanes a candidate
+            for (int i0 = 0; i0 < n; i0 += kChoose / 8) {
+                const int i = i0 + (tid >> 3);
+                const Offer mine = buffer[min(i, n - 1)];
+                int rank = 0;
+                for (int j = tid & 7; j < n; j += 8) rank += before(buffer[j], mine);
+                rank += __shfl_xor(rank, 1);
+                rank += __shfl_xor(rank, 2);
+                rank += __shfl_xor(rank, 4);
+                if (i < n && (tid & 7) == 0 && rank < d.select) kept[rank] = mine;
+            }
+            __syncthreads();
+            if (tid < m) buffer[tid] = kept[tid];
+        } else {                                              // sorted (2048 candidates: 170 us ranked)
+            int size = 512;
+            while (size < n) size <<= 1;
+            for (int i = n + tid; i < size; i += kChoose) buffer[i] = {-INFINITY, INT32_MAX, 0};
+            for (int run = 2; run <= size; run <<= 1)
+                for (int step = run >> 1; step; step >>= 1) {
+                    __syncthreads();
+                    if (tid < size / 2) {
+                        const int i = (tid / step) * 2 * step + tid % step, j = i + step;
+                        const Offer x = buffer[i], y = buffer[j];
+                        if (before(y, x) == ((i & run) == 0)) {
+                            buffer[i] = y;
+                            buffer[j] = x;
+                        }
+                    }
+                }
+            __syncthreads();
         }
-        __syncthreads();
-        const int m = min(n, d.select);
-        if (tid < m) buffer[tid] = kept[tid];
         if (tid == 0) {
             held = m;
-            if (m == d.select) bound = kept[m - 1];
+            if (m == d.select) bound = n <= 256 ? kept[m - 1] : buffer[m - 1];
         }
         __syncthreads();
     };
-    for (int64_t i0 = 0; i0 < pieces; i0 += kChoose) {
-        const int64_t i = i0 + tid;
-        if (i < pieces) {
+    for (int64_t i0 = 0; i0 < pieces; i0 += kNear) {
+        for (int64_t i = i0 + tid; i < pieces && i < i0 + kNear; i += kChoose) {
             const double s = best_of((int32_t)i);
             if (s > -INFINITY && s >= bound.score) list[atomicAdd(&listed, 1)] = (int32_t)i;
         }
         __syncthreads();
         const int n = listed;
-        for (int j0 = 0; j0 < n; j0 += kChooseWaves) {
-            Offer mine[kE];
-            int count = 0;
-            auto passing = [&]() {
-                count = 0;
+        for (int j0 = 0; j0 < n; j0 += kChooseWaves * kTwo) {
+            float x[kTwo][kE];
+            double own[kTwo], norm[kTwo];
+            int beam[kTwo], v0[kTwo];
+            bool live[kTwo];
+            T raw[kTwo][kE];
 #pragma unroll
-                for (int e = 0; e < kE; ++e) count += mine[e].score > -INFINITY && before(mine[e], bound);
-                for (int x = 1; x < 64; x <<= 1) count += __shfl_xor(count, x);
-            };
-            const bool busy = j0 + wave < n;
-            if (busy) {
-                const int32_t i = list[j0 + wave];
-                const int b = i / a.n_pieces;
-                const int32_t v0 = (i - b * a.n_pieces) * kPiece<T>;
-                const T* x = (const T*)a.logits + (row0 + b) * d.logits_stride;
+            for (int u = 0; u < kTwo; ++u) {                  // all loads before any of them is looked at
+                const int j = j0 + u * kChooseWaves + wave, i = list[min(j, n - 1)], b = i / a.n_pieces;
+                const T* row = row_of(b);
+                beam[u] = j < n ? b : -1;
+                v0[u] = (i - b * a.n_pieces) * kPiece<T> - lead_of(row) + lane;
 #pragma unroll
-                for (int e = 0; e < kE; ++e) {
-                    const int32_t v = v0 + e * 64 + lane;
-                    double s = -INFINITY;
-                    if (v < d.vocab) s = alive[b] ? offer(b, (float)x[v]) : v == d.end_token ? score[b] : -INFINITY;
-                    mine[e] = {s, b, v};
-                }
-                passing();
+                for (int e = 0; e < kE; ++e) raw[u][e] = row[max(0, min(v0[u] + e * 64, d.vocab - 1))];
+                live[u] = alive[b];
+                own[u] = score[b];
+                norm[u] = live[u] ? lse[b] : 0.0;
             }
-            if (lane == 0) wave_count[wave] = count;
-            __syncthreads();
-            int all = held;
-            for (int w = 0; w < kChooseWaves; ++w) all += wave_count[w];
-            __syncthreads();
-            auto push = [&]() {
+#pragma unroll
+            for (int u = 0; u < kTwo; ++u) {
 #pragma unroll
                 for (int e = 0; e < kE; ++e) {
-                    const bool go = mine[e].score > -INFINITY && before(mine[e], bound);
+                    const int32_t v = v0[u] + e * 64;
+                    x[u][e] = (uint32_t)v >= (uint32_t)d.vocab ? -INFINITY : live[u] ? (float)raw[u][e] : v == d.end_token ? 0.0f : -INFINITY;
+                }
+            }
+            auto one = [&](int u, int e) -> Offer {
+                return {live[u] ? offered(own[u] + ((double)x[u][e] - norm[u])) : own[u], beam[u], v0[u] + e * 64};
+            };
+            // What a value must at least be for its offer to pass, a little lower than it is: few are looked at in 64 bits
+            // (by the roundings of both sides: offers of a beam whose score is large may be equal for many values).
+            float least[kTwo];
+            auto near_enough = [&](int u, int e) { return x[u][e] > -INFINITY && x[u][e] >= least[u]; };
+            auto count = [&]() {
+                const Offer limit = bound;
+                int mine = 0;
+#pragma unroll
+                for (int u = 0; u < kTwo; ++u) {
+                    const double f = limit.score - own[u] + norm[u];
+                    const double slack = fabs(f) * 0x1p-20 + (fabs(limit.score) + fabs(own[u]) + fabs(norm[u])) * 0x1p-49;
+                    least[u] = live[u] && limit.score > -INFINITY && own[u] > -INFINITY ? (float)(f - slack) : -INFINITY;
+                    if (beam[u] >= 0) {
+#pragma unroll
+                        for (int e = 0; e < kE; ++e) mine += __popcll(__builtin_amdgcn_ballot_w64(near_enough(u, e)));
+                    }
+                }
+                if (lane == 0) wave_count[wave] = mine;
+                __syncthreads();
+                int all = held;
+                for (int w = 0; w < kChooseWaves; ++w) all += wave_count[w];
+                __syncthreads();
+                return all;
+            };
+            int all = count();
+            if (all > held + 256) {
+                // pieces are few or alike: each lane's best offer is a bound of its own (16 beams of 500 tokens, 32 chosen: 600 -> 25 us)
+                double mine = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < kTwo; ++u)
+                    if (beam[u] >= 0) {
+#pragma unroll
+                        for (int e = 0; e < kE; ++e)
+                            if (x[u][e] > -INFINITY) mine = fmax(mine, one(u, e).score);
+                    }
+                raise(mine, 4);
+                all = count();
+            }
+            auto push = [&](int u) {
+                if (beam[u] < 0) return;
+                const Offer now = bound;
+#pragma unroll
+                for (int e = 0; e < kE; ++e) {
+                    if (!__builtin_amdgcn_ballot_w64(near_enough(u, e))) continue;
+                    const Offer o = one(u, e);
+                    const bool go = near_enough(u, e) && o.score > -INFINITY && before(o, now);
                     const uint64_t who = __builtin_amdgcn_ballot_w64(go);
                     if (!who) continue;
                     int at = 0;
                     if (lane == 0) at = atomicAdd(&held, __popcll(who));
                     at = __shfl(at, 0) + __popcll(who & ((1ull << lane) - 1));
-                    if (go) buffer[at] = mine[e];
+                    if (go) buffer[at] = o;
                 }
             };
             if (all <= kBuffer) {
-                if (busy) push();
+#pragma unroll
+                for (int u = 0; u < kTwo; ++u) push(u);
                 __syncthreads();
             } else {
-                for (int w = 0; w < kChooseWaves; ++w) {      // one wavefront after another, cut in between
-                    if (held + kPiece<T> > kBuffer) cut();
-                    if (wave == w && busy) push();
-                    __syncthreads();
-                }
+                for (int w = 0; w < kChooseWaves; ++w)        // one piece after another, cut in between
+#pragma unroll
+                    for (int u = 0; u < kTwo; ++u) {
+                        if (held + kPiece<T> > kBuffer) cut();
+                        if (wave == w) push(u);
+                        __syncthreads();
+                    }
             }
         }
         __syncthreads();
@@ -237,7 +344,7 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
     if (found == d.select) return;
     // Fewer offers than places: the rest at -infinity, in order.  All offers above it are in the buffer, fewer than
     // select, so the first 2 * select places hold enough of the others.
-    int rank = 0;
+    int rank = found;
     const int64_t p = tid;
     bool none = false;
     if (p < 2 * d.select && p < (int64_t)d.beams * d.vocab) {
@@ -250,7 +357,7 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
     if (lane == 0) wave_count[wave] = __popcll(who);
     __syncthreads();
     for (int w = 0; w < wave; ++w) rank += wave_count[w];
-    rank += __popcll(who & ((1ull << lane) - 1)) + found;
+    rank += __popcll(who & ((1ull << lane) - 1));
     if (none && rank < d.select) {
         a.best[out + rank] = -INFINITY;
         a.parents[out + rank] = (int32_t)(row0 + p / d.vocab);
@@ -265,7 +372,8 @@ int run_select(const char* what, SelectArgs a, void* stream) {
     return launch(what, beam_choose<T>, dim3((unsigned)a.d.requests), dim3(kChoose), a, stream);
 }
 
-int32_t pieces_of(const reef_beam_select_desc& d) { return (int32_t)(((int64_t)d.vocab * type_bytes(d.type) + 1023) / 1024); }
+// (with a lead of up to 127 bytes)
+int32_t pieces_of(const reef_beam_select_desc& d) { return (int32_t)(((int64_t)d.vocab * type_bytes(d.type) + 127 + 1023) / 1024); }
 
 int check_select(const char* what, const reef_beam_select_desc* d) {
     if (!d) return refuse(what, "null argument");

@@ -387,7 +387,8 @@ def run_select(kind, requests, beams, logits, n, scores=None, ended=None, end_to
 
 @pytest.mark.parametrize("kind", [F32, F16, BF16])
 @pytest.mark.parametrize("requests,beams,vocab,n", [(1, 1, 1, 1), (1, 1, 7, 7), (2, 3, 5, 15), (1, 4, 1000, 8), (3, 2, 511, 4), (2, 2, 512, 4), (2, 2, 513, 5),
-                                                    (1, 8, 30522, 16), (5, 5, 4097, 1), (2, 1, 70001, 128), (1, 128, 300, 128), (2, 16, 8193, 64)])
+                                                    (1, 8, 30522, 16), (5, 5, 4097, 1), (2, 1, 70001, 128), (1, 128, 300, 128), (2, 16, 8193, 64), (2, 16, 500, 32),
+                                                    (1, 64, 1100, 128), (3, 128, 40, 128), (1, 90, 40000, 10)])
 @pytest.mark.parametrize("pad", [0, 1])
 def test_select(kind, requests, beams, vocab, n, pad):
     """Values that no two rows share, but 16-bit types make ties inside rows."""
@@ -443,6 +444,8 @@ def test_select_scores_and_ended_beams(kind):
     run_select(kind, 2, 4, x, 16, ended=[0, 1] * 4, end_token=6006)
     run_select(kind, 2, 4, x, 16, ended=[0, 1] * 4, end_token=6007)
     run_select(kind, 2, 4, x, 8, scores=[-1e30, -5, -1e8, -4] * 2)
+    run_select(kind, 2, 4, x, 40, scores=[-1e30, -1e30, -2e30, -3e38] * 2)     # so large that every token offers the same
+    run_select(kind, 2, 4, x, 8, scores=[3e38, 1e20, 3e38, -1] * 2)
     x[1] = np.nan                                                              # an ended beam's logits are not read
     run_select(kind, 2, 4, x, 8, ended=[0, 1, 0, 0, 0, 0, 0, 0])
 
