@@ -7,9 +7,8 @@
 namespace {
 using namespace reef_ops;
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
-constexpr int kMaxShares = 512;
+constexpr int kThreads = 256;                // of a workgroup of four wavefronts, and of the join's
+constexpr int kGroups = 512;                 // workgroups that the shares of all sequences are to make, about two a CU
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Args {
@@ -18,21 +17,69 @@ struct Args {
     const int32_t *table, *lengths;
     void* out;
     float* lse;
-    float* parts;           // [request][head][share][head_dim], sums that are not divided yet
-    float2* stats;          // [request][head][share]: maximum (of scores * log2 e) and sum
+    float* parts;           // [share][head][head_dim], sums that are not divided yet
+    float2* stats;          // [share][head]: maximum (of scores * log2 e) and sum
+    int2* info;             // [request]: its first share and how many they are
     int32_t group, tiles;   // query heads a cache head; tiles of 16 of them
-    int32_t shares, least;  // a sequence's shares at most, tokens a share at least
+    int32_t budget;         // shares that all tokens are cut into, beside one a request; 0: sequences are not split
 };
 
-// Shares of a sequence of n tokens, and tokens of a share (the last one may be shorter).
-struct Shares {
-    int32_t n, tokens;
+constexpr int32_t kLeast = 128;              // tokens a share at least
+
+struct Share {
+    int32_t request, number, first, count;   // the number-th of `count` shares of the request, which start with share `first` of all
+    int32_t tokens;                          // of a share, the last one may be shorter
 };
-__host__ __device__ inline Shares shares_of(int32_t n, int32_t most, int32_t least) {
-    const int32_t by_size = (int32_t)(((int64_t)n + least - 1) / least), k = by_size < most ? by_size : most;
-    if (k <= 1) return {k, n};
-    const int32_t tokens = (int32_t)((((int64_t)n + k - 1) / k + 31) / 32 * 32);
-    return {(int32_t)(((int64_t)n + tokens - 1) / tokens), tokens};
+
+__device__ inline int32_t seen_tokens(const Args& a, int32_t r) {
+    const int32_t held = held_length(a.lengths[r], a.d.max_blocks, a.d.cache.block_size);
+    return a.d.window && held > a.d.window ? a.d.window : held;
+}
+
+// Finds share `id` of all: of equal size but for the last one of each sequence, so that long sequences among short ones, or few of
+// them, keep the device as busy as many.  Every workgroup adds up the lengths for itself; with the sum rounded up by
+// more than 32-bit additions lose, sum ceil(seen / tokens) <= budget + requests, the size of the grid.  number < 0: there is no such share.
+template <int THREADS>
+__device__ inline Share find_share(const Args& a, int32_t id) {
+    constexpr int kWaves = THREADS / 64;
+    __shared__ float sums[kWaves];
+    __shared__ int32_t counts[kWaves];
+    __shared__ Share found;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int32_t R = a.d.requests, per = (R + THREADS - 1) / THREADS, lo = min(R, tid * per), hi = min(R, lo + per);
+    float total = 0.0f;
+    for (int32_t r = lo; r < hi; ++r) total += (float)seen_tokens(a, r);
+    for (int x = 32; x; x >>= 1) total += __shfl_xor(total, x);
+    if (lane == 0) sums[wave] = total;
+    if (tid == 0) found.number = -1;
+    __syncthreads();
+    total = 0.0f;
+    for (int w = 0; w < kWaves; ++w) total += sums[w];
+    // (at most 2^24 requests: 2^18 additions a thread, each off by 2^-24 of the sum at most)
+    const float each = total * 1.02f / (float)a.budget;
+    const int32_t tokens = each < 2.0e9f ? max(kLeast, ((int32_t)each + 32) / 32 * 32) : INT32_MAX;
+    int32_t mine = 0;
+    for (int32_t r = lo; r < hi; ++r) mine += max(1, (int32_t)(((int64_t)seen_tokens(a, r) + tokens - 1) / tokens));
+    int32_t at = mine;
+    for (int x = 1; x < 64; x <<= 1) {
+        const int32_t o = __shfl_up(at, x);
+        if (lane >= x) at += o;
+    }
+    if (lane == 63) counts[wave] = at;
+    __syncthreads();
+    at -= mine;
+    for (int w = 0; w < wave; ++w) at += counts[w];
+    if (id >= at && id < at + mine)
+        for (int32_t r = lo; r < hi; ++r) {
+            const int32_t n = max(1, (int32_t)(((int64_t)seen_tokens(a, r) + tokens - 1) / tokens));
+            if (id < at + n) {
+                found = {r, id - at, at, n, tokens};
+                break;
+            }
+            at += n;
+        }
+    __syncthreads();
+    return found;
 }
 
 // Four values of an output row: divided by the sum of the weights and rounded once, 0 where there are none.
@@ -95,8 +142,8 @@ __device__ inline void two_terms(float a, float b, uint32_t* first, uint32_t* se
 // 16-bit types use 16x16x32 products with weights in two terms of the type (a single one would put 2^-9 on bf16 outputs that
 // are off by 2^-9 at most from their own rounding); 32-bit queries use 16x16x4 products on 32-bit values, exact for 16-bit
 // caches.
-template <class Q, class C, int DP, bool WHOLE>
-__global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attention(Args a) {
+template <class Q, class C, int DP, bool WHOLE, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) paged_attention(Args a) {
     constexpr bool kNarrow = sizeof(Q) == 2;                  // products in the 16-bit type
     constexpr int kPiece = 16 / sizeof(C);                    // values of 16 bytes
     constexpr int kTile = sizeof(C) == 2 ? 32 : 16, kSub = kTile / 16;
@@ -107,17 +154,21 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attention(A
     constexpr int kRow = DP + 4;                              // of the join, against bank conflicts
 
     const reef_paged_attention_desc& d = a.d;
-    int64_t id = blockIdx.x;
-    const int kvh = (int)(id % d.cache.kv_heads);
+    int32_t id = blockIdx.x;
+    const int kvh = id % d.cache.kv_heads;
     id /= d.cache.kv_heads;
-    const int tile16 = (int)(id % a.tiles);
+    const int tile16 = id % a.tiles;
     id /= a.tiles;
-    const int share = (int)(id % a.shares), r = (int)(id / a.shares);
+    Share of = {id, 0, 0, 1, 0};
+    if (a.budget) {
+        of = find_share<WAVES * 64>(a, id);
+        if (of.number < 0) return;
+        if (of.number == 0 && blockIdx.x % (d.cache.kv_heads * a.tiles) == 0 && threadIdx.x == 0) a.info[of.request] = make_int2(of.first, of.count);
+    }
+    const int32_t r = of.request;
     const int32_t held = held_length(a.lengths[r], d.max_blocks, d.cache.block_size);
     const int32_t first = d.window && held > d.window ? held - d.window : 0;
-    const Shares of = shares_of(held - first, a.shares, a.least);
-    if (share >= of.n && !(share == 0)) return;
-    const int32_t begin = first + share * of.tokens, end = (int32_t)min((int64_t)held, (int64_t)begin + of.tokens);
+    const int32_t begin = first + of.number * of.tokens, end = of.count > 1 ? (int32_t)min((int64_t)held, (int64_t)begin + of.tokens) : held;
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const int D = d.cache.head_dim;
@@ -127,9 +178,9 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attention(A
     const C* values = (const C*)a.value_cache + kvh * d.cache.head_stride;
     const int32_t* table = a.table + (int64_t)r * d.table_stride;
 
-    __shared__ int64_t offsets[kWaves][2][kTile];
-    __shared__ float o_part[kWaves][16][kRow];
-    __shared__ float m_part[kWaves][16], l_part[kWaves][16];
+    __shared__ int64_t offsets[WAVES][2][kTile];
+    __shared__ float o_part[WAVES][16][kRow];
+    __shared__ float m_part[WAVES][16], l_part[WAVES][16];
 
     // the queries: head n, the pieces that this lane's keys have
     uint32_t q[kQ];
@@ -207,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attention(A
             }
     };
 
-    constexpr int32_t kStride = kWaves * kTile;
+    constexpr int32_t kStride = WAVES * kTile;
     int32_t t0 = begin + wave * kTile;
     uint32_t there = 0, there_next = 0;
     int32_t entry = -1;
@@ -348,26 +399,26 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attention(A
     }
     __syncthreads();
     const int quads = D / 4;
-    for (int x = threadIdx.x; x < heads * quads; x += kThreads) {
+    for (int x = threadIdx.x; x < heads * quads; x += WAVES * 64) {
         const int h = x / quads, at = (x - h * quads) * 4;
         float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) top = fmaxf(top, m_part[w][h]);
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, m_part[w][h]);
         const float base = top == -INFINITY ? 0.0f : top;
         f32x4 all = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             const float f = __builtin_amdgcn_exp2f(m_part[w][h] - base);
             sum += f * l_part[w][h];
             all += f * *(const f32x4*)&o_part[w][h][at];
         }
-        const int64_t row = (int64_t)r * d.heads + head0 + h;
-        if (of.n > 1) {
-            *(f32x4*)(a.parts + (row * a.shares + share) * D + at) = all;
-            if (at == 0) a.stats[row * a.shares + share] = make_float2(top, sum);
+        if (of.count > 1) {
+            const int64_t row = (int64_t)(of.first + of.number) * d.heads + head0 + h;
+            *(f32x4*)(a.parts + row * D + at) = all;
+            if (at == 0) a.stats[row] = make_float2(top, sum);
         } else {
             put4((Q*)a.out + r * d.out_stride + (head0 + h) * d.out_head_stride + at, all, sum);
-            if (at == 0 && a.lse) a.lse[row] = sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
+            if (at == 0 && a.lse) a.lse[(int64_t)r * d.heads + head0 + h] = sum == 0.0f ? -INFINITY : (top + __log2f(sum)) * kLn2;
         }
     }
 }
@@ -375,25 +426,27 @@ __global__ void __launch_bounds__(kThreads, DP == 256 ? 1 : 2) paged_attention(A
 // The shares of a sequence of one query head: a workgroup, lanes over quads of the head, groups of them over the shares.
 template <class Q>
 __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
+    constexpr int kWaves = kThreads / 64;
     const reef_paged_attention_desc& d = a.d;
-    const int64_t row = blockIdx.x;
-    const int r = (int)(row / d.heads), h = (int)(row - (int64_t)r * d.heads), D = d.cache.head_dim;
-    const int32_t held = held_length(a.lengths[r], d.max_blocks, d.cache.block_size);
-    const Shares of = shares_of(d.window && held > d.window ? d.window : held, a.shares, a.least);
-    if (of.n <= 1) return;
-    __shared__ float weight[kMaxShares];
+    const int r = blockIdx.x / d.heads, h = blockIdx.x % d.heads, D = d.cache.head_dim;
+    const int2 of = a.info[r];
+    if (of.y <= 1) return;
+    __shared__ float weight[kGroups + 2];
     __shared__ float red[2][kWaves];
     __shared__ f32x4 sums[kThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const float2* stats = a.stats + (int64_t)of.x * d.heads + h;
+    const float* parts = a.parts + ((int64_t)of.x * d.heads + h) * D;
+    const int64_t step = (int64_t)d.heads * D;
     float m = -INFINITY, l = 0.0f;
-    for (int s = tid; s < of.n; s += kThreads) m = fmaxf(m, a.stats[row * a.shares + s].x);
+    for (int s = tid; s < of.y; s += kThreads) m = fmaxf(m, stats[(int64_t)s * d.heads].x);
     for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
     if (lane == 0) red[0][wave] = m;
     __syncthreads();
     for (int w = 0; w < kWaves; ++w) m = fmaxf(m, red[0][w]);
     const float base = m == -INFINITY ? 0.0f : m;
-    for (int s = tid; s < of.n; s += kThreads) {
-        const float2 x = a.stats[row * a.shares + s];
+    for (int s = tid; s < of.y; s += kThreads) {
+        const float2 x = stats[(int64_t)s * d.heads];
         weight[s] = __builtin_amdgcn_exp2f(x.x - base);
         l += weight[s] * x.y;
     }
@@ -404,14 +457,16 @@ __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
     for (int w = 0; w < kWaves; ++w) l += red[1][w];
     const int quads = D / 4, groups = kThreads / quads, mine = tid / quads, at = (tid - mine * quads) * 4;
     f32x4 all = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (mine < groups)
-        for (int s = mine; s < of.n; s += groups) all += weight[s] * *(const f32x4*)(a.parts + (row * a.shares + s) * D + at);
+    if (mine < groups) {
+#pragma unroll 4
+        for (int s = mine; s < of.y; s += groups) all += weight[s] * *(const f32x4*)(parts + s * step + at);
+    }
     sums[tid] = all;
     __syncthreads();
     if (mine) return;
     for (int x = 1; x < groups; ++x) all += sums[x * quads + tid];
     put4((Q*)a.out + r * d.out_stride + h * d.out_head_stride + at, all, l);
-    if (tid == 0 && a.lse) a.lse[row] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
+    if (tid == 0 && a.lse) a.lse[(int64_t)r * d.heads + h] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
 int check(const char* what, const reef_paged_attention_desc* d) {
@@ -431,49 +486,62 @@ int check(const char* what, const reef_paged_attention_desc* d) {
     return 0;
 }
 
-// Into how many shares sequences are split.
-struct Split {
-    int32_t tiles, shares, least;
-    size_t stats_bytes, bytes;
+// How a call is laid out.
+struct Plan {
+    int32_t tiles, budget;
+    bool wide;              // workgroups of more wavefronts
+    int64_t groups;         // workgroups
+    size_t info_bytes, stats_bytes, bytes;
 };
-Split split_of(const reef_paged_attention_desc& d) {
-    const int32_t group = d.heads / d.cache.kv_heads, tiles = (group + 15) / 16;
+// Wavefronts of a wide workgroup: as many as the registers of one kernel allow a CU, none for heads over 128.
+constexpr int wide_waves(int dp) { return dp <= 64 ? 16 : dp <= 128 ? 8 : 4; }
+Plan plan_of(const reef_paged_attention_desc& d) {
+    const int32_t group = d.heads / d.cache.kv_heads, tiles = (group + 15) / 16, rows = d.cache.kv_heads * tiles;
     int64_t longest = (int64_t)d.max_blocks * d.cache.block_size;
     if (d.longest && d.longest < longest) longest = d.longest;
     if (d.window && d.window < longest) longest = d.window;
-    const int64_t rows = (int64_t)d.requests * d.cache.kv_heads * tiles;
-    int32_t least = 512;
-    int64_t shares = std::min<int64_t>((longest + least - 1) / least, kMaxShares);
-    shares = std::max<int64_t>(1, std::min<int64_t>(shares, (int64_t)(1ll << 30) / std::max<int64_t>(rows, 1)));
-    Split s{tiles, (int32_t)shares, least, 0, 0};
-    if (shares > 1) {
-        const int64_t n = (int64_t)d.requests * d.heads * shares;
-        s.stats_bytes = (size_t)(n * 8 + 15) / 16 * 16;
-        s.bytes = s.stats_bytes + (size_t)n * d.cache.head_dim * 4;
-    }
-    return s;
+    const int64_t all = (int64_t)d.requests * rows;
+    const int tile = d.cache.type == REEF_TYPE_F32 ? 16 : 32, D = d.cache.head_dim, wide = wide_waves(D <= 64 ? 64 : D <= 128 ? 128 : 256);
+    Plan p{};
+    p.tiles = tiles;
+    p.wide = all < kGroups && longest <= (int64_t)4 * wide * tile;
+    p.groups = all;
+    if (p.wide || longest <= 4 * 4 * tile) return p;
+    p.budget = std::max(1, kGroups / rows);
+    const int64_t shares = (int64_t)p.budget + d.requests;
+    p.groups = shares * rows;
+    p.info_bytes = ((size_t)d.requests * 8 + 15) / 16 * 16;
+    p.stats_bytes = ((size_t)shares * d.heads * 8 + 15) / 16 * 16;
+    p.bytes = p.info_bytes + p.stats_bytes + (size_t)shares * d.heads * D * 4;
+    return p;
+}
+
+template <class Q, class C, int DP, bool WHOLE>
+int run_waves(const char* what, const Args& a, const Plan& p, void* stream) {
+    constexpr int kWide = wide_waves(DP);
+    const dim3 grid((unsigned)p.groups);
+    if (p.wide && kWide > 4) return launch(what, paged_attention<Q, C, DP, WHOLE, kWide>, grid, dim3(kWide * 64), a, stream);
+    return launch(what, paged_attention<Q, C, DP, WHOLE, 4>, grid, dim3(kThreads), a, stream);
 }
 
 template <class Q, class C>
-int run(const char* what, const Args& a, const Split& s, void* stream) {
-    const reef_paged_attention_desc& d = a.d;
-    const dim3 grid((unsigned)((int64_t)d.requests * d.cache.kv_heads * s.tiles * s.shares)), block(kThreads);
-    const int D = d.cache.head_dim;
-    const int rc = D == 64    ? launch(what, paged_attention<Q, C, 64, true>, grid, block, a, stream)
-                   : D < 64   ? launch(what, paged_attention<Q, C, 64, false>, grid, block, a, stream)
-                   : D == 128 ? launch(what, paged_attention<Q, C, 128, true>, grid, block, a, stream)
-                   : D < 128  ? launch(what, paged_attention<Q, C, 128, false>, grid, block, a, stream)
-                   : D == 256 ? launch(what, paged_attention<Q, C, 256, true>, grid, block, a, stream)
-                              : launch(what, paged_attention<Q, C, 256, false>, grid, block, a, stream);
-    if (rc || s.shares == 1) return rc;
-    return launch(what, join_shares<Q>, dim3((unsigned)(d.requests * d.heads)), block, a, stream);
+int run(const char* what, const Args& a, const Plan& p, void* stream) {
+    const int D = a.d.cache.head_dim;
+    const int rc = D == 64    ? run_waves<Q, C, 64, true>(what, a, p, stream)
+                   : D < 64   ? run_waves<Q, C, 64, false>(what, a, p, stream)
+                   : D == 128 ? run_waves<Q, C, 128, true>(what, a, p, stream)
+                   : D < 128  ? run_waves<Q, C, 128, false>(what, a, p, stream)
+                   : D == 256 ? run_waves<Q, C, 256, true>(what, a, p, stream)
+                              : run_waves<Q, C, 256, false>(what, a, p, stream);
+    if (rc || !p.budget) return rc;
+    return launch(what, join_shares<Q>, dim3((unsigned)(a.d.requests * a.d.heads)), dim3(kThreads), a, stream);
 }
 
 }  // namespace
 
 extern "C" int64_t reef_ops_paged_attention_workspace(const reef_paged_attention_desc* d) {
     if (check("reef_ops_paged_attention_workspace", d)) return -1;
-    return (int64_t)split_of(*d).bytes;
+    return (int64_t)plan_of(*d).bytes;
 }
 
 extern "C" int reef_ops_paged_attention(const reef_paged_attention_desc* d, const void* query, const void* key_cache, const void* value_cache,
@@ -484,16 +552,18 @@ extern "C" int reef_ops_paged_attention(const reef_paged_attention_desc* d, cons
     if (!d->requests) return 0;
     if (!rows16(query) || !rows16(key_cache) || !rows16(value_cache) || !rows16(out) || !words(table) || !words(lengths) || !aligned(lse, 4))
         return refuse(what, "null or unaligned argument");
-    const Split s = split_of(*d);
-    if (s.bytes && (!rows16(workspace) || workspace_bytes < (int64_t)s.bytes))
-        return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", s.bytes, (long long)workspace_bytes);
-    const Args a{*d, query, key_cache, value_cache, table, lengths, out, lse, (float*)((char*)workspace + s.stats_bytes), (float2*)workspace,
-                 d->heads / d->cache.kv_heads, s.tiles, s.shares, s.least};
+    const Plan p = plan_of(*d);
+    if (p.groups >= 1ll << 31) return refuse(what, "%lld workgroups are too many", (long long)p.groups);
+    if (p.bytes && (!rows16(workspace) || workspace_bytes < (int64_t)p.bytes))
+        return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", p.bytes, (long long)workspace_bytes);
+    char* w = (char*)workspace;
+    const Args a{*d, query, key_cache, value_cache, table, lengths, out, lse, (float*)(w + p.info_bytes + p.stats_bytes), (float2*)(w + p.info_bytes),
+                 (int2*)w, d->heads / d->cache.kv_heads, p.tiles, p.budget};
     switch (d->type * 4 + d->cache.type) {
-        case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, s, stream);
-        case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return run<float, _Float16>(what, a, s, stream);
-        case REEF_TYPE_F32 * 4 + REEF_TYPE_BF16: return run<float, __bf16>(what, a, s, stream);
-        case REEF_TYPE_F16 * 4 + REEF_TYPE_F16: return run<_Float16, _Float16>(what, a, s, stream);
-        default: return run<__bf16, __bf16>(what, a, s, stream);
+        case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, p, stream);
+        case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return run<float, _Float16>(what, a, p, stream);
+        case REEF_TYPE_F32 * 4 + REEF_TYPE_BF16: return run<float, __bf16>(what, a, p, stream);
+        case REEF_TYPE_F16 * 4 + REEF_TYPE_F16: return run<_Float16, _Float16>(what, a, p, stream);
+        default: return run<__bf16, __bf16>(what, a, p, stream);
     }
 }
