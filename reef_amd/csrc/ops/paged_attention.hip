@@ -107,8 +107,7 @@ __device__ inline float over_rows_sum(float x) {
 
 template <class C>
 __device__ inline float to_float(uint32_t word, int odd) {
-    if constexpr (sizeof(C) == 4) return __uint_as_float(word);
-    else if constexpr (__is_same(C, __bf16)) return __uint_as_float(odd ? word & 0xFFFF0000u : word << 16);
+    if constexpr (__is_same(C, __bf16)) return __uint_as_float(odd ? word & 0xFFFF0000u : word << 16);
     else return (float)__builtin_bit_cast(_Float16, (uint16_t)(odd ? word >> 16 : word));
 }
 
@@ -116,18 +115,30 @@ __device__ inline f32x4 product(f16x8 a, f16x8 b, f32x4 c) { return __builtin_am
 __device__ inline f32x4 product(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ inline f32x4 product(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-// Two weights as two terms of the type: the first cut, the second what is left of it.
-__device__ inline void two_terms(float a, float b, uint32_t* first, uint32_t* second, __bf16) {
-    *first = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+// Two values as `N` terms of a 16-bit type each, whose sums they are but for what the last rounds off: two terms keep 16 (bf16) or
+// 22 (fp16) bits, three all 24.  All but the last are cut, so that what is left has their sign.
+template <int N>
+__device__ inline void terms(float a, float b, uint32_t (&t)[N], __bf16) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    const bf16x2 rest = {(__bf16)(a - __uint_as_float(__float_as_uint(a) & 0xFFFF0000u)), (__bf16)(b - __uint_as_float(__float_as_uint(b) & 0xFFFF0000u))};
-    *second = __builtin_bit_cast(uint32_t, rest);
+#pragma unroll
+    for (int i = 0; i < N - 1; ++i) {
+        t[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+        a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+        b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+    }
+    const bf16x2 last = {(__bf16)a, (__bf16)b};
+    t[N - 1] = __builtin_bit_cast(uint32_t, last);
 }
-__device__ inline void two_terms(float a, float b, uint32_t* first, uint32_t* second, _Float16) {
+template <int N>
+__device__ inline void terms(float a, float b, uint32_t (&t)[N], _Float16) {
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    const f16x2 cut = {(_Float16)a, (_Float16)b}, rest = {(_Float16)(a - (float)cut[0]), (_Float16)(b - (float)cut[1])};
-    *first = __builtin_bit_cast(uint32_t, cut);
-    *second = __builtin_bit_cast(uint32_t, rest);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const f16x2 x = {(_Float16)a, (_Float16)b};
+        t[i] = __builtin_bit_cast(uint32_t, x);
+        a -= (float)x[0];
+        b -= (float)x[1];
+    }
 }
 
 // One share of a sequence, one cache head, up to 16 of its query heads: a workgroup whose wavefronts take tiles of 32 tokens (16
@@ -139,18 +150,21 @@ __device__ inline void two_terms(float a, float b, uint32_t* first, uint32_t* se
 //   V^T P^T: S^T leaves lane (head, g) the tokens 4g..4g+3 of a tile, so these are its k; lane (m, g) loads of each
 //   of them the m-th piece, whose e-th values are row m of the e-th product (dim = pieces * m + e).
 // So weights stay in the lane that made them, and a head's maximum, sum and rescaling are one value a lane.
-// 16-bit types use 16x16x32 products with weights in two terms of the type (a single one would put 2^-9 on bf16 outputs that
-// are off by 2^-9 at most from their own rounding); 32-bit queries use 16x16x4 products on 32-bit values, exact for 16-bit
-// caches.
+// 16-bit caches use 16x16x32 products.  Weights are two terms of the cache's type (a single one would put 2^-9 on bf16 outputs that are
+// off by 2^-9 at most from their own rounding); 32-bit queries are three terms, and so are their weights, which keeps all 24
+// bits at a fifth of the time of 16x16x4 products on 32-bit values.  Terms of fp16 need room below: queries are scaled by a power of
+// two to 2^13 a head, weights are up to 2^14.  32-bit caches use the 16x16x4 products.
 template <class Q, class C, int DP, bool WHOLE, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) paged_attention(Args a) {
-    constexpr bool kNarrow = sizeof(Q) == 2;                  // products in the 16-bit type
+    constexpr bool kNarrow = sizeof(C) == 2;                  // products in the cache's 16-bit type
+    constexpr bool kHalf = __is_same(C, _Float16);
+    constexpr int kTermsQ = sizeof(Q) == sizeof(C) ? 1 : 3, kTermsP = sizeof(Q) == 2 ? 2 : 3;
+    constexpr float kShift = kHalf ? 14.0f : 0.0f;            // weights are up to 2^kShift
     constexpr int kPiece = 16 / sizeof(C);                    // values of 16 bytes
     constexpr int kTile = sizeof(C) == 2 ? 32 : 16, kSub = kTile / 16;
     constexpr int kSteps = DP / (4 * kPiece);                 // pieces of a key row a lane
     constexpr int kV = DP / 16 < kPiece ? DP / 16 : kPiece;   // values of a value row a lane and slab
     constexpr int kSlabs = DP / (16 * kV), kVWords = kV * sizeof(C) / 4;
-    constexpr int kQ = kNarrow ? kSteps * 4 : kSteps * kPiece;   // words of the query a lane
     constexpr int kRow = DP + 4;                              // of the join, against bank conflicts
 
     const reef_paged_attention_desc& d = a.d;
@@ -183,24 +197,53 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     __shared__ float m_part[WAVES][16], l_part[WAVES][16];
 
     // the queries: head n, the pieces that this lane's keys have
-    uint32_t q[kQ];
+    float scale = d.scale * kLog2e;
+    u32x4 q[kTermsQ][kSteps];
     {
         const Q* query = (const Q*)a.query + r * d.query_stride + (head0 + n) * d.query_head_stride;
+        constexpr int kWords = kPiece * sizeof(Q) / 4;
+        uint32_t raw[kSteps][kWords];
 #pragma unroll
         for (int s = 0; s < kSteps; ++s) {
             const int at = (s * 4 + g) * kPiece;
-            const bool there = n < heads && at < D;
 #pragma unroll
-            for (int w = 0; w < kQ / kSteps; w += 4) {
+            for (int w = 0; w < kWords; w += 4) {
                 u32x4 v = {0, 0, 0, 0};
-                if (there) v = *(const u32x4*)(query + at + w * 4 / sizeof(Q));
+                if (n < heads && at < D) v = *(const u32x4*)(query + at + w * 4 / sizeof(Q));
 #pragma unroll
-                for (int i = 0; i < 4; ++i) q[s * (kQ / kSteps) + w + i] = v[i];
+                for (int i = 0; i < 4; ++i) raw[s][w + i] = v[i];
             }
+        }
+        if constexpr (kTermsQ == 1) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) q[0][s] = {raw[s][0], raw[s][1], raw[s][2], raw[s][3]};
+        } else {
+            float grow = 1.0f;
+            if constexpr (kHalf) {
+                float top = 0.0f;
+#pragma unroll
+                for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                    for (int w = 0; w < kWords; ++w) top = fmaxf(top, fabsf(__uint_as_float(raw[s][w])));
+                top = over_rows_max(top);
+                if (top > 0.0f && top < INFINITY) {
+                    const int by = max(-100, min(100, 13 - (int)((__float_as_uint(top) >> 23) - 127)));
+                    grow = __uint_as_float((uint32_t)(127 + by) << 23);
+                    scale *= __uint_as_float((uint32_t)(127 - by) << 23);
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t t[kTermsQ];
+                    terms(__uint_as_float(raw[s][2 * w]) * grow, __uint_as_float(raw[s][2 * w + 1]) * grow, t, C());
+#pragma unroll
+                    for (int x = 0; x < kTermsQ; ++x) q[x][s][w] = t[x];
+                }
         }
     }
 
-    const float scale = d.scale * kLog2e;
     float m = -INFINITY, l = 0.0f;
     f32x4 o[kSlabs][kV];
 #pragma unroll
@@ -290,14 +333,42 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
                     if ((c * 4 + g) * kPiece >= D) kk = {0, 0, 0, 0};
                 if constexpr (kNarrow) {
                     typedef C C8 __attribute__((ext_vector_type(8)));
-                    const u32x4 qq = {q[c * 4], q[c * 4 + 1], q[c * 4 + 2], q[c * 4 + 3]};
-                    s[t] = product(__builtin_bit_cast(C8, kk), __builtin_bit_cast(C8, qq), s[t]);
+#pragma unroll
+                    for (int x = kTermsQ - 1; x >= 0; --x) s[t] = product(__builtin_bit_cast(C8, kk), __builtin_bit_cast(C8, q[x][c]), s[t]);
                 } else {
 #pragma unroll
-                    for (int e = 0; e < kPiece; ++e)
-                        s[t] = product(to_float<C>(kk[sizeof(C) == 2 ? e / 2 : e], e & 1), __uint_as_float(q[c * kPiece + e]), s[t]);
+                    for (int e = 0; e < kPiece; ++e) s[t] = product(__uint_as_float(kk[e]), __uint_as_float(q[0][c][e]), s[t]);
                 }
             }
+        if constexpr (kTermsQ > 1) {
+            // An infinite key times a term that is 0 or of the other sign: the sum is made again on 32-bit values, as it is written.
+            bool odd = false;
+#pragma unroll
+            for (int t = 0; t < kSub; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) odd |= s[t][i] != s[t][i];
+            if (__builtin_amdgcn_ballot_w64(odd)) {
+#pragma unroll
+                for (int t = 0; t < kSub; ++t) s[t] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+                    for (int e = 0; e < kPiece; ++e) {
+                        float x = 0.0f;
+#pragma unroll
+                        for (int i = kTermsQ - 1; i >= 0; --i) {
+                            uint32_t y = q[i][c][e / 2];
+                            asm volatile("" : "+v"(y));       // (or the sums are made ahead of the loop, and held in registers for it)
+                            x += to_float<C>(y, e & 1);
+                        }
+#pragma unroll
+                        for (int t = 0; t < kSub; ++t) {
+                            const bool inside = WHOLE || (c * 4 + g) * kPiece < D;
+                            s[t] = product(inside ? to_float<C>(k[t][c][e / 2], e & 1) : 0.0f, x, s[t]);
+                        }
+                    }
+            }
+        }
         if (more) load_k(buffer ^ 1);
         // weights
         const bool all = there == (kTile == 32 ? 0xFFFFFFFFu : 0xFFFFu);
@@ -311,9 +382,9 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
                 top = fmaxf(top, s[t][i]);
             }
         top = over_rows_max(top);
-        const float base = top == -INFINITY ? 0.0f : top;
+        const float base = top == -INFINITY ? 0.0f : top - kShift;
         if (__builtin_amdgcn_ballot_w64(top != m)) {
-            const float f = __builtin_amdgcn_exp2f(m - base);
+            const float f = __builtin_amdgcn_exp2f(m - kShift - base);
             l *= f;
 #pragma unroll
             for (int c = 0; c < kSlabs; ++c)
@@ -343,13 +414,13 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
         }
         if constexpr (kNarrow) {
             typedef C C8 __attribute__((ext_vector_type(8)));
-            u32x4 p1, p2;
+            u32x4 p[kTermsP];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                uint32_t x, y;
-                two_terms(s[w >> 1][(w & 1) * 2], s[w >> 1][(w & 1) * 2 + 1], &x, &y, C());
-                p1[w] = x;
-                p2[w] = y;
+                uint32_t x[kTermsP];
+                terms(s[w >> 1][(w & 1) * 2], s[w >> 1][(w & 1) * 2 + 1], x, C());
+#pragma unroll
+                for (int i = 0; i < kTermsP; ++i) p[i][w] = x[i];
             }
 #pragma unroll
             for (int c = 0; c < kSlabs; ++c)
@@ -359,8 +430,8 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
 #pragma unroll
                     for (int w = 0; w < 4; ++w)
                         x[w] = __builtin_amdgcn_perm(v[w >> 1][(w & 1) * 2 + 1][c][e / 2], v[w >> 1][(w & 1) * 2][c][e / 2], e & 1 ? 0x07060302 : 0x05040100);
-                    o[c][e] = product(__builtin_bit_cast(C8, x), __builtin_bit_cast(C8, p1), o[c][e]);
-                    o[c][e] = product(__builtin_bit_cast(C8, x), __builtin_bit_cast(C8, p2), o[c][e]);
+#pragma unroll
+                    for (int i = kTermsP - 1; i >= 0; --i) o[c][e] = product(__builtin_bit_cast(C8, x), __builtin_bit_cast(C8, p[i]), o[c][e]);
                 }
         } else {
 #pragma unroll
@@ -371,7 +442,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
                     for (int c = 0; c < kSlabs; ++c)
 #pragma unroll
                         for (int e = 0; e < kV; ++e)
-                            o[c][e] = product(to_float<C>(v[t][i][c][sizeof(C) == 2 ? e / 2 : e], e & 1), s[t][i], o[c][e]);
+                            o[c][e] = product(__uint_as_float(v[t][i][c][e]), s[t][i], o[c][e]);
         }
         if (more) load_v(buffer ^ 1);
         there = there_next;
@@ -393,7 +464,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
                     *(f32x4*)&o_part[wave][n][(c * 16 + g * 4 + i) * kV + e] = x;
                 }
         if (g == 0) {
-            m_part[wave][n] = m;
+            m_part[wave][n] = m - kShift;
             l_part[wave][n] = l;
         }
     }
@@ -493,15 +564,15 @@ struct Plan {
     int64_t groups;         // workgroups
     size_t info_bytes, stats_bytes, bytes;
 };
-// Wavefronts of a wide workgroup: as many as the registers of one kernel allow a CU, none for heads over 128.
-constexpr int wide_waves(int dp) { return dp <= 64 ? 16 : dp <= 128 ? 8 : 4; }
+// Wavefronts of a wide workgroup: as many as the registers allow a CU; for heads over 128 those of any.
+constexpr int wide_waves(int dp, bool terms) { return dp <= 64 && !terms ? 16 : dp <= 128 ? 8 : 4; }
 Plan plan_of(const reef_paged_attention_desc& d) {
     const int32_t group = d.heads / d.cache.kv_heads, tiles = (group + 15) / 16, rows = d.cache.kv_heads * tiles;
     int64_t longest = (int64_t)d.max_blocks * d.cache.block_size;
     if (d.longest && d.longest < longest) longest = d.longest;
     if (d.window && d.window < longest) longest = d.window;
     const int64_t all = (int64_t)d.requests * rows;
-    const int tile = d.cache.type == REEF_TYPE_F32 ? 16 : 32, D = d.cache.head_dim, wide = wide_waves(D <= 64 ? 64 : D <= 128 ? 128 : 256);
+    const int tile = d.cache.type == REEF_TYPE_F32 ? 16 : 32, D = d.cache.head_dim, wide = wide_waves(D, d.type != d.cache.type);
     Plan p{};
     p.tiles = tiles;
     p.wide = all < kGroups && longest <= (int64_t)4 * wide * tile;
@@ -518,7 +589,7 @@ Plan plan_of(const reef_paged_attention_desc& d) {
 
 template <class Q, class C, int DP, bool WHOLE>
 int run_waves(const char* what, const Args& a, const Plan& p, void* stream) {
-    constexpr int kWide = wide_waves(DP);
+    constexpr int kWide = wide_waves(DP, sizeof(Q) != sizeof(C));
     const dim3 grid((unsigned)p.groups);
     if (p.wide && kWide > 4) return launch(what, paged_attention<Q, C, DP, WHOLE, kWide>, grid, dim3(kWide * 64), a, stream);
     return launch(what, paged_attention<Q, C, DP, WHOLE, 4>, grid, dim3(kThreads), a, stream);
