@@ -8,7 +8,10 @@ namespace {
 using namespace reef_ops;
 
 constexpr int kThreads = 256;                // of a workgroup of four wavefronts, and of the join's
-constexpr int kGroups = 512;                 // workgroups that the shares of all sequences are to make, about two a CU
+// Workgroups that the shares of all sequences are to make: what runs at once (two a CU; one for heads over 128) less an eighth, as each
+// sequence's last share is a shorter one more.  Just above what runs at once the last round is nearly empty: of
+// 128 .. 4096, 448 takes 282 us for 3 x 131071 tokens (512: 281, 640: 327), 190 for 14 x 15754 (512: 238), 65 for 64 mixed (1024: 62).
+constexpr int kGroups = 448;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Args {
@@ -578,7 +581,7 @@ Plan plan_of(const reef_paged_attention_desc& d) {
     p.wide = all < kGroups && longest <= (int64_t)4 * wide * tile;
     p.groups = all;
     if (p.wide || longest <= 4 * 4 * tile) return p;
-    p.budget = std::max(1, kGroups / rows);
+    p.budget = std::max(1, (D > 128 ? kGroups / 2 : kGroups) / rows);
     const int64_t shares = (int64_t)p.budget + d.requests;
     p.groups = shares * rows;
     p.info_bytes = ((size_t)d.requests * 8 + 15) / 16 * 16;
