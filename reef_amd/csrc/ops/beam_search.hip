@@ -26,14 +26,16 @@ constexpr int kPiece = 1024 / sizeof(T);
 template <class T>
 __device__ inline int lead_of(const T* row) { return (int)((uintptr_t)row & 127) / (int)sizeof(T); }
 
-// A candidate: its score, its place beam * vocab + token.  Whether one goes before another.
+// A candidate, in two whole numbers: its score, in an order that whole numbers have too, and its place, beam then token.
 struct Offer {
-    double score;
-    int32_t beam, token;
+    uint64_t key, place;
 };
-__device__ inline bool before(const Offer& a, const Offer& b) {
-    return a.score != b.score ? a.score > b.score : a.beam != b.beam ? a.beam < b.beam : a.token < b.token;
+__device__ inline uint64_t key_of(double score) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, score + 0.0);      // (-0 counts as 0)
+    return bits >> 63 ? ~bits : bits | 1ull << 63;
 }
+__device__ inline double score_of(uint64_t key) { return __builtin_bit_cast(double, key >> 63 ? key & ~(1ull << 63) : ~key); }
+__device__ inline bool before(const Offer& a, const Offer& b) { return (a.key > b.key) | ((a.key == b.key) & (a.place < b.place)); }
 // Anything that is not a finite number counts as -infinity.
 __device__ inline double offered(double s) { return s < INFINITY && s > -INFINITY ? s : -INFINITY; }
 
@@ -93,7 +95,7 @@ __global__ void __launch_bounds__(kThreads) row_pieces(SelectArgs a) {
     if ((lane & 7) == 0 && piece < a.n_pieces) a.pieces[row * a.n_pieces + piece] = make_float2(m, s);
 }
 
-constexpr int kChoose = 1024, kChooseWaves = kChoose / 64;
+constexpr int kChoose = 512, kChooseWaves = kChoose / 64;
 constexpr int kBuffer = 2048;                 // candidates held; at least kMaxSelect and a piece
 constexpr int kNear = 4096;                   // pieces that are held near; more are read from memory again
 
@@ -109,8 +111,8 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
     const int64_t row0 = (int64_t)blockIdx.x * d.beams;
     __shared__ double lse[kMaxBeams], score[kMaxBeams];
     __shared__ bool alive[kMaxBeams];
-    __shared__ float tops[256];
-    __shared__ int ranks[256];
+    __shared__ __align__(16) uint32_t tops[kChoose];
+    __shared__ int ranks[kChoose];
     __shared__ Offer buffer[kBuffer], kept[kMaxSelect], bound;
     __shared__ int32_t list[kNear];
     __shared__ float2 near[kNear];
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
     }
     if (tid == 0) {
         held = listed = 0;
-        bound = {-INFINITY, d.beams, 0};
+        bound = {key_of(-INFINITY), 0};       // whatever is above -infinity passes
     }
     __syncthreads();
     auto row_of = [&](int b) { return (const T*)a.logits + (row0 + b) * d.logits_stride; };
@@ -157,42 +159,66 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
         if (alive[b]) return offer(b, piece(i).x);
         return d.end_token >= 0 && d.end_token < d.vocab && (d.end_token + lead_of(row_of(b))) / kPiece<T> == p ? score[b] : -INFINITY;
     };
-    double top = -INFINITY;
-    for (int64_t i = tid; i < pieces; i += kChoose) top = fmax(top, best_of((int32_t)i));
-    // Raises the bound by one offer a thread (or -infinity): of groups of `per` threads, at least `select` of them, the maxima in
-    // 32 bits, rounded down, ranked by all threads together.
-    auto raise = [&](double top, int per) {
-        const int groups = kChoose / per;
+    double best[kNear / kChoose], top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kNear / kChoose; ++k) {
+        const int32_t i = k * kChoose + tid;
+        best[k] = i < pieces ? best_of(i) : -INFINITY;
+        top = fmax(top, best[k]);
+    }
+    for (int64_t i = kNear + tid; i < pieces; i += kChoose) top = fmax(top, best_of((int32_t)i));
+
+    // Raises the bound by one offer a thread (or -infinity), of the first `threads`: the maxima of groups of neighbours, `want` of them at
+    // least if there are so many threads, rounded down to 22 bits and made unique by their numbers, are ranked by all threads
+    // together, and the select-th best is the bound.
+    auto raise = [&](double top, int threads, int want) {
+        int per = 16, places = 64;
+        while (per > 1 && threads / per < want) per >>= 1;
+        const int groups = (threads + per - 1) / per;
+        while (places < groups) places <<= 1;
         float low = (float)top;
         low -= fabsf(low) * 0x1p-23f + 1e-37f;
         if (top == -INFINITY) low = -INFINITY;
         for (int x = 1; x < per; x <<= 1) low = fmaxf(low, __shfl_xor(low, x));
-        if ((tid & (per - 1)) == 0) {
-            tops[tid / per] = low;
+        if (tid % per == 0 && tid / per < places) {
+            const uint32_t bits = __float_as_uint(low), order = low == -INFINITY ? 0 : bits >> 31 ? ~bits : bits | 1u << 31;
+            tops[tid / per] = tid / per < groups ? (order & ~1023u) | (1023 - tid / per) : 0;
             ranks[tid / per] = 0;
         }
         __syncthreads();
-        const int mine = tid & (groups - 1), others = groups / per, o0 = tid / groups * others;
-        const float value = tops[mine];
-        int rank = 0;
+        // (threads that have no group of their own write what their slice does not have)
+        const int mine = tid & (places - 1), slices = kChoose / places, others = ((groups + slices - 1) / slices + 3) / 4 * 4, o0 = tid / places * others;
+        if (mine < groups) {
+            const uint32_t value = tops[mine];
+            int rank = 0;
 #pragma unroll 4
-        for (int o = o0; o < o0 + others; ++o) rank += tops[o] > value || (tops[o] == value && o < mine);
-        atomicAdd(&ranks[mine], rank);
+            for (int o = o0; o < min(places, o0 + others); o += 4) {
+                const u32x4 t = *(const u32x4*)&tops[o];
+                rank += (int)(t[0] > value) + (int)(t[1] > value) + (int)(t[2] > value) + (int)(t[3] > value);
+            }
+            if (rank) atomicAdd(&ranks[mine], rank);
+        }
         __syncthreads();
-        if (tid < groups && ranks[tid] == d.select - 1 && (double)value > bound.score) bound = {(double)value, d.beams, 0};
+        if (tid < groups && ranks[tid] == d.select - 1) {
+            const uint32_t order = tops[tid] & ~1023u;
+            const double least = (double)__uint_as_float(order >> 31 ? order & ~(1u << 31) : ~order);
+            if (order && key_of(least) > bound.key) bound = {key_of(least), ~0ull};
+        }
         __syncthreads();
     };
-    raise(top, d.select <= 32 ? 16 : 4);
+    // (up to as many groups a beam as are chosen: often one beam has them all)
+    raise(top, min(pieces, kChoose), max(2 * d.select, min(256, d.beams * d.select)));
 
     // The best `select` of the buffer, in order; the last of them bounds what follows.
     auto cut = [&]() {
         const int n = held, m = min(n, d.select);
         __syncthreads();
-        if (n <= 256) {                                       // ranked, eight lanes a candidate
+        if (n <= 512) {                                       // ranked, eight lanes a candidate
             for (int i0 = 0; i0 < n; i0 += kChoose / 8) {
                 const int i = i0 + (tid >> 3);
                 const Offer mine = buffer[min(i, n - 1)];
                 int rank = 0;
+#pragma unroll 4
                 for (int j = tid & 7; j < n; j += 8) rank += before(buffer[j], mine);
                 rank += __shfl_xor(rank, 1);
                 rank += __shfl_xor(rank, 2);
@@ -202,33 +228,36 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
             __syncthreads();
             if (tid < m) buffer[tid] = kept[tid];
         } else {                                              // sorted (2048 candidates: 170 us ranked)
-            int size = 512;
-            while (size < n) size <<= 1;
-            for (int i = n + tid; i < size; i += kChoose) buffer[i] = {-INFINITY, INT32_MAX, 0};
+            const int size = n <= 1024 ? 1024 : 2048;
+            for (int i = n + tid; i < size; i += kChoose) buffer[i] = {0, ~0ull};
+            __syncthreads();
             for (int run = 2; run <= size; run <<= 1)
                 for (int step = run >> 1; step; step >>= 1) {
-                    __syncthreads();
-                    if (tid < size / 2) {
-                        const int i = (tid / step) * 2 * step + tid % step, j = i + step;
+                    for (int t = tid; t < size / 2; t += kChoose) {
+                        const int i = (t / step) * 2 * step + t % step, j = i + step;
                         const Offer x = buffer[i], y = buffer[j];
                         if (before(y, x) == ((i & run) == 0)) {
                             buffer[i] = y;
                             buffer[j] = x;
                         }
                     }
+                    __syncthreads();
                 }
-            __syncthreads();
         }
         if (tid == 0) {
             held = m;
-            if (m == d.select) bound = n <= 256 ? kept[m - 1] : buffer[m - 1];
+            if (m == d.select) bound = n <= 512 ? kept[m - 1] : buffer[m - 1];
         }
         __syncthreads();
     };
     for (int64_t i0 = 0; i0 < pieces; i0 += kNear) {
-        for (int64_t i = i0 + tid; i < pieces && i < i0 + kNear; i += kChoose) {
-            const double s = best_of((int32_t)i);
-            if (s > -INFINITY && s >= bound.score) list[atomicAdd(&listed, 1)] = (int32_t)i;
+        const double least = score_of(bound.key);
+#pragma unroll
+        for (int k = 0; k < kNear / kChoose; ++k) {
+            const int64_t i = i0 + k * kChoose + tid;
+            if (i >= pieces) continue;
+            const double x = i0 ? best_of((int32_t)i) : best[k];
+            if (x > -INFINITY && x >= least) list[atomicAdd(&listed, 1)] = (int32_t)i;
         }
         __syncthreads();
         const int n = listed;
@@ -238,11 +267,18 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
             int beam[kTwo], v0[kTwo];
             bool live[kTwo];
             T raw[kTwo][kE];
+            const double least_now = score_of(bound.key);
 #pragma unroll
             for (int u = 0; u < kTwo; ++u) {                  // all loads before any of them is looked at
-                const int j = j0 + u * kChooseWaves + wave, i = list[min(j, n - 1)], b = i / a.n_pieces;
+                const int j = j0 + u * kChooseWaves + wave;
+                beam[u] = -1;
+                own[u] = norm[u] = 0.0;
+                live[u] = false;
+                v0[u] = 0;
+                if (j >= n || best_of(list[j]) < least_now) continue;     // (the bound rises on the way)
+                const int32_t i = list[j], b = i / a.n_pieces;
                 const T* row = row_of(b);
-                beam[u] = j < n ? b : -1;
+                beam[u] = b;
                 v0[u] = (i - b * a.n_pieces) * kPiece<T> - lead_of(row) + lane;
 #pragma unroll
                 for (int e = 0; e < kE; ++e) raw[u][e] = row[max(0, min(v0[u] + e * 64, d.vocab - 1))];
@@ -255,64 +291,70 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
 #pragma unroll
                 for (int e = 0; e < kE; ++e) {
                     const int32_t v = v0[u] + e * 64;
-                    x[u][e] = (uint32_t)v >= (uint32_t)d.vocab ? -INFINITY : live[u] ? (float)raw[u][e] : v == d.end_token ? 0.0f : -INFINITY;
+                    x[u][e] = beam[u] < 0 || (uint32_t)v >= (uint32_t)d.vocab ? -INFINITY : live[u] ? (float)raw[u][e] : v == d.end_token ? 0.0f : -INFINITY;
                 }
             }
             auto one = [&](int u, int e) -> Offer {
-                return {live[u] ? offered(own[u] + ((double)x[u][e] - norm[u])) : own[u], beam[u], v0[u] + e * 64};
+                return {key_of(live[u] ? offered(own[u] + ((double)x[u][e] - norm[u])) : own[u]), (uint64_t)beam[u] << 32 | (uint32_t)(v0[u] + e * 64)};
             };
             // What a value must at least be for its offer to pass, a little lower than it is: few are looked at in 64 bits
             // (by the roundings of both sides: offers of a beam whose score is large may be equal for many values).
-            float least[kTwo];
-            auto near_enough = [&](int u, int e) { return x[u][e] > -INFINITY && x[u][e] >= least[u]; };
+            float least_x[kTwo];
+            auto near_enough = [&](int u, int e) { return x[u][e] > -INFINITY && x[u][e] >= least_x[u]; };
+            int had = 0;                                      // held before this step
             auto count = [&]() {
-                const Offer limit = bound;
+                const double limit = score_of(bound.key);
                 int mine = 0;
 #pragma unroll
                 for (int u = 0; u < kTwo; ++u) {
-                    const double f = limit.score - own[u] + norm[u];
-                    const double slack = fabs(f) * 0x1p-20 + (fabs(limit.score) + fabs(own[u]) + fabs(norm[u])) * 0x1p-49;
-                    least[u] = live[u] && limit.score > -INFINITY && own[u] > -INFINITY ? (float)(f - slack) : -INFINITY;
-                    if (beam[u] >= 0) {
+                    if (beam[u] < 0) continue;
+                    const double f = limit - own[u] + norm[u];
+                    const double slack = fabs(f) * 0x1p-20 + (fabs(limit) + fabs(own[u]) + fabs(norm[u])) * 0x1p-49;
+                    least_x[u] = live[u] && limit > -INFINITY && own[u] > -INFINITY ? (float)(f - slack) : -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < kE; ++e) mine += __popcll(__builtin_amdgcn_ballot_w64(near_enough(u, e)));
-                    }
+                    for (int e = 0; e < kE; ++e) mine += __popcll(__builtin_amdgcn_ballot_w64(near_enough(u, e)));
                 }
                 if (lane == 0) wave_count[wave] = mine;
                 __syncthreads();
-                int all = held;
+                had = held;
+                int all = had;
                 for (int w = 0; w < kChooseWaves; ++w) all += wave_count[w];
                 __syncthreads();
                 return all;
             };
             int all = count();
-            if (all > held + 256) {
+            if (all > had + d.select + 128) {
                 // pieces are few or alike: each lane's best offer is a bound of its own (16 beams of 500 tokens, 32 chosen: 600 -> 25 us)
                 double mine = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < kTwo; ++u)
-                    if (beam[u] >= 0) {
+                for (int u = 0; u < kTwo; ++u) {
+                    float high = -INFINITY;
 #pragma unroll
-                        for (int e = 0; e < kE; ++e)
-                            if (x[u][e] > -INFINITY) mine = fmax(mine, one(u, e).score);
-                    }
-                raise(mine, 4);
+                    for (int e = 0; e < kE; ++e) high = fmaxf(high, x[u][e]);
+                    if (high > -INFINITY) mine = fmax(mine, live[u] ? offered(own[u] + ((double)high - norm[u])) : own[u]);
+                }
+                raise(mine, min(n - j0, kChooseWaves) * 64, max(2 * d.select, min(128, 8 * d.select)));
                 all = count();
             }
-            auto push = [&](int u) {
+            auto push = [&](int u) {                          // one place in the buffer for all that pass
                 if (beam[u] < 0) return;
                 const Offer now = bound;
+                uint64_t who[kE];
+                int total = 0;
 #pragma unroll
                 for (int e = 0; e < kE; ++e) {
-                    if (!__builtin_amdgcn_ballot_w64(near_enough(u, e))) continue;
-                    const Offer o = one(u, e);
-                    const bool go = near_enough(u, e) && o.score > -INFINITY && before(o, now);
-                    const uint64_t who = __builtin_amdgcn_ballot_w64(go);
-                    if (!who) continue;
-                    int at = 0;
-                    if (lane == 0) at = atomicAdd(&held, __popcll(who));
-                    at = __shfl(at, 0) + __popcll(who & ((1ull << lane) - 1));
-                    if (go) buffer[at] = o;
+                    who[e] = 0;
+                    if (__builtin_amdgcn_ballot_w64(near_enough(u, e))) who[e] = __builtin_amdgcn_ballot_w64(near_enough(u, e) && before(one(u, e), now));
+                    total += __popcll(who[e]);
+                }
+                if (!total) return;
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&held, total);
+                at = __builtin_amdgcn_readfirstlane(at);
+#pragma unroll
+                for (int e = 0; e < kE; ++e) {
+                    if (who[e] >> lane & 1) buffer[at + __popcll(who[e] & ((1ull << lane) - 1))] = one(u, e);
+                    at += __popcll(who[e]);
                 }
             };
             if (all <= kBuffer) {
@@ -323,7 +365,9 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
                 for (int w = 0; w < kChooseWaves; ++w)        // one piece after another, cut in between
 #pragma unroll
                     for (int u = 0; u < kTwo; ++u) {
-                        if (held + kPiece<T> > kBuffer) cut();
+                        const bool full = held + kPiece<T> > kBuffer;
+                        __syncthreads();                      // (all have read it)
+                        if (full) cut();
                         if (wave == w) push(u);
                         __syncthreads();
                     }
@@ -337,9 +381,9 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
     const int found = held;
     const int64_t out = (int64_t)blockIdx.x * d.select;
     if (tid < found) {
-        a.best[out + tid] = (float)buffer[tid].score;
-        a.parents[out + tid] = (int32_t)(row0 + buffer[tid].beam);
-        a.tokens[out + tid] = buffer[tid].token;
+        a.best[out + tid] = (float)score_of(buffer[tid].key);
+        a.parents[out + tid] = (int32_t)(row0 + (buffer[tid].place >> 32));
+        a.tokens[out + tid] = (int32_t)buffer[tid].place;
     }
     if (found == d.select) return;
     // Fewer offers than places: the rest at -infinity, in order.  All offers above it are in the buffer, fewer than
@@ -351,7 +395,7 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
         const int b = (int)(p / d.vocab);
         const int32_t v = (int32_t)(p - (int64_t)b * d.vocab);
         none = true;
-        for (int j = 0; j < found; ++j) none = none && !(buffer[j].beam == b && buffer[j].token == v);
+        for (int j = 0; j < found; ++j) none = none && buffer[j].place != ((uint64_t)b << 32 | (uint32_t)v);
     }
     const uint64_t who = __builtin_amdgcn_ballot_w64(none);
     if (lane == 0) wave_count[wave] = __popcll(who);
