@@ -348,7 +348,8 @@ int reef_ops_beam_select(const reef_beam_select_desc* d, const void* logits, con
  * spare[i], which takes its place (a block number outside the pool, either one: entry -1 and nothing is copied).  lengths_out[i] = n.
  * Entries behind stay as they are, and so does a row whose parent is not a row.
  * table [table_rows][table_stride], table_out [rows][out_stride]: not the same memory.  spare: `rows` blocks that no row of `table`
- * uses, no two alike.  The pools hold `layers` caches of the layout, layer_stride elements from one to the next. */
+ * uses, no two alike.  The pools hold `layers` caches of the layout, layer_stride elements from one to the next; a block of one
+ * is less than 2^30 values. */
 typedef struct {
     reef_cache_layout cache;
     int32_t rows, table_rows, max_blocks, table_stride, out_stride, layers;

@@ -187,6 +187,11 @@ def test_reorder_refusals(change, text):
     refused(B.ops_beam_reorder(reorder(layout(), **change), P, P, P, P, 2 * P, P, P, P), text)
 
 
+def test_reorder_of_huge_blocks():
+    c = layout(block_size=1 << 23, slot_stride=128, block_stride=1 << 30)
+    refused(B.ops_beam_reorder(reorder(c, max_blocks=1, table_stride=1, out_stride=1), P, P, P, P, 2 * P, 3 * P, P, P), "too large")
+
+
 def test_reorder_pointers():
     d = reorder(layout(), layers=2, layer_stride=20480)
     good = [P, P, P, P, 2 * P, 3 * P, P, P]
