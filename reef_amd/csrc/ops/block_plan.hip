@@ -6,9 +6,7 @@
 namespace {
 using namespace reef_ops;
 
-constexpr int kThreads = 256;
-constexpr int kMine = 4;                     // requests a thread and round
-constexpr int kRound = kThreads * kMine;
+constexpr int kThreads = 512;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMostGroups = 512;
 
@@ -46,10 +44,12 @@ __device__ inline uint32_t scan(uint32_t v, uint32_t* sums, uint32_t* total) {
 __device__ inline uint32_t up(uint32_t n, uint32_t d) { return n / d + (n % d != 0); }
 
 // Two prefix sums over the requests (new tokens, new blocks) decide everything, and each place of the outputs is a function
-// of them.  Every workgroup makes all sums for itself (a round of 1024 requests takes 2 us, less than a launch for them
-// alone) and writes its share of slots and table rows; none waits for another.  A slot's block comes from the free list itself where
+// of them.  Every workgroup makes all sums for itself (a round takes 2 us, less than a launch for them alone) and writes its share of slots and table rows; none waits for another.  A slot's block comes from the free list itself where
 // it is new, so the table is only read where no workgroup writes it.
+// kMine: requests a thread and round.
+template <int kMine>
 __global__ void __launch_bounds__(kThreads) block_plan(Args a) {
+    constexpr int kRound = kThreads * kMine;
     const reef_block_plan_desc& d = a.d;
     const uint32_t bs = d.block_size, room = (uint32_t)d.max_blocks * bs, max_tokens = d.max_tokens;
     __shared__ uint32_t sums[kWaves];
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads) block_plan(Args a) {
             for (uint32_t j = lane; j < need_[r]; j += 64) to[j] = a.free_list[taken[r] + j];
         }
         // The slots of the round's tokens.  Where requests bring four and more, four in a row a thread: one search, and their blocks are
-        // mostly one (2000 prompts, 0.8 M tokens: 13 against 33 us).  In decode steps each has a block of its own, and four loads in a row
+        // mostly one (2000 prompts, 0.8 M tokens: 13 against 33 us, four requests a thread and 256 threads).  In decode steps each has a block of its own, and four loads in a row
         // would wait for each other (four requests: 7.0 against 4.9 us).
         const uint32_t hi = min(tokens, max_tokens), per = (hi - lo) / 4 >= (uint32_t)count ? 4 : 1;
         for (uint64_t t0 = lo / per * per + (uint64_t)per * (blockIdx.x * kThreads + threadIdx.x); t0 < hi; t0 += (uint64_t)per * gridDim.x * kThreads) {
@@ -181,7 +181,11 @@ extern "C" int reef_ops_block_plan(const reef_block_plan_desc* d, const int32_t*
     const Span in[] = {{cached, 4 * n}, {added, 4 * n}, {free_list, 4ll * d->free_blocks}};
     if (overlap(out, in)) return refuse(what, "an output overlaps an input");
     // a workgroup for about 1024 slots or 16 table rows
-    const int64_t want = std::max((d->max_tokens + 1023ll) / 1024, (std::min(d->requests, kRound) + 15ll) / 16);
+    const int64_t want = std::max((d->max_tokens + 1023ll) / 1024, (std::min(d->requests, 1024) + 15ll) / 16);
     const dim3 grid((unsigned)std::min<int64_t>(std::max<int64_t>(want, 1), kMostGroups));
-    return launch(what, block_plan, grid, dim3(kThreads), Args{*d, cached, added, free_list, table, lengths, starts, slots, counts}, stream);
+    const Args a{*d, cached, added, free_list, table, lengths, starts, slots, counts};
+    // Up to 1024 requests go through in one round of two a thread, more in rounds of four: 2000 prompts 10.5 against 12.8 us, 4000
+    // decode steps 10.5 against 13.8, but four requests 5.3 against 4.6.
+    if (d->requests <= 2 * kThreads) return launch(what, block_plan<2>, grid, dim3(kThreads), a, stream);
+    return launch(what, block_plan<4>, grid, dim3(kThreads), a, stream);
 }
