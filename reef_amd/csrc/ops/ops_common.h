@@ -85,6 +85,19 @@ struct PagedView {
 __host__ __device__ inline int64_t paged_row(const PagedView& v, int32_t entry, int32_t place) {
     return (uint32_t)entry < (uint32_t)v.blocks ? (int64_t)entry * v.block_stride + (int64_t)place * v.slot_stride : -1;
 }
+// t / by for 0 <= t < 2^31, without a division: with 2^(l-1) < by <= 2^l, floor(t m / 2^(31+l)) for m = floor(2^(31+l) / by) + 1, whose
+// excess of at most by over the true quotient's multiple is too small to count below 2^31.  m = 0: by is 1.
+struct Divider {
+    uint32_t by, m, shift;
+};
+inline Divider divider(uint32_t by) {
+    if (by <= 1) return {1, 0, 0};
+    uint32_t l = 1;
+    while (l < 31 && (1ull << l) < by) ++l;
+    return {by, (uint32_t)((1ull << (31 + l)) / by + 1), l - 1};
+}
+__host__ __device__ inline uint32_t divided(uint32_t t, const Divider& d) { return d.m ? (uint32_t)((uint64_t)t * d.m >> 32) >> d.shift : t; }
+
 // What a request's length counts for: [0, what a row of the table holds].
 __host__ __device__ inline int32_t held_length(int32_t n, int32_t max_blocks, int32_t block_size) {
     const int64_t room = (int64_t)max_blocks * block_size;

@@ -25,6 +25,7 @@ struct Args {
     int2* info;             // [request]: its first share and how many they are
     int32_t group, tiles;   // query heads a cache head; tiles of 16 of them
     int32_t budget;         // shares that all tokens are cut into, beside one a request; 0: sequences are not split
+    Divider block;          // by the block size
 };
 
 constexpr int32_t kLeast = 128;              // tokens a share at least
@@ -94,6 +95,24 @@ __device__ inline void put4(Q* to, f32x4 v, float sum) {
     *(Q4*)to = x;
 }
 
+// The maximum or sum over the 16 lanes of a row, for all of them.
+template <int BY>
+__device__ inline float rotated(float x) {
+    return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), 0x120 | BY, 0xF, 0xF, true));
+}
+__device__ inline float over_lanes_max(float x) {
+    x = fmaxf(x, rotated<8>(x));
+    x = fmaxf(x, rotated<4>(x));
+    x = fmaxf(x, rotated<2>(x));
+    return fmaxf(x, rotated<1>(x));
+}
+__device__ inline float over_lanes_sum(float x) {
+    x += rotated<8>(x);
+    x += rotated<4>(x);
+    x += rotated<2>(x);
+    return x + rotated<1>(x);
+}
+
 // The maximum or sum over the four rows of 16 lanes.
 __device__ inline float over_rows_max(float x) {
     auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -144,6 +163,9 @@ __device__ inline void terms(float a, float b, uint32_t (&t)[N], _Float16) {
     }
 }
 
+// Tokens of a tile: 32, or 16 where 32 take too many registers.
+constexpr int tile_of(int bytes) { return bytes == 2 ? 32 : 16; }
+
 // One share of a sequence, one cache head, up to 16 of its query heads: a workgroup whose wavefronts take tiles of 32 tokens (16
 // of a 32-bit cache) in turn, each with a running maximum, sum and output, and join at the end.
 //
@@ -156,15 +178,16 @@ __device__ inline void terms(float a, float b, uint32_t (&t)[N], _Float16) {
 // 16-bit caches use 16x16x32 products.  Weights are two terms of the cache's type (a single one would put 2^-9 on bf16 outputs that are
 // off by 2^-9 at most from their own rounding); 32-bit queries are three terms, and so are their weights, which keeps all 24
 // bits at a fifth of the time of 16x16x4 products on 32-bit values.  Terms of fp16 need room below: queries are scaled by a power of
-// two to 2^13 a head, weights are up to 2^14.  32-bit caches use the 16x16x4 products.
-template <class Q, class C, int DP, bool WHOLE, int WAVES>
+// two to 2^13 a head, weights are up to 2^14.  32-bit caches use the 16x16x4 products, but for FEW query heads a cache head, where
+// these would be nearly all padding: there the same pieces are multiplied and added by the lanes, a head after the other.
+template <class Q, class C, int DP, bool WHOLE, int WAVES, int FEW>
 __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) paged_attention(Args a) {
     constexpr bool kNarrow = sizeof(C) == 2;                  // products in the cache's 16-bit type
     constexpr bool kHalf = __is_same(C, _Float16);
     constexpr int kTermsQ = sizeof(Q) == sizeof(C) ? 1 : 3, kTermsP = sizeof(Q) == 2 ? 2 : 3;
     constexpr float kShift = kHalf ? 14.0f : 0.0f;            // weights are up to 2^kShift
     constexpr int kPiece = 16 / sizeof(C);                    // values of 16 bytes
-    constexpr int kTile = sizeof(C) == 2 ? 32 : 16, kSub = kTile / 16;
+    constexpr int kTile = tile_of(sizeof(C)), kSub = kTile / 16;
     constexpr int kSteps = DP / (4 * kPiece);                 // pieces of a key row a lane
     constexpr int kV = DP / 16 < kPiece ? DP / 16 : kPiece;   // values of a value row a lane and slab
     constexpr int kSlabs = DP / (16 * kV), kVWords = kV * sizeof(C) / 4;
@@ -196,13 +219,26 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     const int32_t* table = a.table + (int64_t)r * d.table_stride;
 
     __shared__ int64_t offsets[WAVES][2][kTile];
-    __shared__ float o_part[WAVES][16][kRow];
-    __shared__ float m_part[WAVES][16], l_part[WAVES][16];
+    constexpr int kHeads = FEW ? FEW : 16;
+    __shared__ float o_part[WAVES][kHeads][kRow];
+    __shared__ float m_part[WAVES][kHeads], l_part[WAVES][kHeads];
 
     // the queries: head n, the pieces that this lane's keys have
     float scale = d.scale * kLog2e;
-    u32x4 q[kTermsQ][kSteps];
-    {
+    u32x4 q[FEW ? 1 : kTermsQ][FEW ? 1 : kSteps];
+    float fq[FEW ? FEW : 1][kSteps][4];
+    if constexpr (FEW) {                      // (for each head)
+#pragma unroll
+        for (int h = 0; h < FEW; ++h)
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) {
+                const int at = (s * 4 + g) * kPiece;
+                f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (h < heads && at < D) v = *(const f32x4*)((const float*)a.query + r * d.query_stride + (head0 + h) * d.query_head_stride + at);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) fq[h][s][e] = v[e];
+            }
+    } else {
         const Q* query = (const Q*)a.query + r * d.query_stride + (head0 + n) * d.query_head_stride;
         constexpr int kWords = kPiece * sizeof(Q) / 4;
         uint32_t raw[kSteps][kWords];
@@ -248,22 +284,33 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     }
 
     float m = -INFINITY, l = 0.0f;
-    f32x4 o[kSlabs][kV];
+    f32x4 o[FEW ? 1 : kSlabs][FEW ? 1 : kV];
+    float fm[FEW ? FEW : 1], fl[FEW ? FEW : 1], fo[FEW ? FEW : 1][kSlabs][kV];   // FEW: of each head; fo over this row's tokens
 #pragma unroll
-    for (int s = 0; s < kSlabs; ++s)
+    for (int s = 0; s < (FEW ? 1 : kSlabs); ++s)
 #pragma unroll
-        for (int e = 0; e < kV; ++e) o[s][e] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int e = 0; e < (FEW ? 1 : kV); ++e) o[s][e] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int h = 0; h < (FEW ? FEW : 1); ++h) {
+        fm[h] = -INFINITY;
+        fl[h] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+            for (int e = 0; e < kV; ++e) fo[h][c][e] = 0.0f;
+    }
 
     // the table's entry of one token of a tile a lane; -1: no token
     auto entry_of = [&](int32_t t0) -> int32_t {
         const int64_t t = (int64_t)t0 + lane;
-        return lane < kTile && t < end ? table[(int32_t)t / view.block_size] : -1;
+        return lane < kTile && t < end ? table[divided((uint32_t)t, a.block)] : -1;
     };
     // that token's place, for all lanes to read; which of the tile's tokens there are
     auto place = [&](int32_t t0, int32_t entry, int buffer) -> uint32_t {
         int64_t at = -1;
         if (lane < kTile) {
-            at = paged_row(view, entry, (int32_t)(((int64_t)t0 + lane) % view.block_size));
+            const uint32_t t = (uint32_t)t0 + lane;
+            at = paged_row(view, entry, (int32_t)(t - divided(t, a.block) * a.block.by));
             offsets[wave][buffer][lane] = at < 0 ? 0 : at;
         }
         return (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0);
@@ -323,129 +370,191 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
             entry = t0 < end - 2 * kStride ? entry_of(t0 + 2 * kStride) : -1;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
-        // scores
-        f32x4 s[kSub];
+        const bool all = there == (kTile == 32 ? 0xFFFFFFFFu : 0xFFFFu);
+        if constexpr (FEW) {
+            // scores: token n of each 16, the same in all rows
+            float p[FEW][kSub];
 #pragma unroll
-        for (int t = 0; t < kSub; ++t) s[t] = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int t = 0; t < kSub; ++t)
 #pragma unroll
-        for (int c = 0; c < kSteps; ++c)
+                for (int h = 0; h < FEW; ++h) {
+                    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int t = 0; t < kSub; ++t) {
-                u32x4 kk = k[t][c];
-                if constexpr (!WHOLE)
-                    if ((c * 4 + g) * kPiece >= D) kk = {0, 0, 0, 0};
-                if constexpr (kNarrow) {
-                    typedef C C8 __attribute__((ext_vector_type(8)));
+                    for (int c = 0; c < kSteps; ++c)
 #pragma unroll
-                    for (int x = kTermsQ - 1; x >= 0; --x) s[t] = product(__builtin_bit_cast(C8, kk), __builtin_bit_cast(C8, q[x][c]), s[t]);
-                } else {
+                        for (int e = 0; e < 4; ++e)
+                            if (WHOLE || (c * 4 + g) * kPiece < D) x[e] = fmaf(__uint_as_float(k[t][c][e]), fq[h][c][e], x[e]);
+                    p[h][t] = over_rows_sum((x[0] + x[1]) + (x[2] + x[3])) * scale;
+                    if (!all && !(there >> (t * 16 + n) & 1)) p[h][t] = -INFINITY;
+                }
+            if (more) load_k(buffer ^ 1);
 #pragma unroll
-                    for (int e = 0; e < kPiece; ++e) s[t] = product(__uint_as_float(kk[e]), __uint_as_float(q[0][c][e]), s[t]);
+            for (int h = 0; h < FEW; ++h) {
+                float top = p[h][0];
+                if constexpr (kSub == 2) top = fmaxf(top, p[h][1]);
+                top = fmaxf(over_lanes_max(top), fm[h]);
+                const float base = top == -INFINITY ? 0.0f : top, f = __builtin_amdgcn_exp2f(fm[h] - base);
+                fm[h] = top;
+                fl[h] *= f;
+#pragma unroll
+                for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+                    for (int e = 0; e < kV; ++e) fo[h][c][e] *= f;
+#pragma unroll
+                for (int t = 0; t < kSub; ++t) {
+                    p[h][t] = __builtin_amdgcn_exp2f(p[h][t] - base);
+                    fl[h] += p[h][t];
                 }
             }
-        if constexpr (kTermsQ > 1) {
-            // An infinite key times a term that is 0 or of the other sign: the sum is made again on 32-bit values, as it is written.
-            bool odd = false;
+            // values of places that are no tokens may be anything, and 0 times that too
+            if (!all) {
+#pragma unroll
+                for (int t = 0; t < kSub; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(there >> (t * 16 + g * 4 + i) & 1)) {
+#pragma unroll
+                            for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+                                for (int w = 0; w < kVWords; ++w) v[t][i][c][w] = 0;
+                        }
+            }
 #pragma unroll
             for (int t = 0; t < kSub; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) odd |= s[t][i] != s[t][i];
-            if (__builtin_amdgcn_ballot_w64(odd)) {
+                for (int h = 0; h < FEW; ++h)
 #pragma unroll
-                for (int t = 0; t < kSub; ++t) s[t] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int c = 0; c < kSteps; ++c)
-#pragma unroll
-                    for (int e = 0; e < kPiece; ++e) {
-                        float x = 0.0f;
-#pragma unroll
-                        for (int i = kTermsQ - 1; i >= 0; --i) {
-                            uint32_t y = q[i][c][e / 2];
-                            asm volatile("" : "+v"(y));       // (or the sums are made ahead of the loop, and held in registers for it)
-                            x += to_float<C>(y, e & 1);
-                        }
-#pragma unroll
-                        for (int t = 0; t < kSub; ++t) {
-                            const bool inside = WHOLE || (c * 4 + g) * kPiece < D;
-                            s[t] = product(inside ? to_float<C>(k[t][c][e / 2], e & 1) : 0.0f, x, s[t]);
-                        }
-                    }
-            }
-        }
-        if (more) load_k(buffer ^ 1);
-        // weights
-        const bool all = there == (kTile == 32 ? 0xFFFFFFFFu : 0xFFFFu);
-        float top = m;
-#pragma unroll
-        for (int t = 0; t < kSub; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[t][i] *= scale;
-                if (!all && !(there >> (t * 16 + g * 4 + i) & 1)) s[t][i] = -INFINITY;
-                top = fmaxf(top, s[t][i]);
-            }
-        top = over_rows_max(top);
-        const float base = top == -INFINITY ? 0.0f : top - kShift;
-        if (__builtin_amdgcn_ballot_w64(top != m)) {
-            const float f = __builtin_amdgcn_exp2f(m - kShift - base);
-            l *= f;
-#pragma unroll
-            for (int c = 0; c < kSlabs; ++c)
-#pragma unroll
-                for (int e = 0; e < kV; ++e) o[c][e] *= f;
-        }
-        m = top;
-#pragma unroll
-        for (int t = 0; t < kSub; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - base);
-                l += s[t][i];
-            }
-        // values of places that are no tokens may be anything, and 0 times that too
-        if (!all) {
-#pragma unroll
-            for (int t = 0; t < kSub; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (!(there >> (t * 16 + g * 4 + i) & 1)) {
+                    for (int i = 0; i < 4; ++i) {
+                        const float w = __shfl(p[h][t], g * 4 + i);
 #pragma unroll
                         for (int c = 0; c < kSlabs; ++c)
 #pragma unroll
-                            for (int w = 0; w < kVWords; ++w) v[t][i][c][w] = 0;
+                            for (int e = 0; e < kV; ++e) fo[h][c][e] = fmaf(__uint_as_float(v[t][i][c][e]), w, fo[h][c][e]);
                     }
-        }
-        if constexpr (kNarrow) {
-            typedef C C8 __attribute__((ext_vector_type(8)));
-            u32x4 p[kTermsP];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t x[kTermsP];
-                terms(s[w >> 1][(w & 1) * 2], s[w >> 1][(w & 1) * 2 + 1], x, C());
-#pragma unroll
-                for (int i = 0; i < kTermsP; ++i) p[i][w] = x[i];
-            }
-#pragma unroll
-            for (int c = 0; c < kSlabs; ++c)
-#pragma unroll
-                for (int e = 0; e < kV; ++e) {
-                    u32x4 x;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w)
-                        x[w] = __builtin_amdgcn_perm(v[w >> 1][(w & 1) * 2 + 1][c][e / 2], v[w >> 1][(w & 1) * 2][c][e / 2], e & 1 ? 0x07060302 : 0x05040100);
-#pragma unroll
-                    for (int i = kTermsP - 1; i >= 0; --i) o[c][e] = product(__builtin_bit_cast(C8, x), __builtin_bit_cast(C8, p[i]), o[c][e]);
-                }
         } else {
+            // scores
+            f32x4 s[kSub];
+#pragma unroll
+            for (int t = 0; t < kSub; ++t) s[t] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+                for (int t = 0; t < kSub; ++t) {
+                    u32x4 kk = k[t][c];
+                    if constexpr (!WHOLE)
+                        if ((c * 4 + g) * kPiece >= D) kk = {0, 0, 0, 0};
+                    if constexpr (kNarrow) {
+                        typedef C C8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+                        for (int x = kTermsQ - 1; x >= 0; --x) s[t] = product(__builtin_bit_cast(C8, kk), __builtin_bit_cast(C8, q[x][c]), s[t]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < kPiece; ++e) s[t] = product(__uint_as_float(kk[e]), __uint_as_float(q[0][c][e]), s[t]);
+                    }
+                }
+            if constexpr (kTermsQ > 1) {
+                // An infinite key times a term that is 0 or of the other sign: the sum is made again on 32-bit values, as it is written.
+                bool odd = false;
+#pragma unroll
+                for (int t = 0; t < kSub; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) odd |= s[t][i] != s[t][i];
+                if (__builtin_amdgcn_ballot_w64(odd)) {
+#pragma unroll
+                    for (int t = 0; t < kSub; ++t) s[t] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+                        for (int e = 0; e < kPiece; ++e) {
+                            float x = 0.0f;
+#pragma unroll
+                            for (int i = kTermsQ - 1; i >= 0; --i) {
+                                uint32_t y = q[i][c][e / 2];
+                                asm volatile("" : "+v"(y));       // (or the sums are made ahead of the loop, and held in registers for it)
+                                x += to_float<C>(y, e & 1);
+                            }
+#pragma unroll
+                            for (int t = 0; t < kSub; ++t) {
+                                const bool inside = WHOLE || (c * 4 + g) * kPiece < D;
+                                s[t] = product(inside ? to_float<C>(k[t][c][e / 2], e & 1) : 0.0f, x, s[t]);
+                            }
+                        }
+                }
+            }
+            if (more) load_k(buffer ^ 1);
+            // weights
+            float top = m;
 #pragma unroll
             for (int t = 0; t < kSub; ++t)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 4; ++i) {
+                    s[t][i] *= scale;
+                    if (!all && !(there >> (t * 16 + g * 4 + i) & 1)) s[t][i] = -INFINITY;
+                    top = fmaxf(top, s[t][i]);
+                }
+            top = over_rows_max(top);
+            const float base = top == -INFINITY ? 0.0f : top - kShift;
+            if (__builtin_amdgcn_ballot_w64(top != m)) {
+                const float f = __builtin_amdgcn_exp2f(m - kShift - base);
+                l *= f;
 #pragma unroll
-                    for (int c = 0; c < kSlabs; ++c)
+                for (int c = 0; c < kSlabs; ++c)
 #pragma unroll
-                        for (int e = 0; e < kV; ++e)
-                            o[c][e] = product(__uint_as_float(v[t][i][c][e]), s[t][i], o[c][e]);
+                    for (int e = 0; e < kV; ++e) o[c][e] *= f;
+            }
+            m = top;
+#pragma unroll
+            for (int t = 0; t < kSub; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - base);
+                    l += s[t][i];
+                }
+            // values of places that are no tokens may be anything, and 0 times that too
+            if (!all) {
+#pragma unroll
+                for (int t = 0; t < kSub; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!(there >> (t * 16 + g * 4 + i) & 1)) {
+#pragma unroll
+                            for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+                                for (int w = 0; w < kVWords; ++w) v[t][i][c][w] = 0;
+                        }
+            }
+            if constexpr (kNarrow) {
+                typedef C C8 __attribute__((ext_vector_type(8)));
+                u32x4 p[kTermsP];
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t x[kTermsP];
+                    terms(s[w >> 1][(w & 1) * 2], s[w >> 1][(w & 1) * 2 + 1], x, C());
+#pragma unroll
+                    for (int i = 0; i < kTermsP; ++i) p[i][w] = x[i];
+                }
+#pragma unroll
+                for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+                    for (int e = 0; e < kV; ++e) {
+                        u32x4 x;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                            x[w] = __builtin_amdgcn_perm(v[w >> 1][(w & 1) * 2 + 1][c][e / 2], v[w >> 1][(w & 1) * 2][c][e / 2], e & 1 ? 0x07060302 : 0x05040100);
+#pragma unroll
+                        for (int i = kTermsP - 1; i >= 0; --i) o[c][e] = product(__builtin_bit_cast(C8, x), __builtin_bit_cast(C8, p[i]), o[c][e]);
+                    }
+            } else {
+#pragma unroll
+                for (int t = 0; t < kSub; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+                            for (int e = 0; e < kV; ++e)
+                                o[c][e] = product(__uint_as_float(v[t][i][c][e]), s[t][i], o[c][e]);
+            }
         }
         if (more) load_v(buffer ^ 1);
         there = there_next;
@@ -455,20 +564,38 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     }
 
     // the wavefronts' parts
-    l = over_rows_sum(l);
-    if (n < heads) {
+    if constexpr (FEW) {
 #pragma unroll
-        for (int c = 0; c < kSlabs; ++c)
+        for (int h = 0; h < FEW; ++h) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int c = 0; c < kSlabs; ++c) {
+                f32x4 x;
 #pragma unroll
-                for (int e = 0; e < kV; e += 4) {
-                    f32x4 x = {o[c][e][i], o[c][e + 1][i], o[c][e + 2][i], o[c][e + 3][i]};
-                    *(f32x4*)&o_part[wave][n][(c * 16 + g * 4 + i) * kV + e] = x;
-                }
-        if (g == 0) {
-            m_part[wave][n] = m - kShift;
-            l_part[wave][n] = l;
+                for (int e = 0; e < 4; ++e) x[e] = over_rows_sum(fo[h][c][e]);
+                if (g == 0) *(f32x4*)&o_part[wave][h][(c * 16 + n) * kV] = x;
+            }
+            const float sum = over_lanes_sum(fl[h]);
+            if (lane == 0) {
+                m_part[wave][h] = fm[h];
+                l_part[wave][h] = sum;
+            }
+        }
+    } else {
+        l = over_rows_sum(l);
+        if (n < heads) {
+#pragma unroll
+            for (int c = 0; c < kSlabs; ++c)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < kV; e += 4) {
+                        f32x4 x = {o[c][e][i], o[c][e + 1][i], o[c][e + 2][i], o[c][e + 3][i]};
+                        *(f32x4*)&o_part[wave][n][(c * 16 + g * 4 + i) * kV + e] = x;
+                    }
+            if (g == 0) {
+                m_part[wave][n] = m - kShift;
+                l_part[wave][n] = l;
+            }
         }
     }
     __syncthreads();
@@ -567,15 +694,22 @@ struct Plan {
     int64_t groups;         // workgroups
     size_t info_bytes, stats_bytes, bytes;
 };
-// Wavefronts of a wide workgroup: as many as the registers allow a CU; for heads over 128 those of any.
-constexpr int wide_waves(int dp, bool terms) { return dp <= 64 && !terms ? 16 : dp <= 128 ? 8 : 4; }
+// Wavefronts of a wide workgroup: as many as the registers allow a CU; with matrix products for heads over 128 those of any.
+constexpr int wide_waves(int dp, bool terms, int few) {
+    return dp <= 64 && !terms && few <= 1 ? 16 : dp <= 128 ? 8 : 4;
+}
+// Whether lanes do the work of the matrix instructions: 32-bit caches, query heads a cache head up to 4 for heads up to 64, 2 for heads up to 128.
+constexpr int few_of(bool narrow, int dp, int group) {
+    return narrow || dp > 128 ? 0 : group <= 2 ? group : group <= 4 && dp <= 64 ? 4 : 0;
+}
 Plan plan_of(const reef_paged_attention_desc& d) {
     const int32_t group = d.heads / d.cache.kv_heads, tiles = (group + 15) / 16, rows = d.cache.kv_heads * tiles;
     int64_t longest = (int64_t)d.max_blocks * d.cache.block_size;
     if (d.longest && d.longest < longest) longest = d.longest;
     if (d.window && d.window < longest) longest = d.window;
     const int64_t all = (int64_t)d.requests * rows;
-    const int tile = d.cache.type == REEF_TYPE_F32 ? 16 : 32, D = d.cache.head_dim, wide = wide_waves(D, d.type != d.cache.type);
+    const int D = d.cache.head_dim, few = few_of(d.cache.type != REEF_TYPE_F32, D, group), tile = tile_of(type_bytes(d.cache.type)),
+              wide = wide_waves(D, d.type != d.cache.type, few);
     Plan p{};
     p.tiles = tiles;
     p.wide = all < kGroups && longest <= (int64_t)4 * wide * tile;
@@ -590,23 +724,37 @@ Plan plan_of(const reef_paged_attention_desc& d) {
     return p;
 }
 
-template <class Q, class C, int DP, bool WHOLE>
+template <class Q, class C, int DP, bool WHOLE, int FEW>
 int run_waves(const char* what, const Args& a, const Plan& p, void* stream) {
-    constexpr int kWide = wide_waves(DP, sizeof(Q) != sizeof(C));
+    constexpr int kWide = wide_waves(DP, sizeof(Q) != sizeof(C), FEW);
     const dim3 grid((unsigned)p.groups);
-    if (p.wide && kWide > 4) return launch(what, paged_attention<Q, C, DP, WHOLE, kWide>, grid, dim3(kWide * 64), a, stream);
-    return launch(what, paged_attention<Q, C, DP, WHOLE, 4>, grid, dim3(kThreads), a, stream);
+    if (p.wide && kWide > 4) return launch(what, paged_attention<Q, C, DP, WHOLE, kWide, FEW>, grid, dim3(kWide * 64), a, stream);
+    return launch(what, paged_attention<Q, C, DP, WHOLE, 4, FEW>, grid, dim3(kThreads), a, stream);
+}
+
+template <class Q, class C, int DP, bool WHOLE>
+int run_heads(const char* what, const Args& a, const Plan& p, void* stream) {
+    if constexpr (sizeof(C) == 4) {
+        const int few = few_of(false, DP, a.group);
+        if constexpr (DP <= 128) {
+            if (few == 1) return run_waves<Q, C, DP, WHOLE, 1>(what, a, p, stream);
+            if (few == 2) return run_waves<Q, C, DP, WHOLE, 2>(what, a, p, stream);
+        }
+        if constexpr (DP <= 64)
+            if (few == 4) return run_waves<Q, C, DP, WHOLE, 4>(what, a, p, stream);
+    }
+    return run_waves<Q, C, DP, WHOLE, 0>(what, a, p, stream);
 }
 
 template <class Q, class C>
 int run(const char* what, const Args& a, const Plan& p, void* stream) {
     const int D = a.d.cache.head_dim;
-    const int rc = D == 64    ? run_waves<Q, C, 64, true>(what, a, p, stream)
-                   : D < 64   ? run_waves<Q, C, 64, false>(what, a, p, stream)
-                   : D == 128 ? run_waves<Q, C, 128, true>(what, a, p, stream)
-                   : D < 128  ? run_waves<Q, C, 128, false>(what, a, p, stream)
-                   : D == 256 ? run_waves<Q, C, 256, true>(what, a, p, stream)
-                              : run_waves<Q, C, 256, false>(what, a, p, stream);
+    const int rc = D == 64    ? run_heads<Q, C, 64, true>(what, a, p, stream)
+                   : D < 64   ? run_heads<Q, C, 64, false>(what, a, p, stream)
+                   : D == 128 ? run_heads<Q, C, 128, true>(what, a, p, stream)
+                   : D < 128  ? run_heads<Q, C, 128, false>(what, a, p, stream)
+                   : D == 256 ? run_heads<Q, C, 256, true>(what, a, p, stream)
+                              : run_heads<Q, C, 256, false>(what, a, p, stream);
     if (rc || !p.budget) return rc;
     return launch(what, join_shares<Q>, dim3((unsigned)(a.d.requests * a.d.heads)), dim3(kThreads), a, stream);
 }
@@ -632,7 +780,7 @@ extern "C" int reef_ops_paged_attention(const reef_paged_attention_desc* d, cons
         return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", p.bytes, (long long)workspace_bytes);
     char* w = (char*)workspace;
     const Args a{*d, query, key_cache, value_cache, table, lengths, out, lse, (float*)(w + p.info_bytes + p.stats_bytes), (float2*)(w + p.info_bytes),
-                 (int2*)w, d->heads / d->cache.kv_heads, p.tiles, p.budget};
+                 (int2*)w, d->heads / d->cache.kv_heads, p.tiles, p.budget, divider((uint32_t)d->cache.block_size)};
     switch (d->type * 4 + d->cache.type) {
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, p, stream);
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return run<float, _Float16>(what, a, p, stream);
