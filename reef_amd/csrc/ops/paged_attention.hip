@@ -223,6 +223,16 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     __shared__ float o_part[WAVES][kHeads][kRow];
     __shared__ float m_part[WAVES][kHeads], l_part[WAVES][kHeads];
 
+    // the table's entry of one token of a tile a lane; -1: no token
+    auto entry_of = [&](int32_t t0) -> int32_t {
+        const int64_t t = (int64_t)t0 + lane;
+        return lane < kTile && t < end ? table[divided((uint32_t)t, a.block)] : -1;
+    };
+    constexpr int32_t kStride = WAVES * kTile;
+    int32_t t0 = begin + wave * kTile;
+    // (asked for ahead of the queries: keys and values wait for them)
+    int32_t entry = t0 < end ? entry_of(t0) : -1;
+
     // the queries: head n, the pieces that this lane's keys have
     float scale = d.scale * kLog2e;
     u32x4 q[FEW ? 1 : kTermsQ][FEW ? 1 : kSteps];
@@ -300,11 +310,6 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
             for (int e = 0; e < kV; ++e) fo[h][c][e] = 0.0f;
     }
 
-    // the table's entry of one token of a tile a lane; -1: no token
-    auto entry_of = [&](int32_t t0) -> int32_t {
-        const int64_t t = (int64_t)t0 + lane;
-        return lane < kTile && t < end ? table[divided((uint32_t)t, a.block)] : -1;
-    };
     // that token's place, for all lanes to read; which of the tile's tokens there are
     auto place = [&](int32_t t0, int32_t entry, int buffer) -> uint32_t {
         int64_t at = -1;
@@ -351,13 +356,10 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
             }
     };
 
-    constexpr int32_t kStride = WAVES * kTile;
-    int32_t t0 = begin + wave * kTile;
     uint32_t there = 0, there_next = 0;
-    int32_t entry = -1;
     int buffer = 0;
     if (t0 < end) {
-        there = place(t0, entry_of(t0), 0);
+        there = place(t0, entry, 0);
         entry = t0 < end - kStride ? entry_of(t0 + kStride) : -1;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         load_k(0);
