@@ -244,7 +244,7 @@ int reef_ops_release(void);
  * All pointers but the descriptors are device memory of the current device, and `stream` is a
  * hipStream_t of that device (NULL: the default stream).  The calls check what the host can see, enqueue
  * kernels and return; they allocate nothing, keep nothing and may be captured into a graph (kernel
- * nodes only).  Outputs and inputs do not overlap unless said (refused where the host can tell).  A call without rows
+ * nodes only).  Outputs and inputs do not overlap (block plan, beam select and beam reorder refuse it).  A call without rows
  * (requests, tokens or rows 0) succeeds.  Anything refused is Status::Fail with a message, and nothing is launched.
  * The workspace of a call is the caller's: uninitialised memory, 16-byte aligned, that no other call uses at the
  * same time (two graphs that may run at once need one each).  Its size depends on the descriptor alone.

@@ -528,6 +528,7 @@ def _at(x):
 
 
 def _nbytes(x):
+    """Of a workspace, which therefore is no bare address."""
     return 0 if x is None else x.nbytes
 
 

@@ -427,6 +427,7 @@ int check_select(const char* what, const reef_beam_select_desc* d) {
     if (d->select < 1 || d->select > kMaxSelect || d->select > (int64_t)d->beams * d->vocab)
         return refuse(what, "%d of %d beams of %d tokens cannot be selected (up to %d)", d->select, d->beams, d->vocab, kMaxSelect);
     if ((int64_t)d->requests * d->beams > 1 && d->logits_stride < d->vocab) return refuse(what, "rows of logits overlap");
+    if ((int64_t)d->requests * d->beams * d->vocab >= 1ll << 40) return refuse(what, "more than 2^40 logits");
     return 0;
 }
 

@@ -161,7 +161,8 @@ def test_plan_pointers():
 
 @pytest.mark.parametrize("change,text", [(dict(type=5), "type"), (dict(requests=-1), "sizes"), (dict(beams=0), "sizes"), (dict(beams=129), "sizes"),
                                          (dict(vocab=0), "sizes"), (dict(vocab=1 << 24), "sizes"), (dict(requests=1 << 22), "sizes"), (dict(select=0), "select"),
-                                         (dict(select=129), "select"), (dict(vocab=2, logits_stride=2, select=9), "select"), (dict(logits_stride=99), "overlap")])
+                                         (dict(select=129), "select"), (dict(vocab=2, logits_stride=2, select=9), "select"), (dict(logits_stride=99), "overlap"),
+                                         (dict(requests=1 << 18, vocab=1 << 23, logits_stride=1 << 23), "2^40")])
 def test_select_refusals(change, text):
     v = dict(type=F32, requests=2, beams=4, vocab=100, select=8, end_token=2, logits_stride=100)
     v.update(change)

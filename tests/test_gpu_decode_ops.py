@@ -28,7 +28,7 @@ class Pools:
     """Key and value pools on the host (float64 values as the device has them) and on the device, in either order of heads and tokens,
     with `pad` unused elements behind each innermost row group."""
 
-    def __init__(self, kind, blocks, bs, kv, dim, order="thd", pad=0, layers=None, seed=0):
+    def __init__(self, kind, blocks, bs, kv, dim, order="thd", pad=0, layers=None, seed=0, size=1.0):
         rng = np.random.default_rng(seed)
         if order == "thd":
             head, slot = dim, kv * dim + pad
@@ -39,7 +39,7 @@ class Pools:
         self.kind, self.shape, self.per_layer = kind, (blocks, bs, kv, dim), blocks * block
         self.layers = layers
         n = self.per_layer * (layers or 1)
-        self.raw = [R.encode(rng.standard_normal(n).astype(np.float32), kind) for _ in range(2)]
+        self.raw = [R.encode((rng.standard_normal(n) * size).astype(np.float32), kind) for _ in range(2)]
         self.layout = B.CacheLayout(kind, blocks, bs, kv, dim, block, slot, head)
         self.strides = (block, slot, head, 1)
         self.send()
@@ -127,7 +127,8 @@ def test_append(kind, cache, order, bs, kv, dim, tokens, pad):
     pools = Pools(cache, blocks, bs, kv, dim, order, pad)
     extra = 8
     rows = (rng.standard_normal((tokens, 2, kv, dim + extra)) * 3).astype(np.float32)
-    rows[0, :, 0, :4] = [np.inf, -np.inf, np.nan, 1e30]       # as they round: infinities, NaN, over the 16-bit float's range
+    # as they round: infinities, NaN, over the 16-bit float's range and on its border, subnormal in it, halfway, subnormal in 32 bits
+    rows[0, :, 0, :8] = [np.inf, -np.inf, np.nan, 1e30, 65519.9, 3e-6, 2.0 ** -25 * 3, 1e-39]
     rows = R.encode(rows, kind)
     slots = rng.permutation(blocks * bs)[:tokens].astype(np.int64)
     slots[rng.random(tokens) < 0.1] = -1
@@ -153,13 +154,13 @@ def test_append(kind, cache, order, bs, kv, dim, tokens, pad):
 
 # ---- attention ----------------------------------------------------------------------------------
 def run_attend(kind, cache, order, bs, kv, group, dim, lengths, window=0, pad=0, scale=None, longest=0, seed=0, spoil=True, bad=0.0, q_pad=0, grow=1.0,
-               max_blocks=None, lse=True):
+               max_blocks=None, lse=True, size=1.0):
     rng = np.random.default_rng(seed)
     heads, n = kv * group, len(lengths)
     have = [-(-max(l, 0) // bs) for l in lengths]
     width = max_blocks or max(max(have), 1)
     order_of = rng.permutation(sum(have) + 2)
-    pools = Pools(cache, len(order_of), bs, kv, dim, order, pad, seed=seed + 1)
+    pools = Pools(cache, len(order_of), bs, kv, dim, order, pad, seed=seed + 1, size=size)
     table = np.full((n, width + 3), 2 ** 30, np.int64)         # behind what is used: nonsense
     at = 0
     for i, h in enumerate(have):
@@ -225,7 +226,7 @@ def run_attend(kind, cache, order, bs, kv, group, dim, lengths, window=0, pad=0,
             g = got_lse[i * heads:(i + 1) * heads]
             assert (np.isneginf(g) == np.isneginf(want_lse)).all()
             fine = np.isfinite(want_lse)
-            assert (np.abs(g - want_lse)[fine] <= tol_lse[fine]).all()
+            assert (np.abs(g[fine] - want_lse[fine]) <= tol_lse[fine]).all()
     return got
 
 
@@ -280,6 +281,16 @@ def test_attend_sharp_and_flat_scores(kind, cache):
     run_attend(kind, cache, "thd", 16, 2, 4, 128, [700, 2000], grow=30.0, seed=4)       # one token takes nearly all
     run_attend(kind, cache, "thd", 16, 2, 4, 128, [700, 2000], scale=0.0, seed=5)       # all alike
     run_attend(kind, cache, "thd", 16, 2, 4, 128, [700, 2000], scale=-0.3, seed=6)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("group", [1, 2, 4, 8])
+def test_attend_small_and_large_values(kind, cache, group):
+    """Keys and values that are subnormal in fp16, and ones near its largest; queries far from 1 either way."""
+    run_attend(kind, cache, "thd", 16, 2, group, 64, [300, 40], size=2e-6, scale=1000.0, seed=1)
+    run_attend(kind, cache, "thd", 16, 2, group, 64, [300, 40], size=12000.0, scale=1e-5, seed=2)
+    run_attend(kind, cache, "thd", 16, 2, group, 64, [300, 40], grow=3e-4, scale=300.0, seed=3)
+    run_attend(kind, cache, "thd", 16, 2, group, 64, [300, 40], grow=3e3, scale=3e-5, seed=4)
 
 
 def small_attend(kind, cache, keys, values, q, lengths=None):
@@ -381,7 +392,7 @@ def run_select(kind, requests, beams, logits, n, scores=None, ended=None, end_to
     assert (np.isneginf(got[0]) == np.isneginf(want[0])).all()
     # the sum of the exponentials in 32 bits a piece of a row (at most 512 terms, each off by its argument's rounding and a few steps, which
     # counts as much as the term does), in 64 above: within 2^-17 of it; then one rounding to 32 bits
-    assert (np.abs(got[0] - want[0])[fine] <= 2.0 ** -17 + HALF[F32] * np.abs(want[0])[fine]).all()
+    assert (np.abs(got[0][fine] - want[0][fine]) <= 2.0 ** -17 + HALF[F32] * np.abs(want[0][fine])).all()
     return got
 
 
