@@ -515,16 +515,19 @@ def _op(name):
     return f
 
 
+# address of an operand, by its type
+_address = {type(None): lambda x: None, int: lambda x: x, DeviceBuffer: lambda x: x.ptr}
+
+
 def _at(x):
     """Address of a DeviceBuffer, of anything with data_ptr() (a torch tensor), or an address as it is."""
-    if x is None or isinstance(x, int):
-        return x
-    if isinstance(x, DeviceBuffer):
-        return x.ptr
-    # Loaded before torch, the library has a HIP runtime of its own, whose streams do not wait for torch's.
-    if not _torch_first:
-        raise RuntimeError("tensors of torch: import torch before the library is first used")
-    return x.data_ptr()
+    f = _address.get(type(x))
+    if f is None:
+        # Loaded before torch, the library has a HIP runtime of its own, whose streams do not wait for torch's.
+        if not _torch_first:
+            raise RuntimeError("tensors of torch: import torch before the library is first used")
+        f = _address[type(x)] = type(x).data_ptr
+    return f(x)
 
 
 def _nbytes(x):
