@@ -43,9 +43,34 @@ __device__ inline int32_t seen_tokens(const Args& a, int32_t r) {
 // Finds share `id` of all: of equal size but for the last one of each sequence, so that long sequences among short ones, or few of
 // them, keep the device as busy as many.  Every workgroup adds up the lengths for itself; with the sum rounded up by
 // more than 32-bit additions lose, sum ceil(seen / tokens) <= budget + requests, the size of the grid.  number < 0: there is no such share.
+// (at most 2^24 requests: 2^18 additions a thread, each off by 2^-24 of the sum at most)
+__device__ inline int32_t tokens_of(float total, int32_t budget) {
+    const float each = total * 1.02f / (float)budget;
+    return each < 2.0e9f ? max(kLeast, ((int32_t)each + 32) / 32 * 32) : INT32_MAX;
+}
+__device__ inline int32_t shares_of(int32_t n, int32_t tokens) { return max(1, (int32_t)(((uint32_t)n + tokens - 1) / (uint32_t)tokens)); }
+
 template <int THREADS>
 __device__ inline Share find_share(const Args& a, int32_t id) {
     constexpr int kWaves = THREADS / 64;
+    if (a.d.requests <= 64) {                // a request a lane, each wavefront for itself
+        const int lane = threadIdx.x & 63;
+        const int32_t n = lane < a.d.requests ? seen_tokens(a, lane) : 0;
+        float total = (float)n;
+        for (int x = 32; x; x >>= 1) total += __shfl_xor(total, x);
+        const int32_t tokens = tokens_of(total, a.budget), mine = lane < a.d.requests ? shares_of(n, tokens) : 0;
+        int32_t at = mine;
+        for (int x = 1; x < 64; x <<= 1) {
+            const int32_t o = __shfl_up(at, x);
+            if (lane >= x) at += o;
+        }
+        at -= mine;
+        const uint64_t who = __builtin_amdgcn_ballot_w64(id >= at && id < at + mine);
+        if (!who) return {0, -1, 0, 0, 0};
+        const int r = __builtin_amdgcn_readfirstlane(__builtin_ctzll(who));
+        const int32_t first = __builtin_amdgcn_readlane(at, r);
+        return {r, id - first, first, __builtin_amdgcn_readlane(mine, r), tokens};
+    }
     __shared__ float sums[kWaves];
     __shared__ int32_t counts[kWaves];
     __shared__ Share found;
@@ -59,11 +84,9 @@ __device__ inline Share find_share(const Args& a, int32_t id) {
     __syncthreads();
     total = 0.0f;
     for (int w = 0; w < kWaves; ++w) total += sums[w];
-    // (at most 2^24 requests: 2^18 additions a thread, each off by 2^-24 of the sum at most)
-    const float each = total * 1.02f / (float)a.budget;
-    const int32_t tokens = each < 2.0e9f ? max(kLeast, ((int32_t)each + 32) / 32 * 32) : INT32_MAX;
+    const int32_t tokens = tokens_of(total, a.budget);
     int32_t mine = 0;
-    for (int32_t r = lo; r < hi; ++r) mine += max(1, (int32_t)(((int64_t)seen_tokens(a, r) + tokens - 1) / tokens));
+    for (int32_t r = lo; r < hi; ++r) mine += shares_of(seen_tokens(a, r), tokens);
     int32_t at = mine;
     for (int x = 1; x < 64; x <<= 1) {
         const int32_t o = __shfl_up(at, x);
@@ -75,7 +98,7 @@ __device__ inline Share find_share(const Args& a, int32_t id) {
     for (int w = 0; w < wave; ++w) at += counts[w];
     if (id >= at && id < at + mine)
         for (int32_t r = lo; r < hi; ++r) {
-            const int32_t n = max(1, (int32_t)(((int64_t)seen_tokens(a, r) + tokens - 1) / tokens));
+            const int32_t n = shares_of(seen_tokens(a, r), tokens);
             if (id < at + n) {
                 found = {r, id - at, at, n, tokens};
                 break;
@@ -641,6 +664,15 @@ __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
     const float2* stats = a.stats + (int64_t)of.x * d.heads + h;
     const float* parts = a.parts + ((int64_t)of.x * d.heads + h) * D;
     const int64_t step = (int64_t)d.heads * D;
+    const int quads = D / 4, groups = kThreads / quads, mine = tid / quads, at = (tid - mine * quads) * 4;
+    constexpr int kAhead = 4;                // of a group's parts, on their way while the weights are made
+    f32x4 ahead[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+        const int s = mine + u * groups;
+        ahead[u] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (mine < groups && s < of.y) ahead[u] = *(const f32x4*)(parts + s * step + at);
+    }
     float m = -INFINITY, l = 0.0f;
     for (int s = tid; s < of.y; s += kThreads) m = fmaxf(m, stats[(int64_t)s * d.heads].x);
     for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
@@ -658,11 +690,13 @@ __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
     __syncthreads();
     l = 0.0f;
     for (int w = 0; w < kWaves; ++w) l += red[1][w];
-    const int quads = D / 4, groups = kThreads / quads, mine = tid / quads, at = (tid - mine * quads) * 4;
     f32x4 all = {0.0f, 0.0f, 0.0f, 0.0f};
     if (mine < groups) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (mine + u * groups < of.y) all += weight[mine + u * groups] * ahead[u];
 #pragma unroll 4
-        for (int s = mine; s < of.y; s += groups) all += weight[s] * *(const f32x4*)(parts + s * step + at);
+        for (int s = mine + kAhead * groups; s < of.y; s += groups) all += weight[s] * *(const f32x4*)(parts + s * step + at);
     }
     sums[tid] = all;
     __syncthreads();
