@@ -72,15 +72,15 @@ __global__ void __launch_bounds__(kThreads) row_pieces(SelectArgs a) {
         for (int u = 0; u < 8; ++u) {
             const int32_t i = at + u * 8 * kE;
             if (i >= 0 && i + kE <= d.vocab) raw[u] = *(const Raw*)(x + i);
-            else {
+            else if (i > -kE && i < d.vocab) {
 #pragma unroll
-                for (int e = 0; e < kE; ++e) raw[u][e] = (uint32_t)(i + e) < (uint32_t)d.vocab ? x[i + e] : (T)-INFINITY;
+                for (int e = 0; e < kE; ++e) raw[u][e] = x[max(0, min(i + e, d.vocab - 1))];
             }
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u)
 #pragma unroll
-            for (int e = 0; e < kE; ++e) v[u * kE + e] = (float)raw[u][e];
+            for (int e = 0; e < kE; ++e) v[u * kE + e] = (uint32_t)(at + u * 8 * kE + e) < (uint32_t)d.vocab ? (float)raw[u][e] : -INFINITY;
     }
     float m = v[0];
 #pragma unroll
