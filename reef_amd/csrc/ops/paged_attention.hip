@@ -23,6 +23,7 @@ struct Args {
     float* parts;           // [share][head][head_dim], sums that are not divided yet
     float2* stats;          // [share][head]: maximum (of scores * log2 e) and sum
     int2* info;             // [request]: its first share and how many they are
+    int32_t* list;          // more than kFewRequests: tokens of a share, shares in all, then each share's request; otherwise null
     int32_t group, tiles;   // query heads a cache head; tiles of 16 of them
     int32_t budget;         // shares that all tokens are cut into, beside one a request; 0: sequences are not split
     Divider block;          // by the block size
@@ -40,19 +41,55 @@ __device__ inline int32_t seen_tokens(const Args& a, int32_t r) {
     return a.d.window && held > a.d.window ? a.d.window : held;
 }
 
-// Finds share `id` of all: of equal size but for the last one of each sequence, so that long sequences among short ones, or few of
-// them, keep the device as busy as many.  Every workgroup adds up the lengths for itself; with the sum rounded up by
-// more than 32-bit additions lose, sum ceil(seen / tokens) <= budget + requests, the size of the grid.  number < 0: there is no such share.
-// (at most 2^24 requests: 2^18 additions a thread, each off by 2^-24 of the sum at most)
+// All tokens are cut into shares of equal size but for the last one of each sequence, so that long sequences among short ones, or few
+// of them, keep the device as busy as many.  With the sum of the lengths rounded up by more than its 32-bit additions lose,
+// sum ceil(seen / tokens) <= budget + requests, the size of the grid.  Up to kFewRequests every workgroup adds up the lengths for
+// itself, more are listed by a launch ahead (4096 requests of 8 heads would be read by 33000 workgroups).
+constexpr int32_t kFewRequests = 256, kListHead = 4;
+// (2^24 requests are 2^14 additions a thread, each off by 2^-24 of the sum at most)
 __device__ inline int32_t tokens_of(float total, int32_t budget) {
     const float each = total * 1.02f / (float)budget;
     return each < 2.0e9f ? max(kLeast, ((int32_t)each + 32) / 32 * 32) : INT32_MAX;
 }
 __device__ inline int32_t shares_of(int32_t n, int32_t tokens) { return max(1, (int32_t)(((uint32_t)n + tokens - 1) / (uint32_t)tokens)); }
 
-template <int THREADS>
+// Adds up over the workgroup, exclusively; *all: the sum.
+template <int WAVES>
+__device__ inline int32_t scan(int32_t v, int32_t* counts, int32_t* all) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int32_t at = v;
+    for (int x = 1; x < 64; x <<= 1) {
+        const int32_t o = __shfl_up(at, x);
+        if (lane >= x) at += o;
+    }
+    if (lane == 63) counts[wave] = at;
+    __syncthreads();
+    at -= v;
+    *all = 0;
+    for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) at += counts[w];
+        *all += counts[w];
+    }
+    return at;
+}
+template <int WAVES>
+__device__ inline float sum_of(float v, float* sums) {
+    for (int x = 32; x; x >>= 1) v += __shfl_xor(v, x);
+    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0f;
+    for (int w = 0; w < WAVES; ++w) v += sums[w];
+    return v;
+}
+
+// Share `id` of all; number < 0: there is no such share.
 __device__ inline Share find_share(const Args& a, int32_t id) {
-    constexpr int kWaves = THREADS / 64;
+    if (a.list) {
+        if (id >= a.list[1]) return {0, -1, 0, 0, 0};
+        const int32_t r = a.list[kListHead + id];
+        const int2 info = a.info[r];
+        return {r, id - info.x, info.x, info.y, a.list[0]};
+    }
     if (a.d.requests <= 64) {                // a request a lane, each wavefront for itself
         const int lane = threadIdx.x & 63;
         const int32_t n = lane < a.d.requests ? seen_tokens(a, lane) : 0;
@@ -71,42 +108,43 @@ __device__ inline Share find_share(const Args& a, int32_t id) {
         const int32_t first = __builtin_amdgcn_readlane(at, r);
         return {r, id - first, first, __builtin_amdgcn_readlane(mine, r), tokens};
     }
+    constexpr int kWaves = kThreads / 64;    // a request a thread
     __shared__ float sums[kWaves];
     __shared__ int32_t counts[kWaves];
     __shared__ Share found;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int32_t R = a.d.requests, per = (R + THREADS - 1) / THREADS, lo = min(R, tid * per), hi = min(R, lo + per);
-    float total = 0.0f;
-    for (int32_t r = lo; r < hi; ++r) total += (float)seen_tokens(a, r);
-    for (int x = 32; x; x >>= 1) total += __shfl_xor(total, x);
-    if (lane == 0) sums[wave] = total;
-    if (tid == 0) found.number = -1;
-    __syncthreads();
-    total = 0.0f;
-    for (int w = 0; w < kWaves; ++w) total += sums[w];
-    const int32_t tokens = tokens_of(total, a.budget);
-    int32_t mine = 0;
-    for (int32_t r = lo; r < hi; ++r) mine += shares_of(seen_tokens(a, r), tokens);
-    int32_t at = mine;
-    for (int x = 1; x < 64; x <<= 1) {
-        const int32_t o = __shfl_up(at, x);
-        if (lane >= x) at += o;
-    }
-    if (lane == 63) counts[wave] = at;
-    __syncthreads();
-    at -= mine;
-    for (int w = 0; w < wave; ++w) at += counts[w];
-    if (id >= at && id < at + mine)
-        for (int32_t r = lo; r < hi; ++r) {
-            const int32_t n = shares_of(seen_tokens(a, r), tokens);
-            if (id < at + n) {
-                found = {r, id - at, at, n, tokens};
-                break;
-            }
-            at += n;
-        }
+    const int32_t r = threadIdx.x, n = r < a.d.requests ? seen_tokens(a, r) : 0;
+    if (r == 0) found.number = -1;
+    const int32_t tokens = tokens_of(sum_of<kWaves>((float)n, sums), a.budget), mine = r < a.d.requests ? shares_of(n, tokens) : 0;
+    int32_t all;
+    const int32_t at = scan<kWaves>(mine, counts, &all);
+    if (id >= at && id < at + mine) found = {r, id - at, at, mine, tokens};
     __syncthreads();
     return found;
+}
+
+// The list of shares, by one workgroup: `per` requests a thread.
+constexpr int kListThreads = 1024;
+__global__ void __launch_bounds__(kListThreads) list_shares(Args a) {
+    constexpr int kWaves = kListThreads / 64;
+    __shared__ float sums[kWaves];
+    __shared__ int32_t counts[kWaves];
+    const int32_t R = a.d.requests, per = (R + kListThreads - 1) / kListThreads, lo = min(R, (int32_t)threadIdx.x * per), hi = min(R, lo + per);
+    float total = 0.0f;
+    for (int32_t r = lo; r < hi; ++r) total += (float)seen_tokens(a, r);
+    const int32_t tokens = tokens_of(sum_of<kWaves>(total, sums), a.budget);
+    int32_t mine = 0, all;
+    for (int32_t r = lo; r < hi; ++r) mine += shares_of(seen_tokens(a, r), tokens);
+    int32_t at = scan<kWaves>(mine, counts, &all);
+    for (int32_t r = lo; r < hi; ++r) {
+        const int32_t n = shares_of(seen_tokens(a, r), tokens);
+        a.info[r] = make_int2(at, n);
+        for (int32_t i = 0; i < n; ++i) a.list[kListHead + at + i] = r;
+        at += n;
+    }
+    if (threadIdx.x == 0) {
+        a.list[0] = tokens;
+        a.list[1] = all;
+    }
 }
 
 // Four values of an output row: divided by the sum of the weights and rounded once, 0 where there are none.
@@ -223,10 +261,10 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     const int tile16 = id % a.tiles;
     id /= a.tiles;
     Share of = {id, 0, 0, 1, 0};
-    if (a.budget) {
-        of = find_share<WAVES * 64>(a, id);
+    if (WAVES == 4 && a.budget) {            // (wide workgroups do not split)
+        of = find_share(a, id);
         if (of.number < 0) return;
-        if (of.number == 0 && blockIdx.x % (d.cache.kv_heads * a.tiles) == 0 && threadIdx.x == 0) a.info[of.request] = make_int2(of.first, of.count);
+        if (!a.list && of.number == 0 && blockIdx.x % (d.cache.kv_heads * a.tiles) == 0 && threadIdx.x == 0) a.info[of.request] = make_int2(of.first, of.count);
     }
     const int32_t r = of.request;
     const int32_t held = held_length(a.lengths[r], d.max_blocks, d.cache.block_size);
@@ -728,7 +766,7 @@ struct Plan {
     int32_t tiles, budget;
     bool wide;              // workgroups of more wavefronts
     int64_t groups;         // workgroups
-    size_t info_bytes, stats_bytes, bytes;
+    size_t info_bytes, list_bytes, stats_bytes, bytes;
 };
 // Wavefronts of a wide workgroup: as many as the registers allow a CU; with matrix products for heads over 128 those of any.
 constexpr int wide_waves(int dp, bool terms, int few) {
@@ -756,7 +794,8 @@ Plan plan_of(const reef_paged_attention_desc& d) {
     p.groups = shares * rows;
     p.info_bytes = ((size_t)d.requests * 8 + 15) / 16 * 16;
     p.stats_bytes = ((size_t)shares * d.heads * 8 + 15) / 16 * 16;
-    p.bytes = p.info_bytes + p.stats_bytes + (size_t)shares * d.heads * D * 4;
+    if (d.requests > kFewRequests) p.list_bytes = ((size_t)(kListHead + shares) * 4 + 15) / 16 * 16;
+    p.bytes = p.info_bytes + p.list_bytes + p.stats_bytes + (size_t)shares * d.heads * D * 4;
     return p;
 }
 
@@ -785,6 +824,8 @@ int run_heads(const char* what, const Args& a, const Plan& p, void* stream) {
 template <class Q, class C>
 int run(const char* what, const Args& a, const Plan& p, void* stream) {
     const int D = a.d.cache.head_dim;
+    if (a.list)
+        if (int rc = launch(what, list_shares, dim3(1), dim3(kListThreads), a, stream)) return rc;
     const int rc = D == 64    ? run_heads<Q, C, 64, true>(what, a, p, stream)
                    : D < 64   ? run_heads<Q, C, 64, false>(what, a, p, stream)
                    : D == 128 ? run_heads<Q, C, 128, true>(what, a, p, stream)
@@ -815,8 +856,9 @@ extern "C" int reef_ops_paged_attention(const reef_paged_attention_desc* d, cons
     if (p.bytes && (!rows16(workspace) || workspace_bytes < (int64_t)p.bytes))
         return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", p.bytes, (long long)workspace_bytes);
     char* w = (char*)workspace;
-    const Args a{*d, query, key_cache, value_cache, table, lengths, out, lse, (float*)(w + p.info_bytes + p.stats_bytes), (float2*)(w + p.info_bytes),
-                 (int2*)w, d->heads / d->cache.kv_heads, p.tiles, p.budget, divider((uint32_t)d->cache.block_size)};
+    const size_t list = p.info_bytes, stats = list + p.list_bytes, parts = stats + p.stats_bytes;
+    const Args a{*d, query, key_cache, value_cache, table, lengths, out, lse, (float*)(w + parts), (float2*)(w + stats), (int2*)w,
+                 p.list_bytes ? (int32_t*)(w + list) : nullptr, d->heads / d->cache.kv_heads, p.tiles, p.budget, divider((uint32_t)d->cache.block_size)};
     switch (d->type * 4 + d->cache.type) {
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, p, stream);
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return run<float, _Float16>(what, a, p, stream);

@@ -259,6 +259,16 @@ def test_attend_long_and_ragged(kind, cache, longest):
     run_attend(kind, cache, "thd", 16, 1, 8, 128, [5000, 1, 0, 2047, 2048, 2049, 777, 4096, 511, 512, 513], longest=longest, seed=longest % 97, q_pad=8)
 
 
+@pytest.mark.parametrize("requests", [63, 64, 65, 255, 256, 257, 1023, 1500])
+@pytest.mark.parametrize("window", [0, 700])
+def test_attend_many_requests(requests, window):
+    """A few long sequences among many short and empty ones."""
+    rng = np.random.default_rng(requests)
+    lengths = rng.integers(0, 40, requests)
+    lengths[rng.integers(0, requests, 6)] = [2500, 1100, 600, 513, 512, 0]
+    run_attend(BF16, BF16, "thd", 16, 1, 2, 32, lengths.tolist(), window=window, seed=requests)
+
+
 @pytest.mark.parametrize("kind,cache", PAIRS)
 @pytest.mark.parametrize("window", [1, 2, 16, 31, 100, 128, 1000, 10 ** 9])
 def test_attend_windows(kind, cache, window):
