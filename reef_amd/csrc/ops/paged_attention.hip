@@ -27,6 +27,7 @@ struct Args {
     int32_t group, tiles;   // query heads a cache head; tiles of 16 of them
     int32_t budget;         // shares that all tokens are cut into, beside one a request; 0: sequences are not split
     Divider block;          // by the block size
+    int32_t heads_each;     // of a workgroup of the join
 };
 
 constexpr int32_t kLeast = 128;              // tokens a share at least
@@ -687,61 +688,67 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     }
 }
 
-// The shares of a sequence of one query head: a workgroup, lanes over quads of the head, groups of them over the shares.
+// The shares of a sequence of one query head: a workgroup, lanes over quads of the head, groups of them over the shares.  `heads_each`
+// heads one after the other: most requests of a large batch are not split, and their workgroups only find that out.
 template <class Q>
 __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
     constexpr int kWaves = kThreads / 64;
     const reef_paged_attention_desc& d = a.d;
-    const int r = blockIdx.x / d.heads, h = blockIdx.x % d.heads, D = d.cache.head_dim;
+    const int blocks = (d.heads + a.heads_each - 1) / a.heads_each, r = blockIdx.x / blocks, D = d.cache.head_dim;
     const int2 of = a.info[r];
     if (of.y <= 1) return;
     __shared__ float weight[kGroups + 2];
     __shared__ float red[2][kWaves];
     __shared__ f32x4 sums[kThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const float2* stats = a.stats + (int64_t)of.x * d.heads + h;
-    const float* parts = a.parts + ((int64_t)of.x * d.heads + h) * D;
-    const int64_t step = (int64_t)d.heads * D;
-    const int quads = D / 4, groups = kThreads / quads, mine = tid / quads, at = (tid - mine * quads) * 4;
-    constexpr int kAhead = 4;                // of a group's parts, on their way while the weights are made
-    f32x4 ahead[kAhead];
+    const int h1 = min(d.heads, ((int)blockIdx.x % blocks + 1) * a.heads_each);
+    for (int h = (int)blockIdx.x % blocks * a.heads_each; h < h1; ++h) {
+        const float2* stats = a.stats + (int64_t)of.x * d.heads + h;
+        const float* parts = a.parts + ((int64_t)of.x * d.heads + h) * D;
+        const int64_t step = (int64_t)d.heads * D;
+        const int quads = D / 4, groups = kThreads / quads, mine = tid / quads, at = (tid - mine * quads) * 4;
+        constexpr int kAhead = 4;                // of a group's parts, on their way while the weights are made
+        f32x4 ahead[kAhead];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-        const int s = mine + u * groups;
-        ahead[u] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (mine < groups && s < of.y) ahead[u] = *(const f32x4*)(parts + s * step + at);
-    }
-    float m = -INFINITY, l = 0.0f;
-    for (int s = tid; s < of.y; s += kThreads) m = fmaxf(m, stats[(int64_t)s * d.heads].x);
-    for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
-    if (lane == 0) red[0][wave] = m;
-    __syncthreads();
-    for (int w = 0; w < kWaves; ++w) m = fmaxf(m, red[0][w]);
-    const float base = m == -INFINITY ? 0.0f : m;
-    for (int s = tid; s < of.y; s += kThreads) {
-        const float2 x = stats[(int64_t)s * d.heads];
-        weight[s] = __builtin_amdgcn_exp2f(x.x - base);
-        l += weight[s] * x.y;
-    }
-    for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x);
-    if (lane == 0) red[1][wave] = l;
-    __syncthreads();
-    l = 0.0f;
-    for (int w = 0; w < kWaves; ++w) l += red[1][w];
-    f32x4 all = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (mine < groups) {
+        for (int u = 0; u < kAhead; ++u) {
+            const int s = mine + u * groups;
+            ahead[u] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (mine < groups && s < of.y) ahead[u] = *(const f32x4*)(parts + s * step + at);
+        }
+        float m = -INFINITY, l = 0.0f;
+        for (int s = tid; s < of.y; s += kThreads) m = fmaxf(m, stats[(int64_t)s * d.heads].x);
+        for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
+        if (lane == 0) red[0][wave] = m;
+        __syncthreads();
+        for (int w = 0; w < kWaves; ++w) m = fmaxf(m, red[0][w]);
+        const float base = m == -INFINITY ? 0.0f : m;
+        for (int s = tid; s < of.y; s += kThreads) {
+            const float2 x = stats[(int64_t)s * d.heads];
+            weight[s] = __builtin_amdgcn_exp2f(x.x - base);
+            l += weight[s] * x.y;
+        }
+        for (int x = 32; x; x >>= 1) l += __shfl_xor(l, x);
+        if (lane == 0) red[1][wave] = l;
+        __syncthreads();
+        l = 0.0f;
+        for (int w = 0; w < kWaves; ++w) l += red[1][w];
+        f32x4 all = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (mine < groups) {
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u)
-            if (mine + u * groups < of.y) all += weight[mine + u * groups] * ahead[u];
+            for (int u = 0; u < kAhead; ++u)
+                if (mine + u * groups < of.y) all += weight[mine + u * groups] * ahead[u];
 #pragma unroll 4
-        for (int s = mine + kAhead * groups; s < of.y; s += groups) all += weight[s] * *(const f32x4*)(parts + s * step + at);
+            for (int s = mine + kAhead * groups; s < of.y; s += groups) all += weight[s] * *(const f32x4*)(parts + s * step + at);
+        }
+        sums[tid] = all;
+        __syncthreads();
+        if (!mine) {
+            for (int x = 1; x < groups; ++x) all += sums[x * quads + tid];
+            put4((Q*)a.out + r * d.out_stride + h * d.out_head_stride + at, all, l);
+            if (tid == 0 && a.lse) a.lse[(int64_t)r * d.heads + h] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
+        }
+        __syncthreads();                         // (the next head's weights and sums go where these are)
     }
-    sums[tid] = all;
-    __syncthreads();
-    if (mine) return;
-    for (int x = 1; x < groups; ++x) all += sums[x * quads + tid];
-    put4((Q*)a.out + r * d.out_stride + h * d.out_head_stride + at, all, l);
-    if (tid == 0 && a.lse) a.lse[(int64_t)r * d.heads + h] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
 int check(const char* what, const reef_paged_attention_desc* d) {
@@ -833,7 +840,7 @@ int run(const char* what, const Args& a, const Plan& p, void* stream) {
                    : D == 256 ? run_heads<Q, C, 256, true>(what, a, p, stream)
                               : run_heads<Q, C, 256, false>(what, a, p, stream);
     if (rc || !p.budget) return rc;
-    return launch(what, join_shares<Q>, dim3((unsigned)(a.d.requests * a.d.heads)), dim3(kThreads), a, stream);
+    return launch(what, join_shares<Q>, dim3((unsigned)(a.d.requests * ((a.d.heads + a.heads_each - 1) / a.heads_each))), dim3(kThreads), a, stream);
 }
 
 }  // namespace
@@ -858,7 +865,8 @@ extern "C" int reef_ops_paged_attention(const reef_paged_attention_desc* d, cons
     char* w = (char*)workspace;
     const size_t list = p.info_bytes, stats = list + p.list_bytes, parts = stats + p.stats_bytes;
     const Args a{*d, query, key_cache, value_cache, table, lengths, out, lse, (float*)(w + parts), (float2*)(w + stats), (int2*)w,
-                 p.list_bytes ? (int32_t*)(w + list) : nullptr, d->heads / d->cache.kv_heads, p.tiles, p.budget, divider((uint32_t)d->cache.block_size)};
+                 p.list_bytes ? (int32_t*)(w + list) : nullptr, d->heads / d->cache.kv_heads, p.tiles, p.budget, divider((uint32_t)d->cache.block_size),
+                 d->requests > kFewRequests ? std::min(d->heads, 8) : 1};
     switch (d->type * 4 + d->cache.type) {
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, p, stream);
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return run<float, _Float16>(what, a, p, stream);
