@@ -10,7 +10,7 @@ using namespace reef_ops;
 constexpr int kThreads = 256;                // of a workgroup of four wavefronts, and of the join's
 // Workgroups that the shares of all sequences are to make: what runs at once (two a CU; one for heads over 128) less an eighth, as each
 // sequence's last share is a shorter one more.  Just above what runs at once the last round is nearly empty: of
-// 128 .. 4096, 448 takes 282 us for 3 x 131071 tokens (512: 281, 640: 327), 190 for 14 x 15754 (512: 238), 65 for 64 mixed (1024: 62).
+// 128 .. 2048, 448 takes 280 us for 3 x 131071 tokens (512: 279, 640: 333), 187 for 14 x 15754 (512: 236), 61 for 64 mixed (512: 66).
 constexpr int kGroups = 448;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
