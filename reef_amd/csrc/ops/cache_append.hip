@@ -78,9 +78,12 @@ extern "C" int reef_ops_cache_append(const reef_cache_append_desc* d, const void
 }
 
 extern "C" int reef_ops_paged_row(const reef_cache_layout* c, const int32_t* table_row, int max_blocks, int64_t token, int64_t* offset) {
-    if (!c || !table_row || !offset || c->block_size < 1 || token < 0 || token / c->block_size >= max_blocks) return 0;
+    if (!c || !table_row || !offset || c->block_size < 1 || token < 0 || token >= 1ll << 31) return 0;
+    const Divider by = divider((uint32_t)c->block_size);
+    const uint32_t t = (uint32_t)token, entry = divided(t, by);
+    if ((int64_t)entry >= max_blocks) return 0;
     const PagedView v{c->blocks, c->block_size, max_blocks, c->block_stride, c->slot_stride};
-    const int64_t at = paged_row(v, table_row[token / c->block_size], (int32_t)(token % c->block_size));
+    const int64_t at = paged_row(v, table_row[entry], (int32_t)(t - entry * by.by));
     if (at < 0) return 0;
     *offset = at;
     return 1;

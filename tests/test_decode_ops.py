@@ -34,6 +34,26 @@ def test_places_past_32_bits():
     assert B.ops_paged_row(c, [1, 2], 5) == 2 * 2048 + 2 * 128
 
 
+def test_places_for_any_block_size():
+    """The kernels multiply and shift where this divides."""
+    rng = np.random.default_rng(0)
+    sizes = list(range(1, 70)) + [2 ** k + j for k in range(7, 16) for j in (-1, 0, 1)] + rng.integers(1, 2 ** 16, 40).tolist()
+    row = np.zeros(1 << 14, np.int32)
+    for bs in sizes:
+        c = layout(blocks=1, block_size=bs, slot_stride=8, head_stride=8, head_dim=8, kv_heads=1, block_stride=0)
+        held = min(len(row) * bs, 2 ** 31 - 1)
+        for t in [0, 1, bs - 1, bs, bs + 1, 2 * bs - 1, held - 1, held // bs * bs - 1] + rng.integers(0, held, 30).tolist():
+            assert B.ops_paged_row(c, row, t) == t % bs * 8, (bs, t)
+        if held == len(row) * bs:
+            assert B.ops_paged_row(c, row, held) is None
+    # quotients: a row whose entries name themselves
+    row = np.arange(4096, dtype=np.int32)
+    for bs in (1, 3, 7, 16, 24, 100, 1000, 524287, 524288):
+        c = layout(blocks=4096, block_size=bs, slot_stride=8, head_stride=8, head_dim=8, kv_heads=1, block_stride=2 ** 40)
+        for t in [0, 4095 * bs, min(4096 * bs, 2 ** 31) - 1] + rng.integers(0, min(4096 * bs, 2 ** 31 - 1), 50).tolist():
+            assert B.ops_paged_row(c, row, t) == t // bs * 2 ** 40 + t % bs * 8, (bs, t)
+
+
 BAD_LAYOUTS = [(dict(type=3), "type"), (dict(type=-1), "type"), (dict(blocks=0), "bad cache"), (dict(block_size=0), "bad cache"),
                (dict(kv_heads=0), "bad cache"), (dict(blocks=2 ** 20, block_size=2 ** 11), "bad cache"), (dict(head_dim=60), "head_dim"),
                (dict(head_dim=264), "head_dim"), (dict(head_dim=0), "head_dim"), (dict(head_stride=63), "16 bytes"),
