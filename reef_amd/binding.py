@@ -519,15 +519,17 @@ def _op(name):
 _address = {type(None): lambda x: None, int: lambda x: x, DeviceBuffer: lambda x: x.ptr}
 
 
-def _at(x):
-    """Address of a DeviceBuffer, of anything with data_ptr() (a torch tensor), or an address as it is."""
-    f = _address.get(type(x))
-    if f is None:
-        # Loaded before torch, the library has a HIP runtime of its own, whose streams do not wait for torch's.
-        if not _torch_first:
-            raise RuntimeError("tensors of torch: import torch before the library is first used")
-        f = _address[type(x)] = type(x).data_ptr
-    return f(x)
+def _learn(x):
+    # Loaded before torch, the library has a HIP runtime of its own, whose streams do not wait for torch's.
+    if not _torch_first:
+        raise RuntimeError("tensors of torch: import torch before the library is first used")
+    _address[type(x)] = type(x).data_ptr
+    return x.data_ptr()
+
+
+def _at(*operands):
+    """Addresses of DeviceBuffers, of anything with data_ptr() (torch tensors), or addresses as they are."""
+    return [_address.get(type(x), _learn)(x) for x in operands]
 
 
 def _nbytes(x):
@@ -538,12 +540,11 @@ def _nbytes(x):
 def ops_block_plan(desc, cached, added, free_list, table, lengths, starts, slots, counts, stream=None):
     """reef_ops_block_plan; operands are DeviceBuffers, torch tensors or addresses.  Like the calls below it enqueues,
     does not wait and returns the status."""
-    return _op("block_plan")(ctypes.addressof(desc), _at(cached), _at(added), _at(free_list), _at(table), _at(lengths), _at(starts),
-                             _at(slots), _at(counts), stream)
+    return _op("block_plan")(ctypes.addressof(desc), *_at(cached, added, free_list, table, lengths, starts, slots, counts), stream)
 
 
 def ops_cache_append(desc, key, value, slots, key_cache, value_cache, stream=None):
-    return _op("cache_append")(ctypes.addressof(desc), _at(key), _at(value), _at(slots), _at(key_cache), _at(value_cache), stream)
+    return _op("cache_append")(ctypes.addressof(desc), *_at(key, value, slots, key_cache, value_cache), stream)
 
 
 def _workspace(name, desc):
@@ -561,8 +562,8 @@ def ops_paged_attention_workspace(desc):
 
 
 def ops_paged_attention(desc, query, key_cache, value_cache, table, lengths, out, lse=None, workspace=None, stream=None):
-    return _op("paged_attention")(ctypes.addressof(desc), _at(query), _at(key_cache), _at(value_cache), _at(table), _at(lengths), _at(out),
-                                  _at(lse), _at(workspace), _nbytes(workspace), stream)
+    return _op("paged_attention")(ctypes.addressof(desc), *_at(query, key_cache, value_cache, table, lengths, out, lse, workspace),
+                                  _nbytes(workspace), stream)
 
 
 def ops_beam_select_workspace(desc):
@@ -571,13 +572,11 @@ def ops_beam_select_workspace(desc):
 
 
 def ops_beam_select(desc, logits, scores, ended, best, parents, tokens, workspace=None, stream=None):
-    return _op("beam_select")(ctypes.addressof(desc), _at(logits), _at(scores), _at(ended), _at(best), _at(parents), _at(tokens),
-                              _at(workspace), _nbytes(workspace), stream)
+    return _op("beam_select")(ctypes.addressof(desc), *_at(logits, scores, ended, best, parents, tokens, workspace), _nbytes(workspace), stream)
 
 
 def ops_beam_reorder(desc, parents, lengths, table, spare, table_out, lengths_out, key_cache, value_cache, stream=None):
-    return _op("beam_reorder")(ctypes.addressof(desc), _at(parents), _at(lengths), _at(table), _at(spare), _at(table_out), _at(lengths_out),
-                               _at(key_cache), _at(value_cache), stream)
+    return _op("beam_reorder")(ctypes.addressof(desc), *_at(parents, lengths, table, spare, table_out, lengths_out, key_cache, value_cache), stream)
 
 
 def ops_paged_row(cache, table_row, token):
