@@ -270,6 +270,16 @@ def test_attend_many_requests(requests, window):
 
 
 @pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("requests,kv,group,longest", [(31, 3, 2, 60), (32, 3, 2, 60), (33, 5, 17, 200), (40, 3, 4, 1500), (1, 3, 33, 5000), (290, 3, 1, 700)])
+def test_attend_workgroups_by_xcd(kind, cache, requests, kv, group, longest):
+    """Heads whose rows end inside lines, several tiles of query heads, shares in all numbers modulo eight."""
+    rng = np.random.default_rng(requests)
+    lengths = np.exp(rng.uniform(0, np.log(longest), requests)).astype(int)
+    lengths[0] = longest
+    run_attend(kind, cache, "thd", 16, kv, group, 40, lengths.tolist(), longest=longest, seed=requests)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
 @pytest.mark.parametrize("window", [1, 2, 16, 31, 100, 128, 1000, 10 ** 9])
 def test_attend_windows(kind, cache, window):
     run_attend(kind, cache, "htd", 24, 2, 2, 80, [1, 24, 100, 101, 129, 1500, 3001, 0], window=window, seed=window % 89)
