@@ -9,9 +9,13 @@ using namespace reef_ops;
 
 constexpr int kThreads = 256;                // of a workgroup of four wavefronts, and of the join's
 // Workgroups that the shares of all sequences are to make: what runs at once (two a CU; one for heads over 128) less an eighth, as each
-// sequence's last share is a shorter one more.  Just above what runs at once the last round is nearly empty: of
-// 128 .. 2048, 448 takes 280 us for 3 x 131071 tokens (512: 279, 640: 333), 187 for 14 x 15754 (512: 236), 61 for 64 mixed (512: 66).
-constexpr int kGroups = 448;
+// sequence's number of shares is rounded up.  Just above what runs at once the last round is nearly empty: of 224 .. 3584, 448 takes
+// 80 us for 12 x 8000 tokens, 8 cache heads of 128, bf16 (672: 87, 1344: 88), 21 where these lengths are the longest (672: 26).
+// Where the heads of all sequences are as many by themselves most have one or two shares, and the few long ones decide: twice as many
+// take 95 us instead of 103 for 90 sequences of up to 8000 tokens, 149 instead of 158 for 300 with 4 heads, 306 instead of 326 for
+// 50 x 8000, the same for 300 x 1500, 2 % more for 90 x 8000; 64 x 9000 with heads of 64, which just run at once uncut, lose most: 262
+// instead of 240.  Four times as many win little more (306 -> 303) and lose 7 % for 300 x 8000, heads of 64.
+constexpr int kGroups = 448, kFiner = 2;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Args {
@@ -23,7 +27,7 @@ struct Args {
     float* parts;           // [share][head][head_dim], sums that are not divided yet
     float2* stats;          // [share][head]: maximum (of scores * log2 e) and sum
     int2* info;             // [request]: its first share and how many they are
-    int32_t* list;          // more than kFewRequests: tokens of a share, shares in all, then each share's request; otherwise null
+    int32_t* list;          // more than kFewRequests: the number of shares, then the request of each; otherwise null
     int32_t group, tiles;   // query heads a cache head; tiles of 16 of them
     int32_t budget;         // shares that all tokens are cut into, beside one a request; 0: sequences are not split
     Divider block;          // by the block size
@@ -35,7 +39,6 @@ constexpr int32_t kLeast = 128;              // tokens a share at least
 
 struct Share {
     int32_t request, number, first, count;   // the number-th of `count` shares of the request, which start with share `first` of all
-    int32_t tokens;                          // of a share, the last one may be shorter
 };
 
 __device__ inline int32_t seen_tokens(const Args& a, int32_t r) {
@@ -43,17 +46,23 @@ __device__ inline int32_t seen_tokens(const Args& a, int32_t r) {
     return a.d.window && held > a.d.window ? a.d.window : held;
 }
 
-// All tokens are cut into shares of equal size but for the last one of each sequence, so that long sequences among short ones, or few
-// of them, keep the device as busy as many.  With the sum of the lengths rounded up by more than its 32-bit additions lose,
+// Sequences are cut into shares of at most so many tokens, equal ones, so that long sequences among short ones, or few of them, keep
+// the device as busy as many.  With the sum of the lengths rounded up by more than its 32-bit additions lose,
 // sum ceil(seen / tokens) <= budget + requests, the size of the grid.  Up to kFewRequests every workgroup adds up the lengths for
 // itself, more are listed by a launch ahead (4096 requests of 8 heads would be read by 33000 workgroups).
-constexpr int32_t kFewRequests = 256, kListHead = 4;
+constexpr int32_t kFewRequests = 256, kListHead = 1;
 // (2^24 requests are 2^14 additions a thread, each off by 2^-24 of the sum at most)
 __device__ inline int32_t tokens_of(float total, int32_t budget) {
     const float each = total * 1.02f / (float)budget;
     return each < 2.0e9f ? max(kLeast, ((int32_t)each + 32) / 32 * 32) : INT32_MAX;
 }
 __device__ inline int32_t shares_of(int32_t n, int32_t tokens) { return max(1, (int32_t)(((uint32_t)n + tokens - 1) / (uint32_t)tokens)); }
+// Where share `number` of `count` begins among n tokens: whole tiles of 32, one more for the first ones.  (None is
+// empty: n > 128 (count - 1), so there are 4 count - 3 tiles or more.)
+__device__ inline int32_t begin_of(int32_t n, int32_t number, int32_t count) {
+    const int32_t tiles = (int32_t)(((uint32_t)n + 31) / 32), each = tiles / count;
+    return (number * each + min(number, tiles - each * count)) * 32;
+}
 
 // Adds up over the workgroup, exclusively; *all: the sum.
 template <int WAVES>
@@ -87,10 +96,10 @@ __device__ inline float sum_of(float v, float* sums) {
 // Share `id` of all; number < 0: there is no such share.
 __device__ inline Share find_share(const Args& a, int32_t id) {
     if (a.list) {
-        if (id >= a.list[1]) return {0, -1, 0, 0, 0};
+        if (id >= a.list[0]) return {0, -1, 0, 0};
         const int32_t r = a.list[kListHead + id];
         const int2 info = a.info[r];
-        return {r, id - info.x, info.x, info.y, a.list[0]};
+        return {r, id - info.x, info.x, info.y};
     }
     if (a.d.requests <= 64) {                // a request a lane, each wavefront for itself
         const int lane = threadIdx.x & 63;
@@ -105,10 +114,10 @@ __device__ inline Share find_share(const Args& a, int32_t id) {
         }
         at -= mine;
         const uint64_t who = __builtin_amdgcn_ballot_w64(id >= at && id < at + mine);
-        if (!who) return {0, -1, 0, 0, 0};
+        if (!who) return {0, -1, 0, 0};
         const int r = __builtin_amdgcn_readfirstlane(__builtin_ctzll(who));
         const int32_t first = __builtin_amdgcn_readlane(at, r);
-        return {r, id - first, first, __builtin_amdgcn_readlane(mine, r), tokens};
+        return {r, id - first, first, __builtin_amdgcn_readlane(mine, r)};
     }
     constexpr int kWaves = kThreads / 64;    // a request a thread
     __shared__ float sums[kWaves];
@@ -119,7 +128,7 @@ __device__ inline Share find_share(const Args& a, int32_t id) {
     const int32_t tokens = tokens_of(sum_of<kWaves>((float)n, sums), a.budget), mine = r < a.d.requests ? shares_of(n, tokens) : 0;
     int32_t all;
     const int32_t at = scan<kWaves>(mine, counts, &all);
-    if (id >= at && id < at + mine) found = {r, id - at, at, mine, tokens};
+    if (id >= at && id < at + mine) found = {r, id - at, at, mine};
     __syncthreads();
     return found;
 }
@@ -143,10 +152,7 @@ __global__ void __launch_bounds__(kListThreads) list_shares(Args a) {
         for (int32_t i = 0; i < n; ++i) a.list[kListHead + at + i] = r;
         at += n;
     }
-    if (threadIdx.x == 0) {
-        a.list[0] = tokens;
-        a.list[1] = all;
-    }
+    if (threadIdx.x == 0) a.list[0] = all;
 }
 
 // Four values of an output row: divided by the sum of the weights and rounded once, 0 where there are none.
@@ -267,7 +273,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     id /= a.tiles;
     const int kvh = id % d.cache.kv_heads;
     id /= d.cache.kv_heads;
-    Share of = {id, 0, 0, 1, 0};
+    Share of = {id, 0, 0, 1};
     if (WAVES == 4 && a.budget) {            // (wide workgroups do not split)
         of = find_share(a, id);
         if (of.number < 0) return;
@@ -276,7 +282,11 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     const int32_t r = of.request;
     const int32_t held = held_length(a.lengths[r], d.max_blocks, d.cache.block_size);
     const int32_t first = d.window && held > d.window ? held - d.window : 0;
-    const int32_t begin = first + of.number * of.tokens, end = of.count > 1 ? (int32_t)min((int64_t)held, (int64_t)begin + of.tokens) : held;
+    int32_t begin = first, end = held;
+    if (WAVES == 4 && of.count > 1) {
+        begin = first + begin_of(held - first, of.number, of.count);
+        if (of.number + 1 < of.count) end = first + begin_of(held - first, of.number + 1, of.count);
+    }
 
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const int D = d.cache.head_dim;
@@ -703,7 +713,7 @@ __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
     const int blocks = (d.heads + a.heads_each - 1) / a.heads_each, r = blockIdx.x / blocks, D = d.cache.head_dim;
     const int2 of = a.info[r];
     if (of.y <= 1) return;
-    __shared__ float weight[kGroups + 2];
+    __shared__ float weight[kFiner * kGroups + 2];
     __shared__ float red[2][kWaves];
     __shared__ f32x4 sums[kThreads];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -815,7 +825,8 @@ Plan plan_of(const reef_paged_attention_desc& d) {
         spread(d.requests);
         return p;
     }
-    p.budget = std::max(1, (D > 128 ? kGroups / 2 : kGroups) / rows);
+    const bool finer = all >= kGroups * 7 / 8 && longest >= 4096;     // (90 sequences of up to 1500 tokens: 29 us, 30 with twice as many)
+    p.budget = std::max(1, (D > 128 ? kGroups / 2 : kGroups) * (finer ? kFiner : 1) / rows);
     const int64_t shares = (int64_t)p.budget + d.requests;
     p.groups = shares * rows;
     spread(shares);

@@ -280,6 +280,26 @@ def test_attend_workgroups_by_xcd(kind, cache, requests, kv, group, longest):
 
 
 @pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("window", [0, 450])
+def test_attend_lengths_around_the_cuts(kind, cache, window):
+    """Shares of 128 tokens at most: just below, at and above two, three and more of them, and tiles that they do not divide."""
+    run_attend(kind, cache, "thd", 16, 2, 3, 64, [127, 128, 129, 159, 160, 161, 191, 192, 193, 255, 256, 257, 289, 383, 384, 385, 449, 481, 511, 512, 513, 1025, 1153],
+               window=window, longest=10 ** 6, seed=window)
+
+
+@pytest.mark.parametrize("kind,cache,requests,kv,group,dim,longest,rest", [
+    (F16, F16, 400, 1, 2, 32, 130000, 3), (F32, BF16, 393, 1, 1, 32, 70001, 200), (BF16, BF16, 49, 8, 2, 40, 4200, 4200), (F32, F32, 130, 3, 2, 64, 5003, 900),
+    (BF16, BF16, 100, 4, 1, 256, 4097, 500), (F16, F16, 700, 1, 17, 32, 6000, 60)])
+def test_attend_long_ones_in_large_batches(kind, cache, requests, kv, group, dim, longest, rest):
+    """Batches that fill the device, whose longest sequence alone is cut into hundreds of shares."""
+    rng = np.random.default_rng(longest)
+    lengths = np.exp(rng.uniform(0, np.log(rest), requests)).astype(int)
+    lengths[requests // 2] = longest
+    lengths[-1] = 0
+    run_attend(kind, cache, "thd", 16, kv, group, dim, lengths.tolist(), longest=longest, seed=requests)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
 @pytest.mark.parametrize("window", [1, 2, 16, 31, 100, 128, 1000, 10 ** 9])
 def test_attend_windows(kind, cache, window):
     run_attend(kind, cache, "htd", 24, 2, 2, 80, [1, 24, 100, 101, 129, 1500, 3001, 0], window=window, seed=window % 89)
