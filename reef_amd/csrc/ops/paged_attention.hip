@@ -810,7 +810,12 @@ Plan plan_of(const reef_paged_attention_desc& d) {
               wide = wide_waves(D, d.type != d.cache.type, few);
     Plan p{};
     p.tiles = tiles;
-    p.wide = all < kGroups && longest <= (int64_t)4 * wide * tile;
+    // Whole sequences where a wide workgroup takes the longest in few rounds.  3 / 4 / 5 rounds against shares, heads of 128, bf16: 48 heads in all
+    // 12 / 15 / 17 us against 13 / 14 / 15 (11 / 13 / 16 against 11 where that is the longest), 256 heads 18 / 24 / 33 against 25 / 30 / 39 (12 / 15 / 17
+    // against 13 / 16 / 17).  Eight wavefronts for heads up to 64 have short rounds: 32-bit queries over bf16, 48 heads, 9 / 10 / 12 against 12 / 12 / 13,
+    // 32-bit caches of 4 query heads, 20 heads, 9 / 11 / 12 (6 rounds: 14) against 12.
+    const int rounds = all >= 192 || (wide == 8 && D <= 64) ? 5 : 3;
+    p.wide = all < kGroups && longest <= (int64_t)rounds * wide * tile;
     p.groups = all;
     // The tiles of a cache head, which read the same, go to one XCD and meet in its L2 (32 query heads a cache head, 4 x 30000 tokens: 45 -> 35 us), and
     // so do the heads of a share where rows end inside lines, if there are shares enough for all XCDs (heads of 80, bf16, 64 x 1000 tokens: 46 -> 39).
