@@ -331,7 +331,9 @@ int reef_ops_paged_attention(const reef_paged_attention_desc* d, const void* que
  * a beam with ended[r] != 0 (ended may be NULL) only end_token, at scores[r].  What is not a finite number or lies below all
  * (NaN, infinities of either sign) counts as -infinity.  Of the beams * vocab offers of a request the first
  * `select` in descending order are given: best (the score), parents (the row r) and tokens, [requests][select].  They are
- * compared in 64 bits; equal ones (those at -infinity among them) go by beam, then token, the lower first.
+ * made and compared in 64 bits; equal ones (those at -infinity among them) go by beam, then token, the lower first.
+ * The logarithm is that of a sum in 64 bits of exponentials in 32: within 2^-22 (2 + log vocab) of the true one, and the same to the bit for
+ * rows of the same values, wherever they lie, so that beams with the same logits and scores offer the same.
  * logits: [rows][logits_stride] of `type`, aligned to their own size.  select: up to 128 and beams * vocab; beams: up to 128;
  * vocab: below 2^24. */
 typedef struct {

@@ -15,16 +15,15 @@ struct SelectArgs {
     const uint8_t* ended;
     float* best;
     int32_t *parents, *tokens;
-    float2* pieces;         // [row][piece]: maximum and sum of exp(x - maximum)
+    double* sums;           // [row][piece]: sum of exp(x - maximum)
+    float* tops;            // [row][piece]: maximum
     int32_t n_pieces;       // of a row
 };
 
-// A piece: 1 KiB of a row, from a line of 128 bytes on.  The first one starts with the line that the row starts in, `lead` values
-// in front of it (rows of an odd length start anywhere).
+// A piece: 1 KiB of a row, counted from its first value.  (Not from a line of 128 bytes on: rows of an odd length start anywhere, and rows that
+// hold the same values have to have the same sums, to the bit.)
 template <class T>
 constexpr int kPiece = 1024 / sizeof(T);
-template <class T>
-__device__ inline int lead_of(const T* row) { return (int)((uintptr_t)row & 127) / (int)sizeof(T); }
 
 // A candidate, in two whole numbers: its score, in an order that whole numbers have too, and its place, beam then token.
 struct Offer {
@@ -41,58 +40,126 @@ __device__ inline double offered(double s) { return s < INFINITY && s > -INFINIT
 
 __device__ inline bool lives(const SelectArgs& a, int64_t row) { return !(a.ended && a.ended[row]); }
 
-// Everything that a choice needs of a row beside single values: of each piece the maximum and the sum over it.  Eight lanes a piece, 16
-// bytes a load, 128 bytes of one line a load and piece; a lane keeps its 64 (32) values, so the row is read once, and
-// the sum needs no rescaling.  Bound by memory: some ten operations a value are 60 % of the time that its bytes take.
+// Eight values a lane, reduced over the wavefront: lanes 8 u .. 8 u + 7 have the u-th.  At each of three steps half of the values go to the other half of
+// the lanes, which leaves one; all of it without LDS (through it row_pieces takes 28.6 instead of 20.9 us).
+template <int CONTROL>
+__device__ inline uint32_t moved(uint32_t x) { return __builtin_amdgcn_update_dpp(0, x, CONTROL, 0xF, 0xF, true); }
+template <int CONTROL>
+__device__ inline float moved(float x) { return __uint_as_float(moved<CONTROL>(__float_as_uint(x))); }
+template <int CONTROL>
+__device__ inline double moved(double x) {
+    const u32x2 w = __builtin_bit_cast(u32x2, x), m = {moved<CONTROL>(w[0]), moved<CONTROL>(w[1])};
+    return __builtin_bit_cast(double, m);
+}
+// The upper half of p's lanes against the lower half of q's: of all lanes, or of each 32.
+__device__ inline void swap_words(uint32_t& p, uint32_t& q, bool halves) {
+    const auto x = halves ? __builtin_amdgcn_permlane32_swap(p, q, false, false) : __builtin_amdgcn_permlane16_swap(p, q, false, false);
+    p = x[0];
+    q = x[1];
+}
+template <class V>
+__device__ inline void swap_lanes(V& p, V& q, bool halves) {
+    if constexpr (sizeof(V) == 4) {
+        uint32_t a = __builtin_bit_cast(uint32_t, p), b = __builtin_bit_cast(uint32_t, q);
+        swap_words(a, b, halves);
+        p = __builtin_bit_cast(V, a);
+        q = __builtin_bit_cast(V, b);
+    } else {
+        u32x2 a = __builtin_bit_cast(u32x2, p), b = __builtin_bit_cast(u32x2, q);
+        for (int i = 0; i < 2; ++i) {
+            uint32_t x = a[i], y = b[i];
+            swap_words(x, y, halves);
+            a[i] = x;
+            b[i] = y;
+        }
+        p = __builtin_bit_cast(V, a);
+        q = __builtin_bit_cast(V, b);
+    }
+}
+template <class V, class Join>
+__device__ inline V over_wave(V (&v)[8], Join join) {
+    constexpr int kTurn8 = 0x128, kMirror8 = 0x141, kNext1 = 0xB1, kNext2 = 0x4E;    // rows of 16 by 8 lanes; lane i to 7 - i, i ^ 1, i ^ 2
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        swap_lanes(v[j], v[j + 4], true);
+        v[j] = join(v[j], v[j + 4]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        swap_lanes(v[j], v[j + 2], false);
+        v[j] = join(v[j], v[j + 2]);
+    }
+    const bool upper = threadIdx.x & 8;
+    const V keep = upper ? v[1] : v[0], give = upper ? v[0] : v[1];
+    V x = join(keep, moved<kTurn8>(give));
+    x = join(x, moved<kMirror8>(x));
+    x = join(x, moved<kNext1>(x));
+    return join(x, moved<kNext2>(x));
+}
+
+// Everything that a choice needs of a row beside single values: of each piece the maximum and the sum over it.  A wavefront has eight pieces, 1 KiB a
+// load; a lane keeps its 64 (32) values, so the row is read once, and the sum needs no rescaling.  A row that does not begin
+// at a line costs a ninth line a load.  Exponentials are those of 32 bits, off by 2^-23 of themselves (exp2) and three roundings of the argument, 2^-22 (1 + |x - maximum|)
+// in all; 64 bits would take 38 us instead of 21 for 48 x 8 rows of 128257 (bf16).  They are added in 64 bits, so that rows
+// that differ in one unlikely token have different sums (in 32 bits, in pieces from a line on: 18.6 us).  Bound by memory: 4.2 TB/s, some fourteen operations a value.
 template <class T>
 __global__ void __launch_bounds__(kThreads) row_pieces(SelectArgs a) {
     constexpr int kE = 16 / sizeof(T);
+    typedef T Raw __attribute__((ext_vector_type(kE), aligned(sizeof(T))));
     const reef_beam_select_desc& d = a.d;
     const int lane = threadIdx.x & 63;
     const int32_t rounds = (a.n_pieces + 7) / 8;
     const int64_t id = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), row = id / rounds;
     if (row >= (int64_t)d.requests * d.beams || !lives(a, row)) return;
-    const int32_t piece = (int32_t)(id - row * rounds) * 8 + (lane >> 3);
+    const int32_t piece0 = (int32_t)(id - row * rounds) * 8, at = piece0 * kPiece<T> + lane * kE;
     const T* x = (const T*)a.logits + row * d.logits_stride;
-    const int32_t p0 = piece * kPiece<T> - lead_of(x), at = p0 + (lane & 7) * kE;
-    float v[8 * kE];
-    if (p0 >= 0 && p0 + kPiece<T> <= d.vocab) {
-        typedef T Raw __attribute__((ext_vector_type(kE)));
+    float v[8][kE];
+    if ((piece0 + 8) * kPiece<T> <= d.vocab) {
         Raw raw[8];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) raw[u] = *(const Raw*)(x + at + u * 8 * kE);
+        for (int u = 0; u < 8; ++u) raw[u] = *(const Raw*)(x + at + u * kPiece<T>);
 #pragma unroll
         for (int u = 0; u < 8; ++u)
 #pragma unroll
-            for (int e = 0; e < kE; ++e) v[u * kE + e] = (float)raw[u][e];
-    } else {                                  // the row begins or ends in here
-        typedef T Raw __attribute__((ext_vector_type(kE)));
+            for (int e = 0; e < kE; ++e) v[u][e] = (float)raw[u][e];
+    } else {                                  // the row ends in here
         Raw raw[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
-            const int32_t i = at + u * 8 * kE;
-            if (i >= 0 && i + kE <= d.vocab) raw[u] = *(const Raw*)(x + i);
-            else if (i > -kE && i < d.vocab) {
+            const int32_t i = at + u * kPiece<T>;
+            if (i + kE <= d.vocab) raw[u] = *(const Raw*)(x + i);
+            else if (i < d.vocab) {
 #pragma unroll
-                for (int e = 0; e < kE; ++e) raw[u][e] = x[max(0, min(i + e, d.vocab - 1))];
+                for (int e = 0; e < kE; ++e) raw[u][e] = x[min(i + e, d.vocab - 1)];
             }
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u)
 #pragma unroll
-            for (int e = 0; e < kE; ++e) v[u * kE + e] = (uint32_t)(at + u * 8 * kE + e) < (uint32_t)d.vocab ? (float)raw[u][e] : -INFINITY;
+            for (int e = 0; e < kE; ++e) v[u][e] = at + u * kPiece<T> + e < d.vocab ? (float)raw[u][e] : -INFINITY;
     }
-    float m = v[0];
+    float top[8];
 #pragma unroll
-    for (int i = 1; i < 8 * kE; ++i) m = fmaxf(m, v[i]);
-    m = fmaxf(m, -INFINITY);                  // (a NaN alone)
-    for (int i = 1; i < 8; i <<= 1) m = fmaxf(m, __shfl_xor(m, i));
-    const float base = m == -INFINITY ? 0.0f : m;
-    float s = 0.0f;
+    for (int u = 0; u < 8; ++u) {
+        top[u] = -INFINITY;                   // (where all are NaN)
 #pragma unroll
-    for (int i = 0; i < 8 * kE; ++i) s += __builtin_amdgcn_exp2f((v[i] - base) * 1.4426950408889634f);
-    for (int i = 1; i < 8; i <<= 1) s += __shfl_xor(s, i);
-    if ((lane & 7) == 0 && piece < a.n_pieces) a.pieces[row * a.n_pieces + piece] = make_float2(m, s);
+        for (int e = 0; e < kE; ++e) top[u] = fmaxf(top[u], v[u][e]);
+    }
+    const float m = over_wave(top, [](float p, float q) { return fmaxf(p, q); });
+    double sum[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const float of = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), u * 8)), base = of == -INFINITY ? 0.0f : of;
+        sum[u] = 0.0;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) sum[u] += (double)__builtin_amdgcn_exp2f((v[u][e] - base) * 1.4426950408889634f);
+    }
+    const double s = over_wave(sum, [](double p, double q) { return p + q; });
+    const int32_t piece = piece0 + (lane >> 3);
+    if ((lane & 7) == 0 && piece < a.n_pieces) {
+        a.sums[row * a.n_pieces + piece] = s;
+        a.tops[row * a.n_pieces + piece] = m;
+    }
 }
 
 constexpr int kChoose = 512, kChooseWaves = kChoose / 64;
@@ -115,15 +182,23 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
     __shared__ int ranks[kChoose];
     __shared__ Offer buffer[kBuffer], kept[kMaxSelect], bound;
     __shared__ int32_t list[kNear];
-    __shared__ float2 near[kNear];
+    __shared__ float near[kNear];
     __shared__ int held, listed, wave_count[kChooseWaves];
 
     const int32_t pieces = d.beams * a.n_pieces;
-    const float2* far = a.pieces + row0 * a.n_pieces;
+    const float* far = a.tops + row0 * a.n_pieces;
+    const double* sums = a.sums + row0 * a.n_pieces;
 #pragma unroll
     for (int k = 0; k < kNear / kChoose; ++k) {
         const int32_t i = k * kChoose + tid;
         if (i < pieces) near[i] = far[i];     // (of an ended beam: never used)
+    }
+    constexpr int kAhead = 4;                 // sums a lane of the wavefront's first beam, on their way beside the maxima
+    double ahead[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+        const int i = k * 64 + lane;
+        ahead[k] = sums[min(min(wave, d.beams - 1) * a.n_pieces + i, pieces - 1)];
     }
     for (int b = tid; b < d.beams; b += kChoose) {
         alive[b] = lives(a, row0 + b);
@@ -140,14 +215,19 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
         if (!alive[b]) continue;
         const int32_t p0 = b * a.n_pieces;
         float m = -INFINITY;
-        for (int i = lane; i < a.n_pieces; i += 64) m = fmaxf(m, piece(p0 + i).x);
+        for (int i = lane; i < a.n_pieces; i += 64) m = fmaxf(m, piece(p0 + i));
         for (int x = 32; x; x >>= 1) m = fmaxf(m, __shfl_xor(m, x));
         const float base = m == -INFINITY ? 0.0f : m;
         double sum = 0.0;
-        for (int i = lane; i < a.n_pieces; i += 64) {
-            const float2 p = piece(p0 + i);
-            sum += (double)(p.y * __builtin_amdgcn_exp2f((p.x - base) * 1.4426950408889634f));
+        // (the same roundings in both places: beams with the same values have the same sum)
+        auto add = [&](int i, double s) { sum = __builtin_fma(s, (double)__builtin_amdgcn_exp2f((piece(p0 + i) - base) * 1.4426950408889634f), sum); };
+        int i = lane;
+        if (b == wave) {
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k, i += 64)
+                if (i < a.n_pieces) add(i, ahead[k]);
         }
+        for (; i < a.n_pieces; i += 64) add(i, sums[p0 + i]);
         for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
         if (lane == 0) lse[b] = (double)m + log(sum);
     }
@@ -156,8 +236,8 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
     auto offer = [&](int b, float x) { return offered(score[b] + ((double)x - lse[b])); };
     auto best_of = [&](int32_t i) -> double {
         const int b = i / a.n_pieces, p = i - b * a.n_pieces;
-        if (alive[b]) return offer(b, piece(i).x);
-        return d.end_token >= 0 && d.end_token < d.vocab && (d.end_token + lead_of(row_of(b))) / kPiece<T> == p ? score[b] : -INFINITY;
+        if (alive[b]) return offer(b, piece(i));
+        return d.end_token >= 0 && d.end_token < d.vocab && d.end_token / kPiece<T> == p ? score[b] : -INFINITY;
     };
     double best[kNear / kChoose], top = -INFINITY;
 #pragma unroll
@@ -279,7 +359,7 @@ __global__ void __launch_bounds__(kChoose) beam_choose(SelectArgs a) {
                 const int32_t i = list[j], b = i / a.n_pieces;
                 const T* row = row_of(b);
                 beam[u] = b;
-                v0[u] = (i - b * a.n_pieces) * kPiece<T> - lead_of(row) + lane;
+                v0[u] = (i - b * a.n_pieces) * kPiece<T> + lane;
 #pragma unroll
                 for (int e = 0; e < kE; ++e) raw[u][e] = row[max(0, min(v0[u] + e * 64, d.vocab - 1))];
                 live[u] = alive[b];
@@ -416,8 +496,7 @@ int run_select(const char* what, SelectArgs a, void* stream) {
     return launch(what, beam_choose<T>, dim3((unsigned)a.d.requests), dim3(kChoose), a, stream);
 }
 
-// (with a lead of up to 127 bytes)
-int32_t pieces_of(const reef_beam_select_desc& d) { return (int32_t)(((int64_t)d.vocab * type_bytes(d.type) + 127 + 1023) / 1024); }
+int32_t pieces_of(const reef_beam_select_desc& d) { return (int32_t)(((int64_t)d.vocab * type_bytes(d.type) + 1023) / 1024); }
 
 int check_select(const char* what, const reef_beam_select_desc* d) {
     if (!d) return refuse(what, "null argument");
@@ -488,7 +567,7 @@ __global__ void __launch_bounds__(kThreads) beam_reorder(ReorderArgs a) {
 
 extern "C" int64_t reef_ops_beam_select_workspace(const reef_beam_select_desc* d) {
     if (check_select("reef_ops_beam_select_workspace", d)) return -1;
-    return (int64_t)d->requests * d->beams * pieces_of(*d) * (int64_t)sizeof(float2);
+    return (int64_t)d->requests * d->beams * pieces_of(*d) * (int64_t)(sizeof(double) + sizeof(float));
 }
 
 extern "C" int reef_ops_beam_select(const reef_beam_select_desc* d, const void* logits, const float* scores, const uint8_t* ended, float* best,
@@ -502,7 +581,8 @@ extern "C" int reef_ops_beam_select(const reef_beam_select_desc* d, const void* 
     const Span out[] = {{best, picks}, {parents, picks}, {tokens, picks}, {workspace, reef_ops_beam_select_workspace(d)}};
     const Span in[] = {{logits, ((n - 1) * d->logits_stride + d->vocab) * type_bytes(d->type)}, {scores, 4 * n}, {ended, ended ? n : 0}};
     if (overlap(out, in)) return refuse(what, "an output overlaps an input");
-    const SelectArgs a{*d, logits, scores, ended, best, parents, tokens, (float2*)workspace, pieces_of(*d)};
+    double* const sums = (double*)workspace;
+    const SelectArgs a{*d, logits, scores, ended, best, parents, tokens, sums, (float*)(sums + n * pieces_of(*d)), pieces_of(*d)};
     const int64_t need = reef_ops_beam_select_workspace(d);
     if (!rows16(workspace) || workspace_bytes < need)
         return refuse(what, "a workspace of %lld bytes on 16 is needed, %lld are given", (long long)need, (long long)workspace_bytes);

@@ -739,3 +739,44 @@ def test_calls_on_two_streams_do_not_disturb_each_other():
                 np.testing.assert_array_equal(a, b)
     for j in jobs:
         hip("hipStreamDestroy", j["stream"])
+
+
+# ---- equal and nearly equal offers of different beams ----------------------------------------------
+@pytest.mark.parametrize("kind,beams,vocab,n", [(F32, 4, 30522, 8), (F32, 4, 50257, 8), (F16, 20, 30523, 16), (BF16, 4, 128257, 16), (F32, 4, 701, 5),
+                                                (BF16, 33, 1001, 32), (F32, 12, 70001, 32)])
+def test_select_beams_with_the_same_logits(kind, beams, vocab, n):
+    """Beams that hold the same logits and scores offer the same wherever their rows lie: the lowest beam goes first, and neither the choice nor
+    a bit of the scores depends on the address of the logits."""
+    rng = np.random.default_rng(vocab)
+    requests = 3
+    one = R.encode((rng.standard_normal((requests, vocab)) * 2.5).astype(np.float32), kind)
+    raw = np.repeat(one, beams, axis=0).ravel()
+    scores = np.repeat(-rng.random(requests), beams).astype(np.float32)
+    x = R.decode(one, kind)
+    m = x.max(1, keepdims=True)
+    offers = np.repeat(scores[::beams, None].astype(np.float64) + (x - (m + np.log(np.exp(x - m).sum(1, keepdims=True)))), beams, axis=0)
+    offers = offers.reshape(requests, beams * vocab)
+    at = np.argsort(-offers, axis=1, kind="stable")[:, :n]
+    d = B.BeamSelectDesc(kind, requests, beams, vocab, n, -1, vocab)
+    first = None
+    for ahead in (0, 1, 5, 31):
+        dev = up(np.concatenate([np.zeros(ahead, raw.dtype), raw]))
+        best, parents, tokens, work = B.DeviceBuffer(4 * requests * n), B.DeviceBuffer(4 * requests * n), B.DeviceBuffer(4 * requests * n), B.DeviceBuffer(
+            B.ops_beam_select_workspace(d))
+        ok(B.ops_beam_select(d, dev.ptr.value + ahead * raw.itemsize, up(scores), None, best, parents, tokens, work))
+        np.testing.assert_array_equal(parents.to_array(np.int32).reshape(requests, n), at // vocab + np.arange(requests)[:, None] * beams)
+        np.testing.assert_array_equal(tokens.to_array(np.int32).reshape(requests, n), at % vocab)
+        bits = best.to_array(np.uint32)
+        first = bits if first is None else first
+        np.testing.assert_array_equal(bits, first)
+
+
+@pytest.mark.parametrize("kind,vocab", [(F32, 30522), (F16, 30523), (BF16, 128257), (F32, 999)])
+def test_select_beams_that_differ_in_one_token(kind, vocab):
+    """Beams alike but for one unlikely token: their offers lie 1e-9 to 1e-6 apart, and 64 bits tell them apart."""
+    rng = np.random.default_rng(vocab)
+    x = np.tile((rng.standard_normal(vocab) * 2).astype(np.float32), (8, 1))
+    for b, more in enumerate((7, 3, 5, 0, 2, 6, 1, 4)):
+        x[b, vocab // 3] = -4 + more / 64
+    run_select(kind, 1, 8, x, 24, scores=[-1.0] * 8)
+    run_select(kind, 2, 4, x, 10, scores=[-1.0] * 8)
