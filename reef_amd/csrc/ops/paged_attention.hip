@@ -254,7 +254,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     constexpr bool kNarrow = sizeof(C) == 2;                  // products in the cache's 16-bit type
     constexpr bool kHalf = __is_same(C, _Float16);
     constexpr int kTermsQ = sizeof(Q) == sizeof(C) ? 1 : 3, kTermsP = sizeof(Q) == 2 ? 2 : 3;
-    constexpr float kShift = kHalf ? 14.0f : 0.0f;            // weights are up to 2^kShift
+    constexpr float kGrow = kHalf ? 0x1p14f : 1.0f;           // weights are up to that
     constexpr int kPiece = 16 / sizeof(C);                    // values of 16 bytes
     constexpr int kTile = tile_of(sizeof(C)), kSub = kTile / 16;
     constexpr int kSteps = DP / (4 * kPiece);                 // pieces of a key row a lane
@@ -573,9 +573,9 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
                     top = fmaxf(top, s[t][i]);
                 }
             top = over_rows_max(top);
-            const float base = top == -INFINITY ? 0.0f : top - kShift;
+            const float base = top == -INFINITY ? 0.0f : top;
             if (__builtin_amdgcn_ballot_w64(top != m)) {
-                const float f = __builtin_amdgcn_exp2f(m - kShift - base);
+                const float f = __builtin_amdgcn_exp2f(m - base);
                 l *= f;
 #pragma unroll
                 for (int c = 0; c < kSlabs; ++c)
@@ -588,6 +588,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - base);
+                    if constexpr (kHalf) s[t][i] *= kGrow;    // (not by the exponent: base - 14 would be rounded where scores are large)
                     l += s[t][i];
                 }
             // values of places that are no tokens may be anything, and 0 times that too
@@ -661,7 +662,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
             }
         }
     } else {
-        l = over_rows_sum(l);
+        l = over_rows_sum(l) * (1.0f / kGrow);
         if (n < heads) {
 #pragma unroll
             for (int c = 0; c < kSlabs; ++c)
@@ -670,10 +671,11 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
 #pragma unroll
                     for (int e = 0; e < kV; e += 4) {
                         f32x4 x = {o[c][e][i], o[c][e + 1][i], o[c][e + 2][i], o[c][e + 3][i]};
+                        if constexpr (kHalf) x *= 1.0f / kGrow;
                         *(f32x4*)&o_part[wave][n][(c * 16 + g * 4 + i) * kV + e] = x;
                     }
             if (g == 0) {
-                m_part[wave][n] = m - kShift;
+                m_part[wave][n] = m;
                 l_part[wave][n] = l;
             }
         }

@@ -780,3 +780,42 @@ def test_select_beams_that_differ_in_one_token(kind, vocab):
         x[b, vocab // 3] = -4 + more / 64
     run_select(kind, 1, 8, x, 24, scores=[-1.0] * 8)
     run_select(kind, 2, 4, x, 10, scores=[-1.0] * 8)
+
+
+# ---- scores and queries at the ends of their range ---------------------------------------------------
+def one_request(kind, cache, keys, values, q, scale):
+    """One request, one block: host values [tokens][dim], queries [heads][dim] -> out [heads][dim], lse [heads]."""
+    t, dim = keys.shape
+    heads = q.shape[0]
+    d = B.PagedAttentionDesc(B.CacheLayout(cache, 1, t, 1, dim, t * dim, dim, dim), kind, 1, heads, 1, 1, t, 0, scale, heads * dim, dim, heads * dim, dim)
+    out, ls = B.DeviceBuffer(heads * dim * (4 if kind == F32 else 2)), B.DeviceBuffer(4 * heads)
+    n = B.ops_paged_attention_workspace(d)
+    ok(B.ops_paged_attention(d, up(R.encode(q, kind)), up(R.encode(keys, cache)), up(R.encode(values, cache)), ints([0]), ints([t]), out, ls,
+                             B.DeviceBuffer(n) if n else None))
+    return R.decode(out.to_array(R.np_type(kind)).reshape(heads, dim), kind), ls.to_array()
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("tokens", [40, 200, 3000])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attend_scores_of_any_size(kind, cache, tokens, sign):
+    """Scores from 2^22 to 2^31, where 32 bits keep no fractions: the largest takes everything, two equal ones half each.  One dimension alone
+    is not zero and its products are exact, so all other weights are 0 and the two are 1: the result is the mean of two values but for a
+    rounding of their sum and of the output.  lse: six roundings to 32 bits, each of at most 2^-24 of a number of its size."""
+    rng = np.random.default_rng(tokens)
+    dim = 64
+    values = rng.standard_normal((tokens, dim)).astype(np.float32)
+    v = R.decode(R.encode(values, cache), cache)
+    for binade in range(22, 31):
+        for more in (1.0, 1.25, 1.5, 1.75):
+            keys, q = np.zeros((tokens, dim), np.float32), np.zeros((2, dim), np.float32)
+            win = rng.permutation(tokens)[:2]
+            # (sign < 0: scores are negative, the largest is the one next to zero)
+            keys[:, 5] = 4096 * (rng.integers(1, 5, tokens) / 8 if sign > 0 else 1 + rng.integers(3, 8, tokens) / 8)
+            keys[win, 5] = 4096
+            q[0, 5], q[1, 5] = sign * 4096 * more, sign * 2048 * more
+            out, ls = one_request(kind, cache, keys, values, q, 2.0 ** (binade - 24))
+            want = (v[win[0]] + v[win[1]]) / 2
+            assert (np.abs(out - want) <= HALF[kind] * np.abs(want) + 2.0 ** -23 * np.abs(v[win]).max(0) + (2.0 ** -25 if kind == F16 else 0)).all(), (binade, more)
+            s = np.array([1, 0.5]) * sign * more * 2.0 ** binade
+            assert (np.abs(ls - (s + np.log(2))) <= 8 * 2.0 ** -24 * np.abs(s) + 2.0 ** -20).all(), (binade, more)
