@@ -3,6 +3,7 @@
 #include <cmath>
 
 #include "ops_common.h"
+#include "paged_shares.h"
 
 namespace {
 using namespace reef_ops;
@@ -35,8 +36,6 @@ struct Args {
     int32_t units, together;   // workgroups in `units` groups of `together`, each group on one XCD
 };
 
-constexpr int32_t kLeast = 128;              // tokens a share at least
-
 struct Share {
     int32_t request, number, first, count;   // the number-th of `count` shares of the request, which start with share `first` of all
 };
@@ -46,23 +45,9 @@ __device__ inline int32_t seen_tokens(const Args& a, int32_t r) {
     return a.d.window && held > a.d.window ? a.d.window : held;
 }
 
-// Sequences are cut into shares of at most so many tokens, equal ones, so that long sequences among short ones, or few of them, keep
-// the device as busy as many.  With the sum of the lengths rounded up by more than its 32-bit additions lose,
-// sum ceil(seen / tokens) <= budget + requests, the size of the grid.  Up to kFewRequests every workgroup adds up the lengths for
-// itself, more are listed by a launch ahead (4096 requests of 8 heads would be read by 33000 workgroups).
+// Up to kFewRequests every workgroup adds up the lengths for itself, more are listed by a launch ahead (4096 requests of 8 heads would be
+// read by 33000 workgroups).
 constexpr int32_t kFewRequests = 256, kListHead = 1;
-// (2^24 requests are 2^14 additions a thread, each off by 2^-24 of the sum at most)
-__device__ inline int32_t tokens_of(float total, int32_t budget) {
-    const float each = total * 1.02f / (float)budget;
-    return each < 2.0e9f ? max(kLeast, ((int32_t)each + 32) / 32 * 32) : INT32_MAX;
-}
-__device__ inline int32_t shares_of(int32_t n, int32_t tokens) { return max(1, (int32_t)(((uint32_t)n + tokens - 1) / (uint32_t)tokens)); }
-// Where share `number` of `count` begins among n tokens: whole tiles of 32, one more for the first ones.  (None is
-// empty: n > 128 (count - 1), so there are 4 count - 3 tiles or more.)
-__device__ inline int32_t begin_of(int32_t n, int32_t number, int32_t count) {
-    const int32_t tiles = (int32_t)(((uint32_t)n + 31) / 32), each = tiles / count;
-    return (number * each + min(number, tiles - each * count)) * 32;
-}
 
 // Adds up over the workgroup, exclusively; *all: the sum.
 template <int WAVES>
@@ -307,7 +292,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
         return lane < kTile && t < end ? table[divided((uint32_t)t, a.block)] : -1;
     };
     constexpr int32_t kStride = WAVES * kTile;
-    int32_t t0 = begin + wave * kTile;
+    int32_t t0 = first_of(begin, end, wave * kTile);
     // (asked for ahead of the queries: keys and values wait for them)
     int32_t entry = t0 < end ? entry_of(t0) : -1;
 

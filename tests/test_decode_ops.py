@@ -236,3 +236,55 @@ def test_tensors_of_a_torch_that_came_later_are_refused():
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300,
                        cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode == 0, r.stderr
+
+
+SHARES = r"""
+#include <cstdio>
+#include "paged_shares.h"
+using namespace reef_ops;
+// What the wavefronts of the kernel walk over, for one sequence alone: is every token of its window seen, once, and no other?
+int main() {
+    const int64_t top = 1ll << 31;
+    const int64_t lengths[] = {1, 2, 31, 32, 33, 127, 128, 129, 500, 4097, 70001, top - 1, top - 2, top - 31, top - 32, top - 33, top - 128, top - 479, top - 480, top - 512, top - 513};
+    const int32_t windows[] = {0, 1, 2, 31, 33, 100, 128, 257, 479, 480, 481, 512, 4000, 100000};
+    const int32_t budgets[] = {0, 1, 3, 64, 448, 896};
+    for (int64_t length : lengths)
+        for (int32_t window : windows)
+            for (int32_t budget : budgets)
+                for (int waves : {4, 8, 16})
+                    for (int tile : {16, 32}) {
+                        if (window == 0 && length > 100000 && (budget != 448 || waves != 4 || tile != 32)) continue;    // (many tiles)
+                        const int32_t held = (int32_t)length, first = window && held > window ? held - window : 0, n = held - first;
+                        const int32_t count = budget ? shares_of(n, tokens_of((float)n, budget)) : 1, stride = waves * tile;
+                        if (budget && count > budget + 1) return std::printf("%d shares\n", count), 1;
+                        int64_t seen = 0;
+                        for (int32_t number = 0; number < count; ++number) {
+                            const int32_t begin = first + begin_of(n, number, count), end = number + 1 < count ? first + begin_of(n, number + 1, count) : held;
+                            if (begin < first || begin >= end || end > held) return std::printf("share %d of %d: %d %d of %d\n", number, count, begin, end, held), 1;
+                            for (int wave = 0; wave < waves; ++wave) {
+                                int32_t t0 = first_of(begin, end, wave * tile);
+                                while (t0 < end) {
+                                    if (t0 < begin || (t0 - begin) % stride != wave * tile) return std::printf("wavefront %d at %d of %d .. %d\n", wave, t0, begin, end), 1;
+                                    seen += end - t0 < tile ? end - t0 : tile;
+                                    if (t0 >= end - stride) break;
+                                    t0 += stride;
+                                }
+                            }
+                        }
+                        if (seen != n) return std::printf("%lld of %d seen\n", (long long)seen, n), 1;
+                    }
+    return 0;
+}
+"""
+
+
+def test_shares_cover_sequences_up_to_the_longest(tmp_path):
+    """The kernel's own arithmetic, on the host, for lengths just below 2^31 too."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    (tmp_path / "shares.cpp").write_text(SHARES)
+    subprocess.check_call(["g++", "-O2", "-fwrapv", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", "-I" + os.path.join(root, "reef_amd", "csrc", "ops"),
+                           str(tmp_path / "shares.cpp"), "-o", str(tmp_path / "shares")])
+    r = subprocess.run([str(tmp_path / "shares")], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stdout

@@ -819,3 +819,34 @@ def test_attend_scores_of_any_size(kind, cache, tokens, sign):
             assert (np.abs(out - want) <= HALF[kind] * np.abs(want) + 2.0 ** -23 * np.abs(v[win]).max(0) + (2.0 ** -25 if kind == F16 else 0)).all(), (binade, more)
             s = np.array([1, 0.5]) * sign * more * 2.0 ** binade
             assert (np.abs(ls - (s + np.log(2))) <= 8 * 2.0 ** -24 * np.abs(s) + 2.0 ** -20).all(), (binade, more)
+
+
+# ---- the longest sequences ---------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("group", [1, 4, 20])
+def test_attend_windows_of_sequences_just_below_2_31(kind, cache, group):
+    """A table whose entries all name one large block holds 2^31 - 2 tokens: places near the end of 32 bits, through all wavefronts."""
+    bs, entries, dim = 1549411, 1386, 8
+    assert bs * entries == 2 ** 31 - 2
+    rng = np.random.default_rng(group)
+    raw = [np.zeros((bs, dim), R.np_type(cache)) for _ in range(2)]
+    for r in raw:
+        r[-6000:] = R.encode(rng.standard_normal((6000, dim)).astype(np.float32), cache)
+    k, v = (up(r) for r in raw)
+    table = ints(np.zeros(entries))
+    q = R.encode(rng.standard_normal((1, group, dim)).astype(np.float32), kind)
+    out, ls = B.DeviceBuffer(group * dim * (4 if kind == F32 else 2)), B.DeviceBuffer(4 * group)
+    for window in (1, 33, 100, 479, 481, 700, 5000):
+        d = B.PagedAttentionDesc(B.CacheLayout(cache, 1, bs, 1, dim, 0, dim, 0), kind, 1, group, entries, entries, 0, window, 0.4, group * dim, dim, group * dim, dim)
+        n = B.ops_paged_attention_workspace(d)
+        for length in (2 ** 31 - 2, 2 ** 31 - 1, 2 ** 31 - 100):
+            held = min(length, bs * entries)
+            ok(B.ops_paged_attention(d, up(q), k, v, table, ints([length]), out, ls, B.DeviceBuffer(n) if n else None))
+            at = np.arange(held - window, held) % bs
+            vv = R.decode(raw[1][at], cache)
+            want, want_lse, tol, tol_lse = R.attend(R.decode(q[0], kind), R.decode(raw[0][at], cache)[None], vv[None], 0.4)
+            got, got_lse = R.decode(out.to_array(R.np_type(kind)).reshape(group, dim), kind), ls.to_array()
+            # (weights of 16-bit types as two terms, as in run_attend)
+            extra = (2 * 2.0 ** -16 + (2.0 ** -24 * window if cache == F16 else 0)) * np.abs(vv).max() if cache != F32 and kind != F32 else 0
+            assert (np.abs(got - want) <= tol + extra + HALF[kind] * np.abs(want) + (2.0 ** -25 if kind == F16 else 0)).all(), (window, length)
+            assert (np.abs(got_lse - want_lse) <= tol_lse).all(), (window, length)
