@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     int32_t entry = t0 < end ? entry_of(t0) : -1;
 
     // the queries: head n, the pieces that this lane's keys have
-    float scale = d.scale * kLog2e;
+    float scale = d.scale * kLog2e, shrink = 1.0f;           // scores: products * shrink * scale
     u32x4 q[FEW ? 1 : kTermsQ][FEW ? 1 : kSteps];
     float fq[FEW ? FEW : 1][kSteps][4];
     if constexpr (FEW) {                      // (for each head)
@@ -339,9 +339,13 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
                     for (int w = 0; w < kWords; ++w) top = fmaxf(top, fabsf(__uint_as_float(raw[s][w])));
                 top = over_rows_max(top);
                 if (top > 0.0f && top < INFINITY) {
-                    const int by = max(-100, min(100, 13 - (int)((__float_as_uint(top) >> 23) - 127)));
+                    // (-114 .. 126, so both factors are normal numbers)
+                    const int by = min(126, 13 - (int)((__float_as_uint(top) >> 23) - 127));
                     grow = __uint_as_float((uint32_t)(127 + by) << 23);
-                    scale *= __uint_as_float((uint32_t)(127 - by) << 23);
+                    const float back = __uint_as_float((uint32_t)(127 - by) << 23);
+                    // One factor where it is one: large queries and a large scale may pass 32 bits together where a product is 0.
+                    if (back > 1.0f && fabsf(scale) > 1.0f) shrink = back;
+                    else scale *= back;
                 }
             }
 #pragma unroll
@@ -553,6 +557,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
             for (int t = 0; t < kSub; ++t)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
+                    if constexpr (kHalf && kTermsQ > 1) s[t][i] *= shrink;
                     s[t][i] *= scale;
                     if (!all && !(there >> (t * 16 + g * 4 + i) & 1)) s[t][i] = -INFINITY;
                     top = fmaxf(top, s[t][i]);

@@ -850,3 +850,21 @@ def test_attend_windows_of_sequences_just_below_2_31(kind, cache, group):
             extra = (2 * 2.0 ** -16 + (2.0 ** -24 * window if cache == F16 else 0)) * np.abs(vv).max() if cache != F32 and kind != F32 else 0
             assert (np.abs(got - want) <= tol + extra + HALF[kind] * np.abs(want) + (2.0 ** -25 if kind == F16 else 0)).all(), (window, length)
             assert (np.abs(got_lse - want_lse) <= tol_lse).all(), (window, length)
+
+
+@pytest.mark.parametrize("kind,cache", [(F32, F16), (F32, BF16), (F32, F32)])
+def test_attend_queries_far_from_one(kind, cache):
+    run_attend(kind, cache, "thd", 16, 2, 4, 64, [300, 40, 2500], grow=1e35, scale=3e-36, seed=1)
+    run_attend(kind, cache, "thd", 16, 2, 4, 64, [300, 40, 2500], grow=1e-33, scale=1e32, seed=2)
+    if cache == F16:
+        # products are made on queries brought near 1, so that nothing between runs over or under either
+        run_attend(kind, cache, "thd", 16, 2, 4, 64, [300, 40, 2500], grow=5e37, scale=2e-38, seed=3)
+        run_attend(kind, cache, "thd", 16, 2, 4, 64, [300, 40, 2500], grow=1e-37, scale=2e36, seed=4)
+        run_attend(kind, cache, "thd", 16, 2, 4, 64, [300, 40, 2500], grow=1e-40, scale=2e38, seed=5)
+        rng = np.random.default_rng(6)
+        values = rng.standard_normal((50, 64)).astype(np.float32)
+        for big in (1e38, 1e-38):
+            for scale in (1e6, 2e38):
+                out, ls = one_request(kind, cache, np.zeros((50, 64), np.float32), values, np.full((2, 64), big, np.float32), scale)
+                want, want_lse, tol, tol_lse = R.attend(np.zeros((2, 64)), np.zeros((1, 50, 64)), R.decode(R.encode(values, cache), cache)[None], 1.0)
+                assert (np.abs(out - want) <= tol + HALF[kind] * np.abs(want)).all() and (np.abs(ls - want_lse) <= tol_lse).all()
