@@ -232,7 +232,7 @@ constexpr int tile_of(int bytes) { return bytes == 2 ? 32 : 16; }
 // 16-bit caches use 16x16x32 products.  Weights are two terms of the cache's type (a single one would put 2^-9 on bf16 outputs that are
 // off by 2^-9 at most from their own rounding); 32-bit queries are three terms, and so are their weights, which keeps all 24
 // bits at a fifth of the time of 16x16x4 products on 32-bit values.  Terms of fp16 need room below: queries are scaled by a power of
-// two to 2^13 a head, weights are up to 2^14.  32-bit caches use the 16x16x4 products, but for FEW query heads a cache head, where
+// two to 2^13 a head (for bf16 those below 2^-100 to that), weights are up to 2^14.  32-bit caches use the 16x16x4 products, but for FEW query heads a cache head, where
 // these would be nearly all padding: there the same pieces are multiplied and added by the lanes, a head after the other.
 template <class Q, class C, int DP, bool WHOLE, int WAVES, int FEW>
 __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) paged_attention(Args a) {
@@ -330,23 +330,20 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
 #pragma unroll
             for (int s = 0; s < kSteps; ++s) q[0][s] = {raw[s][0], raw[s][1], raw[s][2], raw[s][3]};
         } else {
-            float grow = 1.0f;
-            if constexpr (kHalf) {
-                float top = 0.0f;
+            float grow = 1.0f, top = 0.0f;
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s)
+            for (int s = 0; s < kSteps; ++s)
 #pragma unroll
-                    for (int w = 0; w < kWords; ++w) top = fmaxf(top, fabsf(__uint_as_float(raw[s][w])));
-                top = over_rows_max(top);
-                if (top > 0.0f && top < INFINITY) {
-                    // (-114 .. 126, so both factors are normal numbers)
-                    const int by = min(126, 13 - (int)((__float_as_uint(top) >> 23) - 127));
-                    grow = __uint_as_float((uint32_t)(127 + by) << 23);
-                    const float back = __uint_as_float((uint32_t)(127 - by) << 23);
-                    // One factor where it is one: large queries and a large scale may pass 32 bits together where a product is 0.
-                    if (back > 1.0f && fabsf(scale) > 1.0f) shrink = back;
-                    else scale *= back;
-                }
+                for (int w = 0; w < kWords; ++w) top = fmaxf(top, fabsf(__uint_as_float(raw[s][w])));
+            top = over_rows_max(top);
+            if (top > 0.0f && top < INFINITY) {
+                // (-114 .. 126, so both factors are normal numbers; bf16 lacks room below 2^-133 only, and keys may be 2^127)
+                const int power = (int)(__float_as_uint(top) >> 23) - 127, by = kHalf ? min(126, 13 - power) : max(0, -100 - power);
+                grow = __uint_as_float((uint32_t)(127 + by) << 23);
+                const float back = __uint_as_float((uint32_t)(127 - by) << 23);
+                // One factor where it is one: large queries and a large scale may pass 32 bits together where a product is 0.
+                if (back > 1.0f && fabsf(scale) > 1.0f) shrink = back;
+                else scale *= back;
             }
 #pragma unroll
             for (int s = 0; s < kSteps; ++s)

@@ -868,3 +868,15 @@ def test_attend_queries_far_from_one(kind, cache):
                 out, ls = one_request(kind, cache, np.zeros((50, 64), np.float32), values, np.full((2, 64), big, np.float32), scale)
                 want, want_lse, tol, tol_lse = R.attend(np.zeros((2, 64)), np.zeros((1, 50, 64)), R.decode(R.encode(values, cache), cache)[None], 1.0)
                 assert (np.abs(out - want) <= tol + HALF[kind] * np.abs(want)).all() and (np.abs(ls - want_lse) <= tol_lse).all()
+
+
+@pytest.mark.parametrize("kind,cache", [(F32, F16), (F32, BF16), (F32, F32)])
+@pytest.mark.parametrize("group", [1, 4, 8])
+@pytest.mark.parametrize("grow,scale", [(1e-35, 1e34), (1e-37, 2e36), (1e-38, 2e37), (1e-39, 2e38)])
+def test_attend_queries_next_to_nothing(kind, cache, group, grow, scale):
+    """Queries that are subnormal, or whose parts in the cache's type would be."""
+    run_attend(kind, cache, "thd", 16, 2, group, 64, [300, 40, 2500], grow=grow, scale=scale, seed=4)
+
+
+def test_attend_small_queries_over_large_keys():
+    run_attend(F32, BF16, "thd", 16, 2, 4, 64, [300, 40, 2500], grow=1e-34, size=1e34, scale=0.125, seed=4)
