@@ -765,7 +765,7 @@ int check(const char* what, const reef_paged_attention_desc* d) {
     if (d->max_blocks < 1 || d->table_stride < d->max_blocks || (int64_t)d->max_blocks * d->cache.block_size >= 1ll << 31)
         return refuse(what, "bad table: rows of %d entries, %d apart, blocks of %d tokens", d->max_blocks, d->table_stride, d->cache.block_size);
     if (d->longest < 0 || d->window < 0) return refuse(what, "negative length or window");
-    if (!std::isfinite(d->scale)) return refuse(what, "scale is not a finite number");
+    if (!std::isfinite(d->scale * kLog2e)) return refuse(what, "scale %g is not a finite number, or not one as a power of two", (double)d->scale);
     const int bytes = type_bytes(d->type);
     if (!stride16(d->requests, d->query_stride, bytes) || !stride16(d->requests, d->out_stride, bytes) || !stride16(d->heads, d->query_head_stride, bytes) ||
         !stride16(d->heads, d->out_head_stride, bytes))

@@ -288,3 +288,13 @@ def test_shares_cover_sequences_up_to_the_longest(tmp_path):
                            str(tmp_path / "shares.cpp"), "-o", str(tmp_path / "shares")])
     r = subprocess.run([str(tmp_path / "shares")], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0, r.stdout
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3.4e38, float("-inf")])
+def test_attention_scales_that_are_no_32_bit_number_as_powers_of_two(scale):
+    """exp(s) is 2^(s log2 e): the factor of the two has to be finite, or scores of 0 would be NaN."""
+    d = attention(layout(), scale=scale)
+    refused(call("paged_attention", d, *[P] * 8, 1 << 40), "scale")
+    with pytest.raises(B.ReefError):
+        B.ops_paged_attention_workspace(d)
+    assert B.ops_paged_attention_workspace(attention(layout(), scale=1.7e38)) >= 0
