@@ -248,7 +248,7 @@ int reef_ops_release(void);
  * (requests, tokens or rows 0) succeeds.  Anything refused is Status::Fail with a message, and nothing is launched.
  * The workspace of a call is the caller's: uninitialised memory, 16-byte aligned, that no other call uses at the
  * same time (two graphs that may run at once need one each).  Its size depends on the descriptor alone.
- * Results depend neither on what else runs nor on earlier calls, bit for bit. */
+ * Results depend neither on what else runs nor on earlier calls, bit for bit (but for one slot named twice, below). */
 
 /* Types of values. */
 enum { REEF_TYPE_F32 = 0, REEF_TYPE_F16 = 1, REEF_TYPE_BF16 = 2 };
@@ -294,7 +294,8 @@ int reef_ops_block_plan(const reef_block_plan_desc* d, const int32_t* cached, co
 
 /* Puts token t's key and value rows ([tokens][kv_heads][head_dim], strides in elements, multiples of 16 bytes, rows 16-byte
  * aligned) at slots[t] of the pools, rounded to the cache's type (to nearest, ties to even).  A slot that is not one of the pool's is skipped.
- * Two tokens with one slot: one of the two, not said which.  type: the cache's, or REEF_TYPE_F32. */
+ * Slots that are not skipped are distinct.  Where two tokens name one, its rows are pieces of 16 bytes of either token's, not said which and
+ * not the same from call to call.  type: the cache's, or REEF_TYPE_F32. */
 typedef struct {
     reef_cache_layout cache;
     int32_t type, tokens;

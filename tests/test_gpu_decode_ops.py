@@ -880,3 +880,32 @@ def test_attend_queries_next_to_nothing(kind, cache, group, grow, scale):
 
 def test_attend_small_queries_over_large_keys():
     run_attend(F32, BF16, "thd", 16, 2, 4, 64, [300, 40, 2500], grow=1e-34, size=1e34, scale=0.125, seed=4)
+
+
+# ---- slots named twice -------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,cache", PAIRS)
+def test_append_of_two_tokens_with_one_slot(kind, cache):
+    """Whatever 16 bytes of the slot hold belongs to one of the two tokens, in their place; all other slots are as ever."""
+    bs, kv, dim, tokens = 16, 3, 72, 600
+    rng = np.random.default_rng(0)
+    pools = Pools(cache, 64, bs, kv, dim)
+    rows = R.encode(rng.standard_normal((tokens, 2, kv, dim)).astype(np.float32), kind)
+    slots = rng.permutation(64 * bs)[:tokens]
+    twice = rng.permutation(tokens)[:100].reshape(2, 50)
+    slots[twice[1]] = slots[twice[0]]
+    row = 2 * kv * dim
+    dev = up(rows)
+    ok(B.ops_cache_append(B.CacheAppendDesc(pools.layout, kind, tokens, row, dim, row, dim), dev.ptr.value, dev.ptr.value + kv * dim * rows.itemsize, ints(slots), *pools.dev))
+    cast = rows if kind == cache else R.encode(rows.astype(np.float32), cache)
+    per = 16 // cast.itemsize
+    for i, got in enumerate(pools.fetch()):
+        have, before = pools.view(got).reshape(64 * bs, kv, dim), pools.view(pools.raw[i]).reshape(64 * bs, kv, dim)
+        named = set(slots.tolist())
+        for s in range(64 * bs):
+            if s not in named:
+                np.testing.assert_array_equal(have[s], before[s])
+                continue
+            who = np.flatnonzero(slots == s)
+            pieces = have[s].reshape(kv, dim // per, per)
+            fits = [(pieces == cast[t, i].reshape(pieces.shape)).all(-1) for t in who]
+            assert np.any(fits, axis=0).all()
