@@ -4,12 +4,14 @@ The library is the product; this module only marshals arguments.  It raises if
 the library has not been built -- there is no fallback path.
 """
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
 import sys
 
 import numpy as np
 
-from .paths import LIB_PATH
+from .paths import LIB_PATH, OPERANDS_PATH
 
 STATUS = {0: "Succ", 1: "Fail", 2: "NotFound", 3: "OutOfRange", 4: "Full"}
 BASE, TRANS, HYBRID = 0, 1, 2
@@ -499,37 +501,70 @@ class BeamReorderDesc(ctypes.Structure):
     _fields_ = [("cache", CacheLayout)] + _fields(("rows", "table_rows", "max_blocks", "table_stride", "out_stride", "layers"), ("layer_stride",))
 
 
-# pointers behind the descriptor (workspaces go with their size)
-_OPS_POINTERS = {"block_plan": 8, "cache_append": 5, "paged_attention": 7, "beam_select": 6, "beam_reorder": 8}
-_OPS_WORKSPACE = ("paged_attention", "beam_select")
+# What each pointer behind the descriptor points at, for operands that are tensors (csrc/python/operands.cpp): int32, bytes, anything, values
+# of the descriptor's type or of its cache's; _S: the descriptor has strides for all but the last dimension.
+_F32, _INTS, _BYTES, _ANY, _ROWS, _CACHE, _S = 0, 3, 4, 5, 6, 7, 8
+_OPS = {
+    "block_plan": (BlockPlanDesc, (_INTS, _INTS, _INTS, _INTS | _S, _INTS, _INTS, _INTS, _INTS)),
+    "cache_append": (CacheAppendDesc, (_ROWS | _S, _ROWS | _S, _INTS, _CACHE | _S, _CACHE | _S)),
+    "paged_attention": (PagedAttentionDesc, (_ROWS | _S, _CACHE | _S, _CACHE | _S, _INTS | _S, _INTS, _ROWS | _S, _F32, _ANY)),
+    "beam_select": (BeamSelectDesc, (_ROWS | _S, _F32, _BYTES, _F32, _INTS, _INTS, _ANY)),
+    "beam_reorder": (BeamReorderDesc, (_INTS, _INTS, _INTS | _S, _INTS, _INTS | _S, _INTS, _CACHE | _S, _CACHE | _S)),
+}
+_OPS_WORKSPACE = ("paged_attention", "beam_select")     # (workspaces go with their size)
 _ops = {}
+_calls = {}
+_operands = None        # the extension
+_call = None
 
 
 def _op(name):
+    """The C function, with addresses as they are."""
     f = _ops.get(name)
     if f is None:
         f = getattr(lib(), "reef_ops_" + name)
         p = ctypes.c_void_p
-        f.argtypes = [p] * (1 + _OPS_POINTERS[name]) + ([p, ctypes.c_int64] if name in _OPS_WORKSPACE else []) + [p]
+        f.argtypes = [p] * (1 + len(_OPS[name][1])) + ([ctypes.c_int64, p] if name in _OPS_WORKSPACE else [p])
         _ops[name] = f
     return f
 
 
-# address of an operand, by its type
-_address = {type(None): lambda x: None, int: lambda x: x, DeviceBuffer: lambda x: x.ptr}
+def _ready(name):
+    """The same for operands as Python has them."""
+    global _operands, _call
+    if _operands is None:
+        if not os.path.exists(OPERANDS_PATH):
+            raise RuntimeError("reef_operands.so is not built: run __graft_entry__.build() (make -C reef_amd/csrc)")
+        loader = importlib.machinery.ExtensionFileLoader("reef_operands", OPERANDS_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("reef_operands", loader))
+        loader.exec_module(module)
+        module.learn(_at)
+        _operands, _call = module, module.call
+    desc, kinds = _OPS[name]
+    at = desc.type.offset if hasattr(desc, "type") else 0
+    _calls[name] = (ctypes.cast(getattr(lib(), "reef_ops_" + name), ctypes.c_void_p).value, bytes(kinds), at)
+    return _calls[name]
 
 
-def _learn(x):
+def _at(x):
+    """The address of an operand that is neither a number nor None nor a tensor; a tensor, where the extension does not know tensors yet: tells it."""
+    if isinstance(x, DeviceBuffer):
+        return x.ptr.value
+    if isinstance(x, ctypes.c_void_p):
+        return x.value
+    if isinstance(x, np.integer):
+        return int(x)
+    torch = sys.modules.get("torch")
+    if torch is None or not isinstance(x, torch.Tensor):
+        raise TypeError("an operand is a DeviceBuffer, a torch tensor, an address or None, not %r" % type(x))
+    lib()
     # Loaded before torch, the library has a HIP runtime of its own, whose streams do not wait for torch's.
     if not _torch_first:
         raise RuntimeError("tensors of torch: import torch before the library is first used")
-    _address[type(x)] = type(x).data_ptr
-    return x.data_ptr()
-
-
-def _at(*operands):
-    """Addresses of DeviceBuffers, of anything with data_ptr() (torch tensors), or addresses as they are."""
-    return [_address.get(type(x), _learn)(x) for x in operands]
+    now = torch.cuda.current_device
+    several = torch.cuda.device_count() > 1
+    _operands.learn(_at, torch.Tensor, (torch.float32, torch.float16, torch.bfloat16, torch.int32, torch.uint8, torch.bool),
+                    (lambda t: t.get_device() != now()) if several else None, int)
 
 
 def _nbytes(x):
@@ -539,12 +574,15 @@ def _nbytes(x):
 
 def ops_block_plan(desc, cached, added, free_list, table, lengths, starts, slots, counts, stream=None):
     """reef_ops_block_plan; operands are DeviceBuffers, torch tensors or addresses.  Like the calls below it enqueues,
-    does not wait and returns the status."""
-    return _op("block_plan")(ctypes.addressof(desc), *_at(cached, added, free_list, table, lengths, starts, slots, counts), stream)
+    does not wait and returns the status.  stream: a hipStream_t; None: the default stream, which is not always torch's current one.  Tensors are looked at (TypeError): on the current device, of the type that the call reads, contiguous (where the
+    descriptor has strides: in the last dimension); their sizes are the caller's, as those of the other operands."""
+    op = _calls.get("block_plan") or _ready("block_plan")
+    return _call(op, desc, None, stream, cached, added, free_list, table, lengths, starts, slots, counts)
 
 
 def ops_cache_append(desc, key, value, slots, key_cache, value_cache, stream=None):
-    return _op("cache_append")(ctypes.addressof(desc), *_at(key, value, slots, key_cache, value_cache), stream)
+    op = _calls.get("cache_append") or _ready("cache_append")
+    return _call(op, desc, None, stream, key, value, slots, key_cache, value_cache)
 
 
 def _workspace(name, desc):
@@ -562,8 +600,8 @@ def ops_paged_attention_workspace(desc):
 
 
 def ops_paged_attention(desc, query, key_cache, value_cache, table, lengths, out, lse=None, workspace=None, stream=None):
-    return _op("paged_attention")(ctypes.addressof(desc), *_at(query, key_cache, value_cache, table, lengths, out, lse, workspace),
-                                  _nbytes(workspace), stream)
+    op = _calls.get("paged_attention") or _ready("paged_attention")
+    return _call(op, desc, _nbytes(workspace), stream, query, key_cache, value_cache, table, lengths, out, lse, workspace)
 
 
 def ops_beam_select_workspace(desc):
@@ -572,11 +610,13 @@ def ops_beam_select_workspace(desc):
 
 
 def ops_beam_select(desc, logits, scores, ended, best, parents, tokens, workspace=None, stream=None):
-    return _op("beam_select")(ctypes.addressof(desc), *_at(logits, scores, ended, best, parents, tokens, workspace), _nbytes(workspace), stream)
+    op = _calls.get("beam_select") or _ready("beam_select")
+    return _call(op, desc, _nbytes(workspace), stream, logits, scores, ended, best, parents, tokens, workspace)
 
 
 def ops_beam_reorder(desc, parents, lengths, table, spare, table_out, lengths_out, key_cache, value_cache, stream=None):
-    return _op("beam_reorder")(ctypes.addressof(desc), *_at(parents, lengths, table, spare, table_out, lengths_out, key_cache, value_cache), stream)
+    op = _calls.get("beam_reorder") or _ready("beam_reorder")
+    return _call(op, desc, None, stream, parents, lengths, table, spare, table_out, lengths_out, key_cache, value_cache)
 
 
 def ops_paged_row(cache, table_row, token):

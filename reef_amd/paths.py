@@ -4,6 +4,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC_DIR = os.path.join(PKG_DIR, "csrc")
 BUILD_DIR = os.path.join(CSRC_DIR, "build")
 LIB_PATH = os.path.join(BUILD_DIR, "libreef_amd.so")
+OPERANDS_PATH = os.path.join(BUILD_DIR, "reef_operands.so")
 
 
 def code_object(flavour):

@@ -298,3 +298,53 @@ def test_attention_scales_that_are_no_32_bit_number_as_powers_of_two(scale):
     with pytest.raises(B.ReefError):
         B.ops_paged_attention_workspace(d)
     assert B.ops_paged_attention_workspace(attention(layout(), scale=1.7e38)) >= 0
+
+
+def in_a_process(code):
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_tensors_of_the_host_are_refused():
+    """Their addresses would be followed on the device; in a process of its own, which imports torch first."""
+    in_a_process("""
+import torch
+from reef_amd import binding as B
+P = 4096
+layout = B.CacheLayout(2, 10, 16, 2, 64, 2048, 128, 64)
+calls = [(B.ops_block_plan, B.BlockPlanDesc(2, 10, 16, 8, 8, 4, 8), 8),
+         (B.ops_cache_append, B.CacheAppendDesc(layout, 2, 3, 128, 64, 128, 64), 5),
+         (B.ops_paged_attention, B.PagedAttentionDesc(layout, 2, 2, 8, 4, 4, 0, 0, 0.125, 512, 64, 512, 64), 8),
+         (B.ops_beam_select, B.BeamSelectDesc(2, 2, 4, 100, 8, 2, 100), 7),
+         (B.ops_beam_reorder, B.BeamReorderDesc(layout, 4, 4, 4, 4, 4, 1, 0), 8)]
+for f, desc, n in calls:
+    for i in range(n):
+        for kind in (torch.int32, torch.bfloat16, torch.float32, torch.uint8):
+            args = [P] * n
+            if f in (B.ops_paged_attention, B.ops_beam_select):
+                args[-1] = None
+            args[i] = torch.zeros(64, dtype=kind)
+            try:
+                f(desc, *args)
+            except TypeError as e:
+                assert "operand %d: a tensor on the current device" % i in str(e), e
+            else:
+                raise SystemExit("%s took operand %d of the host" % (f.__name__, i))
+""")
+
+
+def test_operands_that_are_addresses():
+    """Numbers of any kind, c_void_p and None; refused ones come back as the library refuses them."""
+    d = append(layout())
+    for kind in (int, np.int64, np.uint64, ctypes.c_void_p):
+        assert B.ops_cache_append(append(layout(), tokens=0), *[kind(P)] * 5) == 0
+        refused(B.ops_cache_append(d, *[kind(P)] * 4, kind(P + 8)), "unaligned")
+    refused(B.ops_cache_append(d, P, P, P, P, None), "unaligned")
+    for bad in ("x", 1.5, np.zeros(3), [1]):
+        with pytest.raises(TypeError):
+            B.ops_cache_append(d, P, P, P, P, bad)
+    with pytest.raises(TypeError):
+        B.ops_cache_append(None, P, P, P, P, P)

@@ -909,3 +909,64 @@ def test_append_of_two_tokens_with_one_slot(kind, cache):
             pieces = have[s].reshape(kv, dim // per, per)
             fits = [(pieces == cast[t, i].reshape(pieces.shape)).all(-1) for t in who]
             assert np.any(fits, axis=0).all()
+
+
+# ---- tensors -------------------------------------------------------------------------------------------
+TENSORS = """
+import torch
+from reef_amd import binding as B
+dev = dict(device="cuda")
+ints = lambda *v: torch.tensor(v, dtype=torch.int32, **dev)
+lay = B.CacheLayout(2, 10, 16, 2, 64, 2048, 128, 64)
+rows = torch.randn(5, 2, 2, 64, **dev).bfloat16()
+pools = [torch.zeros(10, 16, 2, 64, dtype=torch.bfloat16, **dev) for _ in range(2)]
+app = B.CacheAppendDesc(lay, 2, 5, 256, 64, 256, 64)
+slots = ints(3, 159, 16, 0, 40)
+"""
+
+
+def in_a_process(code):
+    import os
+    import subprocess
+    import sys
+    r = subprocess.run([sys.executable, "-c", TENSORS + code], capture_output=True, text=True, timeout=110,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_tensors_of_another_type_or_layout_are_refused():
+    in_a_process("""
+def no(f, *args):
+    try:
+        f(*args)
+    except TypeError as e:
+        assert "operand" in str(e), e
+    else:
+        raise SystemExit("taken: %s" % (args,))
+
+good = (rows[:, 0], rows[:, 1], slots, *pools)
+assert B.ops_cache_append(app, *good) == 0, B.last_error()
+for i, bad in ((2, slots.long()), (2, slots.float()), (2, ints(*range(10))[::2]), (0, rows[:, 0].float()), (1, rows[:, 1].half()), (3, pools[0].float()),
+               (0, rows.transpose(-1, -2)), (4, pools[1].cpu())):
+    no(B.ops_cache_append, app, *good[:i], bad, *good[i + 1:])
+lengths, table = ints(5, 0), torch.zeros(2, 1, dtype=torch.int32, **dev)
+q, out, lse = torch.randn(2, 4, 64, **dev).bfloat16(), torch.zeros(2, 4, 64, dtype=torch.bfloat16, **dev), torch.zeros(2, 4, **dev)
+att = B.PagedAttentionDesc(lay, 2, 2, 4, 1, 1, 0, 0, 0.125, 256, 64, 256, 64)
+good = (q, *pools, table, lengths, out, lse, None)
+assert B.ops_paged_attention(att, *good) == 0, B.last_error()
+for i, bad in ((4, lengths.long()), (3, table.long()), (6, lse.double()), (6, lse.half()), (5, out.float()), (0, q.float()), (1, pools[0].half()), (4, ints(5, 5, 0, 0)[::2])):
+    no(B.ops_paged_attention, att, *good[:i], bad, *good[i + 1:])
+wide = B.PagedAttentionDesc(lay, 0, 2, 4, 1, 1, 0, 0, 0.125, 256, 64, 256, 64)
+no(B.ops_paged_attention, wide, *good)
+assert B.ops_paged_attention(wide, q.float(), *pools, table, lengths, out.float(), lse, None) == 0, B.last_error()
+sel = B.BeamSelectDesc(2, 1, 2, 100, 3, 2, 100)
+logits, scores, ended = torch.randn(2, 100, **dev).bfloat16(), torch.zeros(2, **dev), torch.tensor([True, False], **dev)
+best, parents, tokens = torch.zeros(3, **dev), ints(0, 0, 0), ints(0, 0, 0)
+work = torch.empty(B.ops_beam_select_workspace(sel), dtype=torch.uint8, **dev)
+for flags in (ended, ended.to(torch.uint8), None):
+    assert B.ops_beam_select(sel, logits, scores, flags, best, parents, tokens, work) == 0, B.last_error()
+good = (logits, scores, ended, best, parents, tokens, work)
+for i, bad in ((0, logits.float()), (1, scores.half()), (2, ended.int()), (4, parents.long()), (5, tokens.float()), (6, work.cpu())):
+    no(B.ops_beam_select, sel, *good[:i], bad, *good[i + 1:])
+torch.cuda.synchronize()
+""")
