@@ -4,6 +4,7 @@ The library is the product; this module only marshals arguments.  It raises if
 the library has not been built -- there is no fallback path.
 """
 import ctypes
+import functools
 import importlib.machinery
 import importlib.util
 import os
@@ -561,10 +562,10 @@ def _at(x):
     # Loaded before torch, the library has a HIP runtime of its own, whose streams do not wait for torch's.
     if not _torch_first:
         raise RuntimeError("tensors of torch: import torch before the library is first used")
-    now = torch.cuda.current_device
+    now, raw = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
     several = torch.cuda.device_count() > 1
     _operands.learn(_at, torch.Tensor, (torch.float32, torch.float16, torch.bfloat16, torch.int32, torch.uint8, torch.bool),
-                    (lambda t: t.get_device() != now()) if several else None, int)
+                    (lambda t: t.get_device() != now()) if several else None, (lambda: raw(now())) if several else functools.partial(raw, 0))
 
 
 def _nbytes(x):
@@ -574,7 +575,8 @@ def _nbytes(x):
 
 def ops_block_plan(desc, cached, added, free_list, table, lengths, starts, slots, counts, stream=None):
     """reef_ops_block_plan; operands are DeviceBuffers, torch tensors or addresses.  Like the calls below it enqueues,
-    does not wait and returns the status.  stream: a hipStream_t; None: the default stream, which is not always torch's current one.  Tensors are looked at (TypeError): on the current device, of the type that the call reads, contiguous (where the
+    does not wait and returns the status.  stream: a hipStream_t; None: torch's current stream where an operand is a tensor, otherwise the
+    default stream.  Tensors are looked at (TypeError): on the current device, of the type that the call reads, contiguous (where the
     descriptor has strides: in the last dimension); their sizes are the caller's, as those of the other operands."""
     op = _calls.get("block_plan") or _ready("block_plan")
     return _call(op, desc, None, stream, cached, added, free_list, table, lengths, starts, slots, counts)

@@ -970,3 +970,34 @@ for i, bad in ((0, logits.float()), (1, scores.half()), (2, ended.int()), (4, pa
     no(B.ops_beam_select, sel, *good[:i], bad, *good[i + 1:])
 torch.cuda.synchronize()
 """)
+
+
+def test_calls_with_tensors_go_to_the_current_stream_of_torch():
+    """Without a stream of their own, behind what torch was given there, and into a graph that torch captures."""
+    in_a_process("""
+want = [torch.zeros(160, 2, 64, dtype=torch.bfloat16, **dev) for _ in range(2)]
+s = torch.cuda.Stream()
+big = torch.randn(4096, 4096, **dev)
+late = torch.zeros_like(rows)
+torch.cuda.synchronize()
+with torch.cuda.stream(s):
+    for _ in range(30):
+        big = big @ big * 1e-4
+    late.copy_(rows)
+    assert B.ops_cache_append(app, late[:, 0], late[:, 1], slots, *pools) == 0, B.last_error()
+s.synchronize()
+for i in range(2):
+    want[i][slots.long()] = rows[:, i]
+    assert torch.equal(pools[i].view(160, 2, 64), want[i])
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    assert B.ops_cache_append(app, late[:, 0], late[:, 1], slots, *pools) == 0, B.last_error()
+for step in range(4):
+    late.copy_(torch.randn_like(late, dtype=torch.float32).bfloat16())
+    slots.copy_(torch.randperm(160, **dev)[:5].int())
+    graph.replay()
+    torch.cuda.synchronize()
+    for i in range(2):
+        want[i][slots.long()] = late[:, i]
+        assert torch.equal(pools[i].view(160, 2, 64), want[i]), step
+""")
