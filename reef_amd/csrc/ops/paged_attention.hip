@@ -884,7 +884,8 @@ extern "C" int reef_ops_paged_attention(const reef_paged_attention_desc* d, cons
     if (!rows16(query) || !rows16(key_cache) || !rows16(value_cache) || !rows16(out) || !words(table) || !words(lengths) || !aligned(lse, 4))
         return refuse(what, "null or unaligned argument");
     const Plan p = plan_of(*d);
-    if (p.groups >= 1ll << 31) return refuse(what, "%lld workgroups are too many", (long long)p.groups);
+    // (2^32 threads are refused by the launch, which may be the call's second one)
+    if (p.groups >= 1ll << 24) return refuse(what, "%lld workgroups are too many", (long long)p.groups);
     if (p.bytes && (!rows16(workspace) || workspace_bytes < (int64_t)p.bytes))
         return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", p.bytes, (long long)workspace_bytes);
     char* w = (char*)workspace;

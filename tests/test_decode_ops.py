@@ -348,3 +348,10 @@ def test_operands_that_are_addresses():
             B.ops_cache_append(d, P, P, P, P, bad)
     with pytest.raises(TypeError):
         B.ops_cache_append(None, P, P, P, P, P)
+
+
+def test_attention_of_more_workgroups_than_a_launch_takes():
+    """Refused before the first of its launches."""
+    for requests in ((1 << 24) - 1, (1 << 24) - 500):
+        d = attention(layout(kv_heads=1), requests=requests, heads=1, max_blocks=1000, table_stride=1000)
+        refused(call("paged_attention", d, *[P] * 8, 1 << 60), "too many")
