@@ -310,7 +310,7 @@ int reef_ops_cache_append(const reef_cache_append_desc* d, const void* key, cons
  * are in blocks of the pool.  Query head h reads cache head h / (heads / kv_heads).  Without such a token, or where all
  * s_t are -infinity, out is 0 and lse -infinity.  Values in places that are not read (behind a sequence, in front of the window)
  * may be anything; an infinity or a NaN among the values that are read gives infinities or NaN.  Queries are finite; |scale| < 2^127.  type (of query and out): the cache's, or REEF_TYPE_F32; products and sums in 32 bits.
- * query, out: [requests][heads][head_dim], strides in elements, multiples of 16 bytes, 16-byte aligned.
+ * query, out: [requests][heads][head_dim], strides in elements, multiples of 16 bytes, 16-byte aligned; no two rows of out overlap.
  * lse: [requests][heads], may be NULL.  `longest`: the largest length to expect, which sets into how many
  * shares long sequences are split (0: what a row of the table can hold); other lengths are right too.
  * reef_ops_paged_attention_workspace: bytes of workspace, which may be 0 (NULL then); -1: refused. */

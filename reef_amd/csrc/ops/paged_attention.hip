@@ -770,6 +770,16 @@ int check(const char* what, const reef_paged_attention_desc* d) {
     if (!stride16(d->requests, d->query_stride, bytes) || !stride16(d->requests, d->out_stride, bytes) || !stride16(d->heads, d->query_head_stride, bytes) ||
         !stride16(d->heads, d->out_head_stride, bytes))
         return refuse(what, "strides of query or out are not multiples of 16 bytes");
+    // rows of out: heads inside requests or requests inside heads, none over another
+    const bool heads_first = d->requests <= 1 || (d->heads > 1 && d->out_head_stride <= d->out_stride);
+    const int64_t count[2] = {heads_first ? d->heads : d->requests, heads_first ? d->requests : d->heads};
+    const int64_t stride[2] = {heads_first ? d->out_head_stride : d->out_stride, heads_first ? d->out_stride : d->out_head_stride};
+    __int128 extent = d->cache.head_dim;
+    for (int i = 0; i < 2; ++i) {
+        if (count[i] <= 1) continue;
+        if (stride[i] < extent) return refuse(what, "a stride of %lld elements lets rows of out overlap", (long long)stride[i]);
+        extent += (__int128)stride[i] * (count[i] - 1);
+    }
     return 0;
 }
 

@@ -355,3 +355,18 @@ def test_attention_of_more_workgroups_than_a_launch_takes():
     for requests in ((1 << 24) - 1, (1 << 24) - 500):
         d = attention(layout(kv_heads=1), requests=requests, heads=1, max_blocks=1000, table_stride=1000)
         refused(call("paged_attention", d, *[P] * 8, 1 << 60), "too many")
+
+
+@pytest.mark.parametrize("change", [dict(out_head_stride=0), dict(out_stride=0), dict(out_head_stride=56), dict(out_stride=448), dict(out_stride=64, out_head_stride=64),
+                                    dict(out_head_stride=512, out_stride=64, requests=9), dict(heads=2, out_stride=64)])
+def test_attention_rows_of_out_that_overlap(change):
+    d = attention(layout(), **change)
+    refused(call("paged_attention", d, *[P] * 8, 1 << 40), "overlap")
+    with pytest.raises(B.ReefError):
+        B.ops_paged_attention_workspace(d)
+
+
+@pytest.mark.parametrize("change", [dict(query_head_stride=0), dict(query_stride=0), dict(out_head_stride=512, out_stride=64, requests=8), dict(requests=1, out_stride=0),
+                                    dict(heads=2, out_head_stride=512, out_stride=64), dict(out_stride=2 ** 61), dict(requests=1, heads=2, out_stride=0, out_head_stride=64)])
+def test_attention_rows_that_are_apart(change):
+    assert B.ops_paged_attention_workspace(attention(layout(), **change)) >= 0
