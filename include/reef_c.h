@@ -309,7 +309,9 @@ int reef_ops_cache_append(const reef_cache_append_desc* d, const void* key, cons
  * over the tokens t in [max(0, n - window), n) (window 0: [0, n)), n = lengths[i] held to [0, max_blocks * block_size], that
  * are in blocks of the pool.  Query head h reads cache head h / (heads / kv_heads).  Without such a token, or where all
  * s_t are -infinity, out is 0 and lse -infinity.  Values in places that are not read (behind a sequence, in front of the window)
- * may be anything; an infinity or a NaN among the values that are read gives infinities or NaN.  Queries are finite; |scale| < 2^127.  type (of query and out): the cache's, or REEF_TYPE_F32; products and sums in 32 bits.
+ * may be anything; an infinity or a NaN among the values that are read gives infinities or NaN.  Queries are finite; |scale| < 2^127.  type (of query and out): the cache's, or REEF_TYPE_F32.  Scores,
+ * weights and sums are held in 32 bits.  Where type has 16, a weight enters its product with a value as two numbers of that type (2^-16 of
+ * it at most is left out, which is below the output's rounding); 32-bit queries and weights over a cache of 16 bits are three.
  * query, out: [requests][heads][head_dim], strides in elements, multiples of 16 bytes, 16-byte aligned; no two rows of out overlap.
  * lse: [requests][heads], may be NULL.  `longest`: the largest length to expect, which sets into how many
  * shares long sequences are split (0: what a row of the table can hold); other lengths are right too.

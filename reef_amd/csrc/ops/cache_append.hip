@@ -82,7 +82,7 @@ extern "C" int reef_ops_paged_row(const reef_cache_layout* c, const int32_t* tab
     const Divider by = divider((uint32_t)c->block_size);
     const uint32_t t = (uint32_t)token, entry = divided(t, by);
     if ((int64_t)entry >= max_blocks) return 0;
-    const PagedView v{c->blocks, c->block_size, max_blocks, c->block_stride, c->slot_stride};
+    const PagedView v{c->blocks, c->block_stride, c->slot_stride};
     const int64_t at = paged_row(v, table_row[entry], (int32_t)(t - entry * by.by));
     if (at < 0) return 0;
     *offset = at;

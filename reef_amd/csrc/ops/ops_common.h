@@ -77,9 +77,10 @@ inline int check_layout(const char* what, const reef_cache_layout& c, int64_t la
 }
 
 // ---- places in a paged cache, the same on both sides ----------------------------------------------
-// Element offset of a token's first head, or -1: behind the entries, or a block number outside the pool.
+// Element offset of the first head of a block's token `place`, or -1: a block number outside the pool.  (That a token lies within the
+// entries of its row is for callers to see to.)
 struct PagedView {
-    int32_t blocks, block_size, max_blocks;
+    int32_t blocks;
     int64_t block_stride, slot_stride;
 };
 __host__ __device__ inline int64_t paged_row(const PagedView& v, int32_t entry, int32_t place) {

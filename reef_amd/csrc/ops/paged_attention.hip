@@ -276,7 +276,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 15, g = lane >> 4;
     const int D = d.cache.head_dim;
     const int heads = min(16, a.group - tile16 * 16), head0 = kvh * a.group + tile16 * 16;
-    const PagedView view{d.cache.blocks, d.cache.block_size, d.max_blocks, d.cache.block_stride, d.cache.slot_stride};
+    const PagedView view{d.cache.blocks, d.cache.block_stride, d.cache.slot_stride};
     const C* keys = (const C*)a.key_cache + kvh * d.cache.head_stride;
     const C* values = (const C*)a.value_cache + kvh * d.cache.head_stride;
     const int32_t* table = a.table + (int64_t)r * d.table_stride;
@@ -456,9 +456,8 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DP < 256 ? 2 : 1) pa
             if (more) load_k(buffer ^ 1);
 #pragma unroll
             for (int h = 0; h < FEW; ++h) {
-                float top = p[h][0];
-                if constexpr (kSub == 2) top = fmaxf(top, p[h][1]);
-                top = fmaxf(over_lanes_max(top), fm[h]);
+                static_assert(kSub == 1, "32-bit caches have tiles of 16 tokens");
+                const float top = fmaxf(over_lanes_max(p[h][0]), fm[h]);
                 const float base = top == -INFINITY ? 0.0f : top, f = __builtin_amdgcn_exp2f(fm[h] - base);
                 fm[h] = top;
                 fl[h] *= f;
