@@ -15,7 +15,7 @@ constexpr int kThreads = 256;                // of a workgroup of four wavefront
 // Where the heads of all sequences are as many by themselves most have one or two shares, and the few long ones decide: twice as many
 // take 95 us instead of 103 for 90 sequences of up to 8000 tokens, 149 instead of 158 for 300 with 4 heads, 306 instead of 326 for
 // 50 x 8000, the same for 300 x 1500, 2 % more for 90 x 8000; 64 x 9000 with heads of 64, which just run at once uncut, lose most: 262
-// instead of 240.  Four times as many win little more (306 -> 303) and lose 7 % for 300 x 8000, heads of 64.
+// instead of 240 (the rule has no term for batches that do).  Four times as many win little more (306 -> 303) and lose 7 % for 300 x 8000, heads of 64.
 constexpr int kGroups = 448, kFiner = 2;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -811,7 +811,7 @@ Plan plan_of(const reef_paged_attention_desc& d) {
     // Whole sequences where a wide workgroup takes the longest in few rounds.  3 / 4 / 5 rounds against shares, heads of 128, bf16: 48 heads in all
     // 12 / 15 / 17 us against 13 / 14 / 15 (11 / 13 / 16 against 11 where that is the longest), 256 heads 18 / 24 / 33 against 25 / 30 / 39 (12 / 15 / 17
     // against 13 / 16 / 17).  Eight wavefronts for heads up to 64 have short rounds: 32-bit queries over bf16, 48 heads, 9 / 10 / 12 against 12 / 12 / 13,
-    // 32-bit caches of 4 query heads, 20 heads, 9 / 11 / 12 (6 rounds: 14) against 12.
+    // 32-bit caches of 4 query heads, 20 heads, 9 / 11 / 12 (6 rounds: 14) against 12.  (Between 48 and 256 heads nothing was measured.)
     const int rounds = all >= 192 || (wide == 8 && D <= 64) ? 5 : 3;
     p.wide = all < kGroups && longest <= (int64_t)rounds * wide * tile;
     p.groups = all;
