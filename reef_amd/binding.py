@@ -543,7 +543,7 @@ def _ready(name):
         _operands, _call = module, module.call
     desc, kinds = _OPS[name]
     at = desc.type.offset if hasattr(desc, "type") else 0
-    _calls[name] = (ctypes.cast(getattr(lib(), "reef_ops_" + name), ctypes.c_void_p).value, bytes(kinds), at)
+    _calls[name] = (ctypes.cast(getattr(lib(), "reef_ops_" + name), ctypes.c_void_p).value, bytes(kinds), at, ctypes.sizeof(desc))
     return _calls[name]
 
 

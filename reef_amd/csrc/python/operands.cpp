@@ -48,7 +48,8 @@ bool fits(PyObject* x, int kind, int type) {
     return true;
 }
 
-// call(operator, descriptor, bytes of the workspace or None, stream, *operands): the operator is (address, kinds, offset of the type field).
+// call(operator, descriptor, bytes of the workspace or None, stream, *operands): the operator is (address, kinds, offset of the type field,
+// bytes of the descriptor).
 PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     PyObject* const op = args[0];
     const char* const kinds = PyBytes_AS_STRING(PyTuple_GET_ITEM(op, 1));
@@ -60,9 +61,10 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
         Py_buffer* b;
         ~Release() { PyBuffer_Release(b); }
     } release{&desc};
-    const long type_at = PyLong_AsLong(PyTuple_GET_ITEM(op, 2));
+    const long type_at = PyLong_AsLong(PyTuple_GET_ITEM(op, 2)), size = PyLong_AsLong(PyTuple_GET_ITEM(op, 3));
+    if (desc.len != size) return PyErr_Format(PyExc_TypeError, "a descriptor of %ld bytes is needed, not one of %zd", size, desc.len);
     const auto field = [&](long at) {
-        const int32_t v = at + 4 <= desc.len ? *(const int32_t*)((const char*)desc.buf + at) : -1;
+        const int32_t v = *(const int32_t*)((const char*)desc.buf + at);
         return v >= 0 && v <= 2 ? (int)v : (int)kAny;        // (types that there are not: the library refuses them)
     };
     void* p[kMost] = {};

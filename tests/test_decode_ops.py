@@ -346,8 +346,9 @@ def test_operands_that_are_addresses():
     for bad in ("x", 1.5, np.zeros(3), [1]):
         with pytest.raises(TypeError):
             B.ops_cache_append(d, P, P, P, P, bad)
-    with pytest.raises(TypeError):
-        B.ops_cache_append(None, P, P, P, P, P)
+    for desc in (None, layout(), B.BlockPlanDesc(2, 10, 16, 8, 8, 4, 8), b"1234"):
+        with pytest.raises(TypeError):
+            B.ops_cache_append(desc, P, P, P, P, P)
 
 
 def test_attention_of_more_workgroups_than_a_launch_takes():
