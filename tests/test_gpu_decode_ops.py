@@ -929,7 +929,7 @@ def in_a_process(code):
     import os
     import subprocess
     import sys
-    r = subprocess.run([sys.executable, "-c", TENSORS + code], capture_output=True, text=True, timeout=110,
+    r = subprocess.run([sys.executable, "-c", TENSORS + code], capture_output=True, text=True, timeout=600,
                        cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
     assert r.returncode == 0, r.stdout + r.stderr
 
