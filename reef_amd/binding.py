@@ -556,12 +556,16 @@ def _at(x):
     if isinstance(x, np.integer):
         return int(x)
     torch = sys.modules.get("torch")
-    if torch is None or not isinstance(x, torch.Tensor):
+    if torch is None or not hasattr(x, "data_ptr"):
         raise TypeError("an operand is a DeviceBuffer, a torch tensor, an address or None, not %r" % type(x))
     lib()
     # Loaded before torch, the library has a HIP runtime of its own, whose streams do not wait for torch's.
     if not _torch_first:
         raise RuntimeError("tensors of torch: import torch before the library is first used")
+    if not isinstance(x, torch.Tensor):      # a storage, say
+        if not getattr(x, "is_cuda", False):
+            raise TypeError("%r is not on a device" % type(x))
+        return x.data_ptr()
     now, raw = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
     several = torch.cuda.device_count() > 1
     _operands.learn(_at, torch.Tensor, (torch.float32, torch.float16, torch.bfloat16, torch.int32, torch.uint8, torch.bool),

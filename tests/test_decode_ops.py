@@ -333,6 +333,12 @@ for f, desc, n in calls:
                 assert "operand %d: a tensor on the current device" % i in str(e), e
             else:
                 raise SystemExit("%s took operand %d of the host" % (f.__name__, i))
+try:
+    B.ops_cache_append(calls[1][1], P, P, P, P, torch.zeros(64).untyped_storage())
+except TypeError as e:
+    assert "not on a device" in str(e), e
+else:
+    raise SystemExit("a storage of the host was taken")
 """)
 
 

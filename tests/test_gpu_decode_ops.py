@@ -946,6 +946,7 @@ def no(f, *args):
 
 good = (rows[:, 0], rows[:, 1], slots, *pools)
 assert B.ops_cache_append(app, *good) == 0, B.last_error()
+assert B.ops_cache_append(app, *good[:3], torch.nn.Parameter(pools[0]), pools[1].untyped_storage()) == 0, B.last_error()
 for i, bad in ((2, slots.long()), (2, slots.float()), (2, ints(*range(10))[::2]), (0, rows[:, 0].float()), (1, rows[:, 1].half()), (3, pools[0].float()),
                (0, rows.transpose(-1, -2)), (4, pools[1].cpu())):
     no(B.ops_cache_append, app, *good[:i], bad, *good[i + 1:])
