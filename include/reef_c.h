@@ -363,6 +363,99 @@ typedef struct {
 int reef_ops_beam_reorder(const reef_beam_reorder_desc* d, const int32_t* parents, const int32_t* lengths, const int32_t* table,
                           const int32_t* spare, int32_t* table_out, int32_t* lengths_out, void* key_cache, void* value_cache, void* stream);
 
+/* ---- serving many requests over the same cache ----
+ * Beside the steps above, in the order of a server's calls: reef_ops_block_sweep finds the blocks that no request uses, reef_ops_cache_fork
+ * lets requests continue a part of another one, reef_ops_chunk_attention attends for prompts, pieces of prompts and single tokens at once,
+ * reef_ops_token_scores says how likely given tokens were, and reef_ops_cache_compact moves what is in use to the front of the pool.
+ * What is said above of pointers, streams, workspaces and refusals holds for them too. */
+
+/* Attention of the new tokens of all requests over their cached ones, themselves among them (their keys and values are in the cache already).
+ * Request i has the rows [starts[i], starts[i + 1]) of query (both held to [0, tokens]); the k-th of them has place p = cached[i] + k and
+ * attends to the tokens t of [max(0, p + 1 - window), p] (window 0: [0, p]) that are in blocks of the pool, as in reef_ops_paged_attention:
+ *     s_t = scale * query . key_t,   out = sum_t exp(s_t) value_t / sum_t exp(s_t),   lse = log sum_t exp(s_t)
+ * cached, lengths: held to [0, max_blocks * block_size]; starts, cached and lengths are block plan's.  A row whose place is not below
+ * lengths[i] (of a request that the plan refused) attends to nothing.  Without a token, or where all s_t are -infinity, out is 0 and lse -infinity.  Rows in front of
+ * starts[0] or behind starts[requests] are left as they were; starts ascend (where they do not, rows may be left out or belong to either request).
+ * Values that a row does not see (behind its place, in front of its window, behind a sequence, in no block) may be anything; an infinity
+ * or a NaN among the values that it sees gives infinities or NaN in it.  Queries are finite; |scale| < 2^127.  type (of query and out): the cache's, or REEF_TYPE_F32.
+ * Scores, weights' sums and outputs are held in 32 bits.
+ * query, out: [tokens][heads][head_dim], strides in elements, multiples of 16 bytes, 16-byte aligned; no two rows of out overlap.
+ * lse: [tokens][heads], may be NULL.  `longest`: the largest length to expect, which sets into how many shares long sequences are
+ * split (0: what a row of the table can hold); other lengths are right too. */
+typedef struct {
+    reef_cache_layout cache;
+    int32_t type, requests, heads, tokens;
+    int32_t max_blocks, table_stride;
+    int32_t longest, window;
+    float scale;
+    int64_t query_stride, query_head_stride, out_stride, out_head_stride;
+} reef_chunk_attention_desc;
+int64_t reef_ops_chunk_attention_workspace(const reef_chunk_attention_desc* d);
+int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, const void* query, const void* key_cache, const void* value_cache,
+                             const int32_t* table, const int32_t* starts, const int32_t* cached, const int32_t* lengths, void* out, float* lse,
+                             void* workspace, int64_t workspace_bytes, void* stream);
+
+/* How likely the tokens of each row of logits are, m the largest logit and S = sum_u exp(logits[u] - m):
+ *   scores  [rows]: logits[t] - m - log S of the given token t = tokens[row]; -infinity where t is none of the vocabulary
+ *   ranks   [rows]: how many tokens come before it (larger, or equal and with a lower number); -1 where it is none
+ *   entropy [rows]: log S - sum_u exp(logits[u] - m) (logits[u] - m) / S, in natural units
+ *   top_tokens, top_scores [rows][top]: the first `top` tokens, the larger first, equal ones by their number, and their scores
+ * A NaN counts as -infinity.  Where m is an infinity there are no probabilities: scores (of tokens of the vocabulary) and entropy are NaN; ranks and top_tokens go by
+ * the logits all the same.  Exponentials are those of 32 bits, their sums are held in 64.
+ * logits: [rows][logits_stride] of `type`, aligned to their own size.  top: up to 128 and vocab; top_* may be NULL where it is 0.  vocab: below 2^24. */
+typedef struct {
+    int32_t type, rows, vocab, top;
+    int64_t logits_stride;
+} reef_token_scores_desc;
+int64_t reef_ops_token_scores_workspace(const reef_token_scores_desc* d);
+int reef_ops_token_scores(const reef_token_scores_desc* d, const void* logits, const int32_t* tokens, float* scores, int32_t* ranks, float* entropy,
+                          int32_t* top_tokens, float* top_scores, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Which blocks the rows of a block table use.  Row i has n = lengths[i] tokens (held to [0, max_blocks * block_size]; requests that have ended: 0)
+ * and uses its first ceil(n / block_size) entries.
+ *   uses      [blocks]: how many entries name the block
+ *   free_list [blocks]: the blocks that none names, in ascending order; entries behind the last stay as they are
+ *   counts    [3]: blocks that none names; blocks that are named; entries used that name no block of the pool */
+typedef struct {
+    int32_t rows, blocks, block_size;
+    int32_t max_blocks, table_stride;
+} reef_block_sweep_desc;
+int64_t reef_ops_block_sweep_workspace(const reef_block_sweep_desc* d);
+int reef_ops_block_sweep(const reef_block_sweep_desc* d, const int32_t* table, const int32_t* lengths, int32_t* uses, int32_t* free_list,
+                         int32_t* counts, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Row children[i] of the block table becomes the first n tokens of row parents[i], n = tokens[i] held to [0, lengths[parents[i]]] (and that to
+ * [0, max_blocks * block_size]): its entries for full blocks are the parent's.  Where n % block_size tokens are left it takes the next
+ * block of free_list for them, and they are copied there in all layers of both pools (a block number outside the pool, the parent's or the
+ * list's: the entry is -1 and nothing is copied); lengths[children[i]] = n.  Its entries behind stay as they are.
+ * A fork is refused where a row is none of the table's, where a row is to be its own child, or where it needs a block and the list ends before it has one, counting
+ * those that the forks before it need, refused for blocks or not: its row and length stay as they were.
+ * Children are distinct, and no child is a parent of the same call; blocks of the list are used by no row.
+ *   counts [2]: entries of free_list taken; forks refused
+ * free_list may be NULL where free_blocks is 0.  The pools hold `layers` caches of the layout, layer_stride elements from one to the next; a block of one
+ * is less than 2^30 values. */
+typedef struct {
+    reef_cache_layout cache;
+    int32_t forks, table_rows, max_blocks, table_stride, free_blocks, layers;
+    int64_t layer_stride;
+} reef_cache_fork_desc;
+int reef_ops_cache_fork(const reef_cache_fork_desc* d, const int32_t* parents, const int32_t* children, const int32_t* tokens, const int32_t* free_list,
+                        int32_t* table, int32_t* lengths, int32_t* counts, void* key_cache, void* value_cache, void* stream);
+
+/* Moves the blocks in use to the front of the pool.  A block is in use where one of the first ceil(n / block_size) entries of a row names it,
+ * n = lengths[row] held to [0, max_blocks * block_size]; U are in use.  Those whose number is U or more are copied whole, in all layers of both pools, to the
+ * free ones below U: the highest to the lowest, the next to the next.  table_out gets the entries used, with the new numbers (entries that
+ * name no block of the pool as they are); its entries behind stay as they are.  Blocks U, U + 1, ... are free then.
+ * counts [2]: U; blocks moved.  table [rows][table_stride], table_out [rows][out_stride]: not the same memory.  Layers as above. */
+typedef struct {
+    reef_cache_layout cache;
+    int32_t rows, max_blocks, table_stride, out_stride, layers;
+    int64_t layer_stride;
+} reef_cache_compact_desc;
+int64_t reef_ops_cache_compact_workspace(const reef_cache_compact_desc* d);
+int reef_ops_cache_compact(const reef_cache_compact_desc* d, const int32_t* table, const int32_t* lengths, int32_t* table_out, int32_t* counts,
+                           void* key_cache, void* value_cache, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* GPUConfig (src/reef/executor/hip/hip_impl.cpp:9-74) */
 int reef_gpuconfig_num_cus(void);
 int reef_gpuconfig_num_xcds(void);

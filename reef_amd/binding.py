@@ -502,6 +502,27 @@ class BeamReorderDesc(ctypes.Structure):
     _fields_ = [("cache", CacheLayout)] + _fields(("rows", "table_rows", "max_blocks", "table_stride", "out_stride", "layers"), ("layer_stride",))
 
 
+class ChunkAttentionDesc(ctypes.Structure):
+    _fields_ = [("cache", CacheLayout)] + _fields(("type", "requests", "heads", "tokens", "max_blocks", "table_stride", "longest", "window"),
+                                                  ("query_stride", "query_head_stride", "out_stride", "out_head_stride"), ("scale",))
+
+
+class TokenScoresDesc(ctypes.Structure):
+    _fields_ = _fields(("type", "rows", "vocab", "top"), ("logits_stride",))
+
+
+class BlockSweepDesc(ctypes.Structure):
+    _fields_ = _fields(("rows", "blocks", "block_size", "max_blocks", "table_stride"))
+
+
+class CacheForkDesc(ctypes.Structure):
+    _fields_ = [("cache", CacheLayout)] + _fields(("forks", "table_rows", "max_blocks", "table_stride", "free_blocks", "layers"), ("layer_stride",))
+
+
+class CacheCompactDesc(ctypes.Structure):
+    _fields_ = [("cache", CacheLayout)] + _fields(("rows", "max_blocks", "table_stride", "out_stride", "layers"), ("layer_stride",))
+
+
 # What each pointer behind the descriptor points at, for operands that are tensors (csrc/python/operands.cpp): int32, bytes, anything, values
 # of the descriptor's type or of its cache's; _S: the descriptor has strides for all but the last dimension.
 _F32, _INTS, _BYTES, _ANY, _ROWS, _CACHE, _S = 0, 3, 4, 5, 6, 7, 8
@@ -511,8 +532,13 @@ _OPS = {
     "paged_attention": (PagedAttentionDesc, (_ROWS | _S, _CACHE | _S, _CACHE | _S, _INTS | _S, _INTS, _ROWS | _S, _F32, _ANY)),
     "beam_select": (BeamSelectDesc, (_ROWS | _S, _F32, _BYTES, _F32, _INTS, _INTS, _ANY)),
     "beam_reorder": (BeamReorderDesc, (_INTS, _INTS, _INTS | _S, _INTS, _INTS | _S, _INTS, _CACHE | _S, _CACHE | _S)),
+    "chunk_attention": (ChunkAttentionDesc, (_ROWS | _S, _CACHE | _S, _CACHE | _S, _INTS | _S, _INTS, _INTS, _INTS, _ROWS | _S, _F32, _ANY)),
+    "token_scores": (TokenScoresDesc, (_ROWS | _S, _INTS, _F32, _INTS, _F32, _INTS, _F32, _ANY)),
+    "block_sweep": (BlockSweepDesc, (_INTS | _S, _INTS, _INTS, _INTS, _INTS, _ANY)),
+    "cache_fork": (CacheForkDesc, (_INTS, _INTS, _INTS, _INTS, _INTS | _S, _INTS, _INTS, _CACHE | _S, _CACHE | _S)),
+    "cache_compact": (CacheCompactDesc, (_INTS | _S, _INTS, _INTS | _S, _INTS, _CACHE | _S, _CACHE | _S, _ANY)),
 }
-_OPS_WORKSPACE = ("paged_attention", "beam_select")     # (workspaces go with their size)
+_OPS_WORKSPACE = ("paged_attention", "beam_select", "chunk_attention", "token_scores", "block_sweep", "cache_compact")     # (workspaces go with their size)
 _ops = {}
 _calls = {}
 _operands = None        # the extension
@@ -623,6 +649,51 @@ def ops_beam_select(desc, logits, scores, ended, best, parents, tokens, workspac
 def ops_beam_reorder(desc, parents, lengths, table, spare, table_out, lengths_out, key_cache, value_cache, stream=None):
     op = _calls.get("beam_reorder") or _ready("beam_reorder")
     return _call(op, desc, None, stream, parents, lengths, table, spare, table_out, lengths_out, key_cache, value_cache)
+
+
+def ops_chunk_attention_workspace(desc):
+    """Bytes of workspace that reef_ops_chunk_attention wants for this descriptor."""
+    return _workspace("chunk_attention", desc)
+
+
+def ops_chunk_attention(desc, query, key_cache, value_cache, table, starts, cached, lengths, out, lse=None, workspace=None, stream=None):
+    op = _calls.get("chunk_attention") or _ready("chunk_attention")
+    return _call(op, desc, _nbytes(workspace), stream, query, key_cache, value_cache, table, starts, cached, lengths, out, lse, workspace)
+
+
+def ops_token_scores_workspace(desc):
+    """Bytes of workspace that reef_ops_token_scores wants for this descriptor."""
+    return _workspace("token_scores", desc)
+
+
+def ops_token_scores(desc, logits, tokens, scores, ranks, entropy, top_tokens=None, top_scores=None, workspace=None, stream=None):
+    op = _calls.get("token_scores") or _ready("token_scores")
+    return _call(op, desc, _nbytes(workspace), stream, logits, tokens, scores, ranks, entropy, top_tokens, top_scores, workspace)
+
+
+def ops_block_sweep_workspace(desc):
+    """Bytes of workspace that reef_ops_block_sweep wants for this descriptor."""
+    return _workspace("block_sweep", desc)
+
+
+def ops_block_sweep(desc, table, lengths, uses, free_list, counts, workspace=None, stream=None):
+    op = _calls.get("block_sweep") or _ready("block_sweep")
+    return _call(op, desc, _nbytes(workspace), stream, table, lengths, uses, free_list, counts, workspace)
+
+
+def ops_cache_fork(desc, parents, children, tokens, free_list, table, lengths, counts, key_cache, value_cache, stream=None):
+    op = _calls.get("cache_fork") or _ready("cache_fork")
+    return _call(op, desc, None, stream, parents, children, tokens, free_list, table, lengths, counts, key_cache, value_cache)
+
+
+def ops_cache_compact_workspace(desc):
+    """Bytes of workspace that reef_ops_cache_compact wants for this descriptor."""
+    return _workspace("cache_compact", desc)
+
+
+def ops_cache_compact(desc, table, lengths, table_out, counts, key_cache, value_cache, workspace=None, stream=None):
+    op = _calls.get("cache_compact") or _ready("cache_compact")
+    return _call(op, desc, _nbytes(workspace), stream, table, lengths, table_out, counts, key_cache, value_cache, workspace)
 
 
 def ops_paged_row(cache, table_row, token):

@@ -51,6 +51,19 @@ bool overlap(const Span (&out)[N], const Span (&in)[M]) {
 // Whether `count` steps of `stride` elements keep to 16 bytes.
 inline bool stride16(int64_t count, int64_t stride, int bytes) { return count <= 1 || (stride >= 0 && stride * bytes % 16 == 0); }
 
+// Whether rows of `dim` values overlap, `n` and `m` steps of two strides that are not negative where there is more than one.
+inline bool rows_overlap(int64_t n, int64_t stride_n, int64_t m, int64_t stride_m, int64_t dim) {
+    const bool m_first = n <= 1 || (m > 1 && stride_m <= stride_n);
+    const int64_t count[2] = {m_first ? m : n, m_first ? n : m}, stride[2] = {m_first ? stride_m : stride_n, m_first ? stride_n : stride_m};
+    __int128 extent = dim;
+    for (int i = 0; i < 2; ++i) {
+        if (count[i] <= 1) continue;
+        if (stride[i] < extent) return true;
+        extent += (__int128)stride[i] * (count[i] - 1);
+    }
+    return false;
+}
+
 // A layout that the kernels take: rows of 16-byte pieces, none over another, offsets that fit 60 bits.
 inline int check_layout(const char* what, const reef_cache_layout& c, int64_t layers = 1, int64_t layer_stride = 0) {
     const int bytes = type_bytes(c.type);

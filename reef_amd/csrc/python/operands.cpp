@@ -12,7 +12,7 @@ namespace {
 // (its first field); and kStrided, where the descriptor has strides for all but the last dimension.
 enum { kInts = 3, kBytes = 4, kAny = 5, kRows = 6, kCache = 7, kStrided = 8 };
 const char* const kNames[] = {"float32", "float16", "bfloat16", "int32", "uint8 or bool", "any type"};
-constexpr int kMost = 8;                     // operands
+constexpr int kMost = 10;                    // operands
 
 PyObject *tensor_type, *dtypes, *devices_differ, *current_stream, *other_address;     // (learn)
 PyObject *s_dtype, *s_is_cuda, *s_is_contiguous, *s_stride, *s_data_ptr;
@@ -120,9 +120,14 @@ PyObject* call(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Py_BEGIN_ALLOW_THREADS
     switch (operands * 2 + sized) {
         case 10: status = ((int (*)(const void*, P, P, P, P, P, P))f)(d, p[0], p[1], p[2], p[3], p[4], stream); break;
+        case 13: status = ((int (*)(const void*, P, P, P, P, P, P, int64_t, P))f)(d, p[0], p[1], p[2], p[3], p[4], p[5], bytes, stream); break;
         case 15: status = ((int (*)(const void*, P, P, P, P, P, P, P, int64_t, P))f)(d, p[0], p[1], p[2], p[3], p[4], p[5], p[6], bytes, stream); break;
         case 16: status = ((int (*)(const void*, P, P, P, P, P, P, P, P, P))f)(d, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], stream); break;
         case 17: status = ((int (*)(const void*, P, P, P, P, P, P, P, P, int64_t, P))f)(d, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], bytes, stream); break;
+        case 18: status = ((int (*)(const void*, P, P, P, P, P, P, P, P, P, P))f)(d, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], stream); break;
+        case 21:
+            status = ((int (*)(const void*, P, P, P, P, P, P, P, P, P, P, int64_t, P))f)(d, p[0], p[1], p[2], p[3], p[4], p[5], p[6], p[7], p[8], p[9], bytes, stream);
+            break;
         default: known = false;
     }
     Py_END_ALLOW_THREADS

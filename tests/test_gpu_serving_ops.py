@@ -1,0 +1,664 @@
+"""The operators that serve many requests over a paged cache, on the device against plain forms in 64 bits (tests/serving_ref.py): attention
+of new tokens, scores of given tokens, uses of blocks, forks, compaction, and runs of them together."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from reef_amd import binding as B
+from tests import decode_ref as R
+from tests import serving_ref as S
+from tests.decode_ref import BF16, F16, F32, HALF
+from tests.test_gpu_decode_ops import Pools, hip, in_a_process, ints, ok, up
+
+pytestmark = pytest.mark.gpu
+PAIRS = [(F32, F32), (F32, F16), (F32, BF16), (F16, F16), (BF16, BF16)]
+
+
+def work_of(n):
+    """A workspace full of nonsense with some bytes behind it, or none."""
+    if not n:
+        return None
+    w = B.DeviceBuffer(n + 64)
+    w.fill(0xFF)
+    return w
+
+
+def behind(w, n):
+    assert w is None or (w.to_array(np.uint8)[n:n + 64] == 0xFF).all()
+
+
+# ---- attention of new tokens --------------------------------------------------------------------
+def run_chunk(kind, cache, order, bs, kv, group, dim, cached, added, window=0, pad=0, scale=None, longest=0, seed=0, spoil=True, bad=0.0, q_pad=0, grow=1.0,
+              size=1.0, refused=(), extra=5, max_blocks=None, lse=True):
+    rng = np.random.default_rng(seed)
+    heads, requests = kv * group, len(cached)
+    cached, added = np.asarray(cached), np.asarray(added)
+    lengths = np.array([c if i in refused else c + a for i, (c, a) in enumerate(zip(cached, added))])
+    have = [-(-max(int(n), 0) // bs) for n in lengths]
+    width = max_blocks or max(max(have), 1)
+    held = lambda n: S.held(n, width, bs)                                                       # noqa: E731
+    order_of = rng.permutation(sum(min(h, width) for h in have) + 2)
+    pools = Pools(cache, len(order_of), bs, kv, dim, order, pad, seed=seed + 1, size=size)
+    table = np.full((requests, width + 3), 2 ** 30, np.int64)
+    at = 0
+    for i, h in enumerate(have):
+        h = min(h, width)
+        table[i, :h] = order_of[at:at + h]
+        at += h
+        for j in range(h):
+            if rng.random() < bad:
+                table[i, j] = rng.choice([-1, len(order_of), -2 ** 31])
+    in_pool = (table >= 0) & (table < len(order_of))
+    if spoil:
+        # whatever no row sees is NaN or infinite: places behind a sequence, in front of all windows, unused blocks
+        seen = np.zeros((len(order_of), bs), bool)
+        for i in range(requests):
+            n, c = held(lengths[i]), held(cached[i])
+            for t in range(max(0, c + 1 - window) if window else 0, n if added[i] and c < n else 0):
+                if in_pool[i, t // bs]:
+                    seen[table[i, t // bs], t % bs] = True
+        for r, x in zip(pools.raw, (np.nan, np.inf)):
+            pools.view(r)[~seen] = R.encode(np.float32(x).reshape(1), cache)[0]
+        pools.send()
+    starts = extra // 2 + np.concatenate([[0], np.cumsum(added)])       # rows in front of the first request, and behind the last
+    tokens = int(starts[-1]) + extra - extra // 2
+    q = R.encode((rng.standard_normal((tokens, heads + 2, dim + q_pad)) * grow).astype(np.float32), kind)
+    scale = dim ** -0.5 if scale is None else scale
+    d = B.ChunkAttentionDesc(pools.layout, kind, requests, heads, tokens, width, table.shape[1], longest, window, scale, (heads + 2) * (dim + q_pad), dim + q_pad,
+                             (heads + 1) * (dim + 8), dim + 8)
+    item = q.itemsize
+    out = B.DeviceBuffer(tokens * (heads + 1) * (dim + 8) * item)
+    out.fill(0x5A)
+    ls = up(np.full(tokens * heads + 1, 77, np.float32))
+    n_work = B.ops_chunk_attention_workspace(d)
+    work = work_of(n_work)
+    args = (d, up(q), *pools.dev, ints(table), ints(starts), ints(cached), ints(lengths), out, ls if lse else None, work)
+    ok(B.ops_chunk_attention(*args))
+    raw = out.to_array(R.np_type(kind)).reshape(tokens, heads + 1, dim + 8)
+    got_lse = ls.to_array()
+    ok(B.ops_chunk_attention(*args))
+    np.testing.assert_array_equal(raw, out.to_array(R.np_type(kind)).reshape(raw.shape))
+    got = R.decode(raw, kind)
+    sentinel = np.frombuffer(b"\x5a" * item, R.np_type(kind))[0]
+    assert (raw[:, heads] == sentinel).all() and (raw[:, :, dim:] == sentinel).all()
+    outside = np.r_[0:starts[0], starts[-1]:tokens]
+    assert (raw[outside] == sentinel).all() and got_lse[-1] == 77
+    lse_rows = got_lse[:-1].reshape(tokens, heads)
+    assert (lse_rows[outside] == 77).all()
+    behind(work, n_work)
+    qv, kv_, vv = R.decode(q[:, :heads, :dim], kind), pools.values(0), pools.values(1)
+    for i in range(requests):
+        rows, n = slice(starts[i], starts[i + 1]), held(lengths[i])
+        if not added[i]:
+            continue
+        ts = np.arange(n)
+        there = in_pool[i, ts // bs]
+        b = np.where(there, table[i, ts // bs], 0)
+        want, want_lse, tol, tol_lse = S.chunk(qv[rows], kv_[b, ts % bs].transpose(1, 0, 2), vv[b, ts % bs].transpose(1, 0, 2), held(cached[i]), n, scale, window,
+                                               kind, cache, there)
+        err = np.abs(got[rows, :heads, :dim] - want)
+        lim = tol + HALF[kind] * np.abs(want) + (2.0 ** -25 if kind == F16 else 0)              # (its subnormals' half step)
+        assert (err <= lim).all(), (i, int(cached[i]), int(added[i]), float((err / np.maximum(lim, 1e-30)).max()))
+        if lse:
+            g = lse_rows[rows]
+            assert (np.isneginf(g) == np.isneginf(want_lse)).all(), i
+            fine = np.isfinite(want_lse)
+            assert (np.abs(g[fine] - want_lse[fine]) <= tol_lse[fine]).all(), i
+    return got
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("dim", [8, 16, 32, 40, 64, 72, 80, 96, 104, 128, 136, 160, 192, 200, 248, 256])
+def test_chunk_head_sizes(kind, cache, dim):
+    run_chunk(kind, cache, "thd" if dim % 16 else "htd", 16, 2, 3, dim, [0, 200, 13, 77], [1, 5, 0, 90], seed=dim)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("group,kv", [(1, 1), (1, 12), (2, 3), (3, 5), (4, 2), (7, 1), (8, 2), (16, 2), (17, 1), (33, 1), (128, 1), (200, 1)])
+def test_chunk_groups(kind, cache, group, kv):
+    run_chunk(kind, cache, "thd", 16, kv, group, 64, [130, 0, 33], [1, 40, 9], seed=group)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("bs", [1, 2, 3, 8, 16, 24, 33, 64, 128, 1000])
+@pytest.mark.parametrize("order", ["thd", "htd"])
+def test_chunk_block_sizes(kind, cache, bs, order):
+    run_chunk(kind, cache, order, bs, 2, 2, 64, [0, 1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 256], [1, 2, 3, 31, 32, 33, 1, 63, 64, 65, 127, 128, 129], seed=bs, pad=8)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("longest", [0, 1, 700, 10 ** 9])
+@pytest.mark.parametrize("window", [0, 900])
+def test_chunk_long_and_ragged(kind, cache, longest, window):
+    """Long sequences are split, short ones not, whatever the caller expects; whole prompts, pieces and single tokens."""
+    run_chunk(kind, cache, "thd", 16, 1, 4, 128, [4000, 0, 0, 2047, 10, 6000, 511, 0, 1500], [1, 700, 1, 100, 0, 5, 129, 1000, 33], window=window, longest=longest,
+              seed=longest % 97, q_pad=8)
+
+
+@pytest.mark.parametrize("requests", [63, 64, 65, 300, 1500])
+@pytest.mark.parametrize("window", [0, 700])
+def test_chunk_many_requests(requests, window):
+    """A few long sequences and chunks among many short and empty ones."""
+    rng = np.random.default_rng(requests)
+    cached, added = rng.integers(0, 40, requests), rng.integers(0, 4, requests)
+    pick = rng.permutation(requests)[:6]
+    cached[pick] = [2500, 1100, 0, 600, 2900, 0]
+    added[pick] = [1, 70, 500, 200, 0, 129]
+    run_chunk(BF16, BF16, "thd", 16, 1, 2, 32, cached, added, window=window, seed=requests, refused=(int(pick[3]), 5))
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("window", [1, 2, 31, 64, 100, 1000, 2 ** 31 - 1])
+def test_chunk_windows(kind, cache, window):
+    run_chunk(kind, cache, "htd", 24, 2, 2, 80, [0, 24, 1000, 129, 0], [200, 100, 150, 1, 1], window=window, seed=window % 89)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("bad", [0.1, 0.9, 1.0])
+def test_chunk_blocks_that_are_not_in_the_pool(kind, cache, bad):
+    run_chunk(kind, cache, "thd", 4, 2, 2, 64, [1, 24, 100, 1500], [3, 150, 1, 40], bad=bad, seed=3)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+def test_chunk_refused_requests_and_lengths_beyond_the_row(kind, cache):
+    run_chunk(kind, cache, "thd", 16, 2, 2, 64, [100, 0, 64, 33], [200, 3, 70, 1], refused=(0, 2, 3), seed=9)
+    run_chunk(kind, cache, "thd", 16, 2, 2, 64, [40, -5, 200, 64], [60, 30, 5, 1], max_blocks=4, seed=9, spoil=False, lse=False)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+def test_chunk_sharp_and_flat_scores(kind, cache):
+    run_chunk(kind, cache, "thd", 16, 2, 4, 128, [700, 0], [40, 300], grow=30.0, seed=4)        # one token takes nearly all
+    run_chunk(kind, cache, "thd", 16, 2, 4, 128, [700, 0], [40, 300], scale=0.0, seed=5)        # all alike
+    run_chunk(kind, cache, "thd", 16, 2, 4, 128, [700, 0], [40, 300], scale=-0.3, seed=6)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+def test_chunk_small_and_large_values(kind, cache):
+    """Keys and values that are subnormal in fp16, and ones near its largest; queries far from 1 either way."""
+    for kw in (dict(size=2e-6, scale=1000.0), dict(size=12000.0, scale=1e-5), dict(grow=3e-4, scale=300.0), dict(grow=3e3, scale=3e-5)):
+        run_chunk(kind, cache, "thd", 16, 2, 2, 64, [300, 40], [20, 130], seed=1, **kw)
+
+
+@pytest.mark.parametrize("kind,cache", [(F32, F16), (F32, BF16), (F32, F32)])
+def test_chunk_queries_far_from_one(kind, cache):
+    for grow, scale in ((1e35, 3e-36), (1e-33, 1e32)) + (((5e37, 2e-38), (1e-37, 2e36), (1e-40, 2e38)) if cache == F16 else ()):
+        run_chunk(kind, cache, "thd", 16, 2, 2, 64, [300, 2000], [20, 40], grow=grow, scale=scale, seed=1)
+
+
+def one_request(kind, cache, keys, values, q, scale, cached, longest=0):
+    """One request in one block: raw host values keys, values [tokens][dim], q [new][heads][dim] -> out, lse."""
+    t, dim = keys.shape
+    new, heads = q.shape[:2]
+    d = B.ChunkAttentionDesc(B.CacheLayout(cache, 1, t, 1, dim, t * dim, dim, dim), kind, 1, heads, new, 1, 1, longest, 0, scale, heads * dim, dim, heads * dim, dim)
+    out, ls = B.DeviceBuffer(new * heads * dim * (4 if kind == F32 else 2)), B.DeviceBuffer(4 * new * heads)
+    ok(B.ops_chunk_attention(d, up(R.encode(q, kind)), up(R.encode(keys, cache)), up(R.encode(values, cache)), ints([0]), ints([0, new]), ints([cached]), ints([t]), out, ls,
+                             work_of(B.ops_chunk_attention_workspace(d))))
+    return R.decode(out.to_array(R.np_type(kind)).reshape(new, heads, dim), kind), ls.to_array().reshape(new, heads)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("cached,new", [(0, 150), (70, 30), (3000, 140)])
+@pytest.mark.parametrize("dim", [40, 64, 128])
+def test_chunk_rows_do_not_see_infinities_and_nan_behind_them(kind, cache, cached, new, dim):
+    """A key or a value of a later token of the same request is NaN or infinite: rows in front of it are as if it were not there, those from it on show it."""
+    rng = np.random.default_rng(cached + dim)
+    total = cached + new
+    keys, values, q = (rng.standard_normal(s).astype(np.float32) for s in ((total, dim), (total, dim), (new, 2, dim)))
+    clean, clean_lse = one_request(kind, cache, keys, values, q, 0.1, cached)
+    for what in (np.nan, np.inf, -np.inf):
+        for k in (1, new // 2, new - 1):
+            at = cached + k
+            v2 = values.copy()
+            v2[at, 5] = what
+            out, ls = one_request(kind, cache, keys, v2, q, 0.1, cached)
+            np.testing.assert_array_equal(out[:k], clean[:k])
+            assert not np.isfinite(out[k:, :, 5]).any()
+            other = np.arange(dim) != 5
+            np.testing.assert_array_equal(out[k:, :, other], clean[k:, :, other])
+            np.testing.assert_array_equal(ls, clean_lse)
+            k2 = keys.copy()
+            k2[at, 5] = np.nan
+            out, ls = one_request(kind, cache, k2, values, q, 0.1, cached)
+            np.testing.assert_array_equal(out[:k], clean[:k])
+            assert np.isnan(out[k:]).all() and np.isnan(ls[k:]).all()
+            np.testing.assert_array_equal(ls[:k], clean_lse[:k])
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("tokens", [40, 200, 3000])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_chunk_scores_of_any_size(kind, cache, tokens, sign):
+    """Scores from 2^18 to 2^31: the largest takes everything, two equal ones half each.  One dimension alone is not zero and its
+    products are exact, so all other weights are 0 and the two are alike: the result is the mean of two values but for a rounding of their sum and of the output."""
+    rng = np.random.default_rng(tokens)
+    dim, new = 64, 3
+    values = rng.standard_normal((tokens, dim)).astype(np.float32)
+    v = R.decode(R.encode(values, cache), cache)
+    for binade in (18, 20, 21, 23, 24, 25, 27, 29, 30):
+        for more in (1.0, 1.25, 1.75):
+            keys, q = np.zeros((tokens, dim), np.float32), np.zeros((new, 2, dim), np.float32)
+            win = rng.permutation(tokens - new)[:2]
+            keys[:, 5] = 4096 * (rng.integers(1, 5, tokens) / 8 if sign > 0 else 1 + rng.integers(3, 8, tokens) / 8)
+            keys[win, 5] = 4096
+            q[:, 0, 5], q[:, 1, 5] = sign * 4096 * more, sign * 2048 * more
+            out, ls = one_request(kind, cache, keys, values, q, 2.0 ** (binade - 24), tokens - new)
+            want = (v[win[0]] + v[win[1]]) / 2
+            assert (np.abs(out - want) <= HALF[kind] * np.abs(want) + 2.0 ** -22 * np.abs(v[win]).max(0) + (2.0 ** -25 if kind == F16 else 0)).all(), (binade, more)
+            s = np.array([1, 0.5]) * sign * more * 2.0 ** binade
+            assert (np.abs(ls - (s + np.log(2))) <= 8 * 2.0 ** -24 * np.abs(s) + 2.0 ** -20).all(), (binade, more)
+
+
+@pytest.mark.parametrize("kind,cache", PAIRS)
+def test_chunk_of_sequences_just_below_2_31(kind, cache):
+    """A table whose entries all name one large block holds 2^31 - 2 tokens; a window near its end."""
+    bs, entries, dim, group, new = 1549411, 1386, 8, 3, 40
+    rng = np.random.default_rng(group)
+    raw = [np.zeros((bs, dim), R.np_type(cache)) for _ in range(2)]
+    for r in raw:
+        r[-6000:] = R.encode(rng.standard_normal((6000, dim)).astype(np.float32), cache)
+    k, v = (up(r) for r in raw)
+    q = R.encode(rng.standard_normal((new, group, dim)).astype(np.float32), kind)
+    out, ls = B.DeviceBuffer(new * group * dim * (4 if kind == F32 else 2)), B.DeviceBuffer(4 * new * group)
+    for window in (1, 33, 479, 5000):
+        d = B.ChunkAttentionDesc(B.CacheLayout(cache, 1, bs, 1, dim, 0, dim, 0), kind, 1, group, new, entries, entries, 0, window, 0.4, group * dim, dim, group * dim, dim)
+        held = bs * entries
+        ok(B.ops_chunk_attention(d, up(q), k, v, ints(np.zeros(entries)), ints([0, new]), ints([held - new]), ints([2 ** 31 - 1]), out, ls,
+                                 work_of(B.ops_chunk_attention_workspace(d))))
+        n = window + new - 1
+        at = np.arange(held - n, held) % bs
+        want, want_lse, tol, tol_lse = S.chunk(R.decode(q, kind), R.decode(raw[0][at], cache)[None], R.decode(raw[1][at], cache)[None], window - 1, n, 0.4, window, kind, cache)
+        got, got_lse = R.decode(out.to_array(R.np_type(kind)).reshape(new, group, dim), kind), ls.to_array().reshape(new, group)
+        assert (np.abs(got - want) <= tol + HALF[kind] * np.abs(want) + (2.0 ** -25 if kind == F16 else 0)).all(), window
+        assert (np.abs(got_lse - want_lse) <= tol_lse).all(), window
+
+
+@pytest.mark.parametrize("kind,cache,cached,new", [(BF16, BF16, 0, 1500), (F16, F16, 9000, 400), (F32, BF16, 700, 600), (F32, F32, 2000, 300), (BF16, BF16, 30000, 1)])
+def test_chunk_large(kind, cache, cached, new):
+    run_chunk(kind, cache, "thd", 16, 2, 4, 128, [cached], [new], longest=cached + new, seed=new, extra=0)
+
+
+def test_chunk_of_single_tokens_is_paged_attention():
+    """One new token a request: what the operator for single tokens gives, within the roundings of both."""
+    rng = np.random.default_rng(3)
+    kv, group, dim, bs, lengths = 2, 4, 64, 16, [1, 40, 333, 2000]
+    heads, n, width = kv * group, len(lengths), 125
+    pools = Pools(BF16, n * width, bs, kv, dim)
+    table = rng.permutation(n * width).reshape(n, width)
+    q = R.encode(rng.standard_normal((n, heads, dim)).astype(np.float32), BF16)
+    out = [B.DeviceBuffer(n * heads * dim * 2) for _ in range(2)]
+    ls = [B.DeviceBuffer(n * heads * 4) for _ in range(2)]
+    d0 = B.PagedAttentionDesc(pools.layout, BF16, n, heads, width, width, 2000, 0, 0.125, heads * dim, dim, heads * dim, dim)
+    d1 = B.ChunkAttentionDesc(pools.layout, BF16, n, heads, n, width, width, 2000, 0, 0.125, heads * dim, dim, heads * dim, dim)
+    ok(B.ops_paged_attention(d0, up(q), *pools.dev, ints(table), ints(lengths), out[0], ls[0], work_of(B.ops_paged_attention_workspace(d0))))
+    ok(B.ops_chunk_attention(d1, up(q), *pools.dev, ints(table), ints(range(n + 1)), ints(np.array(lengths) - 1), ints(lengths), out[1], ls[1],
+                             work_of(B.ops_chunk_attention_workspace(d1))))
+    a, b = (R.decode(x.to_array(np.uint16), BF16) for x in out)
+    v = np.abs(pools.values(1)).max()
+    assert (np.abs(a - b) <= 3 * HALF[BF16] * v).all()
+    assert np.abs(ls[0].to_array() - ls[1].to_array()).max() <= 2.0 ** -15
+
+
+def test_chunk_starts_that_do_not_ascend_stay_inside():
+    """Nothing is read or written behind the tensors, whatever starts, cached and lengths hold."""
+    rng = np.random.default_rng(1)
+    pools = Pools(BF16, 40, 16, 2, 64)
+    tokens, heads, n = 50, 4, 5
+    q = up(R.encode(rng.standard_normal((tokens, heads, 64)).astype(np.float32), BF16))
+    out = up(np.full(tokens * heads * 64 + 64, 0x4242, np.uint16))
+    d = B.ChunkAttentionDesc(pools.layout, BF16, n, heads, tokens, 8, 8, 0, 0, 0.125, heads * 64, 64, heads * 64, 64)
+    work = work_of(B.ops_chunk_attention_workspace(d))
+    for starts in ([0, 50, 0, 50, 0, 50], [-2 ** 31, 2 ** 31 - 1, 3, -7, 60, 2 ** 31 - 1], [50, 40, 30, 20, 10, 0]):
+        for lengths in ([128] * 5, [2 ** 31 - 1, -5, 0, 64, 10]):
+            ok(B.ops_chunk_attention(d, q, *pools.dev, ints(rng.integers(-3, 50, (n, 8))), ints(starts), ints(rng.integers(-5, 200, n)), ints(lengths), out, None, work))
+    assert (out.to_array(np.uint16)[tokens * heads * 64:] == 0x4242).all()
+    behind(work, B.ops_chunk_attention_workspace(d))
+
+
+# ---- scores of given tokens ----------------------------------------------------------------------
+def run_scores(kind, logits, tokens, top, pad=0):
+    rows, vocab = logits.shape
+    raw = R.encode(np.pad(np.asarray(logits, np.float32), ((0, 0), (0, pad)), constant_values=60), kind)
+    d = B.TokenScoresDesc(kind, rows, vocab, top, vocab + pad)
+    outs = [up(np.full(n + 1, -9, t)) for n, t in ((rows, np.float32), (rows, np.int32), (rows, np.float32), (rows * top, np.int32), (rows * top, np.float32))]
+    n_work = B.ops_token_scores_workspace(d)
+    work = work_of(n_work)
+    args = (d, up(raw), ints(tokens), *outs, work)
+    ok(B.ops_token_scores(*args))
+    got = [o.to_array(t) for o, t in zip(outs, (np.float32, np.int32, np.float32, np.int32, np.float32))]
+    ok(B.ops_token_scores(*args))
+    for g, o in zip(got, outs):
+        np.testing.assert_array_equal(g, o.to_array(g.dtype))
+        assert g[-1] == -9
+    behind(work, n_work)
+    want = S.scores(R.decode(raw[:, :vocab], kind), np.asarray(tokens), top)
+    np.testing.assert_array_equal(got[1][:-1], want[1])
+    np.testing.assert_array_equal(got[3][:-1].reshape(rows, top), want[3])
+    # an exponential in 32 bits is off by 2^-23 of itself and three roundings of its argument, 2^-22 (1 + |x - m|) in all; the sum of them weighs that by
+    # e, and e (1 + |x - m|) / S adds up to at most 2 + log vocab, as an entropy does; sums are in 64 bits.  The entropy's products have the same error again, times |x - m|
+    bound = 2.0 ** -22 * (2 + np.log(vocab))
+    x = R.decode(raw[:, :vocab], kind)
+    x = np.where(np.isnan(x), -np.inf, x)
+    with np.errstate(all="ignore"):
+        y = x - x.max(1)[:, None]
+        e = np.exp(y)
+        second = np.where(e > 0, e * (1 + np.abs(y)) * np.abs(y), 0).sum(1) / e.sum(1)
+    for g, w, more in ((got[0][:-1], want[0], 0), (got[2][:-1], want[2], 2.0 ** -21 * np.where(np.isfinite(second), second, 0)),
+                       (got[4][:-1].reshape(rows, top), want[4], 0)):
+        with np.errstate(over="ignore"):
+            w = np.where(np.isinf(w.astype(np.float32)), w.astype(np.float32), w)       # (differences that 32 bits do not hold)
+        fine = np.isfinite(w)
+        assert (np.isfinite(g) == fine).all() and (np.isnan(g) == np.isnan(w)).all()
+        lim = np.broadcast_to(bound + more if w.ndim == 1 else bound, w.shape) + HALF[F32] * np.abs(np.where(fine, w, 0))
+        assert (np.abs(g - w)[fine] <= lim[fine]).all(), float((np.abs(g - w)[fine] / lim[fine]).max())
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (1, 7), (3, 256), (2, 511), (2, 513), (5, 1000), (1, 30522), (17, 4097), (300, 1025), (2, 70001), (1, 200003)])
+def test_scores_sizes(kind, rows, vocab):
+    rng = np.random.default_rng(vocab)
+    for top in sorted({0, 1, min(5, vocab), min(20, vocab), min(128, vocab)}):
+        tokens = rng.integers(0, vocab, rows)
+        tokens[-1] = rng.choice([0, vocab - 1, -1, vocab, 2 ** 31 - 1, -2 ** 31])
+        run_scores(kind, rng.standard_normal((rows, vocab)) * 2.5, tokens, top, pad=int(rng.integers(0, 4)))
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("vocab", [300, 9001, 66000])
+def test_scores_odd_values(kind, vocab):
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((14, vocab)) * 3
+    x[0] = 1.5                                   # all alike
+    x[1] = rng.integers(0, 3, vocab)             # many alike
+    x[2] = -np.inf                               # nothing
+    x[3, :] = -np.inf
+    x[3, vocab // 2] = 4.0                       # one token alone
+    x[4, rng.permutation(vocab)[:vocab // 2]] = -np.inf
+    x[5, [3, vocab - 2]] = np.nan
+    x[6, 11] = np.inf
+    x[7] = np.nan
+    x[8] = np.arange(vocab) * (10000.0 / vocab)  # ascending: the best are last
+    x[9] = -np.arange(vocab) * (10000.0 / vocab)
+    x[10] = np.where(np.arange(vocab) % 2, 0.0, -0.0)
+    x[11] = np.finfo(np.float16).min
+    x[11, 7] = np.finfo(np.float16).max
+    x[12, 5] = 60000.0                           # takes everything
+    x[13] = 1e-7 * rng.standard_normal(vocab)
+    for top in (1, 20, 128):
+        run_scores(kind, x, rng.integers(0, vocab, 14), top)
+        run_scores(kind, x, [7, vocab - 1, 5, vocab // 2, 4, 3, 11, 0, vocab - 1, 0, 1, 7, 5, 2], top)
+
+
+def test_scores_extremes_of_32_bits():
+    x = np.full((3, 1000), -3e38)
+    x[0, 5], x[1, 5:9], x[2] = 3e38, [1e30, 1e30, -1e30, 2e30], 1e-40
+    run_scores(F32, x, [5, 6, 999], 10)
+
+
+# ---- blocks ---------------------------------------------------------------------------------------
+def run_sweep(table, lengths, blocks, bs, max_blocks):
+    rows, stride = table.shape
+    d = B.BlockSweepDesc(rows, blocks, bs, max_blocks, stride)
+    uses, free, counts = (ints(np.full(n + 1, -7)) for n in (blocks, blocks, 3))
+    n_work = B.ops_block_sweep_workspace(d)
+    work = work_of(n_work)
+    for _ in range(2):
+        ok(B.ops_block_sweep(d, ints(table), ints(lengths), uses, free, counts, work))
+    want = S.sweep(table, lengths, blocks, bs, max_blocks)
+    uses, free, counts = (x.to_array(np.int32) for x in (uses, free, counts))
+    np.testing.assert_array_equal(uses[:-1], want[0])
+    np.testing.assert_array_equal(free[:len(want[1])], want[1])
+    assert (free[len(want[1]):] == -7).all() and uses[-1] == -7 and counts.tolist() == want[2] + [-7]
+    behind(work, n_work)
+
+
+@pytest.mark.parametrize("rows,blocks,bs,max_blocks", [(0, 5, 16, 3), (1, 1, 1, 1), (3, 63, 16, 8), (9, 64, 8, 12), (40, 1025, 16, 20), (100, 8192, 24, 50), (100, 8193, 24, 50),
+                                                       (700, 4096, 16, 64), (513, 40000, 32, 70), (3, 5000, 1, 20000), (2, 12289, 7, 11111)])
+def test_sweep(rows, blocks, bs, max_blocks):
+    rng = np.random.default_rng(blocks)
+    for bad in (0.0, 0.2):
+        table = rng.integers(0, blocks, (rows, max_blocks + 3))
+        table[rng.random(table.shape) < bad] = rng.choice([-1, blocks, 2 ** 31 - 1, -2 ** 31])
+        lengths = rng.integers(-5, max_blocks * bs + 10, rows) * (rng.random(rows) < 0.7)
+        run_sweep(table, lengths, blocks, bs, max_blocks)
+
+
+def test_sweep_of_nothing_and_of_all():
+    table = np.arange(20000).reshape(20, 1000)[:, ::-1].copy()
+    run_sweep(table, np.zeros(20, int), 20000, 4, 1000)
+    run_sweep(table, np.full(20, 4000), 20000, 4, 1000)
+    run_sweep(table, np.full(20, 2 ** 31 - 1), 20000, 4, 1000)
+    run_sweep(np.full((500, 300), 9999), np.full(500, 1200), 10001, 4, 300)      # one block, 150000 times
+
+
+def moved(pools, moves, bs):
+    """The pools on the host after copies of the first tokens of blocks, in all layers."""
+    want = [r.copy() for r in pools.raw]
+    for layer in range(pools.layers or 1):
+        for r, w in zip(pools.raw, want):
+            a, b = pools.view(r, layer), pools.view(w, layer)
+            for m in moves:
+                n = m[2] if len(m) > 2 else bs
+                b[m[1], :n] = a[m[0], :n]
+    return want
+
+
+def run_fork(pools, parents, children, tokens, free, table, lengths, max_blocks):
+    blocks, bs = pools.shape[:2]
+    d = B.CacheForkDesc(pools.layout, len(parents), len(table), max_blocks, table.shape[1], len(free), pools.layers or 1, pools.per_layer)
+    t, ls, counts = up(np.concatenate([table.ravel(), [-7]]).astype(np.int32)), ints(list(lengths) + [-7]), ints([-7] * 3)
+    args = (d, ints(parents), ints(children), ints(tokens), ints(free) if len(free) else None, t, ls, counts, *pools.dev)
+    for _ in range(2):                       # again over its own results: the same
+        ok(B.ops_cache_fork(*args))
+    want = S.fork(parents, children, tokens, free, table, lengths, blocks, bs, max_blocks)
+    np.testing.assert_array_equal(t.to_array(np.int32), np.concatenate([want[0].ravel(), [-7]]))
+    np.testing.assert_array_equal(ls.to_array(np.int32), want[1].tolist() + [-7])
+    assert counts.to_array(np.int32).tolist() == want[2] + [-7]
+    for g, w in zip(pools.fetch(), moved(pools, want[3], bs)):
+        np.testing.assert_array_equal(g, w)
+
+
+@pytest.mark.parametrize("cache,order,bs,kv,dim,layers,forks", [(F32, "thd", 16, 2, 8, 1, 1), (BF16, "htd", 16, 3, 40, 3, 7), (F16, "thd", 1, 1, 64, 2, 20), (F32, "htd", 24, 5, 72, 2, 60),
+                                                                (BF16, "thd", 7, 12, 256, 1, 33), (BF16, "thd", 4, 1, 8, 1, 255), (F16, "htd", 4, 2, 8, 2, 1100)])
+@pytest.mark.parametrize("pad", [0, 16])
+def test_fork(cache, order, bs, kv, dim, layers, forks, pad):
+    rng = np.random.default_rng(forks)
+    base, max_blocks = 1 + forks // 3, 6
+    rows = base + forks
+    used = rows * max_blocks
+    pools = Pools(cache, used + forks + 3, bs, kv, dim, order, pad, layers)
+    numbers = rng.permutation(used + forks + 3)
+    table = np.full((rows, max_blocks + 2), -1, np.int64)
+    table[:, :max_blocks] = numbers[:used].reshape(rows, max_blocks)
+    rows_of = rng.permutation(rows)
+    lengths = rng.integers(0, max_blocks * bs + 1, rows)
+    parents, children = rng.choice(rows_of[:base], forks), rows_of[base:]
+    tokens = rng.integers(0, max_blocks * bs + 5, forks)
+    for free in (forks + 3, forks // 2, 0):
+        pools.send()
+        run_fork(pools, parents, children, tokens, numbers[used:used + free], table, lengths, max_blocks)
+
+
+def test_fork_odd_rows_and_blocks():
+    pools = Pools(F16, 20, 4, 1, 16, layers=2)
+    table = np.array([[0, 1, 99], [2, -1, 3], [4, 5, 6], [7, 8, 9], [10, 11, 12], [13, 14, 15], [-4, -4, -4], [-4, -4, -4], [-4, -4, -4], [-4, -4, -4]])
+    # parents of more tokens than a row holds, of fewer than none, blocks that are none, rows that are none, its own child
+    run_fork(pools, [0, 0, 1, 2, -1, 3, 12, 4], [6, 7, 8, 9, 5, 3, 4, 10], [100, 11, 6, 9, 3, 3, 3, 3], [16, 99, 17, 18], table, [9, 7, 50, 3, 3, 3, 0, 0, 0, 0], 3)
+    pools.send()
+    run_fork(pools, [0, 1], [6, 7], [-5, 3], [16], table, [-9, 2 ** 31 - 1] + [0] * 8, 3)
+    pools.send()
+    run_fork(pools, [], [], [], [16], table, [0] * 10, 3)
+
+
+def run_compact(pools, table, lengths, max_blocks, out_pad=0):
+    blocks, bs = pools.shape[:2]
+    rows, stride = table.shape
+    before = np.full((rows, max_blocks + out_pad), -3)
+    d = B.CacheCompactDesc(pools.layout, rows, max_blocks, stride, max_blocks + out_pad, pools.layers or 1, pools.per_layer)
+    out, counts = up(np.concatenate([before.ravel(), [-7]]).astype(np.int32)), ints([-7] * 3)
+    n_work = B.ops_cache_compact_workspace(d)
+    work = work_of(n_work)
+    for _ in range(2):                       # from the old table again: the same
+        ok(B.ops_cache_compact(d, ints(table), ints(lengths), out, counts, *pools.dev, work))
+    want = S.compact(table, lengths, before, blocks, bs, max_blocks)
+    np.testing.assert_array_equal(out.to_array(np.int32), np.concatenate([want[0].ravel(), [-7]]))
+    assert counts.to_array(np.int32).tolist() == want[1] + [-7]
+    for g, w in zip(pools.fetch(), moved(pools, want[2], bs)):
+        np.testing.assert_array_equal(g, w)
+    behind(work, n_work)
+    return want
+
+
+@pytest.mark.parametrize("cache,order,blocks,bs,kv,dim,layers", [(F32, "thd", 1, 16, 2, 8, 1), (BF16, "htd", 63, 16, 3, 40, 3), (F16, "thd", 500, 1, 1, 64, 2), (F32, "htd", 130, 24, 5, 72, 2),
+                                                                 (BF16, "thd", 90, 7, 12, 256, 1), (BF16, "thd", 9000, 2, 1, 8, 1), (F16, "htd", 20000, 1, 2, 8, 2)])
+@pytest.mark.parametrize("share", [0.0, 0.05, 0.5, 0.95, 1.0])
+def test_compact(cache, order, blocks, bs, kv, dim, layers, share):
+    rng = np.random.default_rng(blocks)
+    used = int(blocks * share)
+    numbers = rng.permutation(blocks)[:used]
+    max_blocks = 1 + used // 7
+    rows = 8 + (used > 0)
+    pools = Pools(cache, blocks, bs, kv, dim, order, 8 if bs > 1 else 0, layers)
+    table, lengths, at = np.full((rows, max_blocks + 1), 2 ** 30), np.zeros(rows, int), 0
+    for i in range(rows):
+        n = min(used - at, max_blocks) if i < 8 else min(3, used, max_blocks)
+        table[i, :n] = numbers[at:at + n] if i < 8 else numbers[:n]             # (the last row shares its blocks)
+        lengths[i] = max(0, n * bs - int(rng.integers(0, bs)))
+        at += n if i < 8 else 0
+    run_compact(pools, table, lengths, max_blocks, out_pad=2)
+
+
+def test_compact_entries_that_are_no_blocks():
+    pools = Pools(BF16, 12, 4, 2, 16, layers=2)
+    run_compact(pools, np.array([[11, -1, 3], [12, 11, 2 ** 31 - 1], [7, 0, 0]]), [12, 100, -4], 3)
+    pools = Pools(BF16, 12, 4, 2, 16)
+    run_compact(pools, np.zeros((0, 3), int), [], 3)
+
+
+# ---- together -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind,cache", [(F32, F32), (F32, F16), (BF16, BF16)])
+@pytest.mark.parametrize("captured", [False, True])
+def test_serving_over_a_paged_cache(kind, cache, captured):
+    """Prompts in pieces, samples forked from them, single tokens of all, requests that end, a compaction now and then: sweep, fork, plan, append,
+    attend, score, compact, each on what the one before left on the device, against rows of plain arrays.  Captured: the calls of a step are
+    recorded into graphs once and replayed."""
+    rng = np.random.default_rng(5)
+    rows, kv, group, dim, bs, vocab, steps = 8, 2, 3, 32, 8, 501, 14
+    heads, width, blocks, room, top = kv * group, 12, 150, 112, 4
+    pools = Pools(cache, blocks, bs, kv, dim)
+    stream = ctypes.c_void_p()
+    hip("hipStreamCreateWithFlags", ctypes.byref(stream), 1)
+    size = 4 if kind == F32 else 2
+    table, table2 = (ints(np.full((rows, width), -1)) for _ in range(2))
+    cached, lengths, added = (ints(np.zeros(rows)) for _ in range(3))
+    parents, children, prefix = (ints(np.full(rows, -1)) for _ in range(3))
+    uses, free, counts, fork_counts, plan_counts = (ints(np.zeros(n)) for n in (blocks, blocks, 3, 2, 3))
+    starts, slots = ints(np.zeros(rows + 1)), ints(np.zeros(room))
+    kv_rows, q, out = B.DeviceBuffer(room * 2 * kv * dim * size), B.DeviceBuffer(room * heads * dim * size), B.DeviceBuffer(room * heads * dim * size)
+    logits, given = B.DeviceBuffer(room * vocab * size), ints(np.zeros(room))
+    score, rank, entropy, best, best_score = (B.DeviceBuffer(4 * n) for n in (room, room, room, room * top, room * top))
+    sw = B.BlockSweepDesc(rows, blocks, bs, width, width)
+    fk = B.CacheForkDesc(pools.layout, rows, rows, width, width, 20, 1, 0)
+    plan = B.BlockPlanDesc(rows, blocks, bs, width, width, 40, room)
+    app = B.CacheAppendDesc(pools.layout, kind, room, 2 * kv * dim, dim, 2 * kv * dim, dim)
+    att = B.ChunkAttentionDesc(pools.layout, kind, rows, heads, room, width, width, width * bs, 0, dim ** -0.5, heads * dim, dim, heads * dim, dim)
+    sc = B.TokenScoresDesc(kind, room, vocab, top, vocab)
+    cm = B.CacheCompactDesc(pools.layout, rows, width, width, width, 1, 0)
+    works = [work_of(n) for n in (B.ops_block_sweep_workspace(sw), B.ops_chunk_attention_workspace(att), B.ops_token_scores_workspace(sc), B.ops_cache_compact_workspace(cm))]
+
+    def put(buf, arr):
+        arr = np.ascontiguousarray(arr)
+        hip("reef_hal_memcpy_h2d", buf.ptr, arr.ctypes.data_as(ctypes.c_void_p), ctypes.c_size_t(arr.nbytes))
+
+    def fork(s):
+        ok(B.ops_block_sweep(sw, table, cached, uses, free, counts, works[0], s))
+        ok(B.ops_cache_fork(fk, parents, children, prefix, free, table, cached, fork_counts, *pools.dev, s))
+        ok(B.ops_block_sweep(sw, table, cached, uses, free, counts, works[0], s))
+
+    def step(s):
+        ok(B.ops_block_plan(plan, cached, added, free, table, lengths, starts, slots, plan_counts, s))
+        ok(B.ops_cache_append(app, kv_rows, kv_rows.ptr.value + kv * dim * size, slots, *pools.dev, s))
+        ok(B.ops_chunk_attention(att, q, *pools.dev, table, starts, cached, lengths, out, None, works[1], s))
+        ok(B.ops_token_scores(sc, logits, given, score, rank, entropy, best, best_score, works[2], s))
+
+    def compact(s):
+        ok(B.ops_cache_compact(cm, table, lengths, table2, counts, *pools.dev, works[3], s))
+
+    calls, graphs = (fork, step, compact), []
+    if captured:
+        for c in calls:
+            graph, run = ctypes.c_void_p(), ctypes.c_void_p()
+            hip("hipStreamBeginCapture", stream, 0)
+            c(stream)
+            hip("hipStreamEndCapture", stream, ctypes.byref(graph))
+            hip("hipGraphInstantiate", ctypes.byref(run), graph, None, None, ctypes.c_size_t(0))
+            graphs.append((graph, run))
+
+    def do(i):
+        if captured:
+            hip("hipGraphLaunch", graphs[i][1], stream)
+        else:
+            calls[i](stream)
+        hip("hipStreamSynchronize", stream)
+
+    seqs = [[] for _ in range(rows)]             # plain: each row's list of (key, value) rows
+    for number in range(steps):
+        # requests that end, samples of others in their place
+        par, chi, pre = np.full(rows, -1), np.full(rows, -1), np.zeros(rows, int)
+        live = [i for i in range(rows) if seqs[i]]
+        if number and live:
+            for i in rng.permutation(rows)[:2]:
+                p = int(rng.choice(live))
+                if p not in chi and i not in par and p != i:
+                    seqs[i] = seqs[p][:int(rng.integers(0, len(seqs[p]) + 1))]
+                    k = int((chi >= 0).sum())
+                    par[k], chi[k], pre[k] = p, i, len(seqs[i])
+                    live = [j for j in live if j != i]
+        put(parents, par.astype(np.int32))
+        put(children, chi.astype(np.int32))
+        put(prefix, pre.astype(np.int32))
+        do(0)
+        assert fork_counts.to_array(np.int32)[1] == (par < 0).sum()
+        assert cached.to_array(np.int32).tolist() == [len(x) for x in seqs]
+        more = np.array([int(rng.integers(1, 14)) if len(seqs[i]) < 20 else 1 for i in range(rows)]) * (rng.random(rows) < 0.8)
+        more = np.minimum(more, [width * bs - len(x) for x in seqs])
+        total = int(more.sum())
+        assert total <= room
+        put(added, more.astype(np.int32))
+        new = R.encode(rng.standard_normal((room, 2, kv, dim)).astype(np.float32), kind)
+        put(kv_rows, new)
+        qv = R.encode(rng.standard_normal((room, heads, dim)).astype(np.float32), kind)
+        put(q, qv)
+        lg = R.encode((rng.standard_normal((room, vocab)) * 2).astype(np.float32), kind)
+        put(logits, lg)
+        tok = rng.integers(0, vocab, room).astype(np.int32)
+        put(given, tok)
+        do(1)
+        assert plan_counts.to_array(np.int32)[1:].tolist() == [total, 0]
+        got, at = R.decode(out.to_array(R.np_type(kind)).reshape(room, heads, dim), kind), 0
+        for i in range(rows):
+            first = len(seqs[i])
+            for t in range(at, at + more[i]):
+                seqs[i].append(R.decode(new[t] if kind == cache else R.encode(new[t].astype(np.float32), cache), cache))
+            if more[i]:
+                have = np.array(seqs[i])
+                want, _, tol, _ = S.chunk(R.decode(qv[at:at + more[i]], kind), have[:, 0].transpose(1, 0, 2), have[:, 1].transpose(1, 0, 2), first, len(have), dim ** -0.5, 0,
+                                          kind, cache)
+                assert (np.abs(got[at:at + more[i]] - want) <= tol + HALF[kind] * np.abs(want)).all(), (number, i)
+            at += more[i]
+        want = S.scores(R.decode(lg, kind), tok, top)
+        np.testing.assert_array_equal(rank.to_array(np.int32), want[1])
+        np.testing.assert_array_equal(best.to_array(np.int32).reshape(room, top), want[3])
+        assert np.abs(score.to_array() - want[0]).max() <= 2.0 ** -18 * (1 + np.abs(want[0]).max())
+        if number % 3 == 2:
+            do(2)
+            used, _ = counts.to_array(np.int32)[:2]
+            t2 = table2.to_array(np.int32).reshape(rows, width)
+            named = {int(t2[i, j]) for i in range(rows) for j in range(-(-len(seqs[i]) // bs))}
+            assert named == set(range(used))
+            put(table, t2)
+        put(cached, np.array([len(x) for x in seqs], np.int32))
+    for graph, run in graphs:
+        hip("hipGraphExecDestroy", run)
+        hip("hipGraphDestroy", graph)
+    hip("hipStreamDestroy", stream)
