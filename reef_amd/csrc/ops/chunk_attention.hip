@@ -1,14 +1,20 @@
 // Attention of the new tokens of all requests over a paged key-value cache (reef_ops_chunk_attention).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "ops_common.h"
 
 namespace {
 using namespace reef_ops;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kRows = 32;                    // query rows of a wavefront: heads of one token next to each other, token after token
+constexpr int kTileRows = kWaves * kRows;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int32_t kLeast = 512;              // cached tokens a share at least
+constexpr int kGroups = 512;                 // workgroups that the shares of all tiles are to make
+constexpr float kSlack = 8.0f;               // powers of two by which weights may pass their reference
 
 struct Args {
     reef_chunk_attention_desc d;
@@ -16,60 +22,678 @@ struct Args {
     const int32_t *table, *starts, *cached, *lengths;
     void* out;
     float* lse;
-    Divider block;
+    int4* info;             // [request], where there are many: first item, shares, first slot, tiles
+    int32_t* list;          // the number of items, then the request of each
+    float* parts;           // [slot][cache head][row of the tile][head_dim], sums that are not divided yet
+    float2* stats;          // [slot][cache head][row of the tile]: power of two that they are to be multiplied by, sum of the weights
+    float scale;            // |scale| log2 e, or log2 e where it is 0
+    uint32_t flip;          // of the queries' sign where scale is negative
+    int32_t zero;           // scale is 0
+    int32_t group;
+    int32_t budget;         // shares that all tiles are cut into, beside one each; 0: tiles are not split
+    int32_t most_items, most_slots;
+    Divider block, by_group;
+};
+
+// A request: the rows of its new tokens, and how they are worked on.
+struct Request {
+    int32_t first, added, cached, n;         // first row, rows; tokens in front of them and in all
+    int32_t tiles;
+};
+// An item: a tile of rows over a share of the tokens that they see.
+struct Item {
+    Request r;
+    int32_t request, tile, share, shares, slot;   // tile < 0: there is no such item; slot of the tile's first share
 };
 
 __device__ inline int32_t start_of(const Args& a, int32_t i) { return max(0, min(a.starts[i], a.d.tokens)); }
+__device__ inline Request request_of(const Args& a, int32_t i) {
+    Request r;
+    r.first = start_of(a, i);
+    r.added = max(0, start_of(a, i + 1) - r.first);
+    r.cached = held_length(a.cached[i], a.d.max_blocks, a.d.cache.block_size);
+    r.n = held_length(a.lengths[i], a.d.max_blocks, a.d.cache.block_size);
+    r.tiles = (r.added * a.group + kTileRows - 1) / kTileRows;
+    return r;
+}
+// The cached tokens [.x, .y) that some row of a tile sees.  (Places may pass 2^31, not 2^32.)
+__device__ inline uint2 span_of(const Args& a, const Request& r, int32_t tile) {
+    const uint32_t last = (uint32_t)min((tile + 1) * kTileRows, r.added * a.group) - 1;
+    const uint32_t p0 = (uint32_t)r.cached + divided((uint32_t)tile * kTileRows, a.by_group), p1 = (uint32_t)r.cached + divided(last, a.by_group);
+    if (p0 >= (uint32_t)r.n) return make_uint2(0, 0);
+    return make_uint2(a.d.window && p0 + 1 > (uint32_t)a.d.window ? p0 + 1 - a.d.window : 0, min((uint32_t)r.n, p1 + 1));
+}
+// What a request's tiles see at most, and on the average (spans grow with the tile, by steps that do not).
+__device__ inline void size_up(const Args& a, const Request& r, float* most, float* all) {
+    *most = *all = 0.0f;
+    if (!r.tiles) return;
+    const uint2 x = span_of(a, r, 0), y = span_of(a, r, r.tiles - 1);
+    const float u = (float)(x.y - x.x), v = (float)(y.y - y.x);
+    *most = fmaxf(u, v);
+    *all = (float)r.tiles * (u + v) * 0.5f;
+}
+// Tokens of a share: sum over the tiles of ceil(most / tokens) <= 2 budget + tiles, as most <= u + v.  (The sum of the requests' sizes is rounded up by more
+// than its additions lose.)
+__device__ inline float tokens_of(float all, int32_t budget) { return fmaxf((float)kLeast, all * 1.02f / (float)budget); }
+__device__ inline int32_t shares_of(float most, float tokens) { return max(1, (int32_t)ceilf(most / tokens)); }
 
-// A wavefront for each row and head, a token of the cache after the other.
-template <class Q, class C>
-__global__ void __launch_bounds__(kThreads) chunk_attention(Args a) {
-    const reef_chunk_attention_desc& d = a.d;
-    const int lane = threadIdx.x & 63, D = d.cache.head_dim;
-    const int64_t id = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-    if (id >= (int64_t)d.tokens * d.heads) return;
-    const int32_t row = (int32_t)(id / d.heads), h = (int32_t)(id - (int64_t)row * d.heads);
-    int32_t lo = 0, hi = d.requests;         // the last request that starts at or in front of the row
-    while (hi - lo > 1) {
-        const int32_t mid = (lo + hi) / 2;
-        if (start_of(a, mid) <= row) lo = mid;
-        else hi = mid;
+template <class V>
+__device__ inline V before_me(V v) {         // exclusive prefix sums over the wavefront
+    V at = v;
+    for (int x = 1; x < 64; x <<= 1) {
+        const V o = __shfl_up(at, x);
+        if ((int)(threadIdx.x & 63) >= x) at += o;
     }
-    const int32_t first = start_of(a, lo);
-    if (row < first || row >= start_of(a, lo + 1)) return;
-    const int32_t n = held_length(a.lengths[lo], d.max_blocks, d.cache.block_size);
-    const int64_t place = (int64_t)held_length(a.cached[lo], d.max_blocks, d.cache.block_size) + (row - first);
-    int32_t begin = 0, end = 0;
-    if (place < n) {
-        end = (int32_t)place + 1;
-        begin = d.window ? max(0, end - d.window) : 0;
+    return at - v;
+}
+
+// Up to kFew requests each wavefront finds its item by itself, a request a lane; more are listed by a launch ahead.
+constexpr int32_t kFew = 64;
+__device__ inline Item find_item(const Args& a, int32_t id) {
+    Item it;
+    it.tile = -1;
+    int32_t local;
+    if (a.list) {
+        if (id >= a.list[0]) return it;
+        it.request = a.list[1 + id];
+        const int4 info = a.info[it.request];
+        it.r = request_of(a, it.request);
+        local = id - info.x;
+        it.shares = info.y;
+        it.slot = info.z;
+    } else {
+        const int lane = threadIdx.x & 63;
+        Request r{};
+        if (lane < a.d.requests) r = request_of(a, lane);
+        int32_t shares = 1;
+        if (a.budget) {
+            float most, all;
+            size_up(a, r, &most, &all);
+            for (int x = 32; x; x >>= 1) all += __shfl_xor(all, x);
+            shares = shares_of(most, tokens_of(all, a.budget));
+        }
+        const int32_t mine = r.tiles * shares, at = before_me(mine), slot = before_me(shares > 1 ? mine : 0);
+        const uint64_t who = __builtin_amdgcn_ballot_w64(id >= at && id < at + mine);
+        if (!who) return it;
+        const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(who));
+        it.request = l;
+        it.r.first = __builtin_amdgcn_readlane(r.first, l);
+        it.r.added = __builtin_amdgcn_readlane(r.added, l);
+        it.r.cached = __builtin_amdgcn_readlane(r.cached, l);
+        it.r.n = __builtin_amdgcn_readlane(r.n, l);
+        it.r.tiles = __builtin_amdgcn_readlane(r.tiles, l);
+        it.shares = __builtin_amdgcn_readlane(shares, l);
+        it.slot = __builtin_amdgcn_readlane(slot, l);
+        local = id - __builtin_amdgcn_readlane(at, l);
+    }
+    // the last tiles, which see most, first
+    const int32_t k = local / it.shares;
+    it.share = local - k * it.shares;
+    it.tile = it.r.tiles - 1 - k;
+    it.slot += k * it.shares;
+    return it;
+}
+
+constexpr int kListThreads = 1024;
+__global__ void __launch_bounds__(kListThreads) list_items(Args a) {
+    constexpr int kListWaves = kListThreads / 64;
+    __shared__ float sums[kListWaves];
+    __shared__ int2 counts[kListWaves];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int32_t R = a.d.requests, per = (R + kListThreads - 1) / kListThreads, lo = min(R, tid * per), hi = min(R, lo + per);
+    float tokens = 0.0f;
+    if (a.budget) {
+        float sum = 0.0f;
+        for (int32_t i = lo; i < hi; ++i) {
+            float most, all;
+            size_up(a, request_of(a, i), &most, &all);
+            sum += all;
+        }
+        for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
+        if (lane == 0) sums[wave] = sum;
+        __syncthreads();
+        sum = 0.0f;
+        for (int w = 0; w < kListWaves; ++w) sum += sums[w];
+        tokens = tokens_of(sum, a.budget);
+    }
+    auto shares_and_tiles = [&](int32_t i) {
+        const Request r = request_of(a, i);
+        int32_t shares = 1;
+        if (a.budget) {
+            float most, all;
+            size_up(a, r, &most, &all);
+            shares = shares_of(most, tokens);
+        }
+        return make_int2(shares, r.tiles);
+    };
+    int32_t items = 0, slots = 0;
+    for (int32_t i = lo; i < hi; ++i) {
+        const int2 x = shares_and_tiles(i);
+        items += x.x * x.y;
+        if (x.x > 1) slots += x.x * x.y;
+    }
+    int32_t item = before_me(items), slot = before_me(slots), all = 0;
+    if (lane == 63) counts[wave] = make_int2(item + items, slot + slots);
+    __syncthreads();
+    for (int w = 0; w < kListWaves; ++w) {
+        if (w < wave) {
+            item += counts[w].x;
+            slot += counts[w].y;
+        }
+        all += counts[w].x;
+    }
+    for (int32_t i = lo; i < hi; ++i) {
+        const int2 x = shares_and_tiles(i);
+        a.info[i] = make_int4(item, x.x, slot, x.y);
+        for (int32_t k = 0; k < x.x * x.y && item + k < a.most_items; ++k) a.list[1 + item + k] = i;
+        item += x.x * x.y;
+        if (x.x > 1) slot += x.x * x.y;
+    }
+    if (tid == 0) a.list[0] = min(all, a.most_items);
+}
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+__device__ inline f32x16 product(u32x4 a, u32x4 b, f32x16 c, _Float16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+__device__ inline f32x16 product(u32x4 a, u32x4 b, f32x16 c, __bf16) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// Two values as N terms of a 16-bit type, whose sums they are but for what the last rounds off.  The first of three is cut, so that it is
+// finite where the value is.
+template <int N>
+__device__ inline void terms(float a, float b, uint32_t (&t)[N], __bf16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    if constexpr (N == 3) {
+        t[0] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+        a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+        b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+        const bf16x2 x = {(__bf16)a, (__bf16)b};
+        t[1] = __builtin_bit_cast(uint32_t, x);
+        a -= __uint_as_float(t[1] << 16);
+        b -= __uint_as_float(t[1] & 0xFFFF0000u);
+    }
+    const bf16x2 last = {(__bf16)a, (__bf16)b};
+    t[N - 1] = __builtin_bit_cast(uint32_t, last);
+}
+template <int N>
+__device__ inline void terms(float a, float b, uint32_t (&t)[N], _Float16) {
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const f16x2 x = {(_Float16)a, (_Float16)b};
+        t[i] = __builtin_bit_cast(uint32_t, x);
+        a -= (float)x[0];
+        b -= (float)x[1];
+    }
+}
+
+// A value of both halves of the wavefront, joined: lanes l and l + 32 have the same row.
+__device__ inline float other_max(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ inline float other_sum(float x) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ inline uint32_t wave_max(uint32_t v) {
+    for (int x = 32; x; x >>= 1) v = max(v, (uint32_t)__shfl_xor(v, x));
+    return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ inline uint32_t wave_min(uint32_t v) { return ~wave_max(~v); }
+
+template <class Q>
+__device__ inline void put4(Q* to, float a, float b, float c, float d) {
+    typedef Q Q4 __attribute__((ext_vector_type(4)));
+    const Q4 x = {(Q)a, (Q)b, (Q)c, (Q)d};
+    *(Q4*)to = x;
+}
+
+// How heads of up to DP values lie in LDS: rows of kPitch bytes, their 16-byte pieces exchanged by the row's number, so that neither 16 rows' same
+// piece nor four rows' same 64 bytes meet in a bank.
+template <int DP>
+struct Near {
+    static constexpr int kPieces = DP <= 64 ? 8 : DP <= 128 ? 16 : 32, kPitch = kPieces * 16;
+    static __device__ inline uint32_t turn(uint32_t row) {
+        return kPieces == 8 ? (row >> 1 & 1) << 2 | (row >> 2 & 3) : (row & 3) << 2 | (row >> 2 & 3);
+    }
+    static __device__ inline uint32_t at(uint32_t row, uint32_t piece) { return row * kPitch + ((piece ^ turn(row)) << 4); }
+};
+
+// A tile of 128 query rows over a share of the tokens they see, one cache head: each wavefront has 32 rows, all of them the keys and values that
+// the workgroup brings to LDS, 64 tokens at a time (32 of heads over 128 and of 32-bit caches).
+//
+// Both products are 32x32x16 MFMAs:  S^T[token][row] = K Q^T, then O^T[dim][row] = V^T P^T.  A product does not care in which order its k
+// runs: S^T leaves lane (row, half h) the tokens 8 j + 4 h + {0..3} of 32, so these are its k, and V^T's operand comes transposed out of LDS four tokens a
+// read.  So weights stay in the lane that made them, and a row's reference, sum and rescaling are one value a lane.
+//
+// Weights are 2^(s c - R): R is a whole number near the largest s c so far (within kSlack above), so that one rounding makes the exponent, and rescaling
+// by 2^(R - R') is exact and rare.  For fp16, whose weights want room below, they are 2^kGrow times larger.
+//
+// 32-bit queries over 16-bit caches are two terms of fp16 or three of bf16 each, and so are their weights; 32-bit caches are three terms of bf16 on
+// both sides, six products (the others are below 2^-22).  Weights of 16-bit types are rounded to the type once: half a step of the type of each at most, which in their mean is
+// no more than the output's own rounding (two terms would take 1.4 times as long).
+template <class Q, class C, int DP>
+__global__ void __launch_bounds__(kThreads, sizeof(Q) == 2 && DP <= 128 ? 2 : 1) chunk_attention(Args a) {
+    using E = std::conditional_t<sizeof(C) == 4, __bf16, C>;                  // what is multiplied
+    constexpr bool kHalf = __is_same(E, _Float16);
+    constexpr int kTermsC = sizeof(C) == 4 ? 3 : 1, kTermsQ = sizeof(Q) == 2 ? 1 : kHalf ? 2 : 3;
+    constexpr float kGrow = kHalf ? 6.0f : 0.0f;                              // 2^(6 + 8 + 1/2) < 65504
+    constexpr int kTile = kTermsC == 3 || DP > 128 ? 32 : 64, kSub = kTile / 32, kBuffers = kTermsC == 3 ? 1 : 2;
+    constexpr int kSteps = DP / 16, kSlabs = DP / 32;
+    using N = Near<DP>;
+    constexpr int kPlane = kTile * N::kPitch, kBuffer = 2 * kTermsC * kPlane;
+    constexpr int kRowPieces = DP * (int)sizeof(C) / 16, kMine = kTile * kRowPieces / kThreads;    // 16-byte pieces of a row in memory; of a thread
+    static_assert(kTile * kRowPieces % kThreads == 0, "");
+    __shared__ __align__(16) unsigned char tiles[kBuffers * kBuffer];
+    __shared__ int64_t offsets[kWaves][2][kTile];
+
+    const reef_chunk_attention_desc& d = a.d;
+    const int32_t kvh = (int32_t)(blockIdx.x % (uint32_t)d.cache.kv_heads);
+    const int32_t id = (int32_t)(blockIdx.x / (uint32_t)d.cache.kv_heads);
+    const Item it = find_item(a, id);
+    if (it.tile < 0) return;
+    const Request& r = it.r;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
+    const int D = d.cache.head_dim;
+
+    // this lane's row
+    const uint32_t rows = (uint32_t)(r.added * a.group), in_tile = (uint32_t)(wave * kRows + n), row = (uint32_t)it.tile * kTileRows + in_tile;
+    const bool valid = row < rows;
+    const uint32_t token = divided(row, a.by_group);
+    const int32_t head = kvh * a.group + (int32_t)(row - token * a.by_group.by);
+    const int64_t out_row = (int64_t)r.first + token;
+    const uint32_t place = (uint32_t)r.cached + token;
+    const uint32_t hi = valid && place < (uint32_t)r.n ? place + 1 : 0, lo = d.window && hi > (uint32_t)d.window ? hi - d.window : 0;
+    // what all rows of the wavefront see, and what some do
+    const uint32_t all_hi = wave_min(valid ? hi : ~0u), all_lo = wave_max(valid ? lo : 0), some_hi = wave_max(hi), some_lo = wave_min(hi ? lo : ~0u);
+
+    const uint2 span = span_of(a, r, it.tile);
+    uint32_t begin = span.x, end = span.y;
+    if (it.shares > 1) {
+        const uint32_t count = (end - begin + kTile - 1) / kTile;
+        const uint32_t x = (uint32_t)((uint64_t)count * it.share / it.shares), y = (uint32_t)((uint64_t)count * (it.share + 1) / it.shares);
+        end = min(end, begin + y * kTile);
+        begin = min(end, begin + x * kTile);
     }
     const PagedView view{d.cache.blocks, d.cache.block_stride, d.cache.slot_stride};
-    const int32_t* table = a.table + (int64_t)lo * d.table_stride;
-    const int kvh = h / (d.heads / d.cache.kv_heads), at = lane * 4;
-    float q[4] = {0, 0, 0, 0}, o[4] = {0, 0, 0, 0}, m = -INFINITY, l = 0.0f;
-    if (at < D)
-        for (int e = 0; e < 4; ++e) q[e] = (float)((const Q*)a.query)[row * d.query_stride + h * d.query_head_stride + at + e] * (d.scale * kLog2e);
-    for (int32_t t = begin; t < end; ++t) {
-        const uint32_t entry = divided((uint32_t)t, a.block);
-        const int64_t from = paged_row(view, table[entry], (int32_t)(t - entry * a.block.by));
-        if (from < 0) continue;
-        const int64_t base = from + kvh * d.cache.head_stride + at;
-        float s = 0.0f, v[4] = {0, 0, 0, 0};
-        if (at < D)
-            for (int e = 0; e < 4; ++e) {
-                s = fmaf(q[e], (float)((const C*)a.key_cache)[base + e], s);
-                v[e] = (float)((const C*)a.value_cache)[base + e];
+    const C* keys = (const C*)a.key_cache + kvh * d.cache.head_stride;
+    const C* values = (const C*)a.value_cache + kvh * d.cache.head_stride;
+    const int32_t* table = a.table + (int64_t)it.request * d.table_stride;
+
+    // the table's entry of one token of a tile a lane; -1: no token
+    auto entry_of = [&](uint32_t t0) -> int32_t {
+        const uint32_t t = t0 + lane;
+        return lane < kTile && t < end ? table[divided(t, a.block)] : -1;
+    };
+    // its place, for all lanes to read; which of the tile's tokens there are
+    auto find = [&](uint32_t t0, int32_t entry, int buffer) -> uint64_t {
+        int64_t at = -1;
+        if (lane < kTile) {
+            const uint32_t t = t0 + lane;
+            at = paged_row(view, entry, (int32_t)(t - divided(t, a.block) * a.block.by));
+            offsets[wave][buffer][lane] = at < 0 ? 0 : at;
+        }
+        return __builtin_amdgcn_ballot_w64(at >= 0);
+    };
+    constexpr uint64_t kAll = kTile == 64 ? ~0ull : 0xFFFFFFFFull;
+    u32x4 k_on_way[kMine], v_on_way[kMine];
+    auto load = [&](int buffer) {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int x = i * kThreads + threadIdx.x, at = x / kRowPieces, piece = x - at * kRowPieces;
+            const int64_t from = offsets[wave][buffer][at] + (piece * 16 < D * (int)sizeof(C) ? piece * (16 / (int)sizeof(C)) : 0);
+            k_on_way[i] = *(const u32x4*)(keys + from);
+            v_on_way[i] = *(const u32x4*)(values + from);
+        }
+    };
+    // into LDS: zeros where there is no token, or no such dimension
+    auto store = [&](int buffer, uint64_t there) {
+        unsigned char* const to = tiles + buffer * kBuffer;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int x = i * kThreads + threadIdx.x, at = x / kRowPieces, piece = x - at * kRowPieces;
+            if (there != kAll || D != DP) {
+                const bool inside = (there >> at & 1) && piece * 16 < D * (int)sizeof(C);
+                if (!inside) k_on_way[i] = v_on_way[i] = {0, 0, 0, 0};
             }
-        for (int x = 32; x; x >>= 1) s += __shfl_xor(s, x);
-        const float top = fmaxf(m, s), of = top == -INFINITY ? 0.0f : top, f = __builtin_amdgcn_exp2f(m - of), p = __builtin_amdgcn_exp2f(s - of);
-        m = top;
-        l = l * f + p;
-        for (int e = 0; e < 4; ++e) o[e] = fmaf(o[e], f, p * v[e]);
+            if constexpr (kTermsC == 1) {
+                *(u32x4*)(to + N::at(at, piece)) = k_on_way[i];
+                *(u32x4*)(to + kPlane + N::at(at, piece)) = v_on_way[i];
+            } else {
+                const uint32_t place = N::at(at, piece >> 1) + (piece & 1) * 8;
+#pragma unroll
+                for (int kv = 0; kv < 2; ++kv) {
+                    const u32x4 w = kv ? v_on_way[i] : k_on_way[i];
+                    uint32_t t[2][3];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const float x0 = __uint_as_float(w[2 * j]), x1 = __uint_as_float(w[2 * j + 1]);
+                        terms(x0, x1, t[j], __bf16());
+                        // an infinity is its first term alone, and so is a NaN, which must not be cut to one
+                        const bool odd0 = !(fabsf(x0) < INFINITY), odd1 = !(fabsf(x1) < INFINITY);
+                        if (odd0 | odd1) {
+                            const uint32_t keep = (odd0 ? 0 : 0xFFFFu) | (odd1 ? 0 : 0xFFFF0000u);
+                            t[j][1] &= keep;
+                            t[j][2] &= keep;
+                            if (x0 != x0) t[j][0] |= 0x7FFFu;
+                            if (x1 != x1) t[j][0] |= 0x7FFF0000u;
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) *(u32x2*)(to + (kv * 3 + x) * kPlane + place) = u32x2{t[0][x], t[1][x]};
+                }
+            }
+        }
+    };
+
+    uint64_t there = 0, there_next = 0;
+    int32_t entry = begin < end ? entry_of(begin) : -1;        // (asked for ahead of the queries: keys and values wait for them)
+
+    // the queries: this lane's row, the pieces that its half of the keys has
+    float scale = a.scale, shrink = 1.0f;    // scores: products * shrink * scale
+    u32x4 q[kTermsQ][kSteps];
+    {
+        const Q* from = (const Q*)a.query + out_row * d.query_stride + head * d.query_head_stride;
+        constexpr int kWords = (int)sizeof(Q) * 2;             // of eight values
+        uint32_t raw[kSteps][kWords];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+            const int at = s * 16 + h * 8;
+#pragma unroll
+            for (int w = 0; w < kWords; w += 4) {
+                u32x4 x = {0, 0, 0, 0};
+                if (valid && at < D && !a.zero) x = *(const u32x4*)(from + at + w * 4 / (int)sizeof(Q));
+#pragma unroll
+                for (int i = 0; i < 4; ++i) raw[s][w + i] = x[i] ^ a.flip;
+            }
+        }
+        if constexpr (kTermsQ == 1) {
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) q[0][s] = {raw[s][0], raw[s][1], raw[s][2], raw[s][3]};
+        } else {
+            // Terms of fp16 need room below: a row is scaled by a power of two to 2^13; bf16 has it but for values below 2^-133, so rows below 2^-100 are
+            // brought there.
+            float grow = 1.0f, top = 0.0f;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int w = 0; w < kWords; ++w) top = fmaxf(top, fabsf(__uint_as_float(raw[s][w])));
+            top = other_max(top);
+            if (top > 0.0f && top < INFINITY) {
+                const int power = (int)(__float_as_uint(top) >> 23) - 127, by = kHalf ? min(126, 13 - power) : max(0, -100 - power);
+                grow = __uint_as_float((uint32_t)(127 + by) << 23);
+                const float back = __uint_as_float((uint32_t)(127 - by) << 23);
+                // One factor where it is one: large queries and a large scale may pass 32 bits together where a product is 0.
+                if (back > 1.0f && scale > 1.0f) shrink = back;
+                else scale *= back;
+            }
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    uint32_t t[kTermsQ];
+                    terms(__uint_as_float(raw[s][2 * w]) * grow, __uint_as_float(raw[s][2 * w + 1]) * grow, t, E());
+#pragma unroll
+                    for (int x = 0; x < kTermsQ; ++x) q[x][s][w] = t[x];
+                }
+        }
+        if (scale == 0.0f) scale = 0x1p-149f;                  // (weights of what is not seen are 2^(-infinity scale))
     }
-    if (at < D)
-        for (int e = 0; e < 4; ++e) ((Q*)a.out)[row * d.out_stride + h * d.out_head_stride + at + e] = (Q)(l == 0.0f ? 0.0f : o[e] / l);
-    if (lane == 0 && a.lse) a.lse[id] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * kLn2;
+
+    float R = -INFINITY, l = 0.0f;
+    f32x16 o[kSlabs];
+#pragma unroll
+    for (int m = 0; m < kSlabs; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[m][i] = 0.0f;
+
+    // where this lane reads: keys' row n; values' rows 4 (lane / 32) + (lane % 16) / 4, four dimensions from 16 (lane / 16 % 2) + 4 (lane % 4) on
+    const int t16 = lane & 15;
+    const uint32_t v_row = (uint32_t)(4 * h + (t16 >> 2)), v_piece = (uint32_t)(2 * (lane >> 4 & 1) + ((t16 & 3) >> 1)), v_byte = (uint32_t)(t16 & 1) * 8;
+
+    auto work = [&](uint32_t t0, int buffer, auto is_masked) {
+        constexpr bool kMasked = decltype(is_masked)::value;
+        const unsigned char* const k_tile = tiles + buffer * kBuffer;
+        const unsigned char* const v_tile = k_tile + kTermsC * kPlane;
+        f32x16 s[kSub];
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                const unsigned char* const from = k_tile + u * 32 * N::kPitch + N::at(n, 2 * c + h);
+                if constexpr (kTermsC == 1) {
+                    const u32x4 k = *(const u32x4*)from;
+#pragma unroll
+                    for (int x = kTermsQ - 1; x >= 0; --x) s[u] = product(k, q[x][c], s[u], E());
+                } else {
+                    u32x4 k[3];
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) k[x] = *(const u32x4*)(from + x * kPlane);
+#pragma unroll
+                    for (int both = 2; both >= 0; --both)
+#pragma unroll
+                        for (int x = both; x >= 0; --x) s[u] = product(k[x], q[both - x][c], s[u], E());
+                }
+            }
+        uint32_t seen[kSub];
+        if constexpr (kMasked) {
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+                const uint32_t in_pool = (uint32_t)(there >> (u * 32));
+                seen[u] = 0;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const uint32_t at = 8 * (i >> 2) + 4 * h + (i & 3), t = t0 + u * 32 + at;
+                    const bool yes = t >= lo && t < hi && (in_pool >> at & 1);
+                    seen[u] |= yes ? 1u << i : 0;
+                    if (!yes) s[u][i] = -INFINITY;
+                }
+            }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                if constexpr (kHalf && kTermsQ > 1) s[u][i] *= shrink;
+                top = fmaxf(top, s[u][i]);
+            }
+        top = other_max(top) * scale;
+        const bool passes = top > R + kSlack;
+        if (__builtin_amdgcn_ballot_w64(passes)) {
+            const float next = passes ? rintf(top) : R;
+            const float f = passes ? __builtin_amdgcn_exp2f(R - next) : 1.0f;
+            R = next;
+            l *= f;
+#pragma unroll
+            for (int m = 0; m < kSlabs; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[m][i] *= f;
+        }
+        const float base = R == -INFINITY ? 0.0f : R;
+        float times = scale, plus = kGrow - base;
+        // From 2^20 on the sum above is not exact: scores are rounded first there.
+        if (__builtin_amdgcn_ballot_w64(fabsf(base) >= 0x1p20f)) {
+#pragma unroll
+            for (int u = 0; u < kSub; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+#pragma clang fp contract(off)
+                    const float x = s[u][i] * scale;
+                    s[u][i] = x - base;
+                }
+            times = 1.0f;
+            plus = kGrow;
+        }
+#pragma unroll
+        for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], times, plus));
+                l += s[u][i];
+            }
+#pragma unroll
+        for (int c = 0; c < kTile / 16; ++c) {
+            u32x4 p[kTermsQ];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t t[kTermsQ];
+                terms(s[c >> 1][(c & 1) * 8 + 2 * w], s[c >> 1][(c & 1) * 8 + 2 * w + 1], t, E());
+#pragma unroll
+                for (int x = 0; x < kTermsQ; ++x) p[x][w] = t[x];
+            }
+#pragma unroll
+            for (int m = 0; m < kSlabs; ++m) {
+                u32x4 v[kTermsC];
+#pragma unroll
+                for (int x = 0; x < kTermsC; ++x) {
+                    typedef short s4 __attribute__((ext_vector_type(4)));
+                    typedef __attribute__((address_space(3))) s4 near_s4;
+                    const unsigned char* const from = v_tile + x * kPlane + c * 16 * N::kPitch + v_byte;
+                    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((near_s4*)(from + N::at(v_row, 4 * m + v_piece))));
+                    const u32x2 z = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((near_s4*)(from + N::at(v_row + 8, 4 * m + v_piece))));
+                    v[x] = {y[0], y[1], z[0], z[1]};
+                }
+                if constexpr (kMasked) {
+                    // Infinities and NaN among the values: no row may have them times 0, those that see them have NaN.
+                    constexpr uint32_t kOdd = kHalf ? 0x7C00u : 0x7F80u, kOne = kHalf ? 0x3C00u : 0x3F80u;
+                    bool odd = false;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) odd |= (v[0][w] & kOdd) == kOdd || (v[0][w] >> 16 & kOdd) == kOdd;
+                    if (__builtin_amdgcn_ballot_w64(odd)) {
+                        u32x4 which, who;
+                        f32x16 bad;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const bool x = (v[0][w] & kOdd) == kOdd, y = (v[0][w] >> 16 & kOdd) == kOdd;
+                            which[w] = (x ? kOne : 0) | (y ? kOne << 16 : 0);
+                            v[0][w] &= (x ? 0 : 0xFFFFu) | (y ? 0 : 0xFFFF0000u);
+                            const uint32_t mine = seen[c >> 1] >> ((c & 1) * 8 + 2 * w);
+                            who[w] = (mine & 1 ? kOne : 0) | (mine & 2 ? kOne << 16 : 0);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) bad[i] = 0.0f;
+                        bad = product(which, who, bad, E());
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[m][i] = bad[i] > 0.0f ? NAN : o[m][i];
+                    }
+                }
+                if constexpr (kTermsC == 1) {
+#pragma unroll
+                    for (int x = kTermsQ - 1; x >= 0; --x) o[m] = product(v[0], p[x], o[m], E());
+                } else {
+#pragma unroll
+                    for (int both = 2; both >= 0; --both)
+#pragma unroll
+                        for (int x = both; x >= 0; --x) o[m] = product(v[x], p[both - x], o[m], E());
+                }
+            }
+        }
+    };
+
+    int buffer = 0, place_at = 0;
+    uint32_t t0 = begin;
+    if (t0 < end) {
+        there = find(t0, entry, 0);
+        entry = t0 + kTile < end ? entry_of(t0 + kTile) : -1;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        load(0);
+        store(0, there);
+        __syncthreads();
+    }
+    while (t0 < end) {
+        const bool more = t0 + kTile < end;
+        if (more) {
+            place_at ^= 1;
+            there_next = find(t0 + kTile, entry, place_at);
+            entry = t0 + 2 * kTile < end ? entry_of(t0 + 2 * kTile) : -1;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            load(place_at);
+        }
+        if (t0 < some_hi && t0 + kTile > some_lo) {
+            if (t0 >= all_lo && t0 + kTile <= all_hi && there == kAll) work(t0, buffer, std::false_type());
+            else work(t0, buffer, std::true_type());
+        }
+        if constexpr (kBuffers == 1) __syncthreads();
+        else buffer ^= 1;
+        if (more) store(buffer, there_next);
+        __syncthreads();
+        there = there_next;
+        t0 += kTile;
+    }
+
+    l = other_sum(l);
+    if (it.shares > 1) {
+        const int32_t slot = it.slot + it.share;
+        if (slot >= a.most_slots) return;                      // (starts that do not ascend)
+        const int64_t at = ((int64_t)slot * d.cache.kv_heads + kvh) * kTileRows + in_tile;
+        if (h == 0) a.stats[at] = make_float2(R == -INFINITY ? -INFINITY : R - kGrow, l);
+#pragma unroll
+        for (int m = 0; m < kSlabs; ++m)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const int dim = m * 32 + i * 2 + h * 4;
+                if (dim < D) *(f32x4*)(a.parts + at * D + dim) = f32x4{o[m][i], o[m][i + 1], o[m][i + 2], o[m][i + 3]};
+            }
+        return;
+    }
+    if (!valid) return;
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    Q* const to = (Q*)a.out + out_row * d.out_stride + head * d.out_head_stride;
+#pragma unroll
+    for (int m = 0; m < kSlabs; ++m)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+            const int dim = m * 32 + i * 2 + h * 4;
+            if (dim < D) put4(to + dim, o[m][i] * f, o[m][i + 1] * f, o[m][i + 2] * f, o[m][i + 3] * f);
+        }
+    if (h == 0 && a.lse) a.lse[out_row * d.heads + head] = l == 0.0f ? -INFINITY : (R + (__log2f(l) - kGrow)) * kLn2;
+}
+
+// The shares of a tile: 32 of its rows a workgroup, a quad of a row a thread, share after share.
+template <class Q>
+__global__ void __launch_bounds__(kThreads) join_shares(Args a) {
+    const reef_chunk_attention_desc& d = a.d;
+    const int32_t part = (int32_t)(blockIdx.x % kWaves);
+    const uint32_t rest = blockIdx.x / kWaves;
+    const int32_t kvh = (int32_t)(rest % (uint32_t)d.cache.kv_heads), id = (int32_t)(rest / (uint32_t)d.cache.kv_heads);
+    const Item it = find_item(a, id);
+    if (it.tile < 0 || it.share || it.shares <= 1) return;
+    const int D = d.cache.head_dim, quads = D / 4;
+    const uint32_t rows = (uint32_t)(it.r.added * a.group), row0 = (uint32_t)it.tile * kTileRows + part * kRows;
+    const int32_t shares = min(it.shares, a.most_slots - it.slot);
+    const int64_t step = (int64_t)d.cache.kv_heads * kTileRows;
+    for (int x = threadIdx.x; x < kRows * quads; x += kThreads) {
+        const int i = x / quads, dim = (x - i * quads) * 4;
+        const uint32_t row = row0 + i;
+        if (row >= rows) continue;
+        const int64_t at = ((int64_t)it.slot * d.cache.kv_heads + kvh) * kTileRows + part * kRows + i;
+        float R = -INFINITY, l = 0.0f;
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int32_t s = 0; s < shares; ++s) {
+            const float2 stat = a.stats[at + s * step];
+            const f32x4 mine = *(const f32x4*)(a.parts + (at + s * step) * D + dim);
+            const float next = fmaxf(R, stat.x), base = next == -INFINITY ? 0.0f : next;
+            const float f = __builtin_amdgcn_exp2f(R - base), g = __builtin_amdgcn_exp2f(stat.x - base);
+            R = next;
+            l = l * f + stat.y * g;
+            o = o * f + mine * g;
+        }
+        const uint32_t token = divided(row, a.by_group);
+        const int32_t head = kvh * a.group + (int32_t)(row - token * a.by_group.by);
+        const int64_t out_row = (int64_t)it.r.first + token;
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+        put4((Q*)a.out + out_row * d.out_stride + head * d.out_head_stride + dim, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+        if (dim == 0 && a.lse) a.lse[out_row * d.heads + head] = l == 0.0f ? -INFINITY : (R + __log2f(l)) * kLn2;
+    }
 }
 
 int check(const char* what, const reef_chunk_attention_desc* d) {
@@ -92,16 +716,53 @@ int check(const char* what, const reef_chunk_attention_desc* d) {
     return 0;
 }
 
+// How a call is laid out.
+struct Plan {
+    int32_t budget;
+    int64_t items, slots;
+    size_t info_bytes, list_bytes, stats_bytes, bytes;
+};
+Plan plan_of(const reef_chunk_attention_desc& d) {
+    const int32_t group = d.heads / d.cache.kv_heads, kv = d.cache.kv_heads;
+    int64_t longest = (int64_t)d.max_blocks * d.cache.block_size;
+    if (d.longest && d.longest < longest) longest = d.longest;
+    if (d.window) longest = std::min(longest, (int64_t)d.window + kTileRows / group);
+    Plan p{};
+    p.items = (int64_t)d.tokens * group / kTileRows + d.requests;
+    if (longest > kLeast) {
+        p.budget = std::max(1, kGroups / kv);
+        p.slots = std::min<int64_t>(4ll * p.budget, 2ll * p.budget + p.items);
+        p.items += 2ll * p.budget;
+        p.stats_bytes = (size_t)p.slots * kv * kTileRows * 8;
+    }
+    if (d.requests > kFew) {
+        p.info_bytes = (size_t)d.requests * 16;
+        p.list_bytes = ((size_t)(1 + p.items) * 4 + 15) / 16 * 16;
+    }
+    p.bytes = p.info_bytes + p.list_bytes + p.stats_bytes + (size_t)p.slots * kv * kTileRows * d.cache.head_dim * 4;
+    return p;
+}
+
 template <class Q, class C>
-int run(const char* what, const Args& a, void* stream) {
-    return launch(what, chunk_attention<Q, C>, dim3((unsigned)(((int64_t)a.d.tokens * a.d.heads + 3) / 4)), dim3(kThreads), a, stream);
+int run(const char* what, const Args& a, const Plan& p, void* stream) {
+    const int D = a.d.cache.head_dim;
+    const dim3 grid((unsigned)(p.items * a.d.cache.kv_heads)), block(kThreads);
+    if (a.list)
+        if (int rc = launch(what, list_items, dim3(1), dim3(kListThreads), a, stream)) return rc;
+    const int rc = D <= 64    ? launch(what, chunk_attention<Q, C, 64>, grid, block, a, stream)
+                   : D <= 96  ? launch(what, chunk_attention<Q, C, 96>, grid, block, a, stream)
+                   : D <= 128 ? launch(what, chunk_attention<Q, C, 128>, grid, block, a, stream)
+                   : D <= 192 ? launch(what, chunk_attention<Q, C, 192>, grid, block, a, stream)
+                              : launch(what, chunk_attention<Q, C, 256>, grid, block, a, stream);
+    if (rc || !p.budget) return rc;
+    return launch(what, join_shares<Q>, dim3(grid.x * kWaves), block, a, stream);
 }
 
 }  // namespace
 
 extern "C" int64_t reef_ops_chunk_attention_workspace(const reef_chunk_attention_desc* d) {
     if (check("reef_ops_chunk_attention_workspace", d)) return -1;
-    return 0;
+    return (int64_t)plan_of(*d).bytes;
 }
 
 extern "C" int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, const void* query, const void* key_cache, const void* value_cache,
@@ -113,12 +774,22 @@ extern "C" int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, cons
     if (!rows16(query) || !rows16(key_cache) || !rows16(value_cache) || !rows16(out) || !words(table) || !words(starts) || !words(cached) || !words(lengths) ||
         !aligned(lse, 4))
         return refuse(what, "null or unaligned argument");
-    const Args a{*d, query, key_cache, value_cache, table, starts, cached, lengths, out, lse, divider((uint32_t)d->cache.block_size)};
+    const Plan p = plan_of(*d);
+    // (2^32 threads are refused by the launch, which may be the call's second one)
+    if (p.items * d->cache.kv_heads * kWaves >= 1ll << 24) return refuse(what, "%lld workgroups are too many", (long long)(p.items * d->cache.kv_heads * kWaves));
+    if (p.bytes && (!rows16(workspace) || workspace_bytes < (int64_t)p.bytes))
+        return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", p.bytes, (long long)workspace_bytes);
+    char* const w = (char*)workspace;
+    const size_t list = p.info_bytes, stats = list + p.list_bytes, parts = stats + p.stats_bytes;
+    const int32_t group = d->heads / d->cache.kv_heads;
+    const Args a{*d, query, key_cache, value_cache, table, starts, cached, lengths, out, lse, (int4*)w, p.list_bytes ? (int32_t*)(w + list) : nullptr, (float*)(w + parts),
+                 (float2*)(w + stats), d->scale == 0.0f ? kLog2e : std::fabs(d->scale) * kLog2e, d->scale < 0.0f ? (d->type == REEF_TYPE_F32 ? 0x80000000u : 0x80008000u) : 0u,
+                 d->scale == 0.0f, group, p.budget, (int32_t)p.items, (int32_t)p.slots, divider((uint32_t)d->cache.block_size), divider((uint32_t)group)};
     switch (d->type * 4 + d->cache.type) {
-        case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, stream);
-        case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return run<float, _Float16>(what, a, stream);
-        case REEF_TYPE_F32 * 4 + REEF_TYPE_BF16: return run<float, __bf16>(what, a, stream);
-        case REEF_TYPE_F16 * 4 + REEF_TYPE_F16: return run<_Float16, _Float16>(what, a, stream);
-        default: return run<__bf16, __bf16>(what, a, stream);
+        case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, p, stream);
+        case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return run<float, _Float16>(what, a, p, stream);
+        case REEF_TYPE_F32 * 4 + REEF_TYPE_BF16: return run<float, __bf16>(what, a, p, stream);
+        case REEF_TYPE_F16 * 4 + REEF_TYPE_F16: return run<_Float16, _Float16>(what, a, p, stream);
+        default: return run<__bf16, __bf16>(what, a, p, stream);
     }
 }

@@ -230,7 +230,9 @@ def test_chunk_rows_do_not_see_infinities_and_nan_behind_them(kind, cache, cache
 @pytest.mark.parametrize("sign", [1, -1])
 def test_chunk_scores_of_any_size(kind, cache, tokens, sign):
     """Scores from 2^18 to 2^31: the largest takes everything, two equal ones half each.  One dimension alone is not zero and its
-    products are exact, so all other weights are 0 and the two are alike: the result is the mean of two values but for a rounding of their sum and of the output."""
+    products are exact, so all other weights are 0 and the two are alike: the result is the mean of two values but for a rounding of their sum and of the output.
+    In 16-bit types the two weights w are rounded to the same w (1 + e), |e| up to half a step, while their sum is not: (w (1 + e) a + w (1 + e) b) / (2 w) is the
+    mean times 1 + e, so that half a step of the mean is added."""
     rng = np.random.default_rng(tokens)
     dim, new = 64, 3
     values = rng.standard_normal((tokens, dim)).astype(np.float32)
@@ -244,7 +246,8 @@ def test_chunk_scores_of_any_size(kind, cache, tokens, sign):
             q[:, 0, 5], q[:, 1, 5] = sign * 4096 * more, sign * 2048 * more
             out, ls = one_request(kind, cache, keys, values, q, 2.0 ** (binade - 24), tokens - new)
             want = (v[win[0]] + v[win[1]]) / 2
-            assert (np.abs(out - want) <= HALF[kind] * np.abs(want) + 2.0 ** -22 * np.abs(v[win]).max(0) + (2.0 ** -25 if kind == F16 else 0)).all(), (binade, more)
+            half = HALF[kind] * (1 if kind == F32 else 2 + HALF[kind])
+            assert (np.abs(out - want) <= half * np.abs(want) + 2.0 ** -22 * np.abs(v[win]).max(0) + (2.0 ** -25 if kind == F16 else 0)).all(), (binade, more)
             s = np.array([1, 0.5]) * sign * more * 2.0 ** binade
             assert (np.abs(ls - (s + np.log(2))) <= 8 * 2.0 ** -24 * np.abs(s) + 2.0 ** -20).all(), (binade, more)
 
