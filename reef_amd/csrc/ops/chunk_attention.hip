@@ -8,9 +8,7 @@
 namespace {
 using namespace reef_ops;
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kRows = 32;                    // query rows of a wavefront: heads of one token next to each other, token after token
-constexpr int kTileRows = kWaves * kRows;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int32_t kLeast = 512;              // cached tokens a share at least
 constexpr int kGroups = 512;                 // workgroups that the shares of all tiles are to make
@@ -30,6 +28,7 @@ struct Args {
     uint32_t flip;          // of the queries' sign where scale is negative
     int32_t zero;           // scale is 0
     int32_t group;
+    int32_t tile_rows;      // of a workgroup
     int32_t budget;         // shares that all tiles are cut into, beside one each; 0: tiles are not split
     int32_t most_items, most_slots;
     Divider block, by_group;
@@ -53,13 +52,13 @@ __device__ inline Request request_of(const Args& a, int32_t i) {
     r.added = max(0, start_of(a, i + 1) - r.first);
     r.cached = held_length(a.cached[i], a.d.max_blocks, a.d.cache.block_size);
     r.n = held_length(a.lengths[i], a.d.max_blocks, a.d.cache.block_size);
-    r.tiles = (r.added * a.group + kTileRows - 1) / kTileRows;
+    r.tiles = (r.added * a.group + a.tile_rows - 1) / a.tile_rows;
     return r;
 }
 // The cached tokens [.x, .y) that some row of a tile sees.  (Places may pass 2^31, not 2^32.)
 __device__ inline uint2 span_of(const Args& a, const Request& r, int32_t tile) {
-    const uint32_t last = (uint32_t)min((tile + 1) * kTileRows, r.added * a.group) - 1;
-    const uint32_t p0 = (uint32_t)r.cached + divided((uint32_t)tile * kTileRows, a.by_group), p1 = (uint32_t)r.cached + divided(last, a.by_group);
+    const uint32_t last = (uint32_t)min((tile + 1) * a.tile_rows, r.added * a.group) - 1;
+    const uint32_t p0 = (uint32_t)r.cached + divided((uint32_t)(tile * a.tile_rows), a.by_group), p1 = (uint32_t)r.cached + divided(last, a.by_group);
     if (p0 >= (uint32_t)r.n) return make_uint2(0, 0);
     return make_uint2(a.d.window && p0 + 1 > (uint32_t)a.d.window ? p0 + 1 - a.d.window : 0, min((uint32_t)r.n, p1 + 1));
 }
@@ -262,12 +261,24 @@ struct Near {
     static __device__ inline uint32_t at(uint32_t row, uint32_t piece) { return row * kPitch + ((piece ^ turn(row)) << 4); }
 };
 
-// A tile of 128 query rows over a share of the tokens they see, one cache head: each wavefront has 32 rows, all of them the keys and values that
-// the workgroup brings to LDS, 64 tokens at a time (32 of heads over 128 and of 32-bit caches).
+constexpr int waves_of(int dp) { return dp <= 128 ? 8 : 4; }
+// How a kernel is laid out, by its types and head size.  TK: tokens of a tile of keys and values; WAVES of 32 rows each share them.
+template <class Q, class C, int DP>
+struct Shape {
+    static constexpr bool kHalf = __is_same(C, _Float16);
+    static constexpr int kTermsC = sizeof(C) == 4 ? 3 : 1, kTermsQ = sizeof(Q) == 2 ? 1 : kHalf ? 2 : 3;
+    static constexpr int kWaves = waves_of(DP), kThreads = kWaves * 64, kTile = kTermsQ == 1 && DP <= 128 ? 64 : 32;
+};
+
+// A tile of query rows over a share of the tokens they see, one cache head: each wavefront has 32 rows, all of them the keys and values that
+// the workgroup brings to LDS.
 //
 // Both products are 32x32x16 MFMAs:  S^T[token][row] = K Q^T, then O^T[dim][row] = V^T P^T.  A product does not care in which order its k
 // runs: S^T leaves lane (row, half h) the tokens 8 j + 4 h + {0..3} of 32, so these are its k, and V^T's operand comes transposed out of LDS four tokens a
 // read.  So weights stay in the lane that made them, and a row's reference, sum and rescaling are one value a lane.
+//
+// Scores are made a tile ahead: the products of the next tile's keys run beside the exponentials of this one's scores, and those of this
+// one's values beside the next one's maximum, so that the matrix cores have work while the lanes have theirs.
 //
 // Weights are 2^(s c - R): R is a whole number near the largest s c so far (within kSlack above), so that one rounding makes the exponent, and rescaling
 // by 2^(R - R') is exact and rare.  For fp16, whose weights want room below, they are 2^kGrow times larger.
@@ -276,19 +287,22 @@ struct Near {
 // both sides, six products (the others are below 2^-22).  Weights of 16-bit types are rounded to the type once: half a step of the type of each at most, which in their mean is
 // no more than the output's own rounding (two terms would take 1.4 times as long).
 template <class Q, class C, int DP>
-__global__ void __launch_bounds__(kThreads, sizeof(Q) == 2 && DP <= 128 ? 2 : 1) chunk_attention(Args a) {
+__global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(Args a) {
     using E = std::conditional_t<sizeof(C) == 4, __bf16, C>;                  // what is multiplied
-    constexpr bool kHalf = __is_same(E, _Float16);
-    constexpr int kTermsC = sizeof(C) == 4 ? 3 : 1, kTermsQ = sizeof(Q) == 2 ? 1 : kHalf ? 2 : 3;
+    using Sh = Shape<Q, C, DP>;
+    constexpr bool kHalf = Sh::kHalf;
+    constexpr int kTermsC = Sh::kTermsC, kTermsQ = Sh::kTermsQ, kTile = Sh::kTile, kSub = kTile / 32, kWaves = Sh::kWaves, kThreads = Sh::kThreads;
     constexpr float kGrow = kHalf ? 6.0f : 0.0f;                              // 2^(6 + 8 + 1/2) < 65504
-    constexpr int kTile = kTermsC == 3 || DP > 128 ? 32 : 64, kSub = kTile / 32, kBuffers = kTermsC == 3 ? 1 : 2;
-    constexpr int kSteps = DP / 16, kSlabs = DP / 32;
+    constexpr int kSteps = DP / 16, kSlabs = DP / 32, kTileRows = kWaves * kRows;
     using N = Near<DP>;
-    constexpr int kPlane = kTile * N::kPitch, kBuffer = 2 * kTermsC * kPlane;
-    constexpr int kRowPieces = DP * (int)sizeof(C) / 16, kMine = kTile * kRowPieces / kThreads;    // 16-byte pieces of a row in memory; of a thread
-    static_assert(kTile * kRowPieces % kThreads == 0, "");
-    __shared__ __align__(16) unsigned char tiles[kBuffers * kBuffer];
+    constexpr int kPlane = kTile * N::kPitch, kBuffer = kTermsC * kPlane;
+    constexpr int kRowPieces = DP * (int)sizeof(C) / 16, kAllPieces = kTile * kRowPieces;    // 16-byte pieces of a row in memory, of a tile
+    constexpr int kMine = (kAllPieces + kThreads - 1) / kThreads;             // of a thread
+    constexpr int kValues = kTermsC == 3 && DP > 128 ? 1 : 2;                 // buffers of values: there is no room for two of three terms of these
+    constexpr bool kEven = kAllPieces % kThreads == 0;
+    __shared__ __align__(16) unsigned char k_near[2 * kBuffer], v_near[kValues * kBuffer];
     __shared__ int64_t offsets[kWaves][2][kTile];
+    __shared__ uint32_t odd_tile[2];         // number of the last tile whose values held infinities or NaN, of even and odd ones
 
     const reef_chunk_attention_desc& d = a.d;
     const int32_t kvh = (int32_t)(blockIdx.x % (uint32_t)d.cache.kv_heads);
@@ -324,72 +338,80 @@ __global__ void __launch_bounds__(kThreads, sizeof(Q) == 2 && DP <= 128 ? 2 : 1)
     const int32_t* table = a.table + (int64_t)it.request * d.table_stride;
 
     // the table's entry of one token of a tile a lane; -1: no token
-    auto entry_of = [&](uint32_t t0) -> int32_t {
+    auto entry_of = [&](uint32_t t0) __attribute__((always_inline)) -> int32_t {
         const uint32_t t = t0 + lane;
         return lane < kTile && t < end ? table[divided(t, a.block)] : -1;
     };
     // its place, for all lanes to read; which of the tile's tokens there are
-    auto find = [&](uint32_t t0, int32_t entry, int buffer) -> uint64_t {
+    auto find = [&](uint32_t t0, int32_t entry, int slot) __attribute__((always_inline)) -> uint64_t {
         int64_t at = -1;
         if (lane < kTile) {
             const uint32_t t = t0 + lane;
             at = paged_row(view, entry, (int32_t)(t - divided(t, a.block) * a.block.by));
-            offsets[wave][buffer][lane] = at < 0 ? 0 : at;
+            offsets[wave][slot][lane] = at < 0 ? 0 : at;
         }
         return __builtin_amdgcn_ballot_w64(at >= 0);
     };
     constexpr uint64_t kAll = kTile == 64 ? ~0ull : 0xFFFFFFFFull;
     u32x4 k_on_way[kMine], v_on_way[kMine];
-    auto load = [&](int buffer) {
+    auto load = [&](const C* pool, u32x4 (&on_way)[kMine], int slot) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             const int x = i * kThreads + threadIdx.x, at = x / kRowPieces, piece = x - at * kRowPieces;
-            const int64_t from = offsets[wave][buffer][at] + (piece * 16 < D * (int)sizeof(C) ? piece * (16 / (int)sizeof(C)) : 0);
-            k_on_way[i] = *(const u32x4*)(keys + from);
-            v_on_way[i] = *(const u32x4*)(values + from);
+            if (!kEven && x >= kAllPieces) continue;
+            on_way[i] = *(const u32x4*)(pool + offsets[wave][slot][at] + (DP == D || piece * 16 < D * (int)sizeof(C) ? piece * (16 / (int)sizeof(C)) : 0));
         }
     };
-    // into LDS: zeros where there is no token, or no such dimension
-    auto store = [&](int buffer, uint64_t there) {
-        unsigned char* const to = tiles + buffer * kBuffer;
+    // Into LDS: zeros where there is no token, or no such dimension.  Where not all rows see all of a tile, infinities and NaN among its values must not
+    // be multiplied by weights of 0: they become 0 as well, and the tile's number is left for spoil().
+    auto store = [&](unsigned char* to, u32x4 (&on_way)[kMine], uint64_t there, bool clean, uint32_t number) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
             const int x = i * kThreads + threadIdx.x, at = x / kRowPieces, piece = x - at * kRowPieces;
+            if (!kEven && x >= kAllPieces) continue;
+            u32x4 w = on_way[i];
             if (there != kAll || D != DP) {
                 const bool inside = (there >> at & 1) && piece * 16 < D * (int)sizeof(C);
-                if (!inside) k_on_way[i] = v_on_way[i] = {0, 0, 0, 0};
+                if (!inside) w = {0, 0, 0, 0};
+            }
+            if (clean) {
+                constexpr uint32_t kOdd = sizeof(C) == 4 ? 0x7F800000u : kHalf ? 0x7C00u : 0x7F80u;
+                bool found = false;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t keep = ~0u;
+                    if constexpr (sizeof(C) == 4) keep = (w[j] & kOdd) == kOdd ? 0 : ~0u;
+                    else keep = ((w[j] & kOdd) == kOdd ? 0 : 0xFFFFu) | ((w[j] >> 16 & kOdd) == kOdd ? 0 : 0xFFFF0000u);
+                    found |= keep != ~0u;
+                    w[j] &= keep;
+                }
+                if (found) odd_tile[number & 1] = number;
             }
             if constexpr (kTermsC == 1) {
-                *(u32x4*)(to + N::at(at, piece)) = k_on_way[i];
-                *(u32x4*)(to + kPlane + N::at(at, piece)) = v_on_way[i];
+                *(u32x4*)(to + N::at(at, piece)) = w;
             } else {
                 const uint32_t place = N::at(at, piece >> 1) + (piece & 1) * 8;
+                uint32_t t[2][3];
 #pragma unroll
-                for (int kv = 0; kv < 2; ++kv) {
-                    const u32x4 w = kv ? v_on_way[i] : k_on_way[i];
-                    uint32_t t[2][3];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float x0 = __uint_as_float(w[2 * j]), x1 = __uint_as_float(w[2 * j + 1]);
-                        terms(x0, x1, t[j], __bf16());
-                        // an infinity is its first term alone, and so is a NaN, which must not be cut to one
-                        const bool odd0 = !(fabsf(x0) < INFINITY), odd1 = !(fabsf(x1) < INFINITY);
-                        if (odd0 | odd1) {
-                            const uint32_t keep = (odd0 ? 0 : 0xFFFFu) | (odd1 ? 0 : 0xFFFF0000u);
-                            t[j][1] &= keep;
-                            t[j][2] &= keep;
-                            if (x0 != x0) t[j][0] |= 0x7FFFu;
-                            if (x1 != x1) t[j][0] |= 0x7FFF0000u;
-                        }
+                for (int j = 0; j < 2; ++j) {
+                    const float x0 = __uint_as_float(w[2 * j]), x1 = __uint_as_float(w[2 * j + 1]);
+                    terms(x0, x1, t[j], __bf16());
+                    // an infinity is its first term alone, and so is a NaN, which must not be cut to one
+                    const bool odd0 = !(fabsf(x0) < INFINITY), odd1 = !(fabsf(x1) < INFINITY);
+                    if (odd0 | odd1) {
+                        const uint32_t keep = (odd0 ? 0 : 0xFFFFu) | (odd1 ? 0 : 0xFFFF0000u);
+                        t[j][1] &= keep;
+                        t[j][2] &= keep;
+                        if (x0 != x0) t[j][0] |= 0x7FFFu;
+                        if (x1 != x1) t[j][0] |= 0x7FFF0000u;
                     }
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) *(u32x2*)(to + (kv * 3 + x) * kPlane + place) = u32x2{t[0][x], t[1][x]};
                 }
+#pragma unroll
+                for (int x = 0; x < 3; ++x) *(u32x2*)(to + x * kPlane + place) = u32x2{t[0][x], t[1][x]};
             }
         }
     };
 
-    uint64_t there = 0, there_next = 0;
     int32_t entry = begin < end ? entry_of(begin) : -1;        // (asked for ahead of the queries: keys and values wait for them)
 
     // the queries: this lane's row, the pieces that its half of the keys has
@@ -452,13 +474,11 @@ __global__ void __launch_bounds__(kThreads, sizeof(Q) == 2 && DP <= 128 ? 2 : 1)
 
     // where this lane reads: keys' row n; values' rows 4 (lane / 32) + (lane % 16) / 4, four dimensions from 16 (lane / 16 % 2) + 4 (lane % 4) on
     const int t16 = lane & 15;
-    const uint32_t v_row = (uint32_t)(4 * h + (t16 >> 2)), v_piece = (uint32_t)(2 * (lane >> 4 & 1) + ((t16 & 3) >> 1)), v_byte = (uint32_t)(t16 & 1) * 8;
+    // (pieces are exchanged by bits, so those of other slabs, and of 8 rows below, are at places with other bits)
+    const uint32_t k_at = N::at(n, h), v_at = N::at(4 * h + (t16 >> 2), 2 * (lane >> 4 & 1) + ((t16 & 3) >> 1)) + (t16 & 1) * 8;
 
-    auto work = [&](uint32_t t0, int buffer, auto is_masked) {
-        constexpr bool kMasked = decltype(is_masked)::value;
-        const unsigned char* const k_tile = tiles + buffer * kBuffer;
-        const unsigned char* const v_tile = k_tile + kTermsC * kPlane;
-        f32x16 s[kSub];
+    // Scores of a tile, as products.
+    auto multiply_keys = [&](f32x16 (&s)[kSub], const unsigned char* k_tile) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kSub; ++u)
 #pragma unroll
@@ -467,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(Q) == 2 && DP <= 128 ? 2 : 1)
         for (int c = 0; c < kSteps; ++c)
 #pragma unroll
             for (int u = 0; u < kSub; ++u) {
-                const unsigned char* const from = k_tile + u * 32 * N::kPitch + N::at(n, 2 * c + h);
+                const unsigned char* const from = k_tile + (k_at ^ c * 32) + u * 32 * N::kPitch;
                 if constexpr (kTermsC == 1) {
                     const u32x4 k = *(const u32x4*)from;
 #pragma unroll
@@ -482,21 +502,29 @@ __global__ void __launch_bounds__(kThreads, sizeof(Q) == 2 && DP <= 128 ? 2 : 1)
                         for (int x = both; x >= 0; --x) s[u] = product(k[x], q[both - x][c], s[u], E());
                 }
             }
-        uint32_t seen[kSub];
-        if constexpr (kMasked) {
+    };
+    // Which of the tokens of 32 that this lane has of a row it sees, a bit each.  (Nothing of it is to be made ahead of the loop, and held in registers.)
+    auto sees = [&](uint32_t t0, uint32_t there) __attribute__((always_inline)) {
+        uint32_t from = t0 + 4 * h - lo, many = hi - lo, in = there >> (4 * h), yes = 0;
+        asm volatile("" : "+v"(from), "+v"(many), "+v"(in));
 #pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-                const uint32_t in_pool = (uint32_t)(there >> (u * 32));
-                seen[u] = 0;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t at = 8 * (i >> 2) + 4 * h + (i & 3), t = t0 + u * 32 + at;
-                    const bool yes = t >= lo && t < hi && (in_pool >> at & 1);
-                    seen[u] |= yes ? 1u << i : 0;
-                    if (!yes) s[u][i] = -INFINITY;
-                }
-            }
+        for (int i = 0; i < 16; ++i) yes |= from + (8 * (i >> 2) + (i & 3)) < many ? 1u << i : 0u;
+        if (there != ~0u) {
+            // bits 0..3, 8..11, 16..19 and 24..27 of `in`
+            const uint32_t x = in & 0x0F0F0F0Fu, y = x | x >> 4;
+            yes &= (y & 0xFFu) | (y >> 8 & 0xFF00u);
         }
+        return yes;
+    };
+    auto hide = [&](f32x16 (&s)[kSub], uint32_t t0, uint64_t there) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < kSub; ++u) {
+            const uint32_t yes = sees(t0 + u * 32, (uint32_t)(there >> (u * 32)));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = yes >> i & 1 ? s[u][i] : -INFINITY;
+        }
+    };
+    auto largest = [&](f32x16 (&s)[kSub]) __attribute__((always_inline)) {
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < kSub; ++u)
@@ -505,7 +533,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(Q) == 2 && DP <= 128 ? 2 : 1)
                 if constexpr (kHalf && kTermsQ > 1) s[u][i] *= shrink;
                 top = fmaxf(top, s[u][i]);
             }
-        top = other_max(top) * scale;
+        return other_max(top) * scale;
+    };
+    auto refer = [&](float top) __attribute__((always_inline)) {
         const bool passes = top > R + kSlack;
         if (__builtin_amdgcn_ballot_w64(passes)) {
             const float next = passes ? rintf(top) : R;
@@ -517,9 +547,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(Q) == 2 && DP <= 128 ? 2 : 1)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[m][i] *= f;
         }
+    };
+    // From 2^20 on a score's product and its difference from the reference are not exact together: it is rounded first there.
+    float times = scale, plus = kGrow;
+    auto approach = [&](f32x16 (&s)[kSub]) __attribute__((always_inline)) {
         const float base = R == -INFINITY ? 0.0f : R;
-        float times = scale, plus = kGrow - base;
-        // From 2^20 on the sum above is not exact: scores are rounded first there.
+        times = scale;
+        plus = kGrow - base;
         if (__builtin_amdgcn_ballot_w64(fabsf(base) >= 0x1p20f)) {
 #pragma unroll
             for (int u = 0; u < kSub; ++u)
@@ -532,101 +566,171 @@ __global__ void __launch_bounds__(kThreads, sizeof(Q) == 2 && DP <= 128 ? 2 : 1)
             times = 1.0f;
             plus = kGrow;
         }
+    };
+    // Weights of a tile, as operands.
+    u32x4 p[kTile / 16][kTermsQ];
+    auto weigh = [&](f32x16 (&s)[kSub]) __attribute__((always_inline)) {
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                s[u][i] = __builtin_amdgcn_exp2f(fmaf(s[u][i], times, plus));
-                l += s[u][i];
-            }
-#pragma unroll
-        for (int c = 0; c < kTile / 16; ++c) {
-            u32x4 p[kTermsQ];
+        for (int c = 0; c < kTile / 16; ++c)
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
+                const int i = (c & 1) * 8 + 2 * w;
+                const float x = __builtin_amdgcn_exp2f(fmaf(s[c >> 1][i], times, plus)), y = __builtin_amdgcn_exp2f(fmaf(s[c >> 1][i + 1], times, plus));
+                sum[w] += x + y;
                 uint32_t t[kTermsQ];
-                terms(s[c >> 1][(c & 1) * 8 + 2 * w], s[c >> 1][(c & 1) * 8 + 2 * w + 1], t, E());
+                terms(x, y, t, E());
 #pragma unroll
-                for (int x = 0; x < kTermsQ; ++x) p[x][w] = t[x];
+                for (int k = 0; k < kTermsQ; ++k) p[c][k][w] = t[k];
             }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    };
+    auto values_of = [&](const unsigned char* v_tile, int c, int m, u32x4 (&v)[kTermsC]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int x = 0; x < kTermsC; ++x) {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s4 near_s4;
+            const unsigned char* const from = v_tile + x * kPlane + c * 16 * N::kPitch;
+            const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((near_s4*)(from + (v_at ^ m * 64))));
+            const u32x2 z = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((near_s4*)(from + 8 * N::kPitch + (v_at ^ (m * 64 + 32)))));
+            v[x] = {y[0], y[1], z[0], z[1]};
+        }
+    };
+    auto multiply_by = [&](u32x4 (&v)[kTermsC], int c, int m) __attribute__((always_inline)) {
+        if constexpr (kTermsC == 1) {
+#pragma unroll
+            for (int x = kTermsQ - 1; x >= 0; --x) o[m] = product(v[0], p[c][x], o[m], E());
+        } else {
+#pragma unroll
+            for (int both = 2; both >= 0; --both)
+#pragma unroll
+                for (int x = both; x >= 0; --x) o[m] = product(v[x], p[c][both - x], o[m], E());
+        }
+    };
+    auto multiply_values = [&](const unsigned char* v_tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int c = 0; c < kTile / 16; ++c)
 #pragma unroll
             for (int m = 0; m < kSlabs; ++m) {
                 u32x4 v[kTermsC];
-#pragma unroll
-                for (int x = 0; x < kTermsC; ++x) {
-                    typedef short s4 __attribute__((ext_vector_type(4)));
-                    typedef __attribute__((address_space(3))) s4 near_s4;
-                    const unsigned char* const from = v_tile + x * kPlane + c * 16 * N::kPitch + v_byte;
-                    const u32x2 y = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((near_s4*)(from + N::at(v_row, 4 * m + v_piece))));
-                    const u32x2 z = __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((near_s4*)(from + N::at(v_row + 8, 4 * m + v_piece))));
-                    v[x] = {y[0], y[1], z[0], z[1]};
-                }
-                if constexpr (kMasked) {
-                    // Infinities and NaN among the values: no row may have them times 0, those that see them have NaN.
-                    constexpr uint32_t kOdd = kHalf ? 0x7C00u : 0x7F80u, kOne = kHalf ? 0x3C00u : 0x3F80u;
-                    bool odd = false;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) odd |= (v[0][w] & kOdd) == kOdd || (v[0][w] >> 16 & kOdd) == kOdd;
-                    if (__builtin_amdgcn_ballot_w64(odd)) {
-                        u32x4 which, who;
-                        f32x16 bad;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const bool x = (v[0][w] & kOdd) == kOdd, y = (v[0][w] >> 16 & kOdd) == kOdd;
-                            which[w] = (x ? kOne : 0) | (y ? kOne << 16 : 0);
-                            v[0][w] &= (x ? 0 : 0xFFFFu) | (y ? 0 : 0xFFFF0000u);
-                            const uint32_t mine = seen[c >> 1] >> ((c & 1) * 8 + 2 * w);
-                            who[w] = (mine & 1 ? kOne : 0) | (mine & 2 ? kOne << 16 : 0);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) bad[i] = 0.0f;
-                        bad = product(which, who, bad, E());
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) o[m][i] = bad[i] > 0.0f ? NAN : o[m][i];
-                    }
-                }
-                if constexpr (kTermsC == 1) {
-#pragma unroll
-                    for (int x = kTermsQ - 1; x >= 0; --x) o[m] = product(v[0], p[x], o[m], E());
-                } else {
-#pragma unroll
-                    for (int both = 2; both >= 0; --both)
-#pragma unroll
-                        for (int x = both; x >= 0; --x) o[m] = product(v[x], p[both - x], o[m], E());
-                }
+                values_of(v_tile, c, m, v);
+                multiply_by(v, c, m);
             }
+    };
+    // Rows that see an infinity or a NaN among the values of a tile have NaN there.  (Rare: the values are read again, token after token.)
+    auto spoil = [&](uint32_t t0) __attribute__((always_inline)) {
+        for (uint32_t t = t0; t < min(end, t0 + kTile); ++t) {
+            const uint32_t page = divided(t, a.block);
+            const int64_t at = paged_row(view, table[page], (int32_t)(t - page * a.block.by));
+            if (at < 0) continue;
+            const bool mine = t >= lo && t < hi;
+            int from = 4 * h;
+            asm volatile("" : "+v"(from));   // (or 64 addresses are made ahead of the loop, and held in registers for it)
+#pragma unroll
+            for (int m = 0; m < kSlabs; ++m)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int dim = m * 32 + 8 * (i >> 2) + (i & 3) + from;
+                    const float v = (float)values[at + (dim < D ? dim : 0)];
+                    if (mine && !(fabsf(v) < INFINITY)) o[m][i] = NAN;
+                }
         }
     };
 
-    int buffer = 0, place_at = 0;
-    uint32_t t0 = begin;
-    if (t0 < end) {
-        there = find(t0, entry, 0);
-        entry = t0 + kTile < end ? entry_of(t0 + kTile) : -1;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        load(0);
-        store(0, there);
-        __syncthreads();
-    }
-    while (t0 < end) {
-        const bool more = t0 + kTile < end;
-        if (more) {
-            place_at ^= 1;
-            there_next = find(t0 + kTile, entry, place_at);
-            entry = t0 + 2 * kTile < end ? entry_of(t0 + 2 * kTile) : -1;
+    const uint32_t count = (end - begin + kTile - 1) / kTile;
+    auto seen_by_all = [&](uint32_t j, uint64_t there) __attribute__((always_inline)) {
+        return begin + j * kTile >= all_lo && begin + (j + 1) * kTile <= all_hi && there == kAll;
+    };
+    // the same of the workgroup's rows, but for tokens that are not there
+    const uint32_t first_place = (uint32_t)r.cached + divided((uint32_t)it.tile * kTileRows, a.by_group);
+    const uint32_t last_place = (uint32_t)r.cached + divided(min((uint32_t)(it.tile + 1) * kTileRows, rows) - 1, a.by_group);
+    auto inside_all = [&](uint32_t j) __attribute__((always_inline)) {
+        const uint32_t t0 = begin + j * kTile;
+        return t0 + kTile <= first_place + 1 && last_place < (uint32_t)r.n && (!d.window || t0 + (uint32_t)d.window > last_place);
+    };
+    // Tile j + 1's keys and tile j's values on their way, and into LDS.
+    uint64_t there = 0, there_next = 0;      // of tiles j and j + 1
+    auto ask = [&](uint32_t j, auto parity) __attribute__((always_inline)) {
+        constexpr int kNow = decltype(parity)::value;          // j % 2
+        if (j + 1 < count) {
+            there_next = find(begin + (j + 1) * kTile, entry, kNow ^ 1);
+            entry = j + 2 < count ? entry_of(begin + (j + 2) * kTile) : -1;
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            load(place_at);
+            load(keys, k_on_way, kNow ^ 1);
         }
-        if (t0 < some_hi && t0 + kTile > some_lo) {
-            if (t0 >= all_lo && t0 + kTile <= all_hi && there == kAll) work(t0, buffer, std::false_type());
-            else work(t0, buffer, std::true_type());
-        }
-        if constexpr (kBuffers == 1) __syncthreads();
-        else buffer ^= 1;
-        if (more) store(buffer, there_next);
+        load(values, v_on_way, kNow);
+    };
+    auto take = [&](uint32_t j, auto parity) __attribute__((always_inline)) {
+        constexpr int kNow = decltype(parity)::value;
+        if (j + 1 < count) store(k_near + (kNow ^ 1) * kBuffer, k_on_way, there_next, false, 0);
+        if constexpr (kValues == 1) __syncthreads();
+        store(v_near + (kValues == 2 ? kNow : 0) * kBuffer, v_on_way, there, !inside_all(j), j);
         __syncthreads();
         there = there_next;
-        t0 += kTile;
+    };
+    constexpr std::integral_constant<int, 0> kEvenOnes;
+    constexpr std::integral_constant<int, 1> kOddOnes;
+    if (count) {
+        if (threadIdx.x < 2) odd_tile[threadIdx.x] = ~0u;
+        there = find(begin, entry, 0);
+        entry = count > 1 ? entry_of(begin + kTile) : -1;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        load(keys, k_on_way, 0);
+        store(k_near, k_on_way, there, false, 0);
+        __syncthreads();
+        if (some_hi == 0) {                  // no rows: this wavefront only brings keys and values
+            for (uint32_t j = 0; j < count; j += 2) {
+                ask(j, kEvenOnes);
+                take(j, kEvenOnes);
+                if (j + 1 == count) break;
+                ask(j + 1, kOddOnes);
+                take(j + 1, kOddOnes);
+            }
+            if (it.shares == 1 && !valid) return;
+        } else {
+            f32x16 even[kSub], odd[kSub];    // scores of even and odd tiles
+            auto look = [&](uint32_t j, f32x16 (&s)[kSub], float top) __attribute__((always_inline)) {
+                if (!seen_by_all(j, there)) {
+                    hide(s, begin + j * kTile, there);
+                    top = largest(s);
+                }
+                refer(top);
+            };
+            // Weights of tile j - 1 go to its values while the scores of tile j are made.
+            auto step = [&](uint32_t j, f32x16 (&s)[kSub], f32x16 (&next)[kSub], auto parity) __attribute__((always_inline)) {
+                constexpr int kNow = decltype(parity)::value;
+                ask(j, parity);
+                approach(s);
+                multiply_keys(next, k_near + kNow * kBuffer);
+                weigh(s);
+                multiply_values(v_near + (kValues == 2 ? kNow ^ 1 : 0) * kBuffer);
+                const float top = largest(next);
+                if (odd_tile[kNow ^ 1] == j - 1) spoil(begin + (j - 1) * kTile);
+                look(j, next, top);
+                take(j, parity);
+            };
+            auto end_with = [&](f32x16 (&s)[kSub], int parity) __attribute__((always_inline)) {
+                approach(s);
+                weigh(s);
+                multiply_values(v_near + (kValues == 2 ? parity : 0) * kBuffer);
+                if (odd_tile[parity] == count - 1) spoil(begin + (count - 1) * kTile);
+            };
+            ask(0, kEvenOnes);
+            multiply_keys(even, k_near);
+            look(0, even, largest(even));
+            take(0, kEvenOnes);
+            uint32_t j = 1;
+            for (; j + 1 < count; j += 2) {
+                step(j, even, odd, kOddOnes);
+                step(j + 1, odd, even, kEvenOnes);
+            }
+            if (j < count) {
+                step(j, even, odd, kOddOnes);
+#pragma unroll
+                for (int u = 0; u < kSub; ++u) even[u] = odd[u];
+            }
+            end_with(even, (count - 1) & 1);
+        }
     }
 
     l = other_sum(l);
@@ -657,24 +761,25 @@ __global__ void __launch_bounds__(kThreads, sizeof(Q) == 2 && DP <= 128 ? 2 : 1)
     if (h == 0 && a.lse) a.lse[out_row * d.heads + head] = l == 0.0f ? -INFINITY : (R + (__log2f(l) - kGrow)) * kLn2;
 }
 
+constexpr int kThreads = 256;                // of the join
 // The shares of a tile: 32 of its rows a workgroup, a quad of a row a thread, share after share.
 template <class Q>
 __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
     const reef_chunk_attention_desc& d = a.d;
-    const int32_t part = (int32_t)(blockIdx.x % kWaves);
-    const uint32_t rest = blockIdx.x / kWaves;
+    const uint32_t parts = (uint32_t)a.tile_rows / kRows, rest = blockIdx.x / parts;
+    const int32_t part = (int32_t)(blockIdx.x - rest * parts);
     const int32_t kvh = (int32_t)(rest % (uint32_t)d.cache.kv_heads), id = (int32_t)(rest / (uint32_t)d.cache.kv_heads);
     const Item it = find_item(a, id);
     if (it.tile < 0 || it.share || it.shares <= 1) return;
     const int D = d.cache.head_dim, quads = D / 4;
-    const uint32_t rows = (uint32_t)(it.r.added * a.group), row0 = (uint32_t)it.tile * kTileRows + part * kRows;
+    const uint32_t rows = (uint32_t)(it.r.added * a.group), row0 = (uint32_t)(it.tile * a.tile_rows + part * kRows);
     const int32_t shares = min(it.shares, a.most_slots - it.slot);
-    const int64_t step = (int64_t)d.cache.kv_heads * kTileRows;
+    const int64_t step = (int64_t)d.cache.kv_heads * a.tile_rows;
     for (int x = threadIdx.x; x < kRows * quads; x += kThreads) {
         const int i = x / quads, dim = (x - i * quads) * 4;
         const uint32_t row = row0 + i;
         if (row >= rows) continue;
-        const int64_t at = ((int64_t)it.slot * d.cache.kv_heads + kvh) * kTileRows + part * kRows + i;
+        const int64_t at = ((int64_t)it.slot * d.cache.kv_heads + kvh) * a.tile_rows + part * kRows + i;
         float R = -INFINITY, l = 0.0f;
         f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
@@ -718,44 +823,50 @@ int check(const char* what, const reef_chunk_attention_desc* d) {
 
 // How a call is laid out.
 struct Plan {
-    int32_t budget;
+    int32_t tile_rows, budget;
     int64_t items, slots;
     size_t info_bytes, list_bytes, stats_bytes, bytes;
 };
 Plan plan_of(const reef_chunk_attention_desc& d) {
     const int32_t group = d.heads / d.cache.kv_heads, kv = d.cache.kv_heads;
+    Plan p{};
+    p.tile_rows = waves_of(d.cache.head_dim) * kRows;
     int64_t longest = (int64_t)d.max_blocks * d.cache.block_size;
     if (d.longest && d.longest < longest) longest = d.longest;
-    if (d.window) longest = std::min(longest, (int64_t)d.window + kTileRows / group);
-    Plan p{};
-    p.items = (int64_t)d.tokens * group / kTileRows + d.requests;
+    if (d.window) longest = std::min(longest, (int64_t)d.window + p.tile_rows / group);
+    p.items = (int64_t)d.tokens * group / p.tile_rows + d.requests;
     if (longest > kLeast) {
         p.budget = std::max(1, kGroups / kv);
         p.slots = std::min<int64_t>(4ll * p.budget, 2ll * p.budget + p.items);
         p.items += 2ll * p.budget;
-        p.stats_bytes = (size_t)p.slots * kv * kTileRows * 8;
+        p.stats_bytes = (size_t)p.slots * kv * p.tile_rows * 8;
     }
     if (d.requests > kFew) {
         p.info_bytes = (size_t)d.requests * 16;
         p.list_bytes = ((size_t)(1 + p.items) * 4 + 15) / 16 * 16;
     }
-    p.bytes = p.info_bytes + p.list_bytes + p.stats_bytes + (size_t)p.slots * kv * kTileRows * d.cache.head_dim * 4;
+    p.bytes = p.info_bytes + p.list_bytes + p.stats_bytes + (size_t)p.slots * kv * p.tile_rows * d.cache.head_dim * 4;
     return p;
 }
 
+template <class Q, class C, int DP>
+int run_heads(const char* what, const Args& a, unsigned groups, void* stream) {
+    static_assert(Shape<Q, C, DP>::kWaves == waves_of(DP), "");
+    return launch(what, chunk_attention<Q, C, DP>, dim3(groups), dim3(Shape<Q, C, DP>::kThreads), a, stream);
+}
 template <class Q, class C>
 int run(const char* what, const Args& a, const Plan& p, void* stream) {
     const int D = a.d.cache.head_dim;
-    const dim3 grid((unsigned)(p.items * a.d.cache.kv_heads)), block(kThreads);
+    const unsigned groups = (unsigned)(p.items * a.d.cache.kv_heads);
     if (a.list)
         if (int rc = launch(what, list_items, dim3(1), dim3(kListThreads), a, stream)) return rc;
-    const int rc = D <= 64    ? launch(what, chunk_attention<Q, C, 64>, grid, block, a, stream)
-                   : D <= 96  ? launch(what, chunk_attention<Q, C, 96>, grid, block, a, stream)
-                   : D <= 128 ? launch(what, chunk_attention<Q, C, 128>, grid, block, a, stream)
-                   : D <= 192 ? launch(what, chunk_attention<Q, C, 192>, grid, block, a, stream)
-                              : launch(what, chunk_attention<Q, C, 256>, grid, block, a, stream);
+    const int rc = D <= 64    ? run_heads<Q, C, 64>(what, a, groups, stream)
+                   : D <= 96  ? run_heads<Q, C, 96>(what, a, groups, stream)
+                   : D <= 128 ? run_heads<Q, C, 128>(what, a, groups, stream)
+                   : D <= 192 ? run_heads<Q, C, 192>(what, a, groups, stream)
+                              : run_heads<Q, C, 256>(what, a, groups, stream);
     if (rc || !p.budget) return rc;
-    return launch(what, join_shares<Q>, dim3(grid.x * kWaves), block, a, stream);
+    return launch(what, join_shares<Q>, dim3(groups * (unsigned)(p.tile_rows / kRows)), dim3(kThreads), a, stream);
 }
 
 }  // namespace
@@ -776,7 +887,8 @@ extern "C" int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, cons
         return refuse(what, "null or unaligned argument");
     const Plan p = plan_of(*d);
     // (2^32 threads are refused by the launch, which may be the call's second one)
-    if (p.items * d->cache.kv_heads * kWaves >= 1ll << 24) return refuse(what, "%lld workgroups are too many", (long long)(p.items * d->cache.kv_heads * kWaves));
+    if (p.items * d->cache.kv_heads * (p.tile_rows / kRows) >= 1ll << 23)
+        return refuse(what, "%lld workgroups are too many", (long long)(p.items * d->cache.kv_heads * (p.tile_rows / kRows)));
     if (p.bytes && (!rows16(workspace) || workspace_bytes < (int64_t)p.bytes))
         return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", p.bytes, (long long)workspace_bytes);
     char* const w = (char*)workspace;
@@ -784,7 +896,7 @@ extern "C" int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, cons
     const int32_t group = d->heads / d->cache.kv_heads;
     const Args a{*d, query, key_cache, value_cache, table, starts, cached, lengths, out, lse, (int4*)w, p.list_bytes ? (int32_t*)(w + list) : nullptr, (float*)(w + parts),
                  (float2*)(w + stats), d->scale == 0.0f ? kLog2e : std::fabs(d->scale) * kLog2e, d->scale < 0.0f ? (d->type == REEF_TYPE_F32 ? 0x80000000u : 0x80008000u) : 0u,
-                 d->scale == 0.0f, group, p.budget, (int32_t)p.items, (int32_t)p.slots, divider((uint32_t)d->cache.block_size), divider((uint32_t)group)};
+                 d->scale == 0.0f, group, p.tile_rows, p.budget, (int32_t)p.items, (int32_t)p.slots, divider((uint32_t)d->cache.block_size), divider((uint32_t)group)};
     switch (d->type * 4 + d->cache.type) {
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, p, stream);
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return run<float, _Float16>(what, a, p, stream);
