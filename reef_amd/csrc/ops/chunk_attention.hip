@@ -243,6 +243,12 @@ __device__ inline uint32_t wave_max(uint32_t v) {
 }
 __device__ inline uint32_t wave_min(uint32_t v) { return ~wave_max(~v); }
 
+// A value that is to be made where it is used, not ahead of a loop and held in registers, of which there are none left.
+__device__ inline uint32_t again(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
 template <class Q>
 __device__ inline void put4(Q* to, float a, float b, float c, float d) {
     typedef Q Q4 __attribute__((ext_vector_type(4)));
@@ -302,7 +308,7 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
     constexpr bool kEven = kAllPieces % kThreads == 0;
     __shared__ __align__(16) unsigned char k_near[2 * kBuffer], v_near[kValues * kBuffer];
     __shared__ int64_t offsets[kWaves][2][kTile];
-    __shared__ uint32_t odd_tile[2];         // number of the last tile whose values held infinities or NaN, of even and odd ones
+    __shared__ uint32_t odd_first, odd_end;  // of the tiles whose values were cleaned
 
     const reef_chunk_attention_desc& d = a.d;
     const int32_t kvh = (int32_t)(blockIdx.x % (uint32_t)d.cache.kv_heads);
@@ -355,25 +361,26 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
     constexpr uint64_t kAll = kTile == 64 ? ~0ull : 0xFFFFFFFFull;
     u32x4 k_on_way[kMine], v_on_way[kMine];
     auto load = [&](const C* pool, u32x4 (&on_way)[kMine], int slot) __attribute__((always_inline)) {
+        const uint32_t tid = again(threadIdx.x);
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
-            const int x = i * kThreads + threadIdx.x, at = x / kRowPieces, piece = x - at * kRowPieces;
+            const uint32_t x = i * kThreads + tid, at = x / kRowPieces, piece = x - at * kRowPieces;
             if (!kEven && x >= kAllPieces) continue;
-            on_way[i] = *(const u32x4*)(pool + offsets[wave][slot][at] + (DP == D || piece * 16 < D * (int)sizeof(C) ? piece * (16 / (int)sizeof(C)) : 0));
+            on_way[i] = *(const u32x4*)(pool + offsets[wave][slot][at] + (piece * 16 < D * (uint32_t)sizeof(C) ? piece * (16 / (uint32_t)sizeof(C)) : 0));
         }
     };
     // Into LDS: zeros where there is no token, or no such dimension.  Where not all rows see all of a tile, infinities and NaN among its values must not
-    // be multiplied by weights of 0: they become 0 as well, and the tile's number is left for spoil().
+    // be multiplied by weights of 0: they become 0 as well, and are looked for again at the end.
     auto store = [&](unsigned char* to, u32x4 (&on_way)[kMine], uint64_t there, bool clean, uint32_t number) __attribute__((always_inline)) {
+        const uint32_t tid = again(threadIdx.x);
 #pragma unroll
         for (int i = 0; i < kMine; ++i) {
-            const int x = i * kThreads + threadIdx.x, at = x / kRowPieces, piece = x - at * kRowPieces;
+            const uint32_t x = i * kThreads + tid, at = x / kRowPieces, piece = x - at * kRowPieces;
             if (!kEven && x >= kAllPieces) continue;
             u32x4 w = on_way[i];
-            if (there != kAll || D != DP) {
-                const bool inside = (there >> at & 1) && piece * 16 < D * (int)sizeof(C);
-                if (!inside) w = {0, 0, 0, 0};
-            }
+            const bool inside = (there >> at & 1) && piece * 16 < D * (uint32_t)sizeof(C);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = inside ? w[j] : 0;
             if (clean) {
                 constexpr uint32_t kOdd = sizeof(C) == 4 ? 0x7F800000u : kHalf ? 0x7C00u : 0x7F80u;
                 bool found = false;
@@ -385,7 +392,10 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
                     found |= keep != ~0u;
                     w[j] &= keep;
                 }
-                if (found) odd_tile[number & 1] = number;
+                if (found) {
+                    atomicMin(&odd_first, number);
+                    atomicMax(&odd_end, number + 1);
+                }
             }
             if constexpr (kTermsC == 1) {
                 *(u32x4*)(to + N::at(at, piece)) = w;
@@ -617,26 +627,6 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
                 multiply_by(v, c, m);
             }
     };
-    // Rows that see an infinity or a NaN among the values of a tile have NaN there.  (Rare: the values are read again, token after token.)
-    auto spoil = [&](uint32_t t0) __attribute__((always_inline)) {
-        for (uint32_t t = t0; t < min(end, t0 + kTile); ++t) {
-            const uint32_t page = divided(t, a.block);
-            const int64_t at = paged_row(view, table[page], (int32_t)(t - page * a.block.by));
-            if (at < 0) continue;
-            const bool mine = t >= lo && t < hi;
-            int from = 4 * h;
-            asm volatile("" : "+v"(from));   // (or 64 addresses are made ahead of the loop, and held in registers for it)
-#pragma unroll
-            for (int m = 0; m < kSlabs; ++m)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int dim = m * 32 + 8 * (i >> 2) + (i & 3) + from;
-                    const float v = (float)values[at + (dim < D ? dim : 0)];
-                    if (mine && !(fabsf(v) < INFINITY)) o[m][i] = NAN;
-                }
-        }
-    };
-
     const uint32_t count = (end - begin + kTile - 1) / kTile;
     auto seen_by_all = [&](uint32_t j, uint64_t there) __attribute__((always_inline)) {
         return begin + j * kTile >= all_lo && begin + (j + 1) * kTile <= all_hi && there == kAll;
@@ -671,7 +661,10 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
     constexpr std::integral_constant<int, 0> kEvenOnes;
     constexpr std::integral_constant<int, 1> kOddOnes;
     if (count) {
-        if (threadIdx.x < 2) odd_tile[threadIdx.x] = ~0u;
+        if (threadIdx.x == 0) {
+            odd_first = ~0u;
+            odd_end = 0;
+        }
         there = find(begin, entry, 0);
         entry = count > 1 ? entry_of(begin + kTile) : -1;
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -704,16 +697,13 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
                 multiply_keys(next, k_near + kNow * kBuffer);
                 weigh(s);
                 multiply_values(v_near + (kValues == 2 ? kNow ^ 1 : 0) * kBuffer);
-                const float top = largest(next);
-                if (odd_tile[kNow ^ 1] == j - 1) spoil(begin + (j - 1) * kTile);
-                look(j, next, top);
+                look(j, next, largest(next));
                 take(j, parity);
             };
             auto end_with = [&](f32x16 (&s)[kSub], int parity) __attribute__((always_inline)) {
                 approach(s);
                 weigh(s);
                 multiply_values(v_near + (kValues == 2 ? parity : 0) * kBuffer);
-                if (odd_tile[parity] == count - 1) spoil(begin + (count - 1) * kTile);
             };
             ask(0, kEvenOnes);
             multiply_keys(even, k_near);
@@ -730,6 +720,19 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
                 for (int u = 0; u < kSub; ++u) even[u] = odd[u];
             }
             end_with(even, (count - 1) & 1);
+            // Rows that see an infinity or a NaN among values have NaN.  (Rare: the values are read again, token after token.)
+            for (uint32_t t = begin + min(odd_first, odd_end) * kTile; t < min(end, begin + odd_end * kTile); ++t) {
+                const uint32_t page = divided(t, a.block);
+                const int64_t at = paged_row(view, table[page], (int32_t)(t - page * a.block.by));
+                if (at < 0 || !(t >= lo && t < hi)) continue;
+#pragma unroll
+                for (int m = 0; m < kSlabs; ++m)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int dim = m * 32 + 8 * (i >> 2) + 4 * h + (i & 3);
+                        if (!(fabsf((float)values[at + (dim < D ? dim : 0)]) < INFINITY)) o[m][i] = NAN;
+                    }
+            }
         }
     }
 
