@@ -10,8 +10,10 @@ using namespace reef_ops;
 
 constexpr int kRows = 32;                    // query rows of a wavefront: heads of one token next to each other, token after token
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr int32_t kLeast = 512;              // cached tokens a share at least
-constexpr int kGroups = 512;                 // workgroups that the shares of all tiles are to make
+constexpr int32_t kLeast = 256, kLeastFew = 512;   // cached tokens a share at least, of tiles of 32 rows for each wavefront and of 32 in all
+constexpr int32_t kCut = 768, kCutFew = 2048;      // up to so many a tile is not cut
+constexpr int kAtOnce = 256;                       // workgroups that run at once, one a CU
+constexpr int kGroups = 3 * kAtOnce;               // workgroups that the shares of all tiles are to make at most
 constexpr float kSlack = 8.0f;               // powers of two by which weights may pass their reference
 
 struct Args {
@@ -20,8 +22,8 @@ struct Args {
     const int32_t *table, *starts, *cached, *lengths;
     void* out;
     float* lse;
-    int4* info;             // [request], where there are many: first item, shares, first slot, tiles
-    int32_t* list;          // the number of items, then the request of each
+    int4* info;             // [request], where there are many: first item, shares, first slot
+    int32_t* list;          // the numbers of items and of slots, then the request of each item
     float* parts;           // [slot][cache head][row of the tile][head_dim], sums that are not divided yet
     float2* stats;          // [slot][cache head][row of the tile]: power of two that they are to be multiplied by, sum of the weights
     float scale;            // |scale| log2 e, or log2 e where it is 0
@@ -29,8 +31,10 @@ struct Args {
     int32_t zero;           // scale is 0
     int32_t group;
     int32_t tile_rows;      // of a workgroup
-    int32_t budget;         // shares that all tiles are cut into, beside one each; 0: tiles are not split
+    int32_t budget;         // workgroups that tiles are cut for, beside one each; 0: they are not cut
     int32_t most_items, most_slots;
+    int32_t* used;          // slots that there are; behind it (int4 aligned) what each belongs to
+    int4* jobs;             // [slot]: request, tile, share, shares
     Divider block, by_group;
 };
 
@@ -43,6 +47,7 @@ struct Request {
 struct Item {
     Request r;
     int32_t request, tile, share, shares, slot;   // tile < 0: there is no such item; slot of the tile's first share
+    int32_t slots;                           // of all
 };
 
 __device__ inline int32_t start_of(const Args& a, int32_t i) { return max(0, min(a.starts[i], a.d.tokens)); }
@@ -71,35 +76,94 @@ __device__ inline void size_up(const Args& a, const Request& r, float* most, flo
     *most = fmaxf(u, v);
     *all = (float)r.tiles * (u + v) * 0.5f;
 }
-// Tokens of a share: sum over the tiles of ceil(most / tokens) <= 2 budget + tiles, as most <= u + v.  (The sum of the requests' sizes is rounded up by more
-// than its additions lose.)
-__device__ inline float tokens_of(float all, int32_t budget) { return fmaxf((float)kLeast, all * 1.02f / (float)budget); }
-__device__ inline int32_t shares_of(float most, float tokens) { return max(1, (int32_t)ceilf(most / tokens)); }
-
-template <class V>
-__device__ inline V before_me(V v) {         // exclusive prefix sums over the wavefront
-    V at = v;
-    for (int x = 1; x < 64; x <<= 1) {
-        const V o = __shfl_up(at, x);
-        if ((int)(threadIdx.x & 63) >= x) at += o;
+// How long shares are: tiles of up to `whole` tokens are not cut, others into shares of `tokens`.  Tiles that are longer than 1.3 rounds' worth are cut into half
+// rounds.  Where there are fewer than kGroups tiles, and those of a request are much alike (not as a prompt's, of which long ones and short ones make up for each other), they are
+// cut into the number n that takes the least rounds of workgroups, ceil(n N / 256) / n.
+// Where that makes more items than there are workgroups for (lengths that were not expected), none is cut.
+struct Cut {
+    float whole, tokens, alike;              // alike: tokens of a share of tiles that are much alike; 0: as others
+};
+__device__ inline Cut cut_of(const Args& a, float all, float tiles) {
+    const float kv = (float)a.d.cache.kv_heads, groups = tiles * kv;
+    Cut c;
+    c.tokens = all * kv * (1.02f / (2 * kAtOnce));
+    c.whole = 2.6f * c.tokens;
+    c.alike = 0.0f;
+    if (groups < (float)a.budget) {
+        float best = ceilf(groups * (1.0f / kAtOnce)), n = 1.0f;
+        for (float k = 2.0f; k * groups <= (float)a.budget && k <= 64.0f; k += 1.0f) {
+            const float rounds = ceilf(k * groups * (1.0f / kAtOnce)) * __builtin_amdgcn_rcpf(k);
+            if (rounds < 0.95f * best) {
+                best = rounds;
+                n = k;
+            }
+        }
+        if (n > 1.0f) c.alike = all * 1.02f / (tiles * n);
     }
-    return at - v;
+    return c;
+}
+__device__ inline int32_t shares_of(const Args& a, const Cut& c, float most, float all, int32_t tiles) {
+    const bool few = a.tile_rows == kRows, alike = c.alike > 0.0f && most * (float)tiles < 1.5f * all;
+    if (most <= fmaxf((float)(few ? kCutFew : kCut), alike ? c.alike : c.whole)) return 1;
+    return (int32_t)ceilf(most / fmaxf((float)(few ? kLeastFew : kLeast), alike ? c.alike : c.tokens));
 }
 
-// Up to kFew requests each wavefront finds its item by itself, a request a lane; more are listed by a launch ahead.
-constexpr int32_t kFew = 64;
+// Items and slots are counted up to 2^32 - 1: more there are only where starts do not ascend, and then nothing may run over.
+__device__ inline uint32_t plus(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+__device__ inline uint32_t product(int32_t tiles, int32_t shares) { return (uint32_t)min((uint64_t)(uint32_t)tiles * (uint32_t)shares, (uint64_t)UINT32_MAX); }
+// Prefix sums over the wavefront without the lane's own value; *all: with all of them.
+template <int CONTROL, int ROWS>
+__device__ inline uint32_t moved(uint32_t x) { return __builtin_amdgcn_update_dpp(0, x, CONTROL, ROWS, 0xF, true); }
+__device__ inline uint32_t before_me(uint32_t v, uint32_t* all) {
+    constexpr int kUp = 0x110, kLast15 = 0x142, kLast31 = 0x143;     // rows of 16 by lanes; the last lane of a row, of a half, to the next
+    const uint32_t mine = v;
+    v = plus(v, moved<kUp | 1, 0xF>(v));
+    v = plus(v, moved<kUp | 2, 0xF>(v));
+    v = plus(v, moved<kUp | 4, 0xF>(v));
+    v = plus(v, moved<kUp | 8, 0xF>(v));
+    v = plus(v, moved<kLast15, 0xA>(v));
+    v = plus(v, moved<kLast31, 0xC>(v));
+    *all = __builtin_amdgcn_readlane(v, 63);
+    return v == UINT32_MAX ? v : v - mine;
+}
+__device__ inline float sum_of(float v) {
+    for (int x = 32; x; x >>= 1) v += __shfl_xor(v, x);
+    return v;
+}
+
+// Up to kFewRequests requests each wavefront finds its item by itself, a request a lane; more are listed by a launch ahead.
+constexpr int32_t kFewRequests = 64, kListHead = 2;
 __device__ inline Item find_item(const Args& a, int32_t id) {
     Item it;
     it.tile = -1;
     int32_t local;
     if (a.list) {
         if (id >= a.list[0]) return it;
-        it.request = a.list[1 + id];
+        it.request = a.list[kListHead + id];
         const int4 info = a.info[it.request];
         it.r = request_of(a, it.request);
         local = id - info.x;
         it.shares = info.y;
         it.slot = info.z;
+        it.slots = a.list[1];
+    } else if (a.d.requests == 1) {
+        it.request = 0;
+        it.r = request_of(a, 0);
+        it.shares = 1;
+        if (a.budget) {
+            float most, all;
+            size_up(a, it.r, &most, &all);
+            it.shares = __builtin_amdgcn_readfirstlane(shares_of(a, cut_of(a, all, (float)it.r.tiles), most, all, it.r.tiles));
+        }
+        uint32_t items = product(it.r.tiles, it.shares);
+        if (items > (uint32_t)a.most_items) {
+            it.shares = 1;
+            items = (uint32_t)it.r.tiles;
+        }
+        if ((uint32_t)id >= items) return it;
+        it.slot = 0;
+        it.slots = it.shares > 1 ? (int32_t)min(items, 1u << 30) : 0;
+        local = id;
     } else {
         const int lane = threadIdx.x & 63;
         Request r{};
@@ -108,11 +172,16 @@ __device__ inline Item find_item(const Args& a, int32_t id) {
         if (a.budget) {
             float most, all;
             size_up(a, r, &most, &all);
-            for (int x = 32; x; x >>= 1) all += __shfl_xor(all, x);
-            shares = shares_of(most, tokens_of(all, a.budget));
+            shares = shares_of(a, cut_of(a, sum_of(all), sum_of((float)r.tiles)), most, all, r.tiles);
         }
-        const int32_t mine = r.tiles * shares, at = before_me(mine), slot = before_me(shares > 1 ? mine : 0);
-        const uint64_t who = __builtin_amdgcn_ballot_w64(id >= at && id < at + mine);
+        uint32_t all_items, all_slots = 0, slot = 0, mine = product(r.tiles, shares), at = before_me(mine, &all_items);
+        if (a.budget && all_items > (uint32_t)a.most_items) {
+            shares = 1;
+            mine = (uint32_t)r.tiles;
+            at = before_me(mine, &all_items);
+        }
+        if (a.budget) slot = before_me(shares > 1 ? mine : 0, &all_slots);
+        const uint64_t who = __builtin_amdgcn_ballot_w64((uint32_t)id >= at && (uint32_t)id - at < mine);
         if (!who) return it;
         const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(who));
         it.request = l;
@@ -122,73 +191,97 @@ __device__ inline Item find_item(const Args& a, int32_t id) {
         it.r.n = __builtin_amdgcn_readlane(r.n, l);
         it.r.tiles = __builtin_amdgcn_readlane(r.tiles, l);
         it.shares = __builtin_amdgcn_readlane(shares, l);
-        it.slot = __builtin_amdgcn_readlane(slot, l);
-        local = id - __builtin_amdgcn_readlane(at, l);
+        it.slot = (int32_t)min(__builtin_amdgcn_readlane(slot, l), 1u << 30);
+        it.slots = (int32_t)min(all_slots, 1u << 30);
+        local = id - (int32_t)__builtin_amdgcn_readlane(at, l);
     }
     // the last tiles, which see most, first
     const int32_t k = local / it.shares;
     it.share = local - k * it.shares;
     it.tile = it.r.tiles - 1 - k;
-    it.slot += k * it.shares;
+    it.slot += local - it.share;
     return it;
 }
 
 constexpr int kListThreads = 1024;
 __global__ void __launch_bounds__(kListThreads) list_items(Args a) {
     constexpr int kListWaves = kListThreads / 64;
-    __shared__ float sums[kListWaves];
-    __shared__ int2 counts[kListWaves];
+    __shared__ float2 sums[kListWaves];
+    __shared__ uint2 counts[kListWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int32_t R = a.d.requests, per = (R + kListThreads - 1) / kListThreads, lo = min(R, tid * per), hi = min(R, lo + per);
-    float tokens = 0.0f;
+    Cut cut{};
     if (a.budget) {
-        float sum = 0.0f;
+        float sum = 0.0f, tiles = 0.0f;
         for (int32_t i = lo; i < hi; ++i) {
+            const Request r = request_of(a, i);
             float most, all;
-            size_up(a, request_of(a, i), &most, &all);
+            size_up(a, r, &most, &all);
             sum += all;
+            tiles += (float)r.tiles;
         }
-        for (int x = 32; x; x >>= 1) sum += __shfl_xor(sum, x);
-        if (lane == 0) sums[wave] = sum;
+        sum = sum_of(sum);
+        tiles = sum_of(tiles);
+        if (lane == 0) sums[wave] = make_float2(sum, tiles);
         __syncthreads();
-        sum = 0.0f;
-        for (int w = 0; w < kListWaves; ++w) sum += sums[w];
-        tokens = tokens_of(sum, a.budget);
+        sum = tiles = 0.0f;
+        for (int w = 0; w < kListWaves; ++w) {
+            sum += sums[w].x;
+            tiles += sums[w].y;
+        }
+        cut = cut_of(a, sum, tiles);
     }
+    bool whole = !a.budget;
     auto shares_and_tiles = [&](int32_t i) {
         const Request r = request_of(a, i);
         int32_t shares = 1;
-        if (a.budget) {
+        if (!whole) {
             float most, all;
             size_up(a, r, &most, &all);
-            shares = shares_of(most, tokens);
+            shares = shares_of(a, cut, most, all, r.tiles);
         }
         return make_int2(shares, r.tiles);
     };
-    int32_t items = 0, slots = 0;
-    for (int32_t i = lo; i < hi; ++i) {
-        const int2 x = shares_and_tiles(i);
-        items += x.x * x.y;
-        if (x.x > 1) slots += x.x * x.y;
-    }
-    int32_t item = before_me(items), slot = before_me(slots), all = 0;
-    if (lane == 63) counts[wave] = make_int2(item + items, slot + slots);
-    __syncthreads();
-    for (int w = 0; w < kListWaves; ++w) {
-        if (w < wave) {
-            item += counts[w].x;
-            slot += counts[w].y;
+    uint32_t all, all_slots, item, slot;
+    auto count = [&]() {
+        uint32_t items = 0, slots = 0, of_wave, slots_of_wave;
+        for (int32_t i = lo; i < hi; ++i) {
+            const int2 x = shares_and_tiles(i);
+            items = plus(items, product(x.x, x.y));
+            if (x.x > 1) slots = plus(slots, product(x.x, x.y));
         }
-        all += counts[w].x;
+        item = before_me(items, &of_wave);
+        slot = before_me(slots, &slots_of_wave);
+        __syncthreads();
+        if (lane == 0) counts[wave] = make_uint2(of_wave, slots_of_wave);
+        __syncthreads();
+        all = all_slots = 0;
+        for (int w = 0; w < kListWaves; ++w) {
+            if (w < wave) {
+                item = plus(item, counts[w].x);
+                slot = plus(slot, counts[w].y);
+            }
+            all = plus(all, counts[w].x);
+            all_slots = plus(all_slots, counts[w].y);
+        }
+    };
+    count();
+    if (!whole && all > (uint32_t)a.most_items) {
+        whole = true;
+        count();
     }
     for (int32_t i = lo; i < hi; ++i) {
         const int2 x = shares_and_tiles(i);
-        a.info[i] = make_int4(item, x.x, slot, x.y);
-        for (int32_t k = 0; k < x.x * x.y && item + k < a.most_items; ++k) a.list[1 + item + k] = i;
-        item += x.x * x.y;
-        if (x.x > 1) slot += x.x * x.y;
+        const uint32_t mine = product(x.x, x.y);
+        a.info[i] = make_int4((int32_t)min(item, 1u << 30), x.x, (int32_t)min(slot, 1u << 30), 0);
+        for (uint32_t k = item; k < min(plus(item, mine), (uint32_t)a.most_items); ++k) a.list[kListHead + k] = i;
+        item = plus(item, mine);
+        if (x.x > 1) slot = plus(slot, mine);
     }
-    if (tid == 0) a.list[0] = min(all, a.most_items);
+    if (tid == 0) {
+        a.list[0] = (int32_t)min(all, (uint32_t)a.most_items);
+        a.list[1] = (int32_t)min(all_slots, 1u << 30);
+    }
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -228,6 +321,11 @@ __device__ inline void terms(float a, float b, uint32_t (&t)[N], _Float16) {
     }
 }
 
+// Which bits of a word hold finite values.
+__device__ inline uint32_t keep_of(uint32_t w, float) { return (w & 0x7F800000u) == 0x7F800000u ? 0 : ~0u; }
+__device__ inline uint32_t keep_of(uint32_t w, __bf16) { return ((w & 0x7F80u) == 0x7F80u ? 0 : 0xFFFFu) | ((w & 0x7F800000u) == 0x7F800000u ? 0 : 0xFFFF0000u); }
+__device__ inline uint32_t keep_of(uint32_t w, _Float16) { return ((w & 0x7C00u) == 0x7C00u ? 0 : 0xFFFFu) | ((w & 0x7C000000u) == 0x7C000000u ? 0 : 0xFFFF0000u); }
+
 // A value of both halves of the wavefront, joined: lanes l and l + 32 have the same row.
 __device__ inline float other_max(float x) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -237,12 +335,6 @@ __device__ inline float other_sum(float x) {
     const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(a[0]) + __uint_as_float(a[1]);
 }
-__device__ inline uint32_t wave_max(uint32_t v) {
-    for (int x = 32; x; x >>= 1) v = max(v, (uint32_t)__shfl_xor(v, x));
-    return __builtin_amdgcn_readfirstlane(v);
-}
-__device__ inline uint32_t wave_min(uint32_t v) { return ~wave_max(~v); }
-
 // A value that is to be made where it is used, not ahead of a loop and held in registers, of which there are none left.
 __device__ inline uint32_t again(uint32_t x) {
     asm volatile("" : "+v"(x));
@@ -273,7 +365,11 @@ template <class Q, class C, int DP>
 struct Shape {
     static constexpr bool kHalf = __is_same(C, _Float16);
     static constexpr int kTermsC = sizeof(C) == 4 ? 3 : 1, kTermsQ = sizeof(Q) == 2 ? 1 : kHalf ? 2 : 3;
-    static constexpr int kWaves = waves_of(DP), kThreads = kWaves * 64, kTile = kTermsQ == 1 && DP <= 128 ? 64 : 32;
+    static constexpr int kWaves = waves_of(DP), kTile = kTermsQ == 1 && DP <= 128 ? 64 : 32;
+    // Tiles of 32 rows in all: registers of what a wavefront holds (keys, values, queries, output, weights), and so how many wavefronts; 0: too many for any.
+    static constexpr int kFewV = DP <= 64 ? 2 : DP <= 128 ? 4 : 8;            // values of a row of V a lane
+    static constexpr int kFewHeld = DP * (int)sizeof(C) / 8 + 16 * kFewV * (int)sizeof(C) / 4 + kTermsQ * DP / 4 + kFewV * 16 + 16 + 8 * kTermsQ;
+    static constexpr int kFewWaves = kFewHeld <= 220 ? 8 : kFewHeld <= 440 ? 4 : 0;
 };
 
 // A tile of query rows over a share of the tokens they see, one cache head: each wavefront has 32 rows, all of them the keys and values that
@@ -292,43 +388,55 @@ struct Shape {
 // 32-bit queries over 16-bit caches are two terms of fp16 or three of bf16 each, and so are their weights; 32-bit caches are three terms of bf16 on
 // both sides, six products (the others are below 2^-22).  Weights of 16-bit types are rounded to the type once: half a step of the type of each at most, which in their mean is
 // no more than the output's own rounding (two terms would take 1.4 times as long).
-template <class Q, class C, int DP>
-__global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(Args a) {
+template <class Q, class C, int DP, bool FEW>
+__global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C, DP>::kWaves) * 64) chunk_attention(Args a) {
     using E = std::conditional_t<sizeof(C) == 4, __bf16, C>;                  // what is multiplied
     using Sh = Shape<Q, C, DP>;
     constexpr bool kHalf = Sh::kHalf;
-    constexpr int kTermsC = Sh::kTermsC, kTermsQ = Sh::kTermsQ, kTile = Sh::kTile, kSub = kTile / 32, kWaves = Sh::kWaves, kThreads = Sh::kThreads;
+    constexpr int kTermsC = Sh::kTermsC, kTermsQ = Sh::kTermsQ, kTile = Sh::kTile, kSub = kTile / 32, kWaves = FEW ? Sh::kFewWaves : Sh::kWaves, kThreads = kWaves * 64;
     constexpr float kGrow = kHalf ? 6.0f : 0.0f;                              // 2^(6 + 8 + 1/2) < 65504
-    constexpr int kSteps = DP / 16, kSlabs = DP / 32, kTileRows = kWaves * kRows;
+    constexpr int kSteps = DP / 16, kSlabs = DP / 32, kTileRows = FEW ? kRows : kWaves * kRows;
     using N = Near<DP>;
     constexpr int kPlane = kTile * N::kPitch, kBuffer = kTermsC * kPlane;
     constexpr int kRowPieces = DP * (int)sizeof(C) / 16, kAllPieces = kTile * kRowPieces;    // 16-byte pieces of a row in memory, of a tile
     constexpr int kMine = (kAllPieces + kThreads - 1) / kThreads;             // of a thread
     constexpr int kValues = kTermsC == 3 && DP > 128 ? 1 : 2;                 // buffers of values: there is no room for two of three terms of these
     constexpr bool kEven = kAllPieces % kThreads == 0;
-    __shared__ __align__(16) unsigned char k_near[2 * kBuffer], v_near[kValues * kBuffer];
+    constexpr int kFewV = Sh::kFewV;
+    constexpr int kKeysNear = 2 * kBuffer, kNear = FEW ? kWaves / 2 * kFewV * 16 * 64 * 4 : kKeysNear + kValues * kBuffer;
+    __shared__ __align__(16) unsigned char near[kNear];
+    unsigned char* const k_near = near;
+    unsigned char* const v_near = near + kKeysNear;
     __shared__ int64_t offsets[kWaves][2][kTile];
     __shared__ uint32_t odd_first, odd_end;  // of the tiles whose values were cleaned
 
     const reef_chunk_attention_desc& d = a.d;
-    const int32_t kvh = (int32_t)(blockIdx.x % (uint32_t)d.cache.kv_heads);
-    const int32_t id = (int32_t)(blockIdx.x / (uint32_t)d.cache.kv_heads);
+    const int32_t id = (int32_t)(blockIdx.x / (uint32_t)d.cache.kv_heads), kvh = (int32_t)(blockIdx.x - (uint32_t)id * (uint32_t)d.cache.kv_heads);
     const Item it = find_item(a, id);
+    if (a.budget && kvh == 0 && threadIdx.x == 0) {
+        if (it.tile >= 0 && it.shares > 1 && it.slot + it.share < a.most_slots) a.jobs[it.slot + it.share] = make_int4(it.request, it.tile, it.share, it.shares);
+        if (id == 0) *a.used = it.tile < 0 ? 0 : min(it.slots, a.most_slots);      // (without a first item there are none)
+    }
     if (it.tile < 0) return;
     const Request& r = it.r;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = lane & 31, h = lane >> 5;
     const int D = d.cache.head_dim;
 
-    // this lane's row
-    const uint32_t rows = (uint32_t)(r.added * a.group), in_tile = (uint32_t)(wave * kRows + n), row = (uint32_t)it.tile * kTileRows + in_tile;
+    // this lane's row; up to 32 of them are those of all wavefronts
+    const uint32_t rows = (uint32_t)(r.added * a.group);
+    const uint32_t in_tile = (uint32_t)((FEW ? 0 : wave * kRows) + n), row = (uint32_t)it.tile * kTileRows + in_tile;
     const bool valid = row < rows;
     const uint32_t token = divided(row, a.by_group);
     const int32_t head = kvh * a.group + (int32_t)(row - token * a.by_group.by);
     const int64_t out_row = (int64_t)r.first + token;
     const uint32_t place = (uint32_t)r.cached + token;
     const uint32_t hi = valid && place < (uint32_t)r.n ? place + 1 : 0, lo = d.window && hi > (uint32_t)d.window ? hi - d.window : 0;
-    // what all rows of the wavefront see, and what some do
-    const uint32_t all_hi = wave_min(valid ? hi : ~0u), all_lo = wave_max(valid ? lo : 0), some_hi = wave_max(hi), some_lo = wave_min(hi ? lo : ~0u);
+    // what all rows of the wavefront see, and what some do (its rows' places ascend)
+    const uint32_t row0 = __builtin_amdgcn_readfirstlane(row), row_end = min(row0 + kRows, rows);
+    const uint32_t place0 = (uint32_t)r.cached + divided(row0, a.by_group), place1 = row0 < rows ? (uint32_t)r.cached + divided(row_end - 1, a.by_group) : place0;
+    const bool sees_any = row0 < rows && place0 < (uint32_t)r.n, see_all = sees_any && place1 < (uint32_t)r.n;
+    const uint32_t some_hi = sees_any ? min(place1 + 1, (uint32_t)r.n) : 0;
+    const uint32_t all_hi = see_all ? place0 + 1 : 0, all_lo = d.window && place1 + 1 > (uint32_t)d.window ? place1 + 1 - d.window : 0;
 
     const uint2 span = span_of(a, r, it.tile);
     uint32_t begin = span.x, end = span.y;
@@ -382,13 +490,10 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
 #pragma unroll
             for (int j = 0; j < 4; ++j) w[j] = inside ? w[j] : 0;
             if (clean) {
-                constexpr uint32_t kOdd = sizeof(C) == 4 ? 0x7F800000u : kHalf ? 0x7C00u : 0x7F80u;
                 bool found = false;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t keep = ~0u;
-                    if constexpr (sizeof(C) == 4) keep = (w[j] & kOdd) == kOdd ? 0 : ~0u;
-                    else keep = ((w[j] & kOdd) == kOdd ? 0 : 0xFFFFu) | ((w[j] >> 16 & kOdd) == kOdd ? 0 : 0xFFFF0000u);
+                    const uint32_t keep = keep_of(w[j], C());
                     found |= keep != ~0u;
                     w[j] &= keep;
                 }
@@ -476,9 +581,9 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
     }
 
     float R = -INFINITY, l = 0.0f;
-    f32x16 o[kSlabs];
+    f32x16 o[FEW ? kFewV : kSlabs];
 #pragma unroll
-    for (int m = 0; m < kSlabs; ++m)
+    for (int m = 0; m < (int)(sizeof(o) / sizeof(o[0])); ++m)
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[m][i] = 0.0f;
 
@@ -526,18 +631,18 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
         }
         return yes;
     };
-    auto hide = [&](f32x16 (&s)[kSub], uint32_t t0, uint64_t there) __attribute__((always_inline)) {
+    auto hide = [&](auto& s, uint32_t t0, uint64_t there) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < kSub; ++u) {
+        for (int u = 0; u < (int)(sizeof(s) / sizeof(s[0])); ++u) {
             const uint32_t yes = sees(t0 + u * 32, (uint32_t)(there >> (u * 32)));
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[u][i] = yes >> i & 1 ? s[u][i] : -INFINITY;
         }
     };
-    auto largest = [&](f32x16 (&s)[kSub]) __attribute__((always_inline)) {
+    auto largest = [&](auto& s) __attribute__((always_inline)) {
         float top = -INFINITY;
 #pragma unroll
-        for (int u = 0; u < kSub; ++u)
+        for (int u = 0; u < (int)(sizeof(s) / sizeof(s[0])); ++u)
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 if constexpr (kHalf && kTermsQ > 1) s[u][i] *= shrink;
@@ -545,7 +650,7 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
             }
         return other_max(top) * scale;
     };
-    auto refer = [&](float top) __attribute__((always_inline)) {
+    auto refer = [&](float top, auto slabs) __attribute__((always_inline)) {
         const bool passes = top > R + kSlack;
         if (__builtin_amdgcn_ballot_w64(passes)) {
             const float next = passes ? rintf(top) : R;
@@ -553,20 +658,20 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
             R = next;
             l *= f;
 #pragma unroll
-            for (int m = 0; m < kSlabs; ++m)
+            for (int m = 0; m < decltype(slabs)::value; ++m)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[m][i] *= f;
         }
     };
     // From 2^20 on a score's product and its difference from the reference are not exact together: it is rounded first there.
     float times = scale, plus = kGrow;
-    auto approach = [&](f32x16 (&s)[kSub]) __attribute__((always_inline)) {
+    auto approach = [&](auto& s) __attribute__((always_inline)) {
         const float base = R == -INFINITY ? 0.0f : R;
         times = scale;
         plus = kGrow - base;
         if (__builtin_amdgcn_ballot_w64(fabsf(base) >= 0x1p20f)) {
 #pragma unroll
-            for (int u = 0; u < kSub; ++u)
+            for (int u = 0; u < (int)(sizeof(s) / sizeof(s[0])); ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
 #pragma clang fp contract(off)
@@ -579,10 +684,10 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
     };
     // Weights of a tile, as operands.
     u32x4 p[kTile / 16][kTermsQ];
-    auto weigh = [&](f32x16 (&s)[kSub]) __attribute__((always_inline)) {
+    auto weigh = [&](auto& s) __attribute__((always_inline)) {
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < kTile / 16; ++c)
+        for (int c = 0; c < 2 * (int)(sizeof(s) / sizeof(s[0])); ++c)
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
                 const int i = (c & 1) * 8 + 2 * w;
@@ -627,6 +732,238 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
                 multiply_by(v, c, m);
             }
     };
+    if constexpr (FEW) {
+        {
+            // Up to 32 rows in all: each wavefront takes every kWaves-th 32 tokens for itself, its operands from memory as they lie there, without LDS.  Lane (token n, half h)
+            // has the 16-byte pieces 2 c + h of its key; lane (n, h) has of each of its tokens the n-th kFewV values, whose e-th ones are row n of the e-th
+            // product: dimension kFewV n + e.
+            constexpr int kKWords = (int)sizeof(C) * 2, kVWords = kFewV * (int)sizeof(C) / 4;
+            constexpr std::integral_constant<int, kFewV> kAcc;
+            uint32_t k[kSteps][kKWords], v[16][kVWords];
+            int64_t mine = -1;               // place of this lane's token
+            auto entry_at = [&](uint32_t t0) __attribute__((always_inline)) -> int32_t {
+                const uint32_t t = t0 + n;
+                return t < end ? table[divided(t, a.block)] : -1;
+            };
+            auto find_few = [&](uint32_t t0, int32_t entry, int slot) __attribute__((always_inline)) -> uint32_t {
+                const uint32_t t = t0 + n;
+                mine = paged_row(view, entry, (int32_t)(t - divided(t, a.block) * a.block.by));
+                if (h == 0) offsets[wave][slot][n] = mine < 0 ? 0 : mine;
+                const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(mine >= 0);
+                if (mine < 0) mine = 0;
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                return there;
+            };
+            auto load_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int c = 0; c < kSteps; ++c) {
+                    const int at = c * 16 + h * 8;
+#pragma unroll
+                    for (int w = 0; w < kKWords; w += 4) {
+                        const u32x4 x = *(const u32x4*)(keys + mine + (at < D ? at : 0) + w * 4 / (int)sizeof(C));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) k[c][w + i] = x[i];
+                    }
+                }
+            };
+            auto load_v = [&](int slot) __attribute__((always_inline)) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const C* const from = values + offsets[wave][slot][16 * (j >> 3) + 8 * (j >> 2 & 1) + 4 * h + (j & 3)] + (kFewV * n < D ? kFewV * n : 0);
+                    if constexpr (kVWords == 1) {
+                        v[j][0] = *(const uint32_t*)from;
+                    } else if constexpr (kVWords == 2) {
+                        const u32x2 x = *(const u32x2*)from;
+                        v[j][0] = x[0];
+                        v[j][1] = x[1];
+                    } else {
+#pragma unroll
+                        for (int w = 0; w < kVWords; w += 4) {
+                            const u32x4 x = *(const u32x4*)(from + w * 4 / (int)sizeof(C));
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) v[j][w + i] = x[i];
+                        }
+                    }
+                }
+            };
+            constexpr uint32_t kStep = kWaves * 32;
+            uint32_t t0 = begin + wave * 32, odd_from = ~0u, odd_to = 0, there = 0;
+            int slot = 0;
+            int32_t entry = t0 < end ? entry_at(t0) : -1;
+            if (t0 < end) {
+                there = find_few(t0, entry, 0);
+                entry = t0 + kStep < end ? entry_at(t0 + kStep) : -1;
+                load_k();
+                load_v(0);
+            }
+            for (; t0 < end; t0 += kStep) {
+                const bool more = t0 + kStep < end;
+                const uint32_t there_now = there;
+                if (more) {
+                    there = find_few(t0 + kStep, entry, slot ^ 1);
+                    entry = t0 + 2 * kStep < end ? entry_at(t0 + 2 * kStep) : -1;
+                }
+                f32x16 s[1];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[0][i] = 0.0f;
+#pragma unroll
+                for (int c = 0; c < kSteps; ++c) {
+                    const bool inside = c * 16 + h * 8 < D;
+                    if constexpr (kTermsC == 1) {
+                        u32x4 x;
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) x[w] = inside ? k[c][w] : 0;
+#pragma unroll
+                        for (int i = kTermsQ - 1; i >= 0; --i) s[0] = product(x, q[i][c], s[0], E());
+                    } else {
+                        u32x4 x[3];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            uint32_t t[3];
+                            terms(inside ? __uint_as_float(k[c][2 * w]) : 0.0f, inside ? __uint_as_float(k[c][2 * w + 1]) : 0.0f, t, E());
+#pragma unroll
+                            for (int i = 0; i < 3; ++i) x[i][w] = t[i];
+                        }
+#pragma unroll
+                        for (int both = 2; both >= 0; --both)
+#pragma unroll
+                            for (int i = both; i >= 0; --i) s[0] = product(x[i], q[both - i][c], s[0], E());
+                    }
+                }
+                if (more) load_k();
+                const bool by_all = t0 >= all_lo && t0 + 32 <= all_hi;
+                if (!by_all || there_now != ~0u) hide(s, t0, there_now);
+                refer(largest(s), kAcc);
+                approach(s);
+                weigh(s);
+                if (there_now != ~0u) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+                        if (!(there_now >> (4 * h) >> (16 * (j >> 3) + 8 * (j >> 2 & 1) + (j & 3)) & 1)) {
+#pragma unroll
+                            for (int w = 0; w < kVWords; ++w) v[j][w] = 0;
+                        }
+                }
+                if (!by_all) {               // (as in store())
+                    bool found = false;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j)
+#pragma unroll
+                        for (int w = 0; w < kVWords; ++w) {
+                            const uint32_t keep = keep_of(v[j][w], C());
+                            found |= keep != ~0u;
+                            v[j][w] &= keep;
+                        }
+                    if (__builtin_amdgcn_ballot_w64(found)) {
+                        odd_from = min(odd_from, t0);
+                        odd_to = t0 + 32;
+                    }
+                }
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int e = 0; e < kFewV; ++e) {
+                        u32x4 x[kTermsC];
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const int j = c * 8 + 2 * w;
+                            if constexpr (kTermsC == 1) {
+                                x[0][w] = __builtin_amdgcn_perm(v[j + 1][e / 2], v[j][e / 2], e & 1 ? 0x07060302 : 0x05040100);
+                            } else {
+                                uint32_t t[3];
+                                terms(__uint_as_float(v[j][e]), __uint_as_float(v[j + 1][e]), t, E());
+#pragma unroll
+                                for (int i = 0; i < 3; ++i) x[i][w] = t[i];
+                            }
+                        }
+                        if constexpr (kTermsC == 1) {
+#pragma unroll
+                            for (int i = kTermsQ - 1; i >= 0; --i) o[e] = product(x[0], p[c][i], o[e], E());
+                        } else {
+#pragma unroll
+                            for (int both = 2; both >= 0; --both)
+#pragma unroll
+                                for (int i = both; i >= 0; --i) o[e] = product(x[i], p[c][both - i], o[e], E());
+                        }
+                    }
+                slot ^= 1;
+                if (more) load_v(slot);
+            }
+            for (uint32_t t = odd_from; t < min(end, odd_to); ++t) {
+                const uint32_t page = divided(t, a.block);
+                const int64_t at = paged_row(view, table[page], (int32_t)(t - page * a.block.by));
+                if (at < 0 || !(t >= lo && t < hi)) continue;
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+#pragma unroll
+                    for (int e = 0; e < kFewV; ++e) {
+                        const int dim = kFewV * (8 * (i >> 2) + 4 * h + (i & 3)) + e;
+                        if (!(fabsf((float)values[at + (dim < D ? dim : 0)]) < INFINITY)) o[e][i] = NAN;
+                    }
+            }
+            // The wavefronts that had tokens, joined in halves; a lane meets the lanes of its place.
+            l = other_sum(l);
+            float2* const stats = (float2*)offsets;
+            int waves = min((int)((end - begin + 31) / 32), kWaves);
+            while (waves > 1) {
+                const int keep = (waves + 1) / 2;
+                __syncthreads();
+                if (wave >= keep && wave < waves) {
+                    const int at = wave - keep;
+                    stats[at * 64 + lane] = make_float2(R, l);
+#pragma unroll
+                    for (int e = 0; e < kFewV; ++e)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4)
+                            *(f32x4*)(near + (((at * kFewV + e) * 4 + i / 4) * 64 + lane) * 16) = f32x4{o[e][i], o[e][i + 1], o[e][i + 2], o[e][i + 3]};
+                }
+                __syncthreads();
+                if (wave + keep < waves) {
+                    const float2 other = stats[wave * 64 + lane];
+                    const float next = fmaxf(R, other.x), base = next == -INFINITY ? 0.0f : next;
+                    const float f = __builtin_amdgcn_exp2f(R - base), g = __builtin_amdgcn_exp2f(other.x - base);
+                    R = next;
+                    l = l * f + other.y * g;
+#pragma unroll
+                    for (int e = 0; e < kFewV; ++e)
+#pragma unroll
+                        for (int i = 0; i < 16; i += 4) {
+                            const f32x4 x = *(const f32x4*)(near + (((wave * kFewV + e) * 4 + i / 4) * 64 + lane) * 16);
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) o[e][i + y] = o[e][i + y] * f + x[y] * g;
+                        }
+                }
+                waves = keep;
+            }
+            if (wave) return;
+            const int64_t at = ((int64_t)(it.slot + it.share) * d.cache.kv_heads + kvh) * kTileRows + n;
+            if (it.shares > 1) {
+                if (it.slot + it.share >= a.most_slots) return;           // (starts that do not ascend)
+                if (h == 0) a.stats[at] = make_float2(R == -INFINITY ? -INFINITY : R - kGrow, l);
+            }
+            const float f = l == 0.0f ? 0.0f : 1.0f / l;
+            Q* const to = (Q*)a.out + out_row * d.out_stride + head * d.out_head_stride;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int dim = kFewV * (8 * (i >> 2) + 4 * h + (i & 3));
+                if (dim >= D) continue;
+                if (it.shares > 1) {
+#pragma unroll
+                    for (int e = 0; e < kFewV; e += 2) *(float2*)(a.parts + at * D + dim + e) = make_float2(o[e][i], o[e + 1][i]);
+                } else if (valid) {
+#pragma unroll
+                    for (int e = 0; e < kFewV; e += 2) {
+                        typedef Q Q2 __attribute__((ext_vector_type(2)));
+                        const Q2 x = {(Q)(o[e][i] * f), (Q)(o[e + 1][i] * f)};
+                        *(Q2*)(to + dim + e) = x;
+                    }
+                }
+            }
+            if (it.shares == 1 && valid && h == 0 && a.lse) a.lse[out_row * d.heads + head] = l == 0.0f ? -INFINITY : (R + (__log2f(l) - kGrow)) * kLn2;
+            return;
+        }
+    }
+
     const uint32_t count = (end - begin + kTile - 1) / kTile;
     auto seen_by_all = [&](uint32_t j, uint64_t there) __attribute__((always_inline)) {
         return begin + j * kTile >= all_lo && begin + (j + 1) * kTile <= all_hi && there == kAll;
@@ -687,7 +1024,7 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
                     hide(s, begin + j * kTile, there);
                     top = largest(s);
                 }
-                refer(top);
+                refer(top, std::integral_constant<int, kSlabs>());
             };
             // Weights of tile j - 1 go to its values while the scores of tile j are made.
             auto step = [&](uint32_t j, f32x16 (&s)[kSub], f32x16 (&next)[kSub], auto parity) __attribute__((always_inline)) {
@@ -739,7 +1076,7 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
     l = other_sum(l);
     if (it.shares > 1) {
         const int32_t slot = it.slot + it.share;
-        if (slot >= a.most_slots) return;                      // (starts that do not ascend)
+        if (slot >= a.most_slots) return;                 // (starts that do not ascend)
         const int64_t at = ((int64_t)slot * d.cache.kv_heads + kvh) * kTileRows + in_tile;
         if (h == 0) a.stats[at] = make_float2(R == -INFINITY ? -INFINITY : R - kGrow, l);
 #pragma unroll
@@ -765,24 +1102,24 @@ __global__ void __launch_bounds__((Shape<Q, C, DP>::kThreads)) chunk_attention(A
 }
 
 constexpr int kThreads = 256;                // of the join
-// The shares of a tile: 32 of its rows a workgroup, a quad of a row a thread, share after share.
+// The shares of a tile, one cache head: a workgroup for each of its slots, which take the tile's rows among them, a quad of a row a thread, share after share.
 template <class Q>
 __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
     const reef_chunk_attention_desc& d = a.d;
-    const uint32_t parts = (uint32_t)a.tile_rows / kRows, rest = blockIdx.x / parts;
-    const int32_t part = (int32_t)(blockIdx.x - rest * parts);
-    const int32_t kvh = (int32_t)(rest % (uint32_t)d.cache.kv_heads), id = (int32_t)(rest / (uint32_t)d.cache.kv_heads);
-    const Item it = find_item(a, id);
-    if (it.tile < 0 || it.share || it.shares <= 1) return;
+    const int32_t id = (int32_t)(blockIdx.x / (uint32_t)d.cache.kv_heads), kvh = (int32_t)(blockIdx.x - (uint32_t)id * (uint32_t)d.cache.kv_heads);
+    if (id >= *a.used) return;
+    const int4 job = a.jobs[id];
+    // (where starts do not ascend there may be none)
+    if ((uint32_t)job.x >= (uint32_t)d.requests || job.z < 0 || job.z >= job.w || job.z > id) return;
+    const Request r = request_of(a, job.x);
     const int D = d.cache.head_dim, quads = D / 4;
-    const uint32_t rows = (uint32_t)(it.r.added * a.group), row0 = (uint32_t)(it.tile * a.tile_rows + part * kRows);
-    const int32_t shares = min(it.shares, a.most_slots - it.slot);
+    if ((uint32_t)job.y >= (uint32_t)r.tiles) return;
+    const int32_t rows = min(a.tile_rows, r.added * a.group - job.y * a.tile_rows), slot = id - job.z, shares = min(job.w, a.most_slots - slot);
+    const int32_t from = (int32_t)((int64_t)rows * quads * job.z / job.w), to = (int32_t)((int64_t)rows * quads * (job.z + 1) / job.w);
     const int64_t step = (int64_t)d.cache.kv_heads * a.tile_rows;
-    for (int x = threadIdx.x; x < kRows * quads; x += kThreads) {
-        const int i = x / quads, dim = (x - i * quads) * 4;
-        const uint32_t row = row0 + i;
-        if (row >= rows) continue;
-        const int64_t at = ((int64_t)it.slot * d.cache.kv_heads + kvh) * a.tile_rows + part * kRows + i;
+    for (int32_t x = from + (int32_t)threadIdx.x; x < to; x += kThreads) {
+        const int32_t i = x / quads, dim = (x - i * quads) * 4;
+        const int64_t at = ((int64_t)slot * d.cache.kv_heads + kvh) * a.tile_rows + i;
         float R = -INFINITY, l = 0.0f;
         f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
@@ -795,9 +1132,9 @@ __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
             l = l * f + stat.y * g;
             o = o * f + mine * g;
         }
-        const uint32_t token = divided(row, a.by_group);
+        const uint32_t row = (uint32_t)(job.y * a.tile_rows + i), token = divided(row, a.by_group);
         const int32_t head = kvh * a.group + (int32_t)(row - token * a.by_group.by);
-        const int64_t out_row = (int64_t)it.r.first + token;
+        const int64_t out_row = (int64_t)r.first + token;
         const float f = l == 0.0f ? 0.0f : 1.0f / l;
         put4((Q*)a.out + out_row * d.out_stride + head * d.out_head_stride + dim, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
         if (dim == 0 && a.lse) a.lse[out_row * d.heads + head] = l == 0.0f ? -INFINITY : (R + __log2f(l)) * kLn2;
@@ -824,52 +1161,74 @@ int check(const char* what, const reef_chunk_attention_desc* d) {
     return 0;
 }
 
+template <class Q, class C>
+bool has_few(int dim) {
+    return dim <= 64 ? Shape<Q, C, 64>::kFewWaves : dim <= 96 ? Shape<Q, C, 96>::kFewWaves : dim <= 128 ? Shape<Q, C, 128>::kFewWaves : dim <= 192 ? Shape<Q, C, 192>::kFewWaves
+                                                                                                                                      : Shape<Q, C, 256>::kFewWaves;
+}
+bool has_few(const reef_chunk_attention_desc& d) {
+    const int dim = d.cache.head_dim;
+    if (d.type != REEF_TYPE_F32) return d.type == REEF_TYPE_F16 ? has_few<_Float16, _Float16>(dim) : has_few<__bf16, __bf16>(dim);
+    return d.cache.type == REEF_TYPE_F32 ? has_few<float, float>(dim) : d.cache.type == REEF_TYPE_F16 ? has_few<float, _Float16>(dim) : has_few<float, __bf16>(dim);
+}
+
 // How a call is laid out.
 struct Plan {
     int32_t tile_rows, budget;
-    int64_t items, slots;
-    size_t info_bytes, list_bytes, stats_bytes, bytes;
+    bool few;               // tiles of 32 rows in all
+    int64_t items, slots, groups;      // groups: workgroups
+    size_t info_bytes, list_bytes, jobs_bytes, stats_bytes, bytes;
 };
 Plan plan_of(const reef_chunk_attention_desc& d) {
     const int32_t group = d.heads / d.cache.kv_heads, kv = d.cache.kv_heads;
+    const int64_t rows = (int64_t)d.tokens * group;
     Plan p{};
-    p.tile_rows = waves_of(d.cache.head_dim) * kRows;
+    // Up to 32 rows a request on the average: tiles of so many, whose wavefronts share the tokens, else tiles of so many for each wavefront, which share keys and values.
+    p.few = rows <= (int64_t)kRows * d.requests && has_few(d);
+    p.tile_rows = p.few ? kRows : waves_of(d.cache.head_dim) * kRows;
     int64_t longest = (int64_t)d.max_blocks * d.cache.block_size;
     if (d.longest && d.longest < longest) longest = d.longest;
     if (d.window) longest = std::min(longest, (int64_t)d.window + p.tile_rows / group);
-    p.items = (int64_t)d.tokens * group / p.tile_rows + d.requests;
-    if (longest > kLeast) {
-        p.budget = std::max(1, kGroups / kv);
-        p.slots = std::min<int64_t>(4ll * p.budget, 2ll * p.budget + p.items);
-        p.items += 2ll * p.budget;
+    p.items = rows / p.tile_rows + d.requests;
+    const int64_t cut = p.few ? kCutFew : kCut, least = p.few ? kLeastFew : kLeast;
+    if (longest > cut) {
+        // Workgroups that find no item take 2 us a round for their look: there are no more than are likely to have one.
+        const int64_t shares = (longest + least - 1) / least, tiles = p.items;
+        p.budget = tiles * kv <= kAtOnce / 2 ? kAtOnce : kGroups;
+        p.items = std::min(tiles * shares, tiles + (p.budget + kv - 1) / kv);
+        p.slots = p.items;
+        p.jobs_bytes = 16 * (size_t)(1 + p.slots);
         p.stats_bytes = (size_t)p.slots * kv * p.tile_rows * 8;
     }
-    if (d.requests > kFew) {
+    p.groups = p.items * kv;
+    if (d.requests > kFewRequests) {
         p.info_bytes = (size_t)d.requests * 16;
-        p.list_bytes = ((size_t)(1 + p.items) * 4 + 15) / 16 * 16;
+        p.list_bytes = ((size_t)(kListHead + p.items) * 4 + 15) / 16 * 16;
     }
-    p.bytes = p.info_bytes + p.list_bytes + p.stats_bytes + (size_t)p.slots * kv * p.tile_rows * d.cache.head_dim * 4;
+    p.bytes = p.info_bytes + p.list_bytes + p.jobs_bytes + p.stats_bytes + (size_t)p.slots * kv * p.tile_rows * d.cache.head_dim * 4;
     return p;
 }
 
 template <class Q, class C, int DP>
-int run_heads(const char* what, const Args& a, unsigned groups, void* stream) {
-    static_assert(Shape<Q, C, DP>::kWaves == waves_of(DP), "");
-    return launch(what, chunk_attention<Q, C, DP>, dim3(groups), dim3(Shape<Q, C, DP>::kThreads), a, stream);
+int run_heads(const char* what, const Args& a, const Plan& p, unsigned groups, void* stream) {
+    using Sh = Shape<Q, C, DP>;
+    if constexpr (Sh::kFewWaves != 0)
+        if (p.few) return launch(what, chunk_attention<Q, C, DP, true>, dim3(groups), dim3(Sh::kFewWaves * 64), a, stream);
+    return launch(what, chunk_attention<Q, C, DP, false>, dim3(groups), dim3(Sh::kWaves * 64), a, stream);
 }
 template <class Q, class C>
 int run(const char* what, const Args& a, const Plan& p, void* stream) {
     const int D = a.d.cache.head_dim;
-    const unsigned groups = (unsigned)(p.items * a.d.cache.kv_heads);
+    const unsigned groups = (unsigned)p.groups;
     if (a.list)
         if (int rc = launch(what, list_items, dim3(1), dim3(kListThreads), a, stream)) return rc;
-    const int rc = D <= 64    ? run_heads<Q, C, 64>(what, a, groups, stream)
-                   : D <= 96  ? run_heads<Q, C, 96>(what, a, groups, stream)
-                   : D <= 128 ? run_heads<Q, C, 128>(what, a, groups, stream)
-                   : D <= 192 ? run_heads<Q, C, 192>(what, a, groups, stream)
-                              : run_heads<Q, C, 256>(what, a, groups, stream);
+    const int rc = D <= 64    ? run_heads<Q, C, 64>(what, a, p, groups, stream)
+                   : D <= 96  ? run_heads<Q, C, 96>(what, a, p, groups, stream)
+                   : D <= 128 ? run_heads<Q, C, 128>(what, a, p, groups, stream)
+                   : D <= 192 ? run_heads<Q, C, 192>(what, a, p, groups, stream)
+                              : run_heads<Q, C, 256>(what, a, p, groups, stream);
     if (rc || !p.budget) return rc;
-    return launch(what, join_shares<Q>, dim3(groups * (unsigned)(p.tile_rows / kRows)), dim3(kThreads), a, stream);
+    return launch(what, join_shares<Q>, dim3((unsigned)(p.slots * a.d.cache.kv_heads)), dim3(kThreads), a, stream);
 }
 
 }  // namespace
@@ -890,16 +1249,16 @@ extern "C" int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, cons
         return refuse(what, "null or unaligned argument");
     const Plan p = plan_of(*d);
     // (2^32 threads are refused by the launch, which may be the call's second one)
-    if (p.items * d->cache.kv_heads * (p.tile_rows / kRows) >= 1ll << 23)
-        return refuse(what, "%lld workgroups are too many", (long long)(p.items * d->cache.kv_heads * (p.tile_rows / kRows)));
+    if (p.groups >= 1ll << 23) return refuse(what, "%lld workgroups are too many", (long long)p.groups);
     if (p.bytes && (!rows16(workspace) || workspace_bytes < (int64_t)p.bytes))
         return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", p.bytes, (long long)workspace_bytes);
     char* const w = (char*)workspace;
-    const size_t list = p.info_bytes, stats = list + p.list_bytes, parts = stats + p.stats_bytes;
+    const size_t list = p.info_bytes, jobs = list + p.list_bytes, stats = jobs + p.jobs_bytes, parts = stats + p.stats_bytes;
     const int32_t group = d->heads / d->cache.kv_heads;
     const Args a{*d, query, key_cache, value_cache, table, starts, cached, lengths, out, lse, (int4*)w, p.list_bytes ? (int32_t*)(w + list) : nullptr, (float*)(w + parts),
                  (float2*)(w + stats), d->scale == 0.0f ? kLog2e : std::fabs(d->scale) * kLog2e, d->scale < 0.0f ? (d->type == REEF_TYPE_F32 ? 0x80000000u : 0x80008000u) : 0u,
-                 d->scale == 0.0f, group, p.tile_rows, p.budget, (int32_t)p.items, (int32_t)p.slots, divider((uint32_t)d->cache.block_size), divider((uint32_t)group)};
+                 d->scale == 0.0f, group, p.tile_rows, p.budget, (int32_t)p.items, (int32_t)p.slots, (int32_t*)(w + jobs), (int4*)(w + jobs) + 1,
+                 divider((uint32_t)d->cache.block_size), divider((uint32_t)group)};
     switch (d->type * 4 + d->cache.type) {
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, p, stream);
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F16: return run<float, _Float16>(what, a, p, stream);
