@@ -403,7 +403,7 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
     constexpr int kValues = kTermsC == 3 && DP > 128 ? 1 : 2;                 // buffers of values: there is no room for two of three terms of these
     constexpr bool kEven = kAllPieces % kThreads == 0;
     constexpr int kFewV = Sh::kFewV;
-    constexpr int kKeysNear = 2 * kBuffer, kNear = FEW ? kWaves / 2 * kFewV * 16 * 64 * 4 : kKeysNear + kValues * kBuffer;
+    constexpr int kKeysNear = 2 * kBuffer, kNear = FEW ? kWaves * kFewV * 16 * 64 * 4 : kKeysNear + kValues * kBuffer;
     __shared__ __align__(16) unsigned char near[kNear];
     unsigned char* const k_near = near;
     unsigned char* const v_near = near + kKeysNear;
@@ -734,37 +734,41 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
     };
     if constexpr (FEW) {
         {
-            // Up to 32 rows in all: each wavefront takes every kWaves-th 32 tokens for itself, its operands from memory as they lie there, without LDS.  Lane (token n, half h)
-            // has the 16-byte pieces 2 c + h of its key; lane (n, h) has of each of its tokens the n-th kFewV values, whose e-th ones are row n of the e-th
-            // product: dimension kFewV n + e.
-            constexpr int kKWords = (int)sizeof(C) * 2, kVWords = kFewV * (int)sizeof(C) / 4;
+            // Up to 32 rows in all: each wavefront takes every kWaves-th 32 tokens for itself.  Keys go through a part of LDS of its own, so that their rows are read from
+            // memory whole (32 bytes a row and load, as the products want them, take 2 us more for 256 tokens).  Values come as the products want
+            // them: lane (n, h) has of each of its tokens the n-th kFewV values, whose e-th ones are row n of the e-th product, dimension kFewV n + e.
+            constexpr int kKLoads = kRowPieces / 2, kVWords = kFewV * (int)sizeof(C) / 4;
             constexpr std::integral_constant<int, kFewV> kAcc;
-            uint32_t k[kSteps][kKWords], v[16][kVWords];
-            int64_t mine = -1;               // place of this lane's token
+            using K = Near<DP * (int)sizeof(C) / 2>;
+            static_assert(kWaves * 32 * K::kPitch <= kNear, "");
+            unsigned char* const k_mine = near + wave * 32 * K::kPitch;
+            u32x4 k[kKLoads];
+            uint32_t v[16][kVWords];
             auto entry_at = [&](uint32_t t0) __attribute__((always_inline)) -> int32_t {
                 const uint32_t t = t0 + n;
                 return t < end ? table[divided(t, a.block)] : -1;
             };
             auto find_few = [&](uint32_t t0, int32_t entry, int slot) __attribute__((always_inline)) -> uint32_t {
                 const uint32_t t = t0 + n;
-                mine = paged_row(view, entry, (int32_t)(t - divided(t, a.block) * a.block.by));
-                if (h == 0) offsets[wave][slot][n] = mine < 0 ? 0 : mine;
-                const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(mine >= 0);
-                if (mine < 0) mine = 0;
+                const int64_t at = paged_row(view, entry, (int32_t)(t - divided(t, a.block) * a.block.by));
+                if (h == 0) offsets[wave][slot][n] = at < 0 ? 0 : at;
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                return there;
+                return (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0);
             };
-            auto load_k = [&]() __attribute__((always_inline)) {
+            auto load_k = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
-                for (int c = 0; c < kSteps; ++c) {
-                    const int at = c * 16 + h * 8;
-#pragma unroll
-                    for (int w = 0; w < kKWords; w += 4) {
-                        const u32x4 x = *(const u32x4*)(keys + mine + (at < D ? at : 0) + w * 4 / (int)sizeof(C));
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) k[c][w + i] = x[i];
-                    }
+                for (int i = 0; i < kKLoads; ++i) {
+                    const uint32_t x = i * 64 + lane, row = x / kRowPieces, piece = x - row * kRowPieces;
+                    k[i] = *(const u32x4*)(keys + offsets[wave][slot][row] + (piece * 16 < D * (uint32_t)sizeof(C) ? piece * (16 / (uint32_t)sizeof(C)) : 0));
                 }
+            };
+            auto store_k = [&]() __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < kKLoads; ++i) {
+                    const uint32_t x = i * 64 + lane, row = x / kRowPieces, piece = x - row * kRowPieces;
+                    *(u32x4*)(k_mine + K::at(row, piece)) = piece * 16 < D * (uint32_t)sizeof(C) ? k[i] : u32x4{0, 0, 0, 0};
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             };
             auto load_v = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
@@ -793,36 +797,39 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
             if (t0 < end) {
                 there = find_few(t0, entry, 0);
                 entry = t0 + kStep < end ? entry_at(t0 + kStep) : -1;
-                load_k();
+                load_k(0);
                 load_v(0);
             }
             for (; t0 < end; t0 += kStep) {
                 const bool more = t0 + kStep < end;
                 const uint32_t there_now = there;
+                store_k();
                 if (more) {
                     there = find_few(t0 + kStep, entry, slot ^ 1);
                     entry = t0 + 2 * kStep < end ? entry_at(t0 + 2 * kStep) : -1;
+                    load_k(slot ^ 1);
                 }
                 f32x16 s[1];
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[0][i] = 0.0f;
 #pragma unroll
                 for (int c = 0; c < kSteps; ++c) {
-                    const bool inside = c * 16 + h * 8 < D;
                     if constexpr (kTermsC == 1) {
-                        u32x4 x;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) x[w] = inside ? k[c][w] : 0;
+                        const u32x4 x = *(const u32x4*)(k_mine + (K::at(n, h) ^ c * 32));
 #pragma unroll
                         for (int i = kTermsQ - 1; i >= 0; --i) s[0] = product(x, q[i][c], s[0], E());
                     } else {
                         u32x4 x[3];
 #pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            uint32_t t[3];
-                            terms(inside ? __uint_as_float(k[c][2 * w]) : 0.0f, inside ? __uint_as_float(k[c][2 * w + 1]) : 0.0f, t, E());
+                        for (int y = 0; y < 2; ++y) {
+                            const f32x4 z = *(const f32x4*)(k_mine + (K::at(n, 2 * h + y) ^ c * 64));
 #pragma unroll
-                            for (int i = 0; i < 3; ++i) x[i][w] = t[i];
+                            for (int w = 0; w < 2; ++w) {
+                                uint32_t t[3];
+                                terms(z[2 * w], z[2 * w + 1], t, E());
+#pragma unroll
+                                for (int i = 0; i < 3; ++i) x[i][2 * y + w] = t[i];
+                            }
                         }
 #pragma unroll
                         for (int both = 2; both >= 0; --both)
@@ -830,7 +837,7 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
                             for (int i = both; i >= 0; --i) s[0] = product(x[i], q[both - i][c], s[0], E());
                     }
                 }
-                if (more) load_k();
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 const bool by_all = t0 >= all_lo && t0 + 32 <= all_hi;
                 if (!by_all || there_now != ~0u) hide(s, t0, there_now);
                 refer(largest(s), kAcc);
@@ -901,65 +908,66 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
                         if (!(fabsf((float)values[at + (dim < D ? dim : 0)]) < INFINITY)) o[e][i] = NAN;
                     }
             }
-            // The wavefronts that had tokens, joined in halves; a lane meets the lanes of its place.
+            // The wavefronts that had tokens, joined: neighbouring dimensions of a row next to each other, lane after lane; then a unit of them a thread.
+            constexpr int kUnit = kFewV < 4 ? kFewV : 4, kUnits = kFewV / kUnit * 16;
+            typedef float UnitF __attribute__((ext_vector_type(kUnit)));
+            typedef Q UnitQ __attribute__((ext_vector_type(kUnit)));
             l = other_sum(l);
+            const int waves = min((int)((end - begin + 31) / 32), kWaves);
             float2* const stats = (float2*)offsets;
-            int waves = min((int)((end - begin + 31) / 32), kWaves);
-            while (waves > 1) {
-                const int keep = (waves + 1) / 2;
-                __syncthreads();
-                if (wave >= keep && wave < waves) {
-                    const int at = wave - keep;
-                    stats[at * 64 + lane] = make_float2(R, l);
+            __syncthreads();                 // (the places are read)
+            if (wave < waves) {
+                if (h == 0) stats[wave * 32 + n] = make_float2(R, l);
 #pragma unroll
-                    for (int e = 0; e < kFewV; ++e)
+                for (int i = 0; i < 16; ++i)
 #pragma unroll
-                        for (int i = 0; i < 16; i += 4)
-                            *(f32x4*)(near + (((at * kFewV + e) * 4 + i / 4) * 64 + lane) * 16) = f32x4{o[e][i], o[e][i + 1], o[e][i + 2], o[e][i + 3]};
-                }
-                __syncthreads();
-                if (wave + keep < waves) {
-                    const float2 other = stats[wave * 64 + lane];
-                    const float next = fmaxf(R, other.x), base = next == -INFINITY ? 0.0f : next;
-                    const float f = __builtin_amdgcn_exp2f(R - base), g = __builtin_amdgcn_exp2f(other.x - base);
-                    R = next;
-                    l = l * f + other.y * g;
+                    for (int e = 0; e < kFewV; e += kUnit) {
+                        UnitF x;
 #pragma unroll
-                    for (int e = 0; e < kFewV; ++e)
-#pragma unroll
-                        for (int i = 0; i < 16; i += 4) {
-                            const f32x4 x = *(const f32x4*)(near + (((wave * kFewV + e) * 4 + i / 4) * 64 + lane) * 16);
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) o[e][i + y] = o[e][i + y] * f + x[y] * g;
-                        }
-                }
-                waves = keep;
-            }
-            if (wave) return;
-            const int64_t at = ((int64_t)(it.slot + it.share) * d.cache.kv_heads + kvh) * kTileRows + n;
-            if (it.shares > 1) {
-                if (it.slot + it.share >= a.most_slots) return;           // (starts that do not ascend)
-                if (h == 0) a.stats[at] = make_float2(R == -INFINITY ? -INFINITY : R - kGrow, l);
-            }
-            const float f = l == 0.0f ? 0.0f : 1.0f / l;
-            Q* const to = (Q*)a.out + out_row * d.out_stride + head * d.out_head_stride;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int dim = kFewV * (8 * (i >> 2) + 4 * h + (i & 3));
-                if (dim >= D) continue;
-                if (it.shares > 1) {
-#pragma unroll
-                    for (int e = 0; e < kFewV; e += 2) *(float2*)(a.parts + at * D + dim + e) = make_float2(o[e][i], o[e + 1][i]);
-                } else if (valid) {
-#pragma unroll
-                    for (int e = 0; e < kFewV; e += 2) {
-                        typedef Q Q2 __attribute__((ext_vector_type(2)));
-                        const Q2 x = {(Q)(o[e][i] * f), (Q)(o[e + 1][i] * f)};
-                        *(Q2*)(to + dim + e) = x;
+                        for (int y = 0; y < kUnit; ++y) x[y] = o[e + y][i];
+                        ((UnitF*)near)[(wave * kUnits + i * (kFewV / kUnit) + e / kUnit) * 64 + lane] = x;
                     }
+            }
+            __syncthreads();
+            float top = -INFINITY, sum = 0.0f, weight[kWaves];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w)
+                if (w < waves) top = fmaxf(top, stats[w * 32 + n].x);
+            const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                weight[w] = 0.0f;
+                if (w < waves) {
+                    const float2 x = stats[w * 32 + n];
+                    weight[w] = __builtin_amdgcn_exp2f(x.x - base);
+                    sum += weight[w] * x.y;
                 }
             }
-            if (it.shares == 1 && valid && h == 0 && a.lse) a.lse[out_row * d.heads + head] = l == 0.0f ? -INFINITY : (R + (__log2f(l) - kGrow)) * kLn2;
+            const int32_t slot_of = it.slot + it.share;
+            if (!valid || (it.shares > 1 && slot_of >= a.most_slots)) return;      // (the latter where starts do not ascend)
+            const int64_t at = ((int64_t)slot_of * d.cache.kv_heads + kvh) * kTileRows + n;
+            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+            Q* const to = (Q*)a.out + out_row * d.out_stride + head * d.out_head_stride;
+            for (int u = wave; u < kUnits; u += kWaves) {
+                const int i = u / (kFewV / kUnit), dim = kFewV * (8 * (i >> 2) + 4 * h + (i & 3)) + (u - i * (kFewV / kUnit)) * kUnit;
+                if (dim >= D) continue;
+                UnitF all = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kWaves; ++w)
+                    if (w < waves) all += weight[w] * ((const UnitF*)near)[(w * kUnits + u) * 64 + lane];
+                if (it.shares > 1) {
+                    *(UnitF*)(a.parts + at * D + dim) = all;
+                } else {
+                    UnitQ x;
+#pragma unroll
+                    for (int y = 0; y < kUnit; ++y) x[y] = (Q)(all[y] * f);
+                    *(UnitQ*)(to + dim) = x;
+                }
+            }
+            if (wave == 0 && h == 0) {
+                if (it.shares > 1) a.stats[at] = make_float2(top == -INFINITY ? -INFINITY : top - kGrow, sum);
+                else if (a.lse) a.lse[out_row * d.heads + head] = sum == 0.0f ? -INFINITY : (top + (__log2f(sum) - kGrow)) * kLn2;
+            }
             return;
         }
     }
