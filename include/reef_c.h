@@ -401,7 +401,8 @@ int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, const void* que
  *   entropy [rows]: log S - sum_u exp(logits[u] - m) (logits[u] - m) / S, in natural units
  *   top_tokens, top_scores [rows][top]: the first `top` tokens, the larger first, equal ones by their number, and their scores
  * A NaN counts as -infinity.  Where m is an infinity there are no probabilities: scores (of tokens of the vocabulary) and entropy are NaN; ranks and top_tokens go by
- * the logits all the same.  Exponentials are those of 32 bits, their sums are held in 64.
+ * the logits all the same.  Exponentials are those of 32 bits, and so are sums of up to eight of them; all other sums
+ * are held in 64.
  * logits: [rows][logits_stride] of `type`, aligned to their own size.  top: up to 128 and vocab; top_* may be NULL where it is 0.  vocab: below 2^24. */
 typedef struct {
     int32_t type, rows, vocab, top;

@@ -4,7 +4,6 @@
 namespace {
 using namespace reef_ops;
 
-constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kMaxTop = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -20,74 +19,384 @@ struct Args {
 };
 
 // A NaN counts as -infinity.
-template <class T>
-__device__ inline float value_of(T x) {
-    const float v = (float)x;
-    return v == v ? v : -INFINITY;
+__device__ inline float cleaned(float v) { return v == v ? v : -INFINITY; }
+// Whole numbers that are ordered as values are (-0 as 0), and with a token behind them, the lower first.
+__device__ inline uint32_t order_of(float v) {
+    const uint32_t bits = __float_as_uint(v + 0.0f);
+    return bits >> 31 ? ~bits : bits | 1u << 31;
+}
+__device__ inline float value_of(uint32_t order) { return __uint_as_float(order >> 31 ? order & ~(1u << 31) : ~order); }
+__device__ inline uint64_t key_of(uint32_t order, int32_t token) { return (uint64_t)order << 32 | (uint32_t)~token; }
+
+// v - m, or what has an exponential of 0 all the same where that is below, or is -infinity less itself.
+__device__ inline float less(float v, float m) { return fmaxf(v - m, -1000.0f); }
+
+template <int CONTROL>
+__device__ inline float moved(float x) { return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CONTROL, 0xF, 0xF, true)); }
+// The maximum over the 16 lanes of a row, for all of them.
+__device__ inline float over_row(float x) {
+    x = fmaxf(x, moved<0x128>(x));
+    x = fmaxf(x, moved<0x124>(x));
+    x = fmaxf(x, moved<0x122>(x));
+    return fmaxf(x, moved<0x121>(x));
 }
 
-template <class V, class Join>
-__device__ inline V over_group(V v, V* parts, Join join) {
-    for (int x = 32; x; x >>= 1) v = join(v, (V)__shfl_xor(v, x));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) parts[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = parts[0];
-    for (int w = 1; w < kWaves; ++w) v = join(v, parts[w]);
-    return v;
-}
+constexpr int kLoads = 8;                    // of a wavefront in flight, 1 KiB each: a unit
+constexpr int kGroups = 4096;                // maxima of groups that are held
+constexpr int kHeld = 2048;                  // candidates that are held
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) token_scores(Args a) {
+// A row a workgroup, read once: a lane keeps its 16 bytes of eight units, their maximum and sums relative to the largest so far, and how many of its values come
+// before the given token.  Exponentials are those of 32 bits, off by 2^-23 of themselves and three roundings of the argument; those of 16 bytes are added
+// in 32 bits, three roundings, and everything else in 64.
+//
+// The best tokens: of the maxima of groups of neighbours (16 lanes of a unit, or one where units are few), held near, as many as wanted reach a bound that is
+// found by halving; only groups that reach it are read again.  Their values that reach it are candidates.  Where there are more than are held (values that ascend with their
+// numbers, many alike) the bound is raised by halving again, down to one value, and of the tokens that have it the first ones are taken in order.
+template <class T, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
+    constexpr int kThreads = WAVES * 64, kE = 16 / sizeof(T), kUnit = 64 * kE, kMine = kGroups / kThreads;
+    typedef T Raw __attribute__((ext_vector_type(kE), aligned(sizeof(T))));
     const reef_token_scores_desc& d = a.d;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t row = blockIdx.x;
     const T* x = (const T*)a.logits + row * d.logits_stride;
-    __shared__ float parts[kWaves];
-    __shared__ double sums[kWaves];
-    __shared__ int32_t counts[kWaves];
-    __shared__ uint64_t keys[kWaves];
+    const int32_t units = (d.vocab + kUnit - 1) / kUnit;
+    // a group: 16 lanes of `per` units, or a lane of one unit
+    const bool fine = units <= kGroups / 64;
+    const int32_t per = fine ? 1 : (units + kGroups / 4 - 1) / (kGroups / 4), groups = fine ? units * 64 : (units + per - 1) / per * 4;
+
+    __shared__ uint32_t maxima[kGroups];
+    __shared__ uint64_t held[kHeld];
+    __shared__ double sums[2][WAVES];
+    __shared__ float tops[WAVES];
+    __shared__ int32_t counts[2][WAVES], n_held;
+
     const int32_t t = a.tokens[row];
     const bool given = (uint32_t)t < (uint32_t)d.vocab;
-    const float mine = given ? value_of(x[t]) : 0.0f;
+    const float mine = given ? cleaned((float)x[t]) : INFINITY;
+    if (d.top && (per > 1 || !fine)) {
+        for (int i = tid; i < groups; i += kThreads) maxima[i] = 0;
+        __syncthreads();
+    }
     float m = -INFINITY;
-    int32_t rank = 0;
-    for (int32_t i = threadIdx.x; i < d.vocab; i += kThreads) {
-        const float v = value_of(x[i]);
-        m = fmaxf(m, v);
-        rank += v > mine || (v == mine && i < t);
-    }
-    m = over_group(m, parts, [](float p, float q) { return fmaxf(p, q); });
-    rank = over_group(rank, counts, [](int32_t p, int32_t q) { return p + q; });
     double s = 0.0, near = 0.0;
-    for (int32_t i = threadIdx.x; i < d.vocab; i += kThreads) {
-        const float y = value_of(x[i]) - m, e = __builtin_amdgcn_exp2f(y * kLog2e);
-        s += e;
-        if (e > 0.0f) near += (double)e * y;
+    int32_t rank = 0;
+    // 16 bytes from value i of the row on, -infinity behind its end
+    auto fetch = [&](int32_t i, float (&v)[kE]) __attribute__((always_inline)) {
+        if (i + kE <= d.vocab) {
+            const Raw raw = *(const Raw*)(x + i);
+#pragma unroll
+            for (int e = 0; e < kE; ++e) v[e] = (float)raw[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < kE; ++e) v[e] = i + e < d.vocab ? (float)x[i + e] : -INFINITY;
+        }
+    };
+    for (int32_t u0 = wave * kLoads; u0 < units; u0 += WAVES * kLoads) {
+        float v[kLoads][kE];
+        if ((int64_t)(u0 + kLoads) * kUnit <= d.vocab) {
+            Raw raw[kLoads];
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u) raw[u] = *(const Raw*)(x + (u0 + u) * kUnit + lane * kE);
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u)
+#pragma unroll
+                for (int e = 0; e < kE; ++e) v[u][e] = cleaned((float)raw[u][e]);
+        } else {
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u) {
+                fetch((u0 + u) * kUnit + lane * kE, v[u]);
+#pragma unroll
+                for (int e = 0; e < kE; ++e) v[u][e] = cleaned(v[u][e]);
+            }
+        }
+        float top[kLoads], all = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            top[u] = v[u][0];
+#pragma unroll
+            for (int e = 1; e < kE; ++e) top[u] = fmaxf(top[u], v[u][e]);
+            all = fmaxf(all, top[u]);
+        }
+        // those that come before the given token: at least as large in front of it, larger behind it
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            const int32_t first = (u0 + u) * kUnit;
+            if (t >= first + kUnit) {
+#pragma unroll
+                for (int e = 0; e < kE; ++e) rank += v[u][e] >= mine ? 1 : 0;
+            } else if (t < first) {
+#pragma unroll
+                for (int e = 0; e < kE; ++e) rank += v[u][e] > mine ? 1 : 0;
+            } else {
+#pragma unroll
+                for (int e = 0; e < kE; ++e) rank += first + lane * kE + e < t ? v[u][e] >= mine : v[u][e] > mine;
+            }
+        }
+        if (all > m) {
+            const float y = less(m, all), f = __builtin_amdgcn_exp2f(y * kLog2e);
+            near = (near + s * (double)y) * f;
+            s *= f;
+            m = all;
+        }
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            float e1[kE], e2[kE];
+#pragma unroll
+            for (int e = 0; e < kE; ++e) {
+                const float y = less(v[u][e], m);
+                e1[e] = __builtin_amdgcn_exp2f(y * kLog2e);
+                e2[e] = e1[e] * y;
+            }
+#pragma unroll
+            for (int step = 1; step < kE; step <<= 1)
+#pragma unroll
+                for (int e = 0; e < kE; e += 2 * step) {
+                    e1[e] += e1[e + step];
+                    e2[e] += e2[e + step];
+                }
+            s += (double)e1[0];
+            near += (double)e2[0];
+        }
+        if (d.top) {
+#pragma unroll
+            for (int u = 0; u < kLoads; ++u) {
+                if (u0 + u >= units) continue;
+                if (fine) {
+                    maxima[(u0 + u) * 64 + lane] = order_of(top[u]);
+                } else {
+                    const uint32_t o = order_of(over_row(top[u]));
+                    if ((lane & 15) == 0) {
+                        if (per == 1) maxima[(u0 + u) * 4 + lane / 16] = o;
+                        else atomicMax(&maxima[(u0 + u) / per * 4 + lane / 16], o);
+                    }
+                }
+            }
+        }
     }
-    s = over_group(s, sums, [](double p, double q) { return p + q; });
-    near = over_group(near, sums, [](double p, double q) { return p + q; });
-    const bool none = !(m > -INFINITY && m < INFINITY);
-    const double log_s = none ? NAN : log(s);
-    if (threadIdx.x == 0) {
-        a.scores[row] = given ? (float)((double)mine - (double)m - log_s) : -INFINITY;
+    // the row's: first of the wavefront's lanes, then of the wavefronts
+    float all = m;
+    for (int i = 32; i; i >>= 1) {
+        all = fmaxf(all, __shfl_xor(all, i));
+        rank += __shfl_xor(rank, i);
+    }
+    if (lane == 0) {
+        tops[wave] = all;
+        counts[0][wave] = rank;
+    }
+    if (tid == 0) n_held = 0;
+    __syncthreads();
+    rank = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        all = fmaxf(all, tops[w]);
+        rank += counts[0][w];
+    }
+    const bool none = !(all > -INFINITY && all < INFINITY);
+    if (m > -INFINITY && !none) {
+        const float y = less(m, all);
+        const double f = (double)__builtin_amdgcn_exp2f(y * kLog2e);
+        near = (near + s * (double)y) * f;
+        s *= f;
+    } else {
+        s = near = 0.0;
+    }
+    for (int i = 32; i; i >>= 1) {
+        s += __shfl_xor(s, i);
+        near += __shfl_xor(near, i);
+    }
+    if (lane == 0) {
+        sums[0][wave] = s;
+        sums[1][wave] = near;
+    }
+    __syncthreads();
+    s = near = 0.0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) {
+        s += sums[0][w];
+        near += sums[1][w];
+    }
+    const double log_s = none ? (double)NAN : log(s);
+    auto score = [&](float v) { return (float)((double)v - (double)all - log_s); };
+    if (tid == 0) {
+        a.scores[row] = given ? score(mine) : -INFINITY;
         a.ranks[row] = given ? rank : -1;
         a.entropy[row] = (float)(log_s - near / s);
     }
-    uint64_t last = ~0ull;                   // an order of values, the larger first, then of tokens
-    for (int k = 0; k < d.top; ++k) {
-        uint64_t best = 0;
-        for (int32_t i = threadIdx.x; i < d.vocab; i += kThreads) {
-            const uint32_t bits = __float_as_uint(value_of(x[i]) + 0.0f);
-            const uint64_t key = (uint64_t)(bits >> 31 ? ~bits : bits | 1u << 31) << 32 | (uint32_t)~i;
-            if (key < last && key > best) best = key;
+    if (!d.top) return;
+
+    // A bound that `top` groups or more reach, not many more.  (0 is below all.)
+    int turn = 0;
+    auto over_waves = [&](int32_t n) __attribute__((always_inline)) {
+        if (lane == 0) counts[turn][wave] = n;
+        __syncthreads();
+        n = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) n += counts[turn][w];
+        turn ^= 1;
+        return n;
+    };
+    uint32_t near_me[kMine];
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) near_me[k] = k * kThreads + tid < groups ? maxima[k * kThreads + tid] : 0;
+    turn = 1;
+    auto groups_from = [&](uint32_t bound) __attribute__((always_inline)) {
+        int32_t n = 0;
+#pragma unroll
+        for (int k = 0; k < kMine; ++k)
+            if (k * kThreads < groups) n += (int32_t)__popcll(__builtin_amdgcn_ballot_w64(near_me[k] >= bound));
+        return over_waves(n);
+    };
+    const uint32_t best = order_of(all);
+    const int32_t enough = d.top + d.top / 2 + 8;
+    uint32_t low = 0, high = best + 1;       // groups_from(low) >= top (or all there are), groups_from(high) < top
+    if (groups >= d.top) {
+        // down from the best by steps that double, then halving
+        for (uint32_t step = 1u << 18; low == 0 && step; step <<= 1) {
+            const uint32_t bound = best > step ? best - step : 1;
+            const int32_t n = groups_from(bound);
+            if (n >= d.top) {
+                low = bound;
+                if (n <= enough) break;
+            } else {
+                high = bound;
+            }
+            if (bound == 1) break;
         }
-        last = over_group(best, keys, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
-        if (threadIdx.x == 0) {
-            const int32_t i = (int32_t)~(uint32_t)last;
-            a.top_tokens[row * d.top + k] = i;
-            a.top_scores[row * d.top + k] = (float)((double)value_of(x[i]) - (double)m - log_s);
+        while (high - low > 1) {
+            const uint32_t bound = low + (high - low) / 2;
+            const int32_t n = groups_from(bound);
+            if (n >= d.top) {
+                low = bound;
+                if (n <= enough) break;
+            } else {
+                high = bound;
+            }
         }
     }
+    // The values of those groups from a bound on: all are counted, some are held.  16 lanes a group, or one.
+    const uint32_t groups_bound = low;
+    auto values_from = [&](uint32_t bound) __attribute__((always_inline)) {
+        __syncthreads();
+        if (tid == 0) n_held = 0;
+        __syncthreads();
+        auto offer = [&](int32_t i) __attribute__((always_inline)) {
+            float v[kE];
+            fetch(i, v);
+#pragma unroll
+            for (int e = 0; e < kE; ++e) {
+                const uint32_t o = order_of(cleaned(v[e]));
+                if (o >= bound && i + e < d.vocab) {
+                    const int32_t at = atomicAdd(&n_held, 1);
+                    if (at < kHeld) held[at] = key_of(o, i + e);
+                }
+            }
+        };
+        if (fine) {
+            for (int g = tid; g < groups; g += kThreads)
+                if (maxima[g] >= groups_bound) offer(g * kE);
+        } else {
+            // (64 groups a wavefront looked at at once, then four of them at a time)
+            for (int g0 = wave * 64; g0 < groups; g0 += WAVES * 64) {
+                uint64_t who = __builtin_amdgcn_ballot_w64(g0 + lane < groups && maxima[min(g0 + lane, groups - 1)] >= groups_bound);
+                while (who) {
+                    int32_t g = -1;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        if (lane / 16 == k && who) g = g0 + __builtin_ctzll(who);
+                        who &= who - 1;
+                    }
+                    if (g < 0) continue;
+                    for (int32_t u = g / 4 * per; u < min(units, (g / 4 + 1) * per); ++u) {
+                        const int32_t i = u * kUnit + ((g & 3) * 16 + (lane & 15)) * kE;
+                        if (i < d.vocab) offer(i);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        return n_held;
+    };
+    int32_t n = values_from(low);
+    int32_t ties = 0;
+    if (n > kHeld) {
+        high = best + 1;                     // values_from(low) > kHeld, values_from(high) < top
+        while (high - low > 1) {
+            const uint32_t bound = low + (high - low) / 2;
+            n = values_from(bound);
+            if (n < d.top) high = bound;
+            else low = bound;
+            if (n >= d.top && n <= kHeld) break;
+        }
+        if (n > kHeld || n < d.top) {
+            n = high > best ? 0 : values_from(high);           // fewer than top
+            ties = d.top - n;
+        }
+    }
+    if (ties) {
+        // of the tokens whose value is `low` the first ones, in order
+        __syncthreads();
+        for (int32_t i0 = 0; ties && i0 < d.vocab; i0 += kThreads) {
+            const int32_t i = i0 + tid;
+            const bool is = i < d.vocab && order_of(cleaned((float)x[i])) == low;
+            const uint64_t who = __builtin_amdgcn_ballot_w64(is);
+            if (lane == 0) counts[turn][wave] = (int32_t)__popcll(who);
+            __syncthreads();
+            int32_t before = (int32_t)__popcll(who & ((1ull << lane) - 1)), found = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                if (w < wave) before += counts[turn][w];
+                found += counts[turn][w];
+            }
+            turn ^= 1;
+            if (is && before < ties) held[n + before] = key_of(low, i);
+            n += min(found, ties);
+            ties -= min(found, ties);
+        }
+        __syncthreads();
+    }
+    auto put = [&](int32_t place, uint64_t key) {
+        a.top_tokens[row * d.top + place] = (int32_t)~(uint32_t)key;
+        a.top_scores[row * d.top + place] = score(value_of((uint32_t)(key >> 32)));
+    };
+    if (n <= 512) {                          // ranked, eight lanes a candidate
+        for (int i0 = 0; i0 < n; i0 += kThreads / 8) {
+            const int i = i0 + (tid >> 3);
+            const uint64_t key = held[min(i, n - 1)];
+            int32_t place = 0;
+#pragma unroll 4
+            for (int j = tid & 7; j < n; j += 8) place += held[j] > key;
+            place += __shfl_xor(place, 1);
+            place += __shfl_xor(place, 2);
+            place += __shfl_xor(place, 4);
+            if (i < n && (tid & 7) == 0 && place < d.top) put(place, key);
+        }
+        return;
+    }
+    int size = 1024;                         // sorted
+    while (size < n) size <<= 1;
+    for (int i = n + tid; i < size; i += kThreads) held[i] = 0;
+    __syncthreads();
+    for (int run = 2; run <= size; run <<= 1)
+        for (int step = run >> 1; step; step >>= 1) {
+            for (int k = tid; k < size / 2; k += kThreads) {
+                const int i = (k / step) * 2 * step + k % step, j = i + step;
+                const uint64_t p = held[i], q = held[j];
+                if ((q > p) == ((i & run) == 0)) {
+                    held[i] = q;
+                    held[j] = p;
+                }
+            }
+            __syncthreads();
+        }
+    for (int i = tid; i < d.top; i += kThreads) put(i, held[i]);
+}
+
+// Sixteen wavefronts a row where rows are few, four where they fill the device.
+template <class T>
+int run(const char* what, const Args& a, void* stream) {
+    if (a.d.rows <= 256) return launch(what, token_scores<T, 16>, dim3((unsigned)a.d.rows), dim3(16 * 64), a, stream);
+    return launch(what, token_scores<T, 4>, dim3((unsigned)a.d.rows), dim3(4 * 64), a, stream);
 }
 
 int check(const char* what, const reef_token_scores_desc* d) {
@@ -122,10 +431,9 @@ extern "C" int reef_ops_token_scores(const reef_token_scores_desc* d, const void
     const Span in[] = {{logits, ((n - 1) * d->logits_stride + d->vocab) * type_bytes(d->type)}, {tokens, 4 * n}};
     if (overlap(out, in)) return refuse(what, "an output overlaps an input");
     const Args a{*d, logits, tokens, scores, ranks, entropy, top_tokens, top_scores};
-    const dim3 grid((unsigned)n), block(kThreads);
     switch (d->type) {
-        case REEF_TYPE_F32: return launch(what, token_scores<float>, grid, block, a, stream);
-        case REEF_TYPE_F16: return launch(what, token_scores<_Float16>, grid, block, a, stream);
-        default: return launch(what, token_scores<__bf16>, grid, block, a, stream);
+        case REEF_TYPE_F32: return run<float>(what, a, stream);
+        case REEF_TYPE_F16: return run<_Float16>(what, a, stream);
+        default: return run<__bf16>(what, a, stream);
     }
 }
