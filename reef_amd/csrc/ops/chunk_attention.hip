@@ -1109,7 +1109,7 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
     if (h == 0 && a.lse) a.lse[out_row * d.heads + head] = l == 0.0f ? -INFINITY : (R + (__log2f(l) - kGrow)) * kLn2;
 }
 
-constexpr int kThreads = 256;                // of the join
+constexpr int kThreads = 1024;               // of the join
 // The shares of a tile, one cache head: a workgroup for each of its slots, which take the tile's rows among them, a quad of a row a thread, share after share.
 template <class Q>
 __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
