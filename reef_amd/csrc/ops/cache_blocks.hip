@@ -28,7 +28,6 @@ struct Use {
     int32_t *source, *target;        // of a compaction: [moves]
 };
 constexpr int32_t kSegment = 4096;
-constexpr int kEach = kSegment / kThreads;   // blocks of a segment a lane
 
 __global__ void __launch_bounds__(kThreads) clear(Use a) {
     const int64_t n = (int64_t)a.t.blocks + a.n_segments + 1;
@@ -76,16 +75,26 @@ __device__ inline int32_t over_waves(int32_t mine, int32_t* counts, int32_t* all
     return at;
 }
 
-__global__ void __launch_bounds__(kThreads) count_segments(Use a) {
-    __shared__ int32_t counts[kWaves];
-    const int64_t first = (int64_t)blockIdx.x * kSegment;
-    int32_t mine = 0, all;
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        const int64_t b = first + k * kThreads + threadIdx.x;
-        mine += (int32_t)__popcll(__builtin_amdgcn_ballot_w64(b < a.t.blocks && a.uses[b] != 0));
+// A segment a workgroup, four blocks a thread: whether each is in use.
+constexpr int kWide = kSegment / 4, kWideWaves = kWide / 64;
+__device__ inline uint32_t in_use(const Use& a, int64_t b) {
+    uint32_t who = 0;
+    if (b + 4 <= a.t.blocks && aligned(a.uses, 16)) {
+        const int4 n = *(const int4*)(a.uses + b);
+        who = (n.x != 0) | (n.y != 0) << 1 | (n.z != 0) << 2 | (n.w != 0) << 3;
+    } else {
+        for (int k = 0; k < 4; ++k) who |= b + k < a.t.blocks && a.uses[b + k] != 0 ? 1u << k : 0;
     }
-    over_waves(mine, counts, &all);
+    return who;
+}
+__device__ inline int32_t sum_of(int32_t v) {
+    for (int x = 32; x; x >>= 1) v += __shfl_xor(v, x);
+    return v;
+}
+__global__ void __launch_bounds__(kWide) count_segments(Use a) {
+    __shared__ int32_t counts[kWideWaves];
+    int32_t all;
+    over_waves(sum_of(__popc(in_use(a, (int64_t)blockIdx.x * kSegment + threadIdx.x * 4))), counts, &all);
     if (threadIdx.x == 0) a.segments[blockIdx.x] = all;
 }
 
@@ -118,42 +127,35 @@ __device__ inline void place_counts(const Use& a, int32_t used, int32_t outside)
     }
 }
 
-// A segment a workgroup, 1024 blocks a wavefront, 64 at a time.
 template <bool kSweep>
-__global__ void __launch_bounds__(kThreads) place_blocks(Use a) {
-    __shared__ int32_t counts[kWaves];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ void __launch_bounds__(kWide) place_blocks(Use a) {
+    __shared__ int32_t counts[kWideWaves];
+    const int lane = threadIdx.x & 63;
+    const int64_t b = (int64_t)blockIdx.x * kSegment + threadIdx.x * 4;
+    const uint32_t who = in_use(a, b);
     int32_t before = 0, used = 0;            // blocks in use of the segments in front, and of all
-    for (int32_t s = threadIdx.x; s < a.n_segments; s += kThreads) {
+    for (int32_t s = threadIdx.x; s < a.n_segments; s += kWide) {
         const int32_t n = a.segments[s];
         used += n;
         if (s < (int32_t)blockIdx.x) before += n;
     }
-    for (int x = 32; x; x >>= 1) {
-        used += __shfl_xor(used, x);
-        before += __shfl_xor(before, x);
-    }
     int32_t sum;
-    over_waves(used, counts, &sum);
+    over_waves(sum_of(used), counts, &sum);
     used = sum;
-    over_waves(before, counts, &sum);
+    over_waves(sum_of(before), counts, &sum);
     before = sum;
     if (blockIdx.x == 0 && threadIdx.x == 0) place_counts<kSweep>(a, used, a.segments[a.n_segments]);
-    const int64_t first = (int64_t)blockIdx.x * kSegment + wave * (kEach * 64);
-    uint64_t who[kEach];
-    int32_t mine = 0;
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        const int64_t b = first + k * 64 + lane;
-        who[k] = __builtin_amdgcn_ballot_w64(b < a.t.blocks && a.uses[b] != 0);
-        mine += (int32_t)__popcll(who[k]);
+    const int32_t mine = __popc(who);
+    int32_t at = mine;
+    for (int x = 1; x < 64; x <<= 1) {
+        const int32_t o = __shfl_up(at, x);
+        if (lane >= x) at += o;
     }
-    before += over_waves(mine, counts, &sum);
+    before += over_waves(__shfl(at, 63), counts, &sum) + at - mine;
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        const int64_t b = first + k * 64 + lane;
-        if (b < a.t.blocks) place_block<kSweep>(a, (int32_t)b, who[k] >> lane & 1, before + (int32_t)__popcll(who[k] & ((1ull << lane) - 1)), used);
-        before += (int32_t)__popcll(who[k]);
+    for (int k = 0; k < 4; ++k) {
+        if (b + k < a.t.blocks) place_block<kSweep>(a, (int32_t)(b + k), who >> k & 1, before, used);
+        before += who >> k & 1;
     }
 }
 
@@ -213,8 +215,8 @@ int place(const char* what, const Use& a, void* stream) {
     const unsigned clears = (unsigned)std::min<int64_t>(((int64_t)a.t.blocks + a.n_segments + kThreads) / kThreads, 2048);
     if (int rc = launch(what, clear, dim3(clears), dim3(kThreads), a, stream)) return rc;
     if (int rc = launch(what, name_blocks<kSweep>, rows_grid(a.t), dim3(kThreads), a, stream)) return rc;
-    if (int rc = launch(what, count_segments, dim3((unsigned)a.n_segments), dim3(kThreads), a, stream)) return rc;
-    return launch(what, place_blocks<kSweep>, dim3((unsigned)a.n_segments), dim3(kThreads), a, stream);
+    if (int rc = launch(what, count_segments, dim3((unsigned)a.n_segments), dim3(kWide), a, stream)) return rc;
+    return launch(what, place_blocks<kSweep>, dim3((unsigned)a.n_segments), dim3(kWide), a, stream);
 }
 
 int check_table(const char* what, int32_t rows, int32_t blocks, int32_t block_size, int32_t max_blocks, int32_t stride) {

@@ -30,7 +30,7 @@ int launch(const char* what, void (*kernel)(Args), dim3 grid, dim3 block, Args a
 }
 
 inline int type_bytes(int type) { return type == REEF_TYPE_F32 ? 4 : type == REEF_TYPE_F16 || type == REEF_TYPE_BF16 ? 2 : 0; }
-inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+__host__ __device__ inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 // Two int32 arrays and the like: a pointer that is there and aligned.
 inline bool words(const void* p) { return p && aligned(p, 4); }
 inline bool rows16(const void* p) { return p && aligned(p, 16); }
