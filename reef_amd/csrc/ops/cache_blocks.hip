@@ -404,8 +404,9 @@ int check_compact(const char* what, const reef_cache_compact_desc* d) {
 Table table_of(const reef_cache_compact_desc& d, const int32_t* table, const int32_t* lengths) {
     return {d.rows, d.cache.blocks, d.cache.block_size, d.max_blocks, d.table_stride, table, lengths};
 }
-// Places of moves, both ends; numbers of blocks; sums of segments.
-int64_t compact_bytes(const reef_cache_compact_desc& d) { return 4 * (2 * ((int64_t)d.cache.blocks / 2 + 1) + d.cache.blocks + segments_of(d.cache.blocks) + 1); }
+// Places of moves, both ends; numbers of blocks, on 16 bytes; sums of segments.
+int64_t most_moves(int32_t blocks) { return ((int64_t)blocks / 2 + 2) / 2 * 2; }
+int64_t compact_bytes(const reef_cache_compact_desc& d) { return 4 * (2 * most_moves(d.cache.blocks) + d.cache.blocks + segments_of(d.cache.blocks) + 1); }
 
 }  // namespace
 
@@ -465,7 +466,7 @@ extern "C" int reef_ops_cache_compact(const reef_cache_compact_desc* d, const in
     const Span out[] = {{table_out, table_bytes(d->rows, d->max_blocks, d->out_stride)}, {counts, 8}, {workspace, need}};
     const Span in[] = {{table, table_bytes(d->rows, d->max_blocks, d->table_stride)}, {lengths, 4ll * d->rows}};
     if (overlap(out, in)) return refuse(what, "an output overlaps an input");
-    const int64_t half = (int64_t)d->cache.blocks / 2 + 1;
+    const int64_t half = most_moves(d->cache.blocks);
     int32_t* const w = (int32_t*)workspace;
     const Use use{table_of(*d, table, lengths), w + 2 * half, w + 2 * half + d->cache.blocks, segments_of(d->cache.blocks), nullptr, counts, w, w + half};
     if (int rc = place<false>(what, use, stream)) return rc;

@@ -733,243 +733,241 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
             }
     };
     if constexpr (FEW) {
-        {
-            // Up to 32 rows in all: each wavefront takes every kWaves-th 32 tokens for itself.  Keys go through a part of LDS of its own, so that their rows are read from
-            // memory whole (32 bytes a row and load, as the products want them, take 2 us more for 256 tokens).  Values come as the products want
-            // them: lane (n, h) has of each of its tokens the n-th kFewV values, whose e-th ones are row n of the e-th product, dimension kFewV n + e.
-            constexpr int kKLoads = kRowPieces / 2, kVWords = kFewV * (int)sizeof(C) / 4;
-            constexpr std::integral_constant<int, kFewV> kAcc;
-            using K = Near<DP * (int)sizeof(C) / 2>;
-            static_assert(kWaves * 32 * K::kPitch <= kNear, "");
-            unsigned char* const k_mine = near + wave * 32 * K::kPitch;
-            u32x4 k[kKLoads];
-            uint32_t v[16][kVWords];
-            auto entry_at = [&](uint32_t t0) __attribute__((always_inline)) -> int32_t {
-                const uint32_t t = t0 + n;
-                return t < end ? table[divided(t, a.block)] : -1;
-            };
-            auto find_few = [&](uint32_t t0, int32_t entry, int slot) __attribute__((always_inline)) -> uint32_t {
-                const uint32_t t = t0 + n;
-                const int64_t at = paged_row(view, entry, (int32_t)(t - divided(t, a.block) * a.block.by));
-                if (h == 0) offsets[wave][slot][n] = at < 0 ? 0 : at;
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                return (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0);
-            };
-            auto load_k = [&](int slot) __attribute__((always_inline)) {
+        // Up to 32 rows in all: each wavefront takes every kWaves-th 32 tokens for itself.  Keys go through a part of LDS of its own, so that their rows are read from
+        // memory whole (32 bytes a row and load, as the products want them, take 2 us more for 256 tokens).  Values come as the products want
+        // them: lane (n, h) has of each of its tokens the n-th kFewV values, whose e-th ones are row n of the e-th product, dimension kFewV n + e.
+        constexpr int kKLoads = kRowPieces / 2, kVWords = kFewV * (int)sizeof(C) / 4;
+        constexpr std::integral_constant<int, kFewV> kAcc;
+        using K = Near<DP * (int)sizeof(C) / 2>;
+        static_assert(kWaves * 32 * K::kPitch <= kNear, "");
+        unsigned char* const k_mine = near + wave * 32 * K::kPitch;
+        u32x4 k[kKLoads];
+        uint32_t v[16][kVWords];
+        auto entry_at = [&](uint32_t t0) __attribute__((always_inline)) -> int32_t {
+            const uint32_t t = t0 + n;
+            return t < end ? table[divided(t, a.block)] : -1;
+        };
+        auto find_few = [&](uint32_t t0, int32_t entry, int slot) __attribute__((always_inline)) -> uint32_t {
+            const uint32_t t = t0 + n;
+            const int64_t at = paged_row(view, entry, (int32_t)(t - divided(t, a.block) * a.block.by));
+            if (h == 0) offsets[wave][slot][n] = at < 0 ? 0 : at;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            return (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0);
+        };
+        auto load_k = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < kKLoads; ++i) {
-                    const uint32_t x = i * 64 + lane, row = x / kRowPieces, piece = x - row * kRowPieces;
-                    k[i] = *(const u32x4*)(keys + offsets[wave][slot][row] + (piece * 16 < D * (uint32_t)sizeof(C) ? piece * (16 / (uint32_t)sizeof(C)) : 0));
-                }
-            };
-            auto store_k = [&]() __attribute__((always_inline)) {
+            for (int i = 0; i < kKLoads; ++i) {
+                const uint32_t x = i * 64 + lane, row = x / kRowPieces, piece = x - row * kRowPieces;
+                k[i] = *(const u32x4*)(keys + offsets[wave][slot][row] + (piece * 16 < D * (uint32_t)sizeof(C) ? piece * (16 / (uint32_t)sizeof(C)) : 0));
+            }
+        };
+        auto store_k = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < kKLoads; ++i) {
-                    const uint32_t x = i * 64 + lane, row = x / kRowPieces, piece = x - row * kRowPieces;
-                    *(u32x4*)(k_mine + K::at(row, piece)) = piece * 16 < D * (uint32_t)sizeof(C) ? k[i] : u32x4{0, 0, 0, 0};
-                }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            };
-            auto load_v = [&](int slot) __attribute__((always_inline)) {
+            for (int i = 0; i < kKLoads; ++i) {
+                const uint32_t x = i * 64 + lane, row = x / kRowPieces, piece = x - row * kRowPieces;
+                *(u32x4*)(k_mine + K::at(row, piece)) = piece * 16 < D * (uint32_t)sizeof(C) ? k[i] : u32x4{0, 0, 0, 0};
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        };
+        auto load_v = [&](int slot) __attribute__((always_inline)) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const C* const from = values + offsets[wave][slot][16 * (j >> 3) + 8 * (j >> 2 & 1) + 4 * h + (j & 3)] + (kFewV * n < D ? kFewV * n : 0);
-                    if constexpr (kVWords == 1) {
-                        v[j][0] = *(const uint32_t*)from;
-                    } else if constexpr (kVWords == 2) {
-                        const u32x2 x = *(const u32x2*)from;
-                        v[j][0] = x[0];
-                        v[j][1] = x[1];
-                    } else {
+            for (int j = 0; j < 16; ++j) {
+                const C* const from = values + offsets[wave][slot][16 * (j >> 3) + 8 * (j >> 2 & 1) + 4 * h + (j & 3)] + (kFewV * n < D ? kFewV * n : 0);
+                if constexpr (kVWords == 1) {
+                    v[j][0] = *(const uint32_t*)from;
+                } else if constexpr (kVWords == 2) {
+                    const u32x2 x = *(const u32x2*)from;
+                    v[j][0] = x[0];
+                    v[j][1] = x[1];
+                } else {
 #pragma unroll
-                        for (int w = 0; w < kVWords; w += 4) {
-                            const u32x4 x = *(const u32x4*)(from + w * 4 / (int)sizeof(C));
+                    for (int w = 0; w < kVWords; w += 4) {
+                        const u32x4 x = *(const u32x4*)(from + w * 4 / (int)sizeof(C));
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) v[j][w + i] = x[i];
-                        }
+                        for (int i = 0; i < 4; ++i) v[j][w + i] = x[i];
                     }
                 }
-            };
-            constexpr uint32_t kStep = kWaves * 32;
-            uint32_t t0 = begin + wave * 32, odd_from = ~0u, odd_to = 0, there = 0;
-            int slot = 0;
-            int32_t entry = t0 < end ? entry_at(t0) : -1;
-            if (t0 < end) {
-                there = find_few(t0, entry, 0);
-                entry = t0 + kStep < end ? entry_at(t0 + kStep) : -1;
-                load_k(0);
-                load_v(0);
             }
-            for (; t0 < end; t0 += kStep) {
-                const bool more = t0 + kStep < end;
-                const uint32_t there_now = there;
-                store_k();
-                if (more) {
-                    there = find_few(t0 + kStep, entry, slot ^ 1);
-                    entry = t0 + 2 * kStep < end ? entry_at(t0 + 2 * kStep) : -1;
-                    load_k(slot ^ 1);
-                }
-                f32x16 s[1];
+        };
+        constexpr uint32_t kStep = kWaves * 32;
+        uint32_t t0 = begin + wave * 32, odd_from = ~0u, odd_to = 0, there = 0;
+        int slot = 0;
+        int32_t entry = t0 < end ? entry_at(t0) : -1;
+        if (t0 < end) {
+            there = find_few(t0, entry, 0);
+            entry = t0 + kStep < end ? entry_at(t0 + kStep) : -1;
+            load_k(0);
+            load_v(0);
+        }
+        for (; t0 < end; t0 += kStep) {
+            const bool more = t0 + kStep < end;
+            const uint32_t there_now = there;
+            store_k();
+            if (more) {
+                there = find_few(t0 + kStep, entry, slot ^ 1);
+                entry = t0 + 2 * kStep < end ? entry_at(t0 + 2 * kStep) : -1;
+                load_k(slot ^ 1);
+            }
+            f32x16 s[1];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[0][i] = 0.0f;
+            for (int i = 0; i < 16; ++i) s[0][i] = 0.0f;
 #pragma unroll
-                for (int c = 0; c < kSteps; ++c) {
-                    if constexpr (kTermsC == 1) {
-                        const u32x4 x = *(const u32x4*)(k_mine + (K::at(n, h) ^ c * 32));
+            for (int c = 0; c < kSteps; ++c) {
+                if constexpr (kTermsC == 1) {
+                    const u32x4 x = *(const u32x4*)(k_mine + (K::at(n, h) ^ c * 32));
 #pragma unroll
-                        for (int i = kTermsQ - 1; i >= 0; --i) s[0] = product(x, q[i][c], s[0], E());
-                    } else {
-                        u32x4 x[3];
+                    for (int i = kTermsQ - 1; i >= 0; --i) s[0] = product(x, q[i][c], s[0], E());
+                } else {
+                    u32x4 x[3];
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const f32x4 z = *(const f32x4*)(k_mine + (K::at(n, 2 * h + y) ^ c * 64));
+                    for (int y = 0; y < 2; ++y) {
+                        const f32x4 z = *(const f32x4*)(k_mine + (K::at(n, 2 * h + y) ^ c * 64));
 #pragma unroll
-                            for (int w = 0; w < 2; ++w) {
-                                uint32_t t[3];
-                                terms(z[2 * w], z[2 * w + 1], t, E());
+                        for (int w = 0; w < 2; ++w) {
+                            uint32_t t[3];
+                            terms(z[2 * w], z[2 * w + 1], t, E());
 #pragma unroll
-                                for (int i = 0; i < 3; ++i) x[i][2 * y + w] = t[i];
-                            }
+                            for (int i = 0; i < 3; ++i) x[i][2 * y + w] = t[i];
                         }
+                    }
+#pragma unroll
+                    for (int both = 2; both >= 0; --both)
+#pragma unroll
+                        for (int i = both; i >= 0; --i) s[0] = product(x[i], q[both - i][c], s[0], E());
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            const bool by_all = t0 >= all_lo && t0 + 32 <= all_hi;
+            if (!by_all || there_now != ~0u) hide(s, t0, there_now);
+            refer(largest(s), kAcc);
+            approach(s);
+            weigh(s);
+            if (there_now != ~0u) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (!(there_now >> (4 * h) >> (16 * (j >> 3) + 8 * (j >> 2 & 1) + (j & 3)) & 1)) {
+#pragma unroll
+                        for (int w = 0; w < kVWords; ++w) v[j][w] = 0;
+                    }
+            }
+            if (!by_all) {               // (as in store())
+                bool found = false;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+#pragma unroll
+                    for (int w = 0; w < kVWords; ++w) {
+                        const uint32_t keep = keep_of(v[j][w], C());
+                        found |= keep != ~0u;
+                        v[j][w] &= keep;
+                    }
+                if (__builtin_amdgcn_ballot_w64(found)) {
+                    odd_from = min(odd_from, t0);
+                    odd_to = t0 + 32;
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < kFewV; ++e) {
+                    u32x4 x[kTermsC];
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int j = c * 8 + 2 * w;
+                        if constexpr (kTermsC == 1) {
+                            x[0][w] = __builtin_amdgcn_perm(v[j + 1][e / 2], v[j][e / 2], e & 1 ? 0x07060302 : 0x05040100);
+                        } else {
+                            uint32_t t[3];
+                            terms(__uint_as_float(v[j][e]), __uint_as_float(v[j + 1][e]), t, E());
+#pragma unroll
+                            for (int i = 0; i < 3; ++i) x[i][w] = t[i];
+                        }
+                    }
+                    if constexpr (kTermsC == 1) {
+#pragma unroll
+                        for (int i = kTermsQ - 1; i >= 0; --i) o[e] = product(x[0], p[c][i], o[e], E());
+                    } else {
 #pragma unroll
                         for (int both = 2; both >= 0; --both)
 #pragma unroll
-                            for (int i = both; i >= 0; --i) s[0] = product(x[i], q[both - i][c], s[0], E());
+                            for (int i = both; i >= 0; --i) o[e] = product(x[i], p[c][both - i], o[e], E());
                     }
                 }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                const bool by_all = t0 >= all_lo && t0 + 32 <= all_hi;
-                if (!by_all || there_now != ~0u) hide(s, t0, there_now);
-                refer(largest(s), kAcc);
-                approach(s);
-                weigh(s);
-                if (there_now != ~0u) {
+            slot ^= 1;
+            if (more) load_v(slot);
+        }
+        for (uint32_t t = odd_from; t < min(end, odd_to); ++t) {
+            const uint32_t page = divided(t, a.block);
+            const int64_t at = paged_row(view, table[page], (int32_t)(t - page * a.block.by));
+            if (at < 0 || !(t >= lo && t < hi)) continue;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (!(there_now >> (4 * h) >> (16 * (j >> 3) + 8 * (j >> 2 & 1) + (j & 3)) & 1)) {
+            for (int i = 0; i < 16; ++i)
 #pragma unroll
-                            for (int w = 0; w < kVWords; ++w) v[j][w] = 0;
-                        }
+                for (int e = 0; e < kFewV; ++e) {
+                    const int dim = kFewV * (8 * (i >> 2) + 4 * h + (i & 3)) + e;
+                    if (!(fabsf((float)values[at + (dim < D ? dim : 0)]) < INFINITY)) o[e][i] = NAN;
                 }
-                if (!by_all) {               // (as in store())
-                    bool found = false;
+        }
+        // The wavefronts that had tokens, joined: neighbouring dimensions of a row next to each other, lane after lane; then a unit of them a thread.
+        constexpr int kUnit = kFewV < 4 ? kFewV : 4, kUnits = kFewV / kUnit * 16;
+        typedef float UnitF __attribute__((ext_vector_type(kUnit)));
+        typedef Q UnitQ __attribute__((ext_vector_type(kUnit)));
+        l = other_sum(l);
+        const int waves = min((int)((end - begin + 31) / 32), kWaves);
+        float2* const stats = (float2*)offsets;
+        __syncthreads();                 // (the places are read)
+        if (wave < waves) {
+            if (h == 0) stats[wave * 32 + n] = make_float2(R, l);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
+            for (int i = 0; i < 16; ++i)
 #pragma unroll
-                        for (int w = 0; w < kVWords; ++w) {
-                            const uint32_t keep = keep_of(v[j][w], C());
-                            found |= keep != ~0u;
-                            v[j][w] &= keep;
-                        }
-                    if (__builtin_amdgcn_ballot_w64(found)) {
-                        odd_from = min(odd_from, t0);
-                        odd_to = t0 + 32;
-                    }
+                for (int e = 0; e < kFewV; e += kUnit) {
+                    UnitF x;
+#pragma unroll
+                    for (int y = 0; y < kUnit; ++y) x[y] = o[e + y][i];
+                    ((UnitF*)near)[(wave * kUnits + i * (kFewV / kUnit) + e / kUnit) * 64 + lane] = x;
                 }
+        }
+        __syncthreads();
+        float top = -INFINITY, sum = 0.0f, weight[kWaves];
 #pragma unroll
-                for (int c = 0; c < 2; ++c)
+        for (int w = 0; w < kWaves; ++w)
+            if (w < waves) top = fmaxf(top, stats[w * 32 + n].x);
+        const float base = top == -INFINITY ? 0.0f : top;
 #pragma unroll
-                    for (int e = 0; e < kFewV; ++e) {
-                        u32x4 x[kTermsC];
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            const int j = c * 8 + 2 * w;
-                            if constexpr (kTermsC == 1) {
-                                x[0][w] = __builtin_amdgcn_perm(v[j + 1][e / 2], v[j][e / 2], e & 1 ? 0x07060302 : 0x05040100);
-                            } else {
-                                uint32_t t[3];
-                                terms(__uint_as_float(v[j][e]), __uint_as_float(v[j + 1][e]), t, E());
-#pragma unroll
-                                for (int i = 0; i < 3; ++i) x[i][w] = t[i];
-                            }
-                        }
-                        if constexpr (kTermsC == 1) {
-#pragma unroll
-                            for (int i = kTermsQ - 1; i >= 0; --i) o[e] = product(x[0], p[c][i], o[e], E());
-                        } else {
-#pragma unroll
-                            for (int both = 2; both >= 0; --both)
-#pragma unroll
-                                for (int i = both; i >= 0; --i) o[e] = product(x[i], p[c][both - i], o[e], E());
-                        }
-                    }
-                slot ^= 1;
-                if (more) load_v(slot);
+        for (int w = 0; w < kWaves; ++w) {
+            weight[w] = 0.0f;
+            if (w < waves) {
+                const float2 x = stats[w * 32 + n];
+                weight[w] = __builtin_amdgcn_exp2f(x.x - base);
+                sum += weight[w] * x.y;
             }
-            for (uint32_t t = odd_from; t < min(end, odd_to); ++t) {
-                const uint32_t page = divided(t, a.block);
-                const int64_t at = paged_row(view, table[page], (int32_t)(t - page * a.block.by));
-                if (at < 0 || !(t >= lo && t < hi)) continue;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-#pragma unroll
-                    for (int e = 0; e < kFewV; ++e) {
-                        const int dim = kFewV * (8 * (i >> 2) + 4 * h + (i & 3)) + e;
-                        if (!(fabsf((float)values[at + (dim < D ? dim : 0)]) < INFINITY)) o[e][i] = NAN;
-                    }
-            }
-            // The wavefronts that had tokens, joined: neighbouring dimensions of a row next to each other, lane after lane; then a unit of them a thread.
-            constexpr int kUnit = kFewV < 4 ? kFewV : 4, kUnits = kFewV / kUnit * 16;
-            typedef float UnitF __attribute__((ext_vector_type(kUnit)));
-            typedef Q UnitQ __attribute__((ext_vector_type(kUnit)));
-            l = other_sum(l);
-            const int waves = min((int)((end - begin + 31) / 32), kWaves);
-            float2* const stats = (float2*)offsets;
-            __syncthreads();                 // (the places are read)
-            if (wave < waves) {
-                if (h == 0) stats[wave * 32 + n] = make_float2(R, l);
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-#pragma unroll
-                    for (int e = 0; e < kFewV; e += kUnit) {
-                        UnitF x;
-#pragma unroll
-                        for (int y = 0; y < kUnit; ++y) x[y] = o[e + y][i];
-                        ((UnitF*)near)[(wave * kUnits + i * (kFewV / kUnit) + e / kUnit) * 64 + lane] = x;
-                    }
-            }
-            __syncthreads();
-            float top = -INFINITY, sum = 0.0f, weight[kWaves];
+        }
+        const int32_t slot_of = it.slot + it.share;
+        if (!valid || (it.shares > 1 && slot_of >= a.most_slots)) return;      // (the latter where starts do not ascend)
+        const int64_t at = ((int64_t)slot_of * d.cache.kv_heads + kvh) * kTileRows + n;
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+        Q* const to = (Q*)a.out + out_row * d.out_stride + head * d.out_head_stride;
+        for (int u = wave; u < kUnits; u += kWaves) {
+            const int i = u / (kFewV / kUnit), dim = kFewV * (8 * (i >> 2) + 4 * h + (i & 3)) + (u - i * (kFewV / kUnit)) * kUnit;
+            if (dim >= D) continue;
+            UnitF all = 0.0f;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w)
-                if (w < waves) top = fmaxf(top, stats[w * 32 + n].x);
-            const float base = top == -INFINITY ? 0.0f : top;
+                if (w < waves) all += weight[w] * ((const UnitF*)near)[(w * kUnits + u) * 64 + lane];
+            if (it.shares > 1) {
+                *(UnitF*)(a.parts + at * D + dim) = all;
+            } else {
+                UnitQ x;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                weight[w] = 0.0f;
-                if (w < waves) {
-                    const float2 x = stats[w * 32 + n];
-                    weight[w] = __builtin_amdgcn_exp2f(x.x - base);
-                    sum += weight[w] * x.y;
-                }
+                for (int y = 0; y < kUnit; ++y) x[y] = (Q)(all[y] * f);
+                *(UnitQ*)(to + dim) = x;
             }
-            const int32_t slot_of = it.slot + it.share;
-            if (!valid || (it.shares > 1 && slot_of >= a.most_slots)) return;      // (the latter where starts do not ascend)
-            const int64_t at = ((int64_t)slot_of * d.cache.kv_heads + kvh) * kTileRows + n;
-            const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-            Q* const to = (Q*)a.out + out_row * d.out_stride + head * d.out_head_stride;
-            for (int u = wave; u < kUnits; u += kWaves) {
-                const int i = u / (kFewV / kUnit), dim = kFewV * (8 * (i >> 2) + 4 * h + (i & 3)) + (u - i * (kFewV / kUnit)) * kUnit;
-                if (dim >= D) continue;
-                UnitF all = 0.0f;
-#pragma unroll
-                for (int w = 0; w < kWaves; ++w)
-                    if (w < waves) all += weight[w] * ((const UnitF*)near)[(w * kUnits + u) * 64 + lane];
-                if (it.shares > 1) {
-                    *(UnitF*)(a.parts + at * D + dim) = all;
-                } else {
-                    UnitQ x;
-#pragma unroll
-                    for (int y = 0; y < kUnit; ++y) x[y] = (Q)(all[y] * f);
-                    *(UnitQ*)(to + dim) = x;
-                }
-            }
-            if (wave == 0 && h == 0) {
-                if (it.shares > 1) a.stats[at] = make_float2(top == -INFINITY ? -INFINITY : top - kGrow, sum);
-                else if (a.lse) a.lse[out_row * d.heads + head] = sum == 0.0f ? -INFINITY : (top + (__log2f(sum) - kGrow)) * kLn2;
-            }
-            return;
         }
+        if (wave == 0 && h == 0) {
+            if (it.shares > 1) a.stats[at] = make_float2(top == -INFINITY ? -INFINITY : top - kGrow, sum);
+            else if (a.lse) a.lse[out_row * d.heads + head] = sum == 0.0f ? -INFINITY : (top + (__log2f(sum) - kGrow)) * kLn2;
+        }
+        return;
     }
 
     const uint32_t count = (end - begin + kTile - 1) / kTile;
@@ -1256,8 +1254,8 @@ extern "C" int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, cons
         !aligned(lse, 4))
         return refuse(what, "null or unaligned argument");
     const Plan p = plan_of(*d);
-    // (2^32 threads are refused by the launch, which may be the call's second one)
-    if (p.groups >= 1ll << 23) return refuse(what, "%lld workgroups are too many", (long long)p.groups);
+    // (2^32 threads are refused by the launch, which may be the call's last one)
+    if (p.groups >= 1ll << (p.budget ? 22 : 23)) return refuse(what, "%lld workgroups are too many", (long long)p.groups);
     if (p.bytes && (!rows16(workspace) || workspace_bytes < (int64_t)p.bytes))
         return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", p.bytes, (long long)workspace_bytes);
     char* const w = (char*)workspace;
