@@ -9,6 +9,18 @@ using namespace reef_ops;
 constexpr int kMaxTop = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 
+constexpr int kGroups = 1024;                // maxima of groups that are held
+// Groups of neighbours: 2^bits lanes' 16 bytes of the units that a wavefront reads at once (a batch), and of `per` batches where there are more than 256.
+struct Groups {
+    int32_t batches, per, bits, groups;
+};
+Groups groups_of(int32_t units, int32_t loads) {
+    Groups g{(units + loads - 1) / loads, 1, 0, 0};
+    while (g.bits < 4 && g.batches * 64 > kGroups << g.bits) ++g.bits;
+    g.per = (g.batches + kGroups / 4 - 1) / (kGroups / 4);
+    g.groups = (g.batches + g.per - 1) / g.per * (64 >> g.bits);
+    return g;
+}
 struct Args {
     reef_token_scores_desc d;
     const void* logits;
@@ -21,6 +33,7 @@ struct Args {
     struct Part* parts;     // [row][slice]
     uint32_t* maxima;       // [row][groups]
     int32_t slices, slice_units;
+    Groups by;
 };
 // What a part of a row comes to: its maximum, the sums relative to it, values that come before the given token.
 struct Part {
@@ -39,8 +52,30 @@ __device__ inline uint32_t order_of(float v) {
 __device__ inline float value_of(uint32_t order) { return __uint_as_float(order >> 31 ? order & ~(1u << 31) : ~order); }
 __device__ inline uint64_t key_of(uint32_t order, int32_t token) { return (uint64_t)order << 32 | (uint32_t)~token; }
 
-// v - m, or what has an exponential of 0 all the same where that is below, or is -infinity less itself.
+// v - m, or what has an exponential of 0 all the same where that is below, or is an infinity less itself.
 __device__ inline float less(float v, float m) { return fmaxf(v - m, -1000.0f); }
+// Exponentials relative to m are 2^(v c - M), c = log2 e and M = m c of 32 bits each, so that one rounding makes the exponent: larger by
+// 2^(m c - M) than they should be, which is taken off at the end.  Where M is so large that this could be much they are 2^((v - m) c).
+__device__ inline bool plain(float M) { return fabsf(M) < 0x1p20f; }
+__device__ inline float exponent(float v, float m, float M) { return plain(M) ? fmaxf(fmaf(v, kLog2e, -M), -1000.0f) : less(v, m) * kLog2e; }
+__device__ inline float excess(float m, float M) { return plain(M) ? fmaf(m, kLog2e, -M) : 0.0f; }
+// By which power of two sums relative to m0 are to be multiplied to be such relative to m1 >= m0.
+__device__ inline float step(float m0, float m1) {
+    const float M0 = m0 * kLog2e, M1 = m1 * kLog2e;
+    return plain(M0) && plain(M1) ? fmaxf(M0 - M1, -1000.0f) : less(m0, m1) * kLog2e + excess(m1, M1) - excess(m0, M0);
+}
+// A signalling NaN as a quiet one, which maxima pass over.
+__device__ inline float quiet(float v) {
+    float x;
+    asm("v_max_f32 %0, %1, %1" : "=v"(x) : "v"(v));
+    return x;
+}
+// The largest of three, of which none signals.
+__device__ inline float largest(float a, float b, float c) {
+    float x;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(x) : "v"(a), "v"(b), "v"(c));
+    return x;
+}
 
 // Sums and maxima over lanes without LDS: rows of 16 turned by 8, 4, 2, 1 lanes, then halves of halves and halves exchanged.
 template <int CONTROL, class V>
@@ -65,20 +100,14 @@ __device__ inline V swapped(V x) {
     __builtin_memcpy(&x, w, sizeof(V));
     return x;
 }
-template <class V, class Join>
-__device__ inline V over_four(V x, Join join) {
-    x = join(x, moved<0xB1>(x));             // lane i ^ 1
-    return join(x, moved<0x4E>(x));          // lane i ^ 2
-}
-template <class V, class Join>
-__device__ inline V over_row(V x, Join join) {
-    x = over_four(x, join);
-    x = join(x, moved<0x141>(x));            // lane 7 - i of eight
-    return join(x, moved<0x128>(x));         // by 8 of 16
-}
+// lane i ^ 1; i ^ 2; 7 - i of eight, where fours have the same; i - 8 of sixteen
+constexpr int kOne = 0xB1, kTwo = 0x4E, kFour = 0x141, kEight = 0x128;
 template <class V, class Join>
 __device__ inline V over_wave(V x, Join join) {
-    x = over_row(x, join);
+    x = join(x, moved<kOne>(x));
+    x = join(x, moved<kTwo>(x));
+    x = join(x, moved<kFour>(x));
+    x = join(x, moved<kEight>(x));
     x = join(x, swapped<false>(x));
     return join(x, swapped<true>(x));
 }
@@ -90,21 +119,17 @@ struct Sum {
     __device__ V operator()(V a, V b) const { return a + b; }
 };
 
-constexpr int kGroups = 1024;                // maxima of groups that are held
-// Groups of neighbours: so many lanes' 16 bytes of a unit, and of the next units where there are more than 256.
-__host__ __device__ inline int32_t lanes_of(int32_t units) { return units <= kGroups / 64 ? 1 : units <= kGroups / 16 ? 4 : 16; }
-__host__ __device__ inline int32_t units_each(int32_t units) { return (units + kGroups / 4 - 1) / (kGroups / 4); }
-__host__ __device__ inline int32_t groups_of(int32_t units) {
-    const int32_t per = units_each(units);
-    return (units + per - 1) / per * (64 / lanes_of(units));
-}
+constexpr float kBehind = -0x1p18f;          // (plain)
 constexpr int kHeld = 2048;                  // candidates that are held
 
-// A row a workgroup, read once: a lane keeps its 16 bytes of eight units, their maximum and sums relative to the largest so far, and how many of its values come
-// before the given token.  Exponentials are those of 32 bits, off by 2^-23 of themselves and three roundings of the argument; those of 16 bytes are added
-// in 32 bits, three roundings, and everything else in 64.
+// A row a workgroup, read once: a lane keeps its 16 bytes of a batch of units, their maximum m and sums relative to the largest so far; how many values come
+// before the given token is counted by the wavefront.  Exponentials are those of 32 bits, off by 2^-23 of themselves; those of 16 bytes are
+// added in 32 bits, up to seven roundings, and everything else in 64.
 //
-// The best tokens: of the maxima of groups of neighbours (16 lanes of a unit, or one where units are few), held near, as many as wanted reach a bound that is
+// The lanes' operations are nearly as long as the reads, so nothing is cleaned ahead: maxima pass over a NaN, and the bound that makes exponents no less
+// than -1000 is what a NaN and -infinity come to.  A batch with +infinity, or with a maximum so large that M is not plain, is read again and taken with care.
+//
+// The best tokens: of the maxima of groups of neighbours (up to 16 lanes of a batch), held near, as many as wanted reach a bound that is
 // found by halving; only groups that reach it are read again.  Their values that reach it are candidates.  Where there are more than are held (values that ascend with their
 // numbers, many alike) the bound is raised by halving again, down to one value, and of the tokens that have it the first ones are taken in order.
 //
@@ -113,7 +138,7 @@ enum { kWhole, kSlice, kJoin };
 // LOADS: of a wavefront in flight, 1 KiB each, a unit.
 template <class T, int WAVES, int LOADS, int STAGE>
 __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
-    constexpr int kLoads = LOADS, kThreads = WAVES * 64, kE = 16 / sizeof(T), kUnit = 64 * kE, kMine = kGroups / 64;
+    constexpr int kLoads = LOADS, kThreads = WAVES * 64, kE = 16 / sizeof(T), kUnit = 64 * kE, kMine = kGroups / 64, kLoadBits = LOADS == 8 ? 3 : 2;
     constexpr int kShift = sizeof(T) == 4 ? 0 : __is_same(T, _Float16) ? 13 : 16;
     typedef T Raw __attribute__((ext_vector_type(kE), aligned(sizeof(T))));
     const reef_token_scores_desc& d = a.d;
@@ -121,7 +146,7 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
     const int64_t row = STAGE == kSlice ? blockIdx.x / (uint32_t)a.slices : blockIdx.x;
     const T* x = (const T*)a.logits + row * d.logits_stride;
     const int32_t units = (d.vocab + kUnit - 1) / kUnit;
-    const int32_t per = units_each(units), wide = lanes_of(units), in_unit = 64 / wide, groups = groups_of(units);
+    const int32_t per = a.by.per, bits = a.by.bits, wide = 1 << bits, in_batch = 64 >> bits, groups = a.by.groups;
 
     __shared__ uint32_t maxima[kGroups];
     __shared__ uint64_t held[kHeld];
@@ -142,42 +167,36 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
     float m = -INFINITY;
     double s = 0.0, near = 0.0;
     int32_t rank = 0;
-    // 16 bytes from value i of the row on, -infinity behind its end
-    auto fetch = [&](int32_t i, float (&v)[kE]) __attribute__((always_inline)) {
+    // (as a NaN comes after all values but -infinity, and with -infinity by its number)
+    const bool lowest = mine == -INFINITY;
+    const float mine_before = lowest ? NAN : mine;
+    // 16 bytes from value i of the row on, and what is behind its end
+    auto fetch = [&](int32_t i, float (&v)[kE], float behind) __attribute__((always_inline)) {
         if (i + kE <= d.vocab) {
             const Raw raw = *(const Raw*)(x + i);
 #pragma unroll
             for (int e = 0; e < kE; ++e) v[e] = (float)raw[e];
         } else {
 #pragma unroll
-            for (int e = 0; e < kE; ++e) v[e] = i + e < d.vocab ? (float)x[i + e] : -INFINITY;
+            for (int e = 0; e < kE; ++e) v[e] = i + e < d.vocab ? (float)x[i + e] : behind;
         }
     };
     for (int32_t u0 = first_unit + wave * kLoads; u0 < end_unit; u0 += WAVES * kLoads) {
         float v[kLoads][kE];
-        if ((int64_t)(u0 + kLoads) * kUnit <= d.vocab) {
+        const bool full = (u0 + kLoads) * kUnit <= d.vocab;
+        // behind the end: no infinity, none that comes before the given token, and (in front of a lane's real values) none that is its largest
+        const float behind = fminf(mine, kBehind);
+        if (full) {
             Raw raw[kLoads];
 #pragma unroll
             for (int u = 0; u < kLoads; ++u) raw[u] = *(const Raw*)(x + (u0 + u) * kUnit + lane * kE);
 #pragma unroll
             for (int u = 0; u < kLoads; ++u)
 #pragma unroll
-                for (int e = 0; e < kE; ++e) v[u][e] = cleaned((float)raw[u][e]);
+                for (int e = 0; e < kE; ++e) v[u][e] = (float)raw[u][e];
         } else {
 #pragma unroll
-            for (int u = 0; u < kLoads; ++u) {
-                fetch((u0 + u) * kUnit + lane * kE, v[u]);
-#pragma unroll
-                for (int e = 0; e < kE; ++e) v[u][e] = cleaned(v[u][e]);
-            }
-        }
-        float top[kLoads], all = -INFINITY;
-#pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-            top[u] = v[u][0];
-#pragma unroll
-            for (int e = 1; e < kE; ++e) top[u] = fmaxf(top[u], v[u][e]);
-            all = fmaxf(all, top[u]);
+            for (int u = 0; u < kLoads; ++u) fetch((u0 + u) * kUnit + lane * kE, v[u], behind);
         }
         // those that come before the given token: at least as large in front of it, larger behind it
 #pragma unroll
@@ -185,53 +204,94 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
             const int32_t first = (u0 + u) * kUnit;
             if (t >= first + kUnit) {
 #pragma unroll
-                for (int e = 0; e < kE; ++e) rank += v[u][e] >= mine ? 1 : 0;
+                for (int e = 0; e < kE; ++e) rank += (int32_t)__popcll(__builtin_amdgcn_ballot_w64(v[u][e] >= mine_before));
             } else if (t < first) {
 #pragma unroll
-                for (int e = 0; e < kE; ++e) rank += v[u][e] > mine ? 1 : 0;
+                for (int e = 0; e < kE; ++e) rank += (int32_t)__popcll(__builtin_amdgcn_ballot_w64(v[u][e] > mine));
             } else {
 #pragma unroll
-                for (int e = 0; e < kE; ++e) rank += first + lane * kE + e < t ? v[u][e] >= mine : v[u][e] > mine;
+                for (int e = 0; e < kE; ++e)
+                    rank += (int32_t)__popcll(__builtin_amdgcn_ballot_w64(first + lane * kE + e < t ? v[u][e] >= mine_before : v[u][e] > mine));
             }
         }
-        if (all > m) {
-            const float y = less(m, all), f = __builtin_amdgcn_exp2f(y * kLog2e);
-            near = (near + s * (double)y) * f;
-            s *= f;
-            m = all;
-        }
+        constexpr bool kQuiet = __is_same(T, _Float16);       // (conversions make them so)
+        auto value = [&](int i) __attribute__((always_inline)) { return kQuiet ? v[i / kE][i % kE] : quiet(v[i / kE][i % kE]); };
+        float all = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kLoads * kE; i += 2) all = largest(all, value(i), value(i + 1));
+        const float next = largest(m, m, all), base = next * kLog2e;
+        float e1[kLoads], e2[kLoads];
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
-            float e1[kE], e2[kE];
+            e1[u] = e2[u] = 0.0f;
 #pragma unroll
             for (int e = 0; e < kE; ++e) {
-                const float y = less(v[u][e], m);
-                e1[e] = __builtin_amdgcn_exp2f(y * kLog2e);
-                e2[e] = e1[e] * y;
+                const float y = fmaxf(fmaf(v[u][e], kLog2e, -base), -1000.0f), w = __builtin_amdgcn_exp2f(y);    // (-1000 for a NaN)
+                e1[u] += w;
+                e2[u] = fmaf(w, y, e2[u]);
             }
-#pragma unroll
-            for (int step = 1; step < kE; step <<= 1)
-#pragma unroll
-                for (int e = 0; e < kE; e += 2 * step) {
-                    e1[e] += e1[e + step];
-                    e2[e] += e2[e + step];
+        }
+        const bool any = full || u0 * kUnit + lane * kE < d.vocab;           // of the lane's values are real
+        if (__builtin_amdgcn_ballot_w64(any && !((plain(base) || next == -INFINITY) && (full || all > kBehind))) == 0) {
+            if (any) {
+                if (next > m) {
+                    const float y = step(m, next), f = __builtin_amdgcn_exp2f(y);
+                    near = (near + s * (double)y) * f;
+                    s *= f;
+                    m = next;
                 }
-            s += (double)e1[0];
-            near += (double)e2[0];
+#pragma unroll
+                for (int u = 0; u < kLoads; ++u) {
+                    s += (double)e1[u];
+                    near += (double)e2[u];
+                }
+            } else {
+                all = -INFINITY;
+            }
+        } else {
+            all = -INFINITY;
+#pragma unroll 1
+            for (int u = 0; u < kLoads; ++u) {
+                float z[kE], top = -INFINITY;
+                fetch((u0 + u) * kUnit + lane * kE, z, -INFINITY);
+#pragma unroll
+                for (int e = 0; e < kE; ++e) {
+                    z[e] = cleaned(z[e]);
+                    top = fmaxf(top, z[e]);
+                }
+                all = fmaxf(all, top);
+                if (top > m) {
+                    const float y = step(m, top), f = __builtin_amdgcn_exp2f(y);
+                    near = (near + s * (double)y) * f;
+                    s *= f;
+                    m = top;
+                }
+                const float M = m * kLog2e;
+                float sum = 0.0f, sum2 = 0.0f;
+#pragma unroll
+                for (int e = 0; e < kE; ++e) {
+                    const float y = exponent(z[e], m, M), w = __builtin_amdgcn_exp2f(y);
+                    sum += w;
+                    sum2 = fmaf(w, y, sum2);
+                }
+                s += (double)sum;
+                near += (double)sum2;
+            }
         }
         if (d.top) {
-#pragma unroll
-            for (int u = 0; u < kLoads; ++u) {
-                if (u0 + u >= end_unit) continue;
-                const float of = wide == 1 ? top[u] : wide == 4 ? over_four(top[u], Max()) : over_row(top[u], Max());
-                if (lane % wide == 0) {
-                    uint32_t* const to = &maxima[(u0 + u) / per * in_unit + lane / wide];
-                    if (per == 1) *to = order_of(of);
-                    else atomicMax(to, order_of(of));
-                }
+            float of = all;
+            if (wide > 1) of = fmaxf(of, moved<kOne>(of));
+            if (wide > 2) of = fmaxf(of, moved<kTwo>(of));
+            if (wide > 4) of = fmaxf(of, moved<kFour>(of));
+            if (wide > 8) of = fmaxf(of, moved<kEight>(of));
+            if ((lane & (wide - 1)) == 0) {
+                uint32_t* const to = &maxima[(per == 1 ? u0 / kLoads : u0 / kLoads / per) * in_batch + (lane >> bits)];
+                if (per == 1) *to = order_of(of);
+                else atomicMax(to, order_of(of));
             }
         }
     }
+    if (STAGE != kJoin && lowest && slice == 0 && wave == 0) rank += t;
     if constexpr (STAGE == kJoin) {          // a slice a thread
         if (tid < a.slices) {
             const Part part = a.parts[row * a.slices + tid];
@@ -245,7 +305,7 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
     }
     // the row's: first of the wavefront's lanes, then of the wavefronts
     float all = over_wave(m, Max());
-    rank = over_wave(rank, Sum());
+    if constexpr (STAGE == kJoin) rank = over_wave(rank, Sum());
     if (lane == 0) {
         tops[wave] = all;
         counts[0][wave] = rank;
@@ -260,8 +320,8 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
     }
     const bool none = !(all > -INFINITY && all < INFINITY);
     if (m > -INFINITY && !none) {
-        const float y = less(m, all);
-        const double f = (double)__builtin_amdgcn_exp2f(y * kLog2e);
+        const float y = step(m, all);
+        const double f = (double)__builtin_amdgcn_exp2f(y);
         near = (near + s * (double)y) * f;
         s *= f;
     } else {
@@ -283,15 +343,17 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
     if constexpr (STAGE == kSlice) {
         if (tid == 0) a.parts[row * a.slices + slice] = {s, near, all, rank};
         if (d.top)
-            for (int i = first_unit / per * in_unit + tid; i < (end_unit + per - 1) / per * in_unit; i += kThreads) a.maxima[row * groups + i] = maxima[i];
+            for (int i = first_unit / (kLoads * per) * in_batch + tid; i < (end_unit + kLoads * per - 1) / (kLoads * per) * in_batch; i += kThreads)
+                a.maxima[row * groups + i] = maxima[i];
         return;
     }
-    const double log_s = none ? (double)NAN : log(s);
+    const double off = excess(all, all * kLog2e);
+    const double log_s = none ? (double)NAN : log(s) - off * 0.6931471805599453;
     auto score = [&](float v) { return (float)((double)v - (double)all - log_s); };
     if (tid == 0) {
         a.scores[row] = given ? score(mine) : -INFINITY;
         a.ranks[row] = given ? rank : -1;
-        a.entropy[row] = (float)(log_s - near / s);
+        a.entropy[row] = (float)(log_s - (near / s - off) / (double)kLog2e);
     }
     if (!d.top) return;
 
@@ -339,7 +401,7 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
     auto values_from = [&](uint32_t bound) __attribute__((always_inline)) {
         auto offer = [&](int32_t i) __attribute__((always_inline)) {
             float v[kE];
-            fetch(i, v);
+            fetch(i, v, -INFINITY);
 #pragma unroll
             for (int e = 0; e < kE; ++e) {
                 const uint32_t o = order_of(cleaned(v[e]));
@@ -355,10 +417,11 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
             const int32_t many = (int32_t)__popcll(who);
             if (is) chosen[wave][__popcll(who & ((1ull << lane) - 1))] = (uint16_t)(g0 + lane);
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            for (int32_t k = lane / wide; k < many; k += in_unit) {
-                const int32_t g = chosen[wave][k], first = g / in_unit * per;
-                for (int32_t u = first; u < min(units, first + per); ++u) {
-                    const int32_t i = u * kUnit + (g % in_unit * wide + lane % wide) * kE;
+            const int32_t team_bits = min(6, bits + kLoadBits), team = 1 << team_bits;       // lanes a group
+            for (int32_t k = lane >> team_bits; k < many; k += 64 >> team_bits) {
+                const int32_t g = chosen[wave][k], first = (g >> (6 - bits)) * per * kLoads, end = min(units, first + per * kLoads);
+                for (int32_t u = first + ((lane & (team - 1)) >> bits); u < end; u += team >> bits) {
+                    const int32_t i = u * kUnit + (((g & (in_batch - 1)) << bits) + (lane & (wide - 1))) * kE;
                     if (i < d.vocab) offer(i);
                 }
             }
@@ -450,23 +513,23 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
     for (int i = tid; i < d.top; i += kThreads) put(i, held[i]);
 }
 
-constexpr int kSliceLoads = 8;
 // How a call is laid out: slices of 128 units, which sixteen wavefronts read at once, where rows are few and have more of them.
 struct Plan {
     int32_t slices, slice_units;
-    int64_t groups, parts_bytes, bytes;
+    Groups by;
+    int64_t parts_bytes, bytes;
 };
 Plan plan_of(const reef_token_scores_desc& d) {
-    const int32_t unit = 1024 / type_bytes(d.type), units = (d.vocab + unit - 1) / unit, per = units_each(units);
-    Plan p{1, units, groups_of(units), 0, 0};
+    const int32_t unit = 1024 / type_bytes(d.type), units = (d.vocab + unit - 1) / unit, loads = d.rows <= 512 ? 8 : 4;
+    Plan p{1, units, groups_of(units, loads), 0, 0};
     if (d.rows > 128 || units <= 192) return p;
     const int32_t most = std::min(256 / d.rows, (units + 127) / 128);
-    const int32_t step = per * kSliceLoads;  // no group and no eight loads of a wavefront reach into the next slice
+    const int32_t step = p.by.per * loads;        // no group and no batch reaches into the next slice
     p.slice_units = ((units + most - 1) / most + step - 1) / step * step;
     p.slices = (units + p.slice_units - 1) / p.slice_units;
     if (p.slices <= 1) return p;
     p.parts_bytes = (int64_t)d.rows * p.slices * (int64_t)sizeof(Part);
-    p.bytes = p.parts_bytes + (d.top ? 4 * d.rows * p.groups : 0);
+    p.bytes = p.parts_bytes + (d.top ? 4ll * d.rows * p.by.groups : 0);
     return p;
 }
 // Sixteen wavefronts a row where rows are few, four where they fill the device (1000 rows of 128257, bf16: 89 us; eight 96, sixteen 129).
@@ -474,7 +537,7 @@ template <class T>
 int run(const char* what, const Args& a, const Plan& p, void* stream) {
     const dim3 rows((unsigned)a.d.rows);
     if (p.bytes) {
-        if (int rc = launch(what, token_scores<T, 16, kSliceLoads, kSlice>, dim3((unsigned)(a.d.rows * p.slices)), dim3(16 * 64), a, stream)) return rc;
+        if (int rc = launch(what, token_scores<T, 16, 8, kSlice>, dim3((unsigned)(a.d.rows * p.slices)), dim3(16 * 64), a, stream)) return rc;
         return launch(what, token_scores<T, 16, 8, kJoin>, rows, dim3(16 * 64), a, stream);
     }
     if (a.d.rows <= 256) return launch(what, token_scores<T, 16, 8, kWhole>, rows, dim3(16 * 64), a, stream);
@@ -514,7 +577,7 @@ extern "C" int reef_ops_token_scores(const reef_token_scores_desc* d, const void
     const Span in[] = {{logits, ((n - 1) * d->logits_stride + d->vocab) * type_bytes(d->type)}, {tokens, 4 * n}};
     if (overlap(out, in)) return refuse(what, "an output overlaps an input");
     const Plan p = plan_of(*d);
-    const Args a{*d, logits, tokens, scores, ranks, entropy, top_tokens, top_scores, (Part*)workspace, (uint32_t*)((char*)workspace + p.parts_bytes), p.slices, p.slice_units};
+    const Args a{*d, logits, tokens, scores, ranks, entropy, top_tokens, top_scores, (Part*)workspace, (uint32_t*)((char*)workspace + p.parts_bytes), p.slices, p.slice_units, p.by};
     switch (d->type) {
         case REEF_TYPE_F32: return run<float>(what, a, p, stream);
         case REEF_TYPE_F16: return run<_Float16>(what, a, p, stream);

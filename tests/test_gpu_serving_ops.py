@@ -319,9 +319,10 @@ def test_chunk_starts_that_do_not_ascend_stay_inside():
 
 
 # ---- scores of given tokens ----------------------------------------------------------------------
-def run_scores(kind, logits, tokens, top, pad=0):
+def run_scores(kind, logits, tokens, top, pad=0, raw=None):
     rows, vocab = logits.shape
-    raw = R.encode(np.pad(np.asarray(logits, np.float32), ((0, 0), (0, pad)), constant_values=60), kind)
+    if raw is None:
+        raw = R.encode(np.pad(np.asarray(logits, np.float32), ((0, 0), (0, pad)), constant_values=60), kind)
     d = B.TokenScoresDesc(kind, rows, vocab, top, vocab + pad)
     outs = [up(np.full(n + 1, -9, t)) for n, t in ((rows, np.float32), (rows, np.int32), (rows, np.float32), (rows * top, np.int32), (rows * top, np.float32))]
     n_work = B.ops_token_scores_workspace(d)
@@ -396,6 +397,38 @@ def test_scores_extremes_of_32_bits():
     x = np.full((3, 1000), -3e38)
     x[0, 5], x[1, 5:9], x[2] = 3e38, [1e30, 1e30, -1e30, 2e30], 1e-40
     run_scores(F32, x, [5, 6, 999], 10)
+
+
+@pytest.mark.parametrize("kind,many", [(F32, (0x7F800001, 0xFF800001, 0x7FBFFFFF)), (F16, (0x7C01, 0xFC01)), (BF16, (0x7F81, 0xFFBF))])
+@pytest.mark.parametrize("vocab", [129, 4096, 70001])
+def test_scores_signalling_nan(kind, many, vocab):
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((5, vocab)).astype(np.float32) * 3
+    raw = R.encode(x, kind).copy()
+    for i, share in enumerate((0.0, 0.01, 0.5, 0.99, 1.0)):
+        where = rng.random(vocab) < share
+        raw.view(np.uint32 if kind == F32 else np.uint16)[i, where] = rng.choice(many, int(where.sum()))
+    assert np.isnan(R.decode(raw, kind)[4]).all()
+    run_scores(kind, x, rng.integers(0, vocab, 5), 64, raw=raw)
+    run_scores(kind, x, [0, vocab - 1, 1, 2, 3], 7, raw=raw)
+
+
+# (Values near 2^20 / log2 e, where exponentials are taken otherwise; rows that reach there from below and from above.)
+@pytest.mark.parametrize("vocab", [1000, 30011, 150001])
+def test_scores_of_large_values(vocab):
+    rng = np.random.default_rng(vocab)
+    x = rng.standard_normal((8, vocab)) * 4
+    x[0] += 726817
+    x[1] -= 726817
+    x[2] += 2.0 ** 24
+    x[3] -= 1e30
+    x[4] += np.linspace(726700, 726900, vocab)
+    x[5] -= np.linspace(726700, 726900, vocab)
+    x[6] = np.where(rng.random(vocab) < 0.01, x[6], -3.4e38)
+    x[7] = np.where(np.arange(vocab) < vocab - 3, -250000.0 - np.arange(vocab) % 3, -np.inf)
+    tokens = rng.integers(0, vocab, 8)
+    run_scores(F32, x, tokens, 20)
+    run_scores(F32, x, [vocab - 1] * 8, 0)
 
 
 # ---- blocks ---------------------------------------------------------------------------------------
