@@ -12,8 +12,7 @@ constexpr int kRows = 32;                    // query rows of a wavefront: heads
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int32_t kLeast = 256, kLeastFew = 512;   // cached tokens a share at least, of tiles of 32 rows for each wavefront and of 32 in all
 constexpr int32_t kCut = 768, kCutFew = 2048;      // up to so many a tile is not cut
-constexpr int kAtOnce = 256;                       // workgroups that run at once, one a CU
-constexpr int kGroups = 3 * kAtOnce;               // workgroups that the shares of all tiles are to make at most
+constexpr int kCus = 256;
 constexpr float kSlack = 8.0f;               // powers of two by which weights may pass their reference
 
 struct Args {
@@ -31,6 +30,7 @@ struct Args {
     int32_t zero;           // scale is 0
     int32_t group;
     int32_t tile_rows;      // of a workgroup
+    int32_t at_once;        // workgroups that run at once
     int32_t budget;         // workgroups that tiles are cut for, beside one each; 0: they are not cut
     int32_t most_items, most_slots;
     int32_t* used;          // slots that there are; behind it (int4 aligned) what each belongs to
@@ -77,8 +77,8 @@ __device__ inline void size_up(const Args& a, const Request& r, float* most, flo
     *all = (float)r.tiles * (u + v) * 0.5f;
 }
 // How long shares are: tiles of up to `whole` tokens are not cut, others into shares of `tokens`.  Tiles that are longer than 1.3 rounds' worth are cut into half
-// rounds.  Where there are fewer than kGroups tiles, and those of a request are much alike (not as a prompt's, of which long ones and short ones make up for each other), they are
-// cut into the number n that takes the least rounds of workgroups, ceil(n N / 256) / n.
+// rounds.  Where there are fewer than three rounds of tiles, and those of a request are much alike (not as a prompt's, of which long ones and short ones make up for each other), they are
+// cut into the number n that takes the least rounds of workgroups, ceil(n N / at once) / n.
 // Where that makes more items than there are workgroups for (lengths that were not expected), none is cut.
 struct Cut {
     float whole, tokens, alike;              // alike: tokens of a share of tiles that are much alike; 0: as others
@@ -86,13 +86,14 @@ struct Cut {
 __device__ inline Cut cut_of(const Args& a, float all, float tiles) {
     const float kv = (float)a.d.cache.kv_heads, groups = tiles * kv;
     Cut c;
-    c.tokens = all * kv * (1.02f / (2 * kAtOnce));
+    const float at_once = (float)a.at_once;
+    c.tokens = all * kv * (0.51f / at_once);
     c.whole = 2.6f * c.tokens;
     c.alike = 0.0f;
     if (groups < (float)a.budget) {
-        float best = ceilf(groups * (1.0f / kAtOnce)), n = 1.0f;
+        float best = ceilf(groups / at_once), n = 1.0f;
         for (float k = 2.0f; k * groups <= (float)a.budget && k <= 64.0f; k += 1.0f) {
-            const float rounds = ceilf(k * groups * (1.0f / kAtOnce)) * __builtin_amdgcn_rcpf(k);
+            const float rounds = ceilf(k * groups / at_once) * __builtin_amdgcn_rcpf(k);
             if (rounds < 0.95f * best) {
                 best = rounds;
                 n = k;
@@ -107,6 +108,8 @@ __device__ inline int32_t shares_of(const Args& a, const Cut& c, float most, flo
     if (most <= fmaxf((float)(few ? kCutFew : kCut), alike ? c.alike : c.whole)) return 1;
     return (int32_t)ceilf(most / fmaxf((float)(few ? kLeastFew : kLeast), alike ? c.alike : c.tokens));
 }
+// Shares that are longer than half a round come first, so that none of them begins when the others are nearly done.
+__device__ inline bool comes_first(const Cut& c, float most, int32_t shares) { return most > c.tokens * (float)shares; }
 
 // Items and slots are counted up to 2^32 - 1: more there are only where starts do not ascend, and then nothing may run over.
 __device__ inline uint32_t plus(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
@@ -169,18 +172,25 @@ __device__ inline Item find_item(const Args& a, int32_t id) {
         Request r{};
         if (lane < a.d.requests) r = request_of(a, lane);
         int32_t shares = 1;
+        bool first = true;
         if (a.budget) {
             float most, all;
             size_up(a, r, &most, &all);
-            shares = shares_of(a, cut_of(a, sum_of(all), sum_of((float)r.tiles)), most, all, r.tiles);
+            const Cut cut = cut_of(a, sum_of(all), sum_of((float)r.tiles));
+            shares = shares_of(a, cut, most, all, r.tiles);
+            first = comes_first(cut, most, shares);
         }
-        uint32_t all_items, all_slots = 0, slot = 0, mine = product(r.tiles, shares), at = before_me(mine, &all_items);
-        if (a.budget && all_items > (uint32_t)a.most_items) {
-            shares = 1;
-            mine = (uint32_t)r.tiles;
-            at = before_me(mine, &all_items);
+        uint32_t firsts, others = 0, all_slots = 0, slot = 0, mine = product(r.tiles, shares), at = before_me(first ? mine : 0, &firsts);
+        if (a.budget) {
+            const uint32_t x = before_me(first ? 0 : mine, &others);
+            at = first ? at : plus(firsts, x);
+            if (plus(firsts, others) > (uint32_t)a.most_items) {
+                shares = 1;
+                mine = (uint32_t)r.tiles;
+                at = before_me(mine, &firsts);
+            }
+            slot = before_me(shares > 1 ? mine : 0, &all_slots);
         }
-        if (a.budget) slot = before_me(shares > 1 ? mine : 0, &all_slots);
         const uint64_t who = __builtin_amdgcn_ballot_w64((uint32_t)id >= at && (uint32_t)id - at < mine);
         if (!who) return it;
         const int l = __builtin_amdgcn_readfirstlane(__builtin_ctzll(who));
@@ -207,7 +217,7 @@ constexpr int kListThreads = 1024;
 __global__ void __launch_bounds__(kListThreads) list_items(Args a) {
     constexpr int kListWaves = kListThreads / 64;
     __shared__ float2 sums[kListWaves];
-    __shared__ uint2 counts[kListWaves];
+    __shared__ uint3 counts[kListWaves];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int32_t R = a.d.requests, per = (R + kListThreads - 1) / kListThreads, lo = min(R, tid * per), hi = min(R, lo + per);
     Cut cut{};
@@ -232,38 +242,47 @@ __global__ void __launch_bounds__(kListThreads) list_items(Args a) {
         cut = cut_of(a, sum, tiles);
     }
     bool whole = !a.budget;
+    // shares, tiles, whether it comes first
     auto shares_and_tiles = [&](int32_t i) {
         const Request r = request_of(a, i);
-        int32_t shares = 1;
+        int32_t shares = 1, first = 1;
         if (!whole) {
             float most, all;
             size_up(a, r, &most, &all);
             shares = shares_of(a, cut, most, all, r.tiles);
+            first = comes_first(cut, most, shares);
         }
-        return make_int2(shares, r.tiles);
+        return make_int3(shares, r.tiles, first);
     };
-    uint32_t all, all_slots, item, slot;
+    uint32_t all, all_slots, item, later, slot;            // later: where the next request that does not come first has its items
     auto count = [&]() {
-        uint32_t items = 0, slots = 0, of_wave, slots_of_wave;
+        uint32_t items = 0, others = 0, slots = 0, of_wave, others_of_wave, slots_of_wave;
         for (int32_t i = lo; i < hi; ++i) {
-            const int2 x = shares_and_tiles(i);
-            items = plus(items, product(x.x, x.y));
-            if (x.x > 1) slots = plus(slots, product(x.x, x.y));
+            const int3 x = shares_and_tiles(i);
+            const uint32_t mine = product(x.x, x.y);
+            if (x.z) items = plus(items, mine);
+            else others = plus(others, mine);
+            if (x.x > 1) slots = plus(slots, mine);
         }
         item = before_me(items, &of_wave);
+        later = before_me(others, &others_of_wave);
         slot = before_me(slots, &slots_of_wave);
         __syncthreads();
-        if (lane == 0) counts[wave] = make_uint2(of_wave, slots_of_wave);
+        if (lane == 0) counts[wave] = make_uint3(of_wave, others_of_wave, slots_of_wave);
         __syncthreads();
+        uint32_t firsts = 0;
         all = all_slots = 0;
         for (int w = 0; w < kListWaves; ++w) {
             if (w < wave) {
                 item = plus(item, counts[w].x);
-                slot = plus(slot, counts[w].y);
+                later = plus(later, counts[w].y);
+                slot = plus(slot, counts[w].z);
             }
-            all = plus(all, counts[w].x);
-            all_slots = plus(all_slots, counts[w].y);
+            firsts = plus(firsts, counts[w].x);
+            all = plus(all, plus(counts[w].x, counts[w].y));
+            all_slots = plus(all_slots, counts[w].z);
         }
+        later = plus(later, firsts);
     };
     count();
     if (!whole && all > (uint32_t)a.most_items) {
@@ -271,11 +290,12 @@ __global__ void __launch_bounds__(kListThreads) list_items(Args a) {
         count();
     }
     for (int32_t i = lo; i < hi; ++i) {
-        const int2 x = shares_and_tiles(i);
+        const int3 x = shares_and_tiles(i);
         const uint32_t mine = product(x.x, x.y);
-        a.info[i] = make_int4((int32_t)min(item, 1u << 30), x.x, (int32_t)min(slot, 1u << 30), 0);
-        for (uint32_t k = item; k < min(plus(item, mine), (uint32_t)a.most_items); ++k) a.list[kListHead + k] = i;
-        item = plus(item, mine);
+        uint32_t& at = x.z ? item : later;
+        a.info[i] = make_int4((int32_t)min(at, 1u << 30), x.x, (int32_t)min(slot, 1u << 30), 0);
+        for (uint32_t k = at; k < min(plus(at, mine), (uint32_t)a.most_items); ++k) a.list[kListHead + k] = i;
+        at = plus(at, mine);
         if (x.x > 1) slot = plus(slot, mine);
     }
     if (tid == 0) {
@@ -359,13 +379,13 @@ struct Near {
     static __device__ inline uint32_t at(uint32_t row, uint32_t piece) { return row * kPitch + ((piece ^ turn(row)) << 4); }
 };
 
-constexpr int waves_of(int dp) { return dp <= 128 ? 8 : 4; }
 // How a kernel is laid out, by its types and head size.  TK: tokens of a tile of keys and values; WAVES of 32 rows each share them.
 template <class Q, class C, int DP>
 struct Shape {
     static constexpr bool kHalf = __is_same(C, _Float16);
     static constexpr int kTermsC = sizeof(C) == 4 ? 3 : 1, kTermsQ = sizeof(Q) == 2 ? 1 : kHalf ? 2 : 3;
-    static constexpr int kWaves = waves_of(DP), kTile = kTermsQ == 1 && DP <= 128 ? 64 : 32;
+    static constexpr bool kPair = DP <= 64;
+    static constexpr int kWaves = DP <= 128 && !kPair ? 8 : 4, kTile = kTermsQ == 1 && DP <= 128 ? 64 : 32;
     // Tiles of 32 rows in all: registers of what a wavefront holds (keys, values, queries, output, weights), and so how many wavefronts; 0: too many for any.
     static constexpr int kFewV = DP <= 64 ? 2 : DP <= 128 ? 4 : 8;            // values of a row of V a lane
     static constexpr int kFewHeld = DP * (int)sizeof(C) / 8 + 16 * kFewV * (int)sizeof(C) / 4 + kTermsQ * DP / 4 + kFewV * 16 + 16 + 8 * kTermsQ;
@@ -389,7 +409,7 @@ struct Shape {
 // both sides, six products (the others are below 2^-22).  Weights of 16-bit types are rounded to the type once: half a step of the type of each at most, which in their mean is
 // no more than the output's own rounding (two terms would take 1.4 times as long).
 template <class Q, class C, int DP, bool FEW>
-__global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C, DP>::kWaves) * 64) chunk_attention(Args a) {
+__global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C, DP>::kWaves) * 64, (!FEW && Shape<Q, C, DP>::kPair ? 2 : 1)) chunk_attention(Args a) {
     using E = std::conditional_t<sizeof(C) == 4, __bf16, C>;                  // what is multiplied
     using Sh = Shape<Q, C, DP>;
     constexpr bool kHalf = Sh::kHalf;
@@ -1167,20 +1187,28 @@ int check(const char* what, const reef_chunk_attention_desc* d) {
     return 0;
 }
 
+// What the host asks of a shape.
+struct Waves {
+    int few, each, at_once;
+};
 template <class Q, class C>
-bool has_few(int dim) {
-    return dim <= 64 ? Shape<Q, C, 64>::kFewWaves : dim <= 96 ? Shape<Q, C, 96>::kFewWaves : dim <= 128 ? Shape<Q, C, 128>::kFewWaves : dim <= 192 ? Shape<Q, C, 192>::kFewWaves
-                                                                                                                                      : Shape<Q, C, 256>::kFewWaves;
+Waves waves_of(int dim) {
+    auto of = [](auto dp) {
+        using Sh = Shape<Q, C, decltype(dp)::value>;
+        return Waves{Sh::kFewWaves, Sh::kWaves, Sh::kPair ? 2 * kCus : kCus};
+    };
+    return dim <= 64 ? of(std::integral_constant<int, 64>()) : dim <= 96 ? of(std::integral_constant<int, 96>()) : dim <= 128 ? of(std::integral_constant<int, 128>())
+         : dim <= 192 ? of(std::integral_constant<int, 192>()) : of(std::integral_constant<int, 256>());
 }
-bool has_few(const reef_chunk_attention_desc& d) {
+Waves waves_of(const reef_chunk_attention_desc& d) {
     const int dim = d.cache.head_dim;
-    if (d.type != REEF_TYPE_F32) return d.type == REEF_TYPE_F16 ? has_few<_Float16, _Float16>(dim) : has_few<__bf16, __bf16>(dim);
-    return d.cache.type == REEF_TYPE_F32 ? has_few<float, float>(dim) : d.cache.type == REEF_TYPE_F16 ? has_few<float, _Float16>(dim) : has_few<float, __bf16>(dim);
+    if (d.type != REEF_TYPE_F32) return d.type == REEF_TYPE_F16 ? waves_of<_Float16, _Float16>(dim) : waves_of<__bf16, __bf16>(dim);
+    return d.cache.type == REEF_TYPE_F32 ? waves_of<float, float>(dim) : d.cache.type == REEF_TYPE_F16 ? waves_of<float, _Float16>(dim) : waves_of<float, __bf16>(dim);
 }
 
 // How a call is laid out.
 struct Plan {
-    int32_t tile_rows, budget;
+    int32_t tile_rows, at_once, budget;
     bool few;               // tiles of 32 rows in all
     int64_t items, slots, groups;      // groups: workgroups
     size_t info_bytes, list_bytes, jobs_bytes, stats_bytes, bytes;
@@ -1190,8 +1218,10 @@ Plan plan_of(const reef_chunk_attention_desc& d) {
     const int64_t rows = (int64_t)d.tokens * group;
     Plan p{};
     // Up to 32 rows a request on the average: tiles of so many, whose wavefronts share the tokens, else tiles of so many for each wavefront, which share keys and values.
-    p.few = rows <= (int64_t)kRows * d.requests && has_few(d);
-    p.tile_rows = p.few ? kRows : waves_of(d.cache.head_dim) * kRows;
+    const Waves waves = waves_of(d);
+    p.few = rows <= (int64_t)kRows * d.requests && waves.few;
+    p.tile_rows = p.few ? kRows : waves.each * kRows;
+    p.at_once = p.few ? kCus : waves.at_once;
     int64_t longest = (int64_t)d.max_blocks * d.cache.block_size;
     if (d.longest && d.longest < longest) longest = d.longest;
     if (d.window) longest = std::min(longest, (int64_t)d.window + p.tile_rows / group);
@@ -1200,7 +1230,7 @@ Plan plan_of(const reef_chunk_attention_desc& d) {
     if (longest > cut) {
         // Workgroups that find no item take 2 us a round for their look: there are no more than are likely to have one.
         const int64_t shares = (longest + least - 1) / least, tiles = p.items;
-        p.budget = tiles * kv <= kAtOnce / 2 ? kAtOnce : kGroups;
+        p.budget = tiles * kv <= p.at_once / 2 ? p.at_once : 3 * p.at_once;
         p.items = std::min(tiles * shares, tiles + (p.budget + kv - 1) / kv);
         p.slots = p.items;
         p.jobs_bytes = 16 * (size_t)(1 + p.slots);
@@ -1263,7 +1293,7 @@ extern "C" int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, cons
     const int32_t group = d->heads / d->cache.kv_heads;
     const Args a{*d, query, key_cache, value_cache, table, starts, cached, lengths, out, lse, (int4*)w, p.list_bytes ? (int32_t*)(w + list) : nullptr, (float*)(w + parts),
                  (float2*)(w + stats), d->scale == 0.0f ? kLog2e : std::fabs(d->scale) * kLog2e, d->scale < 0.0f ? (d->type == REEF_TYPE_F32 ? 0x80000000u : 0x80008000u) : 0u,
-                 d->scale == 0.0f, group, p.tile_rows, p.budget, (int32_t)p.items, (int32_t)p.slots, (int32_t*)(w + jobs), (int4*)(w + jobs) + 1,
+                 d->scale == 0.0f, group, p.tile_rows, p.at_once, p.budget, (int32_t)p.items, (int32_t)p.slots, (int32_t*)(w + jobs), (int4*)(w + jobs) + 1,
                  divider((uint32_t)d->cache.block_size), divider((uint32_t)group)};
     switch (d->type * 4 + d->cache.type) {
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, p, stream);
