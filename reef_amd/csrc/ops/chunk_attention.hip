@@ -11,7 +11,8 @@ using namespace reef_ops;
 constexpr int kRows = 32;                    // query rows of a wavefront: heads of one token next to each other, token after token
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int32_t kLeast = 256, kLeastFew = 512;   // cached tokens a share at least, of tiles of 32 rows for each wavefront and of 32 in all
-constexpr int32_t kCut = 768, kCutFew = 2048;      // up to so many a tile is not cut
+constexpr int32_t kLooked = 640, kLookedFew = 2048;  // up to so many tokens no cutting is looked at
+constexpr float kJoin = 420.0f;              // tokens whose time it takes to write and read a share's sums, over the products per token
 constexpr int kCus = 256;
 constexpr float kSlack = 8.0f;               // powers of two by which weights may pass their reference
 
@@ -21,8 +22,8 @@ struct Args {
     const int32_t *table, *starts, *cached, *lengths;
     void* out;
     float* lse;
-    int4* info;             // [request], where there are many: first item, shares, first slot
-    int32_t* list;          // the numbers of items and of slots, then the request of each item
+    int2* info;             // [request], where there are many: first item, first slot
+    int32_t* list;          // numbers of all (kListHead), then the request of each item
     float* parts;           // [slot][cache head][row of the tile][head_dim], sums that are not divided yet
     float2* stats;          // [slot][cache head][row of the tile]: power of two that they are to be multiplied by, sum of the weights
     float scale;            // |scale| log2 e, or log2 e where it is 0
@@ -31,6 +32,7 @@ struct Args {
     int32_t group;
     int32_t tile_rows;      // of a workgroup
     int32_t at_once;        // workgroups that run at once
+    float join;             // tokens whose time a share's sums take
     int32_t budget;         // workgroups that tiles are cut for, beside one each; 0: they are not cut
     int32_t most_items, most_slots;
     int32_t* used;          // slots that there are; behind it (int4 aligned) what each belongs to
@@ -46,7 +48,7 @@ struct Request {
 // An item: a tile of rows over a share of the tokens that they see.
 struct Item {
     Request r;
-    int32_t request, tile, share, shares, slot;   // tile < 0: there is no such item; slot of the tile's first share
+    int32_t request, tile, share, shares, slot;   // tile < 0: there is no such item; slot of the tile's first share, -1: none of the request's has one
     int32_t slots;                           // of all
 };
 
@@ -67,33 +69,62 @@ __device__ inline uint2 span_of(const Args& a, const Request& r, int32_t tile) {
     if (p0 >= (uint32_t)r.n) return make_uint2(0, 0);
     return make_uint2(a.d.window && p0 + 1 > (uint32_t)a.d.window ? p0 + 1 - a.d.window : 0, min((uint32_t)r.n, p1 + 1));
 }
-// What a request's tiles see at most, and on the average (spans grow with the tile, by steps that do not).
-__device__ inline void size_up(const Args& a, const Request& r, float* most, float* all) {
-    *most = *all = 0.0f;
-    if (!r.tiles) return;
-    const uint2 x = span_of(a, r, 0), y = span_of(a, r, r.tiles - 1);
-    const float u = (float)(x.y - x.x), v = (float)(y.y - y.x);
-    *most = fmaxf(u, v);
-    *all = (float)r.tiles * (u + v) * 0.5f;
-}
-// How long shares are: tiles of up to `whole` tokens are not cut, others into shares of `tokens`.  Tiles that are longer than 1.3 rounds' worth are cut into half
-// rounds.  Where there are fewer than three rounds of tiles, and those of a request are much alike (not as a prompt's, of which long ones and short ones make up for each other), they are
-// cut into the number n that takes the least rounds of workgroups, ceil(n N / at once) / n.
-// Where that makes more items than there are workgroups for (lengths that were not expected), none is cut.
-struct Cut {
-    float whole, tokens, alike;              // alike: tokens of a share of tiles that are much alike; 0: as others
+// A request's tiles in four parts, as those of a prompt see more and more: what the tiles of each see at most, and all of them together
+// (spans grow with the tile, by steps that do not).  No products are contracted here and below: what a launch lists the next one has to find again.
+constexpr int kParts = 4;
+struct Sizes {
+    float most[kParts], top, all;
 };
-__device__ inline Cut cut_of(const Args& a, float all, float tiles) {
-    const float kv = (float)a.d.cache.kv_heads, groups = tiles * kv;
+__device__ inline int32_t part_of(const Request& r, int q) { return r.tiles * q / kParts; }
+__device__ inline Sizes size_up(const Args& a, const Request& r) {
+#pragma clang fp contract(off)
+    Sizes s{};
+    if (!r.tiles) return s;
+    const uint2 x = span_of(a, r, 0);
+    float before = (float)(x.y - x.x);
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+        const int32_t from = part_of(r, q), to = part_of(r, q + 1);
+        if (from == to) continue;
+        const uint2 y = span_of(a, r, to - 1);
+        const float v = (float)(y.y - y.x);
+        s.most[q] = fmaxf(before, v);
+        s.top = fmaxf(s.top, s.most[q]);
+        s.all += (float)(to - from) * (before + v) * 0.5f;
+        before = v;
+    }
+    return s;
+}
+// How long shares are.  Let w be the tokens of all tiles over the workgroups that run at once, and c the tokens whose time it takes to write and
+// read a share's sums.  Shares of T tokens take about w (1 + c / T), and 0.7 T until the last are done, least at T = (1.4 w c)^(1/2); a request whose
+// longest tile is done sooner is not cut, nor are its tiles of up to 1.3 T.  (One prompt of 2000 tokens, 32 heads over 8 of 128, bf16: 76 us, cut all the
+// same 90; of 2348, 10 heads over 5 of 64, f32: cut 99 us, else 160.)  Shares under half of w make no difference to the last ones any more.
+// Where there are fewer workgroups than the budget, and tiles of a request are much alike (not as a prompt's, of which long ones and short ones make up for
+// each other), they are cut into the number n that takes the least rounds, ceil(n N / at once) (1 / n + c / tokens).
+// Where all that makes more items than there are workgroups for, shares are made longer, up to four times; then (lengths that were not expected) none is cut.
+struct Cut {
+    float whole, tokens, alike;              // tiles of up to `whole` tokens are not cut, others into shares of `tokens`; alike: of tiles much alike; 0: as others
+};
+__host__ __device__ inline Cut cut_for(float w, float join, bool few) {
     Cut c;
-    const float at_once = (float)a.at_once;
-    c.tokens = all * kv * (0.51f / at_once);
-    c.whole = 2.6f * c.tokens;
+    if (few) {
+        c.tokens = 1.02f * w;
+        c.whole = kLookedFew + 1.3f * w;
+    } else {
+        c.tokens = fmaxf((float)kLeast, fmaxf(0.51f * w, sqrtf(1.4f * w * join)));
+        c.whole = w + w * join / c.tokens;
+    }
     c.alike = 0.0f;
+    return c;
+}
+__device__ inline Cut cut_of(const Args& a, float all, float tiles) {
+    const float at_once = (float)a.at_once, groups = tiles * (float)a.d.cache.kv_heads;
+    Cut c = cut_for(all * (float)a.d.cache.kv_heads / at_once, a.join, a.tile_rows == kRows);
     if (groups < (float)a.budget) {
+        const float join = a.join * tiles / all;
         float best = ceilf(groups / at_once), n = 1.0f;
         for (float k = 2.0f; k * groups <= (float)a.budget && k <= 64.0f; k += 1.0f) {
-            const float rounds = ceilf(k * groups / at_once) * __builtin_amdgcn_rcpf(k);
+            const float rounds = ceilf(k * groups / at_once) * (__builtin_amdgcn_rcpf(k) + join);
             if (rounds < 0.95f * best) {
                 best = rounds;
                 n = k;
@@ -103,17 +134,51 @@ __device__ inline Cut cut_of(const Args& a, float all, float tiles) {
     }
     return c;
 }
-__device__ inline int32_t shares_of(const Args& a, const Cut& c, float most, float all, int32_t tiles) {
-    const bool few = a.tile_rows == kRows, alike = c.alike > 0.0f && most * (float)tiles < 1.5f * all;
-    if (most <= fmaxf((float)(few ? kCutFew : kCut), alike ? c.alike : c.whole)) return 1;
-    return (int32_t)ceilf(most / fmaxf((float)(few ? kLeastFew : kLeast), alike ? c.alike : c.tokens));
+// Into how many shares the tiles of each part are cut.
+struct Shares {
+    int32_t n[kParts];
+    bool any, first;        // shares that are longer than half a round come first, so that none of them begins when the others are nearly done
+};
+__device__ inline Shares shares_of(const Args& a, const Cut& c, const Sizes& s, int32_t tiles) {
+#pragma clang fp contract(off)
+    const bool few = a.tile_rows == kRows, alike = c.alike > 0.0f && s.top * (float)tiles < 1.5f * s.all;
+    const float least = (float)(few ? kLeastFew : kLeast), looked = (float)(few ? kLookedFew : kLooked);
+    const float each = fmaxf(least, alike ? c.alike : c.tokens), whole = fmaxf(1.5f * least, 1.3f * (alike ? c.alike : c.tokens));
+    const bool cut = s.top > fmaxf(looked, alike ? c.alike : c.whole);
+    Shares x;
+    x.any = x.first = false;
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) {
+        x.n[q] = !cut || s.most[q] <= whole ? 1 : (int32_t)ceilf(s.most[q] / each);
+        x.any |= x.n[q] > 1;
+        x.first |= s.most[q] > 0.5f * c.tokens * (float)x.n[q];
+    }
+    return x;
 }
-// Shares that are longer than half a round come first, so that none of them begins when the others are nearly done.
-__device__ inline bool comes_first(const Cut& c, float most, int32_t shares) { return most > c.tokens * (float)shares; }
+__device__ inline Shares not_cut() {
+    Shares x;
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) x.n[q] = 1;
+    x.any = false;
+    x.first = true;
+    return x;
+}
+__device__ inline void cut_less(Cut& c) {
+    c.whole *= 1.5f;
+    c.tokens *= 1.5f;
+    c.alike *= 1.5f;
+}
+constexpr int kTries = 5;
 
 // Items and slots are counted up to 2^32 - 1: more there are only where starts do not ascend, and then nothing may run over.
 __device__ inline uint32_t plus(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 __device__ inline uint32_t product(int32_t tiles, int32_t shares) { return (uint32_t)min((uint64_t)(uint32_t)tiles * (uint32_t)shares, (uint64_t)UINT32_MAX); }
+__device__ inline uint32_t items_of(const Request& r, const Shares& x) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) n = plus(n, product(part_of(r, q + 1) - part_of(r, q), x.n[q]));
+    return n;
+}
 // Prefix sums over the wavefront without the lane's own value; *all: with all of them.
 template <int CONTROL, int ROWS>
 __device__ inline uint32_t moved(uint32_t x) { return __builtin_amdgcn_update_dpp(0, x, CONTROL, ROWS, 0xF, true); }
@@ -135,61 +200,70 @@ __device__ inline float sum_of(float v) {
 }
 
 // Up to kFewRequests requests each wavefront finds its item by itself, a request a lane; more are listed by a launch ahead.
-constexpr int32_t kFewRequests = 64, kListHead = 2;
+constexpr int32_t kFewRequests = 64, kListHead = 6;           // (items, slots, the cut, whether there is one)
 __device__ inline Item find_item(const Args& a, int32_t id) {
     Item it;
     it.tile = -1;
     int32_t local;
+    Shares shares = not_cut();
     if (a.list) {
         if (id >= a.list[0]) return it;
         it.request = a.list[kListHead + id];
-        const int4 info = a.info[it.request];
+        const int2 info = a.info[it.request];
         it.r = request_of(a, it.request);
         local = id - info.x;
-        it.shares = info.y;
-        it.slot = info.z;
+        if (a.list[5]) shares = shares_of(a, {__int_as_float(a.list[2]), __int_as_float(a.list[3]), __int_as_float(a.list[4])}, size_up(a, it.r), it.r.tiles);
+        it.slot = info.y;
         it.slots = a.list[1];
     } else if (a.d.requests == 1) {
         it.request = 0;
         it.r = request_of(a, 0);
-        it.shares = 1;
+        uint32_t items = (uint32_t)it.r.tiles;
         if (a.budget) {
-            float most, all;
-            size_up(a, it.r, &most, &all);
-            it.shares = __builtin_amdgcn_readfirstlane(shares_of(a, cut_of(a, all, (float)it.r.tiles), most, all, it.r.tiles));
-        }
-        uint32_t items = product(it.r.tiles, it.shares);
-        if (items > (uint32_t)a.most_items) {
-            it.shares = 1;
-            items = (uint32_t)it.r.tiles;
+            const Sizes sizes = size_up(a, it.r);
+            Cut cut = cut_of(a, sizes.all, (float)it.r.tiles);
+            for (int tries = 1;; ++tries) {
+                shares = shares_of(a, cut, sizes, it.r.tiles);
+                items = items_of(it.r, shares);
+                if (items <= (uint32_t)a.most_items) break;
+                if (tries == kTries) {
+                    shares = not_cut();
+                    items = (uint32_t)it.r.tiles;
+                    break;
+                }
+                cut_less(cut);
+            }
         }
         if ((uint32_t)id >= items) return it;
         it.slot = 0;
-        it.slots = it.shares > 1 ? (int32_t)min(items, 1u << 30) : 0;
+        it.slots = shares.any ? (int32_t)min(items, 1u << 30) : 0;
         local = id;
     } else {
         const int lane = threadIdx.x & 63;
         Request r{};
         if (lane < a.d.requests) r = request_of(a, lane);
-        int32_t shares = 1;
-        bool first = true;
+        uint32_t firsts, others = 0, all_slots = 0, slot = 0, mine = (uint32_t)r.tiles, at;
         if (a.budget) {
-            float most, all;
-            size_up(a, r, &most, &all);
-            const Cut cut = cut_of(a, sum_of(all), sum_of((float)r.tiles));
-            shares = shares_of(a, cut, most, all, r.tiles);
-            first = comes_first(cut, most, shares);
-        }
-        uint32_t firsts, others = 0, all_slots = 0, slot = 0, mine = product(r.tiles, shares), at = before_me(first ? mine : 0, &firsts);
-        if (a.budget) {
-            const uint32_t x = before_me(first ? 0 : mine, &others);
-            at = first ? at : plus(firsts, x);
-            if (plus(firsts, others) > (uint32_t)a.most_items) {
-                shares = 1;
-                mine = (uint32_t)r.tiles;
-                at = before_me(mine, &firsts);
+            const Sizes sizes = size_up(a, r);
+            Cut cut = cut_of(a, sum_of(sizes.all), sum_of((float)r.tiles));
+            for (int tries = 1;; ++tries) {
+                shares = shares_of(a, cut, sizes, r.tiles);
+                mine = items_of(r, shares);
+                at = before_me(shares.first ? mine : 0, &firsts);
+                const uint32_t x = before_me(shares.first ? 0 : mine, &others);
+                at = shares.first ? at : plus(firsts, x);
+                if (plus(firsts, others) <= (uint32_t)a.most_items) break;
+                if (tries == kTries) {
+                    shares = not_cut();
+                    mine = (uint32_t)r.tiles;
+                    at = before_me(mine, &firsts);
+                    break;
+                }
+                cut_less(cut);
             }
-            slot = before_me(shares > 1 ? mine : 0, &all_slots);
+            slot = before_me(shares.any ? mine : 0, &all_slots);
+        } else {
+            at = before_me(mine, &firsts);
         }
         const uint64_t who = __builtin_amdgcn_ballot_w64((uint32_t)id >= at && (uint32_t)id - at < mine);
         if (!who) return it;
@@ -200,16 +274,33 @@ __device__ inline Item find_item(const Args& a, int32_t id) {
         it.r.cached = __builtin_amdgcn_readlane(r.cached, l);
         it.r.n = __builtin_amdgcn_readlane(r.n, l);
         it.r.tiles = __builtin_amdgcn_readlane(r.tiles, l);
-        it.shares = __builtin_amdgcn_readlane(shares, l);
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) shares.n[q] = __builtin_amdgcn_readlane(shares.n[q], l);
+        shares.any = __builtin_amdgcn_readlane((int32_t)shares.any, l);
         it.slot = (int32_t)min(__builtin_amdgcn_readlane(slot, l), 1u << 30);
         it.slots = (int32_t)min(all_slots, 1u << 30);
         local = id - (int32_t)__builtin_amdgcn_readlane(at, l);
     }
     // the last tiles, which see most, first
-    const int32_t k = local / it.shares;
-    it.share = local - k * it.shares;
-    it.tile = it.r.tiles - 1 - k;
-    it.slot += local - it.share;
+    int32_t before = 0, from = 0, to = 0;
+    it.shares = 1;
+#pragma unroll
+    for (int q = kParts - 1; q >= 0; --q) {
+        const int32_t f = part_of(it.r, q), t = part_of(it.r, q + 1), n = (t - f) * shares.n[q];
+        if (local >= before && local - before < n) {
+            from = before;
+            to = t;
+            it.shares = shares.n[q];
+        }
+        before += n;
+    }
+    const int32_t k = (local - from) / it.shares;
+    it.share = local - from - k * it.shares;
+    it.tile = to - 1 - k;
+    it.slot = __builtin_amdgcn_readfirstlane(shares.any ? it.slot + local - it.share : -1);
+    it.shares = __builtin_amdgcn_readfirstlane(it.shares);
+    it.share = __builtin_amdgcn_readfirstlane(it.share);
+    it.tile = __builtin_amdgcn_readfirstlane(it.tile);
     return it;
 }
 
@@ -225,9 +316,7 @@ __global__ void __launch_bounds__(kListThreads) list_items(Args a) {
         float sum = 0.0f, tiles = 0.0f;
         for (int32_t i = lo; i < hi; ++i) {
             const Request r = request_of(a, i);
-            float most, all;
-            size_up(a, r, &most, &all);
-            sum += all;
+            sum += size_up(a, r).all;
             tiles += (float)r.tiles;
         }
         sum = sum_of(sum);
@@ -241,28 +330,21 @@ __global__ void __launch_bounds__(kListThreads) list_items(Args a) {
         }
         cut = cut_of(a, sum, tiles);
     }
-    bool whole = !a.budget;
-    // shares, tiles, whether it comes first
-    auto shares_and_tiles = [&](int32_t i) {
+    bool is_cut = a.budget != 0;
+    auto shares_and_items = [&](int32_t i, uint32_t* mine) {
         const Request r = request_of(a, i);
-        int32_t shares = 1, first = 1;
-        if (!whole) {
-            float most, all;
-            size_up(a, r, &most, &all);
-            shares = shares_of(a, cut, most, all, r.tiles);
-            first = comes_first(cut, most, shares);
-        }
-        return make_int3(shares, r.tiles, first);
+        const Shares x = is_cut ? shares_of(a, cut, size_up(a, r), r.tiles) : not_cut();
+        *mine = items_of(r, x);
+        return x;
     };
     uint32_t all, all_slots, item, later, slot;            // later: where the next request that does not come first has its items
-    auto count = [&]() {
-        uint32_t items = 0, others = 0, slots = 0, of_wave, others_of_wave, slots_of_wave;
+    for (int tries = 1;; ++tries) {
+        uint32_t items = 0, others = 0, slots = 0, of_wave, others_of_wave, slots_of_wave, mine;
         for (int32_t i = lo; i < hi; ++i) {
-            const int3 x = shares_and_tiles(i);
-            const uint32_t mine = product(x.x, x.y);
-            if (x.z) items = plus(items, mine);
+            const Shares x = shares_and_items(i, &mine);
+            if (x.first) items = plus(items, mine);
             else others = plus(others, mine);
-            if (x.x > 1) slots = plus(slots, mine);
+            if (x.any) slots = plus(slots, mine);
         }
         item = before_me(items, &of_wave);
         later = before_me(others, &others_of_wave);
@@ -283,24 +365,26 @@ __global__ void __launch_bounds__(kListThreads) list_items(Args a) {
             all_slots = plus(all_slots, counts[w].z);
         }
         later = plus(later, firsts);
-    };
-    count();
-    if (!whole && all > (uint32_t)a.most_items) {
-        whole = true;
-        count();
+        if (!is_cut || all <= (uint32_t)a.most_items) break;
+        if (tries == kTries) is_cut = false;
+        else cut_less(cut);
     }
     for (int32_t i = lo; i < hi; ++i) {
-        const int3 x = shares_and_tiles(i);
-        const uint32_t mine = product(x.x, x.y);
-        uint32_t& at = x.z ? item : later;
-        a.info[i] = make_int4((int32_t)min(at, 1u << 30), x.x, (int32_t)min(slot, 1u << 30), 0);
+        uint32_t mine;
+        const Shares x = shares_and_items(i, &mine);
+        uint32_t& at = x.first ? item : later;
+        a.info[i] = make_int2((int32_t)min(at, 1u << 30), (int32_t)min(slot, 1u << 30));
         for (uint32_t k = at; k < min(plus(at, mine), (uint32_t)a.most_items); ++k) a.list[kListHead + k] = i;
         at = plus(at, mine);
-        if (x.x > 1) slot = plus(slot, mine);
+        if (x.any) slot = plus(slot, mine);
     }
     if (tid == 0) {
         a.list[0] = (int32_t)min(all, (uint32_t)a.most_items);
         a.list[1] = (int32_t)min(all_slots, 1u << 30);
+        a.list[2] = __float_as_int(cut.whole);
+        a.list[3] = __float_as_int(cut.tokens);
+        a.list[4] = __float_as_int(cut.alike);
+        a.list[5] = is_cut;
     }
 }
 
@@ -434,7 +518,9 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
     const int32_t id = (int32_t)(blockIdx.x / (uint32_t)d.cache.kv_heads), kvh = (int32_t)(blockIdx.x - (uint32_t)id * (uint32_t)d.cache.kv_heads);
     const Item it = find_item(a, id);
     if (a.budget && kvh == 0 && threadIdx.x == 0) {
-        if (it.tile >= 0 && it.shares > 1 && it.slot + it.share < a.most_slots) a.jobs[it.slot + it.share] = make_int4(it.request, it.tile, it.share, it.shares);
+        // (no shares: tiles that are not cut, of requests that have others that are)
+        if (it.tile >= 0 && it.slot >= 0 && it.slot + it.share < a.most_slots)
+            a.jobs[it.slot + it.share] = make_int4(it.request, it.tile, it.share, it.shares > 1 ? it.shares : 0);
         if (id == 0) *a.used = it.tile < 0 ? 0 : min(it.slots, a.most_slots);      // (without a first item there are none)
     }
     if (it.tile < 0) return;
@@ -1132,38 +1218,40 @@ constexpr int kThreads = 1024;               // of the join
 template <class Q>
 __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
     const reef_chunk_attention_desc& d = a.d;
-    const int32_t id = (int32_t)(blockIdx.x / (uint32_t)d.cache.kv_heads), kvh = (int32_t)(blockIdx.x - (uint32_t)id * (uint32_t)d.cache.kv_heads);
-    if (id >= *a.used) return;
-    const int4 job = a.jobs[id];
-    // (where starts do not ascend there may be none)
-    if ((uint32_t)job.x >= (uint32_t)d.requests || job.z < 0 || job.z >= job.w || job.z > id) return;
-    const Request r = request_of(a, job.x);
     const int D = d.cache.head_dim, quads = D / 4;
-    if ((uint32_t)job.y >= (uint32_t)r.tiles) return;
-    const int32_t rows = min(a.tile_rows, r.added * a.group - job.y * a.tile_rows), slot = id - job.z, shares = min(job.w, a.most_slots - slot);
-    const int32_t from = (int32_t)((int64_t)rows * quads * job.z / job.w), to = (int32_t)((int64_t)rows * quads * (job.z + 1) / job.w);
-    const int64_t step = (int64_t)d.cache.kv_heads * a.tile_rows;
-    for (int32_t x = from + (int32_t)threadIdx.x; x < to; x += kThreads) {
-        const int32_t i = x / quads, dim = (x - i * quads) * 4;
-        const int64_t at = ((int64_t)slot * d.cache.kv_heads + kvh) * a.tile_rows + i;
-        float R = -INFINITY, l = 0.0f;
-        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+    const uint32_t kv_heads = (uint32_t)d.cache.kv_heads, works = (uint32_t)*a.used * kv_heads;
+    for (uint32_t work = blockIdx.x; work < works; work += gridDim.x) {
+        const int32_t id = (int32_t)(work / kv_heads), kvh = (int32_t)(work - (uint32_t)id * kv_heads);
+        const int4 job = a.jobs[id];
+        // (tiles that are not cut; where starts do not ascend there may be none)
+        if ((uint32_t)job.x >= (uint32_t)d.requests || job.z < 0 || job.z >= job.w || job.z > id) continue;
+        const Request r = request_of(a, job.x);
+        if ((uint32_t)job.y >= (uint32_t)r.tiles) continue;
+        const int32_t rows = min(a.tile_rows, r.added * a.group - job.y * a.tile_rows), slot = id - job.z, shares = min(job.w, a.most_slots - slot);
+        const int32_t from = (int32_t)((int64_t)rows * quads * job.z / job.w), to = (int32_t)((int64_t)rows * quads * (job.z + 1) / job.w);
+        const int64_t step = (int64_t)d.cache.kv_heads * a.tile_rows;
+        for (int32_t x = from + (int32_t)threadIdx.x; x < to; x += kThreads) {
+            const int32_t i = x / quads, dim = (x - i * quads) * 4;
+            const int64_t at = ((int64_t)slot * d.cache.kv_heads + kvh) * a.tile_rows + i;
+            float R = -INFINITY, l = 0.0f;
+            f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
-        for (int32_t s = 0; s < shares; ++s) {
-            const float2 stat = a.stats[at + s * step];
-            const f32x4 mine = *(const f32x4*)(a.parts + (at + s * step) * D + dim);
-            const float next = fmaxf(R, stat.x), base = next == -INFINITY ? 0.0f : next;
-            const float f = __builtin_amdgcn_exp2f(R - base), g = __builtin_amdgcn_exp2f(stat.x - base);
-            R = next;
-            l = l * f + stat.y * g;
-            o = o * f + mine * g;
+            for (int32_t s = 0; s < shares; ++s) {
+                const float2 stat = a.stats[at + s * step];
+                const f32x4 mine = *(const f32x4*)(a.parts + (at + s * step) * D + dim);
+                const float next = fmaxf(R, stat.x), base = next == -INFINITY ? 0.0f : next;
+                const float f = __builtin_amdgcn_exp2f(R - base), g = __builtin_amdgcn_exp2f(stat.x - base);
+                R = next;
+                l = l * f + stat.y * g;
+                o = o * f + mine * g;
+            }
+            const uint32_t row = (uint32_t)(job.y * a.tile_rows + i), token = divided(row, a.by_group);
+            const int32_t head = kvh * a.group + (int32_t)(row - token * a.by_group.by);
+            const int64_t out_row = (int64_t)r.first + token;
+            const float f = l == 0.0f ? 0.0f : 1.0f / l;
+            put4((Q*)a.out + out_row * d.out_stride + head * d.out_head_stride + dim, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
+            if (dim == 0 && a.lse) a.lse[out_row * d.heads + head] = l == 0.0f ? -INFINITY : (R + __log2f(l)) * kLn2;
         }
-        const uint32_t row = (uint32_t)(job.y * a.tile_rows + i), token = divided(row, a.by_group);
-        const int32_t head = kvh * a.group + (int32_t)(row - token * a.by_group.by);
-        const int64_t out_row = (int64_t)r.first + token;
-        const float f = l == 0.0f ? 0.0f : 1.0f / l;
-        put4((Q*)a.out + out_row * d.out_stride + head * d.out_head_stride + dim, o[0] * f, o[1] * f, o[2] * f, o[3] * f);
-        if (dim == 0 && a.lse) a.lse[out_row * d.heads + head] = l == 0.0f ? -INFINITY : (R + __log2f(l)) * kLn2;
     }
 }
 
@@ -1189,13 +1277,13 @@ int check(const char* what, const reef_chunk_attention_desc* d) {
 
 // What the host asks of a shape.
 struct Waves {
-    int few, each, at_once;
+    int few, each, at_once, products;
 };
 template <class Q, class C>
 Waves waves_of(int dim) {
     auto of = [](auto dp) {
         using Sh = Shape<Q, C, decltype(dp)::value>;
-        return Waves{Sh::kFewWaves, Sh::kWaves, Sh::kPair ? 2 * kCus : kCus};
+        return Waves{Sh::kFewWaves, Sh::kWaves, Sh::kPair ? 2 * kCus : kCus, Sh::kTermsC == 3 ? 6 : Sh::kTermsQ};
     };
     return dim <= 64 ? of(std::integral_constant<int, 64>()) : dim <= 96 ? of(std::integral_constant<int, 96>()) : dim <= 128 ? of(std::integral_constant<int, 128>())
          : dim <= 192 ? of(std::integral_constant<int, 192>()) : of(std::integral_constant<int, 256>());
@@ -1209,6 +1297,7 @@ Waves waves_of(const reef_chunk_attention_desc& d) {
 // How a call is laid out.
 struct Plan {
     int32_t tile_rows, at_once, budget;
+    float join;
     bool few;               // tiles of 32 rows in all
     int64_t items, slots, groups;      // groups: workgroups
     size_t info_bytes, list_bytes, jobs_bytes, stats_bytes, bytes;
@@ -1222,15 +1311,24 @@ Plan plan_of(const reef_chunk_attention_desc& d) {
     p.few = rows <= (int64_t)kRows * d.requests && waves.few;
     p.tile_rows = p.few ? kRows : waves.each * kRows;
     p.at_once = p.few ? kCus : waves.at_once;
+    p.join = p.few ? 0.0f : kJoin / (float)waves.products;
     int64_t longest = (int64_t)d.max_blocks * d.cache.block_size;
     if (d.longest && d.longest < longest) longest = d.longest;
     if (d.window) longest = std::min(longest, (int64_t)d.window + p.tile_rows / group);
     p.items = rows / p.tile_rows + d.requests;
-    const int64_t cut = p.few ? kCutFew : kCut, least = p.few ? kLeastFew : kLeast;
-    if (longest > cut) {
+    const int64_t least = p.few ? kLeastFew : kLeast;
+    // tokens that a workgroup has at most where all are the longest; of one request the cut is known
+    const int64_t most = p.items * kv * longest / p.at_once;
+    bool whole = false;
+    if (d.requests == 1) {
+        const float tokens = (float)std::min<int64_t>(d.tokens, longest);
+        const Cut c = cut_for((float)most * (1.0f - 0.5f * tokens / (float)longest), p.join, p.few);
+        whole = (float)longest <= c.whole + 0.7f * c.tokens + 0.5f * p.join;
+    }
+    if (longest > (p.few ? kLookedFew : kLooked) && !whole) {
         // Workgroups that find no item take 2 us a round for their look: there are no more than are likely to have one.
         const int64_t shares = (longest + least - 1) / least, tiles = p.items;
-        p.budget = tiles * kv <= p.at_once / 2 ? p.at_once : 3 * p.at_once;
+        p.budget = p.at_once * (tiles * kv <= p.at_once / 2 ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(3, most * waves.products / 1000)));
         p.items = std::min(tiles * shares, tiles + (p.budget + kv - 1) / kv);
         p.slots = p.items;
         p.jobs_bytes = 16 * (size_t)(1 + p.slots);
@@ -1238,7 +1336,7 @@ Plan plan_of(const reef_chunk_attention_desc& d) {
     }
     p.groups = p.items * kv;
     if (d.requests > kFewRequests) {
-        p.info_bytes = (size_t)d.requests * 16;
+        p.info_bytes = ((size_t)d.requests * 8 + 15) / 16 * 16;
         p.list_bytes = ((size_t)(kListHead + p.items) * 4 + 15) / 16 * 16;
     }
     p.bytes = p.info_bytes + p.list_bytes + p.jobs_bytes + p.stats_bytes + (size_t)p.slots * kv * p.tile_rows * d.cache.head_dim * 4;
@@ -1264,7 +1362,7 @@ int run(const char* what, const Args& a, const Plan& p, void* stream) {
                    : D <= 192 ? run_heads<Q, C, 192>(what, a, p, groups, stream)
                               : run_heads<Q, C, 256>(what, a, p, groups, stream);
     if (rc || !p.budget) return rc;
-    return launch(what, join_shares<Q>, dim3((unsigned)(p.slots * a.d.cache.kv_heads)), dim3(kThreads), a, stream);
+    return launch(what, join_shares<Q>, dim3((unsigned)std::min<int64_t>(p.slots * a.d.cache.kv_heads, 2 * kCus)), dim3(kThreads), a, stream);
 }
 
 }  // namespace
@@ -1284,16 +1382,16 @@ extern "C" int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, cons
         !aligned(lse, 4))
         return refuse(what, "null or unaligned argument");
     const Plan p = plan_of(*d);
-    // (2^32 threads are refused by the launch, which may be the call's last one)
-    if (p.groups >= 1ll << (p.budget ? 22 : 23)) return refuse(what, "%lld workgroups are too many", (long long)p.groups);
+    // (2^32 threads are refused by the launch, which may be the call's second one)
+    if (p.groups >= 1ll << 23) return refuse(what, "%lld workgroups are too many", (long long)p.groups);
     if (p.bytes && (!rows16(workspace) || workspace_bytes < (int64_t)p.bytes))
         return refuse(what, "a workspace of %zu bytes on 16 is needed, %lld are given", p.bytes, (long long)workspace_bytes);
     char* const w = (char*)workspace;
     const size_t list = p.info_bytes, jobs = list + p.list_bytes, stats = jobs + p.jobs_bytes, parts = stats + p.stats_bytes;
     const int32_t group = d->heads / d->cache.kv_heads;
-    const Args a{*d, query, key_cache, value_cache, table, starts, cached, lengths, out, lse, (int4*)w, p.list_bytes ? (int32_t*)(w + list) : nullptr, (float*)(w + parts),
+    const Args a{*d, query, key_cache, value_cache, table, starts, cached, lengths, out, lse, (int2*)w, p.list_bytes ? (int32_t*)(w + list) : nullptr, (float*)(w + parts),
                  (float2*)(w + stats), d->scale == 0.0f ? kLog2e : std::fabs(d->scale) * kLog2e, d->scale < 0.0f ? (d->type == REEF_TYPE_F32 ? 0x80000000u : 0x80008000u) : 0u,
-                 d->scale == 0.0f, group, p.tile_rows, p.at_once, p.budget, (int32_t)p.items, (int32_t)p.slots, (int32_t*)(w + jobs), (int4*)(w + jobs) + 1,
+                 d->scale == 0.0f, group, p.tile_rows, p.at_once, p.join, p.budget, (int32_t)p.items, (int32_t)p.slots, (int32_t*)(w + jobs), (int4*)(w + jobs) + 1,
                  divider((uint32_t)d->cache.block_size), divider((uint32_t)group)};
     switch (d->type * 4 + d->cache.type) {
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, p, stream);
