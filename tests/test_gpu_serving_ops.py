@@ -281,6 +281,207 @@ def test_chunk_large(kind, cache, cached, new):
     run_chunk(kind, cache, "thd", 16, 2, 4, 128, [cached], [new], longest=cached + new, seed=new, extra=0)
 
 
+@pytest.mark.parametrize("kind,cache", PAIRS)
+@pytest.mark.parametrize("cached,added,window", [([15], [1300], 0), ([0, 900], [1100, 700], 0), ([3, 0, 2500, 40], [900, 1, 300, 1000], 1500)])
+def test_chunk_prompts_whose_tiles_see_more_and_more(kind, cache, cached, added, window):
+    """Few tiles over many tokens: the late ones are cut, the early ones less or not at all."""
+    run_chunk(kind, cache, "htd", 64, 1, 2, 64, cached, added, longest=max(c + a for c, a in zip(cached, added)), window=window, seed=len(cached))
+    if kind != F32:
+        run_chunk(kind, cache, "thd", 16, 1, 1, 104, cached, added, window=window, seed=7)
+
+
+def test_chunk_many_prompts_and_long_sequences():
+    """More than 64 requests, of which some are cut, some in parts, most not."""
+    rng = np.random.default_rng(2)
+    cached, added = rng.integers(0, 100, 90), rng.integers(1, 40, 90)
+    cached[[3, 50, 77, 80]], added[[3, 50, 77, 80]] = [0, 4000, 700, 0], [1200, 100, 900, 0]
+    for longest in (0, 4100, 50):
+        run_chunk(BF16, BF16, "thd", 16, 1, 2, 64, cached, added, longest=longest, seed=3)
+    run_chunk(F32, F16, "thd", 16, 2, 1, 128, cached, added, longest=4100, seed=4, refused=(77, 5))
+
+
+def test_pools_past_32_bits():
+    """Blocks that start behind 2^32 elements and 2^33 bytes: attention, a fork into one, a compaction out of them."""
+    bs, kv, dim, blocks = 16, 8, 128, 264 * 1024
+    lay = B.CacheLayout(F16, blocks, bs, kv, dim, bs * kv * dim, kv * dim, dim)
+    pools = [B.DeviceBuffer(blocks * bs * kv * dim * 2) for _ in range(2)]
+    rng = np.random.default_rng(1)
+    pick = np.array([blocks - 1, 131072, 131071, 262144, 0, 262143])
+    used = 16 * len(pick) - 3
+    rows = rng.standard_normal((used, 2, kv, dim)).astype(np.float16)
+    slots = [pick[t // bs] * bs + t % bs for t in range(used)]
+    dev, row = up(rows), 2 * kv * dim
+    ok(B.ops_cache_append(B.CacheAppendDesc(lay, F16, used, row, dim, row, dim), dev.ptr.value, dev.ptr.value + kv * dim * 2, ints(slots), *pools))
+
+    def attend(table, new):
+        q = rng.standard_normal((new, 16, dim)).astype(np.float16)
+        d = B.ChunkAttentionDesc(lay, F16, 1, 16, new, len(pick), len(pick), used, 0, 0.1, 16 * dim, dim, 16 * dim, dim)
+        out = B.DeviceBuffer(new * 16 * dim * 2)
+        ok(B.ops_chunk_attention(d, up(q), *pools, table, ints([0, new]), ints([used - new]), ints([used]), out, None, work_of(B.ops_chunk_attention_workspace(d))))
+        want, _, tol, _ = S.chunk(q.astype(np.float64), rows[:, 0].transpose(1, 0, 2).astype(np.float64), rows[:, 1].transpose(1, 0, 2).astype(np.float64), used - new, used, 0.1, 0,
+                                  F16, F16)
+        got = out.to_array(np.float16).reshape(new, 16, dim).astype(np.float64)
+        assert (np.abs(got - want) <= tol + HALF[F16] * np.abs(want) + 2.0 ** -25).all()
+
+    attend(ints(pick), 3)
+    attend(ints(pick), 70)
+    table, lengths, counts = ints(np.stack([pick, np.full(6, -1)])), ints([used, 0]), ints([0, 0])
+    ok(B.ops_cache_fork(B.CacheForkDesc(lay, 1, 2, 6, 6, 1, 1, 0), ints([0]), ints([1]), ints([used]), ints([blocks - 2]), table, lengths, counts, *pools))
+    assert table.to_array(np.int32)[6:].tolist() == pick[:5].tolist() + [blocks - 2] and counts.to_array(np.int32).tolist() == [1, 0]
+    attend(ints(table.to_array(np.int32)[6:]), 3)
+    cm = B.CacheCompactDesc(lay, 2, 6, 6, 6, 1, 0)
+    packed = ints(np.full((2, 6), -1))
+    ok(B.ops_cache_compact(cm, table, lengths, packed, counts, *pools, work_of(B.ops_cache_compact_workspace(cm))))
+    assert counts.to_array(np.int32).tolist() == [7, 6] and sorted(set(packed.to_array(np.int32).tolist())) == list(range(7))
+    for half in np.split(packed.to_array(np.int32), 2):
+        attend(ints(half), 3)
+
+
+def test_calls_on_two_streams_do_not_disturb_each_other():
+    """The calls of two servers side by side, each with workspaces of its own, many times over: the bits of a call alone."""
+    rng = np.random.default_rng(1)
+    jobs = []
+    for s in range(2):
+        pools = Pools(BF16, 12000, 16, 2, 64, seed=s)
+        att = B.ChunkAttentionDesc(pools.layout, BF16, 3, 8, 420, 260, 260, 4100, 0, 0.12, 8 * 64, 64, 8 * 64, 64)
+        sc, sw = B.TokenScoresDesc(BF16, 3, 128257, 20, 128257), B.BlockSweepDesc(3, 12000, 16, 260, 260)
+        stream = ctypes.c_void_p()
+        hip("hipStreamCreateWithFlags", ctypes.byref(stream), 1)
+        jobs.append(dict(stream=stream, pools=pools, att=att, sc=sc, sw=sw, q=up(R.encode(rng.standard_normal((420, 8, 64)), BF16)), table=ints(rng.permutation(12000)[:780]),
+                         starts=ints([0, 300, 301, 420]), cached=ints([700, 4000, 0]), lengths=ints([1000, 4001, 119]), out=B.DeviceBuffer(420 * 8 * 64 * 2),
+                         logits=up(R.encode(rng.standard_normal((3, 128257)), BF16)), tokens=ints([5, 60000, -1]), scores=B.DeviceBuffer(12), ranks=B.DeviceBuffer(12),
+                         entropy=B.DeviceBuffer(12), top=B.DeviceBuffer(240), tops=B.DeviceBuffer(240), uses=B.DeviceBuffer(48000), free=ints(np.zeros(12000)), counts=B.DeviceBuffer(12),
+                         w=[work_of(n) for n in (B.ops_chunk_attention_workspace(att), B.ops_token_scores_workspace(sc), B.ops_block_sweep_workspace(sw))]))
+
+    def go(j):
+        ok(B.ops_chunk_attention(j["att"], j["q"], *j["pools"].dev, j["table"], j["starts"], j["cached"], j["lengths"], j["out"], None, j["w"][0], j["stream"]))
+        ok(B.ops_token_scores(j["sc"], j["logits"], j["tokens"], j["scores"], j["ranks"], j["entropy"], j["top"], j["tops"], j["w"][1], j["stream"]))
+        ok(B.ops_block_sweep(j["sw"], j["table"], j["lengths"], j["uses"], j["free"], j["counts"], j["w"][2], j["stream"]))
+
+    def result(j):
+        hip("hipStreamSynchronize", j["stream"])
+        return [j[k].to_array(np.uint16) for k in ("out", "scores", "ranks", "entropy", "top", "tops", "uses", "free", "counts")]
+
+    assert all(w is not None for j in jobs for w in j["w"])
+    want = []
+    for j in jobs:
+        go(j)
+        want.append(result(j))
+    for _ in range(8):
+        for j in jobs:
+            for k in ("out", "scores", "top"):
+                j[k].fill(0)
+        B.lib().reef_hal_device_sync()
+        for _ in range(15):
+            for j in jobs:
+                go(j)
+        for j, w in zip(jobs, want):
+            for a, b in zip(result(j), w):
+                np.testing.assert_array_equal(a, b)
+    for j in jobs:
+        hip("hipStreamDestroy", j["stream"])
+
+
+SERVING = """
+heads, top, V = 4, 5, 1000
+table, starts, cached, lengths = ints(3, 1, 7, 9).view(2, 2), ints(0, 2, 5), ints(20, 0), ints(22, 3)
+pools = [torch.randn(10, 16, 2, 64, **dev).bfloat16() for _ in range(2)]
+q, out, lse = torch.randn(5, heads, 64, **dev).bfloat16(), torch.zeros(5, heads, 64, dtype=torch.bfloat16, **dev), torch.zeros(5, heads, **dev)
+att = B.ChunkAttentionDesc(lay, 2, 2, heads, 5, 2, 2, 0, 0, 0.125, 256, 64, 256, 64)
+attend = [q, *pools, table, starts, cached, lengths, out, lse, None]
+sc = B.TokenScoresDesc(2, 3, V, top, V)
+logits, tokens = torch.randn(3, V, **dev).bfloat16(), ints(1, 2, 999)
+scores, ranks, entropy, best, bests = torch.zeros(3, **dev), ints(0, 0, 0), torch.zeros(3, **dev), ints(*[0] * 15), torch.zeros(15, **dev)
+score = [logits, tokens, scores, ranks, entropy, best, bests, None]
+sw = B.BlockSweepDesc(2, 10, 16, 2, 2)
+uses, free, counts = ints(*[0] * 10), ints(*[0] * 10), ints(0, 0, 0)
+sweep = [table, lengths, uses, free, counts, None]
+fk = B.CacheForkDesc(lay, 1, 2, 2, 2, 2, 1, 0)
+fork = [ints(0), ints(1), ints(18), ints(5, 6), table.clone(), lengths.clone(), ints(0, 0), *pools]
+cm = B.CacheCompactDesc(lay, 2, 2, 2, 2, 1, 0)
+compact = [table, lengths, torch.zeros_like(table), ints(0, 0), *pools, torch.empty(B.ops_cache_compact_workspace(cm), dtype=torch.uint8, **dev)]
+
+def plain_attention():
+    want = torch.zeros(5, heads, 64)
+    k, v = ([p[table[i].long()].reshape(32, 2, 64).float().cpu().repeat_interleave(2, 1) for i in range(2)] for p in pools)
+    for i in range(2):
+        for n, r in enumerate(range(int(starts[i]), int(starts[i + 1]))):
+            e = int(cached[i]) + n + 1
+            for h in range(heads):
+                w = (k[i][:e, h] @ q[r, h].float().cpu() * 0.125).softmax(0)
+                want[r, h] = w @ v[i][:e, h]
+    return want
+"""
+
+
+def test_tensors_of_another_type_or_layout_are_refused():
+    in_a_process(SERVING + """
+def no(f, *args):
+    try:
+        f(*args)
+    except TypeError as e:
+        assert "operand" in str(e), e
+    else:
+        raise SystemExit("taken: %s" % (args,))
+
+wide = torch.zeros(2, 4, dtype=torch.int32, **dev)[:, ::2]
+for f, d, good, bads in ((B.ops_chunk_attention, att, attend, ((0, q.float()), (0, q.half()), (1, pools[0].half()), (2, pools[1].cpu()), (3, table.long()), (4, starts.float()), (5, cached.long()),
+                                                               (6, ints(0, 0, 0, 0)[::2]), (7, out.float()), (8, lse.half()))),
+                         (B.ops_token_scores, sc, score, ((0, logits.float()), (1, tokens.long()), (2, scores.double()), (3, ranks.float()), (4, entropy.half()), (5, best.long()),
+                                                          (6, bests.double()))),
+                         (B.ops_block_sweep, sw, sweep, ((0, table.long()), (0, wide), (1, lengths.float()), (2, uses.long()), (3, free.float()), (4, counts.cpu()))),
+                         (B.ops_cache_fork, fk, fork, ((0, ints(0).long()), (3, ints(5, 6).float()), (4, table.long()), (6, ints(0, 0).long()), (7, pools[0].half()), (8, pools[1].cpu()))),
+                         (B.ops_cache_compact, cm, compact, ((0, table.long()), (2, table.float()), (3, ints(0, 0).long()), (4, pools[0].float())))):
+    assert f(d, *good) == 0, B.last_error()
+    for i, bad in bads:
+        no(f, d, *good[:i], bad, *good[i + 1:])
+""")
+
+
+def test_calls_with_tensors_go_to_the_current_stream_of_torch():
+    """Behind what torch was given there, and into a graph that torch captures, replayed between other work."""
+    in_a_process(SERVING + """
+def check(step):
+    torch.cuda.synchronize()
+    want = plain_attention()
+    assert (out.float().cpu() - want).abs().max() <= 0.02 * (1 + want.abs().max()), step
+    x = logits.double().log_softmax(1)
+    assert (scores.double() - x.gather(1, tokens.long()[:, None])[:, 0]).abs().max() <= 1e-4, step
+    assert (bests.view(3, top)[:, 1:] <= bests.view(3, top)[:, :-1]).all(), step
+    assert (bests.view(3, top).double() - x.topk(top).values).abs().max() <= 1e-4, step
+    assert uses.tolist() == [sum(int(b) == n for row, l in zip(table.tolist(), lengths.tolist()) for b in row[:-(-l // 16)]) for n in range(10)], step
+    assert counts[2] == 0 and free[:int(counts[0])].tolist() == [n for n in range(10) if uses[n] == 0], step
+
+def calls():
+    assert B.ops_chunk_attention(att, *attend) == 0, B.last_error()
+    assert B.ops_token_scores(sc, *score) == 0, B.last_error()
+    assert B.ops_block_sweep(sw, *sweep) == 0, B.last_error()
+
+s = torch.cuda.Stream()
+big, late_q, late_x = torch.randn(4096, 4096, **dev), torch.randn_like(q.float()).bfloat16(), torch.randn(3, V, **dev).bfloat16()
+torch.cuda.synchronize()
+with torch.cuda.stream(s):
+    for _ in range(30):
+        big = big @ big * 1e-4
+    q.copy_(late_q)
+    logits.copy_(late_x)
+    calls()
+check("stream")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    calls()
+for step in range(4):
+    q.copy_(torch.randn(5, heads, 64, **dev))
+    logits.copy_(torch.randn(3, V, **dev) * 3)
+    tokens.copy_(torch.randint(0, V, (3,), **dev))
+    table.copy_(torch.randperm(10, **dev)[:4].view(2, 2))
+    cached.copy_(ints(step * 7, 28 - step))
+    lengths.copy_(cached + ints(2, 3))
+    graph.replay()
+    check(step)
+""")
+
+
 def test_chunk_of_single_tokens_is_paged_attention():
     """One new token a request: what the operator for single tokens gives, within the roundings of both."""
     rng = np.random.default_rng(3)
