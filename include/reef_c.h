@@ -367,7 +367,7 @@ int reef_ops_beam_reorder(const reef_beam_reorder_desc* d, const int32_t* parent
  * Beside the steps above, in the order of a server's calls: reef_ops_block_sweep finds the blocks that no request uses, reef_ops_cache_fork
  * lets requests continue a part of another one, reef_ops_chunk_attention attends for prompts, pieces of prompts and single tokens at once,
  * reef_ops_token_scores says how likely given tokens were, and reef_ops_cache_compact moves what is in use to the front of the pool.
- * What is said above of pointers, streams, workspaces and refusals holds for them too. */
+ * What is said above of pointers, streams, workspaces and refusals holds for them too (all but the attention refuse outputs that overlap inputs; pools are not looked at). */
 
 /* Attention of the new tokens of all requests over their cached ones, themselves among them (their keys and values are in the cache already).
  * Request i has the rows [starts[i], starts[i + 1]) of query (both held to [0, tokens]); the k-th of them has place p = cached[i] + k and

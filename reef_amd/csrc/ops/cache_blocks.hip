@@ -36,8 +36,8 @@ __global__ void __launch_bounds__(kThreads) clear(Use a) {
         else a.segments[i - a.t.blocks] = 0;
 }
 
-// A row a wavefront; gridDim.y of them go through a row in turn, 1024 entries each.
-constexpr int32_t kRun = 1024;
+// A row a wavefront; gridDim.y of them go through a row in turn, 256 entries each, which are on their way together.
+constexpr int32_t kRun = 256;
 template <bool kCount>
 __global__ void __launch_bounds__(kThreads) name_blocks(Use a) {
     const int lane = threadIdx.x & 63;
@@ -46,15 +46,18 @@ __global__ void __launch_bounds__(kThreads) name_blocks(Use a) {
     const int32_t n = used_entries(a.t, row);
     const int32_t* entries = a.t.entries + row * a.t.stride;
     for (int64_t j0 = (int64_t)blockIdx.y * kRun; j0 < n; j0 += (int64_t)gridDim.y * kRun) {
-        const int32_t end = (int32_t)min((int64_t)n, j0 + kRun);
-        for (int32_t j = (int32_t)j0 + lane; j < end; j += 64) {
-            const int32_t b = entries[j];
-            const bool inside = (uint32_t)b < (uint32_t)a.t.blocks;
+        int32_t b[kRun / 64];
+#pragma unroll
+        for (int u = 0; u < kRun / 64; ++u) b[u] = entries[min((int64_t)n - 1, j0 + u * 64 + lane)];
+#pragma unroll
+        for (int u = 0; u < kRun / 64; ++u) {
+            if (j0 + u * 64 + lane >= n) continue;
+            const bool inside = (uint32_t)b[u] < (uint32_t)a.t.blocks;
             if constexpr (kCount) {
-                if (inside) atomicAdd(a.uses + b, 1);
+                if (inside) atomicAdd(a.uses + b[u], 1);
                 else atomicAdd(a.segments + a.n_segments, 1);
             } else if (inside) {
-                a.uses[b] = 1;               // (whoever comes last: all write the same)
+                a.uses[b[u]] = 1;            // (whoever comes last: all write the same)
             }
         }
     }

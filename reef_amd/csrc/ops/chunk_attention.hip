@@ -490,8 +490,15 @@ struct Shape {
 // by 2^(R - R') is exact and rare.  For fp16, whose weights want room below, they are 2^kGrow times larger.
 //
 // 32-bit queries over 16-bit caches are two terms of fp16 or three of bf16 each, and so are their weights; 32-bit caches are three terms of bf16 on
-// both sides, six products (the others are below 2^-22).  Weights of 16-bit types are rounded to the type once: half a step of the type of each at most, which in their mean is
-// no more than the output's own rounding (two terms would take 1.4 times as long).
+// both sides, six products (the others are below 2^-22).  Weights of 16-bit types are rounded to the type once, half a step of each at most, and their sum is of those
+// that are not rounded: the output is off by no more than the mean |value| times that half step, as much as its own rounding where it is of values' size.  A
+// second term would double the products with the values, and products are what bounds it.
+//
+// One prompt of 8191 tokens, 32 heads over 8 of 128, bf16: 607 us, 0.91 PFLOP/s; three pieces of 509 over 40000, 64 heads over 8, fp16: 2.27 ms, 0.89.  When
+// the former took 646 us, it took 588 without loads, 541 without stores to LDS too, 503 without exponentials too, and 463 with its products alone
+// (1.19 PFLOP/s, what a large matrix product reaches here).  Heads of up to 64 leave room for two workgroups of four wavefronts a CU, which do not wait
+// for each other (four prompts of 2048, 12 heads of 64, bf16: 89 -> 79 us; two pieces of 300 over 20000: 91 -> 99); for heads of 80 and 128 eight wavefronts
+// that share what they read are faster (98 against 104 us, 616 against 688).
 template <class Q, class C, int DP, bool FEW>
 __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C, DP>::kWaves) * 64, (!FEW && Shape<Q, C, DP>::kPair ? 2 : 1)) chunk_attention(Args a) {
     using E = std::conditional_t<sizeof(C) == 4, __bf16, C>;                  // what is multiplied
@@ -1326,7 +1333,7 @@ Plan plan_of(const reef_chunk_attention_desc& d) {
         whole = (float)longest <= c.whole + 0.7f * c.tokens + 0.5f * p.join;
     }
     if (longest > (p.few ? kLookedFew : kLooked) && !whole) {
-        // Workgroups that find no item take 2 us a round for their look: there are no more than are likely to have one.
+        // Workgroups that find no item take 2 us a round for their look (four prompts of 2048: 74 us without, 80 with three rounds): there are no more than are likely to have one.
         const int64_t shares = (longest + least - 1) / least, tiles = p.items;
         p.budget = p.at_once * (tiles * kv <= p.at_once / 2 ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(3, most * waves.products / 1000)));
         p.items = std::min(tiles * shares, tiles + (p.budget + kv - 1) / kv);
