@@ -431,7 +431,7 @@ int reef_ops_block_sweep(const reef_block_sweep_desc* d, const int32_t* table, c
  * list's: the entry is -1 and nothing is copied); lengths[children[i]] = n.  Its entries behind stay as they are.
  * A fork is refused where a row is none of the table's, where a row is to be its own child, or where it needs a block and the list ends before it has one, counting
  * those that the forks before it need, refused for blocks or not: its row and length stay as they were.
- * Children are distinct, and no child is a parent of the same call; blocks of the list are used by no row.
+ * Children are distinct, and no child is a parent of the same call; blocks of the list are used by no row.  forks: up to table_rows and 2^15.
  *   counts [2]: entries of free_list taken; forks refused
  * free_list may be NULL where free_blocks is 0.  The pools hold `layers` caches of the layout, layer_stride elements from one to the next; a block of one
  * is less than 2^30 values. */

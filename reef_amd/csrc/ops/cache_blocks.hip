@@ -262,6 +262,7 @@ __device__ inline void copy_pieces(const Pieces& p, const unsigned char* from, u
         if (k0 + u * kThreads + threadIdx.x < total) *(u32x4*)(to + at[u]) = v[u];
 }
 
+constexpr int32_t kMostForks = 1 << 15;      // (each looks at those in front of it)
 struct ForkArgs {
     reef_cache_fork_desc d;
     const int32_t *parents, *children, *tokens, *free_list;
@@ -439,7 +440,7 @@ extern "C" int reef_ops_cache_fork(const reef_cache_fork_desc* d, const int32_t*
     if (!d) return refuse(what, "null argument");
     if (int rc = check_caches(what, d->cache, d->layers, d->layer_stride)) return rc;
     if (int rc = check_table(what, d->table_rows, d->cache.blocks, d->cache.block_size, d->max_blocks, d->table_stride)) return rc;
-    if (d->forks < 0 || d->forks > d->table_rows || d->free_blocks < 0) return refuse(what, "%d forks in a table of %d rows, %d free blocks", d->forks, d->table_rows, d->free_blocks);
+    if (d->forks < 0 || d->forks > d->table_rows || d->forks > kMostForks || d->free_blocks < 0) return refuse(what, "%d forks in a table of %d rows, %d free blocks", d->forks, d->table_rows, d->free_blocks);
     if (!words(counts) || (d->forks && (!words(parents) || !words(children) || !words(tokens) || !words(table) || !words(lengths) || !rows16(key_cache) || !rows16(value_cache))) ||
         (d->forks && d->free_blocks && !words(free_list)))
         return refuse(what, "null or unaligned argument");

@@ -157,7 +157,7 @@ def test_sweep_pointers():
     refused(call("block_sweep", None, *addresses(6), need), "null")
 
 
-@pytest.mark.parametrize("change,text", [(dict(forks=-1), "forks"), (dict(forks=5), "forks"), (dict(free_blocks=-1), "free"), (dict(layers=0), "layers"), (dict(layers=30001), "layers"),
+@pytest.mark.parametrize("change,text", [(dict(forks=-1), "forks"), (dict(forks=5), "forks"), (dict(forks=32769, table_rows=40000), "forks"), (dict(free_blocks=-1), "free"), (dict(layers=0), "layers"), (dict(layers=30001), "layers"),
                                          (dict(layers=2, layer_stride=64), "overlap"), (dict(table_rows=-1), "rows"), (dict(max_blocks=0), "table"), (dict(table_stride=3), "table")])
 def test_fork_refusals(change, text):
     refused(call("cache_fork", fork(layout(), **change), *addresses(9)), text)
