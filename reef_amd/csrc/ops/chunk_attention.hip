@@ -98,7 +98,8 @@ __device__ inline Sizes size_up(const Args& a, const Request& r) {
 // How long shares are.  Let w be the tokens of all tiles over the workgroups that run at once, and c the tokens whose time it takes to write and
 // read a share's sums.  Shares of T tokens take about w (1 + c / T), and 0.7 T until the last are done, least at T = (1.4 w c)^(1/2); a request whose
 // longest tile is done sooner is not cut, nor are its tiles of up to 1.3 T.  (One prompt of 2000 tokens, 32 heads over 8 of 128, bf16: 76 us, cut all the
-// same 90; of 2348, 10 heads over 5 of 64, f32: cut 99 us, else 160.)  Shares under half of w make no difference to the last ones any more.
+// same 90; of 2348, 10 heads over 5 of 64, f32: cut 99 us, else 160.)  T is half of w at least (two prompts of 2048, 16 heads over 4 of 128, f32: 290 us, 335
+// without that; the one of 2348 would take 91).
 // Where there are fewer workgroups than the budget, and tiles of a request are much alike (not as a prompt's, of which long ones and short ones make up for
 // each other), they are cut into the number n that takes the least rounds, ceil(n N / at once) (1 / n + c / tokens).
 // Where all that makes more items than there are workgroups for, shares are made longer, up to four times; then (lengths that were not expected) none is cut.
