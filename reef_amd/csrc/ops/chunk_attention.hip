@@ -11,7 +11,9 @@ using namespace reef_ops;
 constexpr int kRows = 32;                    // query rows of a wavefront: heads of one token next to each other, token after token
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int32_t kLeast = 256, kLeastFew = 512;   // cached tokens a share at least, of tiles of 32 rows for each wavefront and of 32 in all
-constexpr int32_t kLooked = 640, kLookedFew = 2048;  // up to so many tokens no cutting is looked at
+constexpr int32_t kLooked = 640, kLookedFew = 2048;  // up to so many tokens no cutting is looked at; where a pair takes more than one product, two thirds
+// (four pieces of 100 over 500, 12 heads of 64, f32: 47 us whole, 31 cut; over 300, 16 heads over 4 of 128: 70 whole, 79 cut; bf16, eight pieces of 60 over 400,
+// 32 heads over 8 of 128: 27 whole, 33 cut)
 constexpr float kJoin = 420.0f;              // tokens whose time it takes to write and read a share's sums, over the products per token
 constexpr int kCus = 256;
 constexpr float kSlack = 8.0f;               // powers of two by which weights may pass their reference
@@ -32,6 +34,7 @@ struct Args {
     int32_t group;
     int32_t tile_rows;      // of a workgroup
     int32_t at_once;        // workgroups that run at once
+    int32_t looked;         // tokens up to which no cutting is looked at
     float join;             // tokens whose time a share's sums take
     int32_t budget;         // workgroups that tiles are cut for, beside one each; 0: they are not cut
     int32_t most_items, most_slots;
@@ -143,7 +146,7 @@ struct Shares {
 __device__ inline Shares shares_of(const Args& a, const Cut& c, const Sizes& s, int32_t tiles) {
 #pragma clang fp contract(off)
     const bool few = a.tile_rows == kRows, alike = c.alike > 0.0f && s.top * (float)tiles < 1.5f * s.all;
-    const float least = (float)(few ? kLeastFew : kLeast), looked = (float)(few ? kLookedFew : kLooked);
+    const float least = (float)(few ? kLeastFew : kLeast), looked = (float)a.looked;
     const float each = fmaxf(least, alike ? c.alike : c.tokens), whole = fmaxf(1.5f * least, 1.3f * (alike ? c.alike : c.tokens));
     const bool cut = s.top > fmaxf(looked, alike ? c.alike : c.whole);
     Shares x;
@@ -1304,7 +1307,7 @@ Waves waves_of(const reef_chunk_attention_desc& d) {
 
 // How a call is laid out.
 struct Plan {
-    int32_t tile_rows, at_once, budget;
+    int32_t tile_rows, at_once, looked, budget;
     float join;
     bool few;               // tiles of 32 rows in all
     int64_t items, slots, groups;      // groups: workgroups
@@ -1319,6 +1322,7 @@ Plan plan_of(const reef_chunk_attention_desc& d) {
     p.few = rows <= (int64_t)kRows * d.requests && waves.few;
     p.tile_rows = p.few ? kRows : waves.each * kRows;
     p.at_once = p.few ? kCus : waves.at_once;
+    p.looked = p.few ? kLookedFew : waves.products > 1 ? kLooked * 2 / 3 : kLooked;
     p.join = p.few ? 0.0f : kJoin / (float)waves.products;
     int64_t longest = (int64_t)d.max_blocks * d.cache.block_size;
     if (d.longest && d.longest < longest) longest = d.longest;
@@ -1333,7 +1337,7 @@ Plan plan_of(const reef_chunk_attention_desc& d) {
         const Cut c = cut_for((float)most * (1.0f - 0.5f * tokens / (float)longest), p.join, p.few);
         whole = (float)longest <= c.whole + 0.7f * c.tokens + 0.5f * p.join;
     }
-    if (longest > (p.few ? kLookedFew : kLooked) && !whole) {
+    if (longest > p.looked && !whole) {
         // Workgroups that find no item take 2 us a round for their look (four prompts of 2048: 74 us without, 80 with three rounds): there are no more than are likely to have one.
         const int64_t shares = (longest + least - 1) / least, tiles = p.items;
         p.budget = p.at_once * (tiles * kv <= p.at_once / 2 ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(3, most * waves.products / 1000)));
@@ -1399,7 +1403,7 @@ extern "C" int reef_ops_chunk_attention(const reef_chunk_attention_desc* d, cons
     const int32_t group = d->heads / d->cache.kv_heads;
     const Args a{*d, query, key_cache, value_cache, table, starts, cached, lengths, out, lse, (int2*)w, p.list_bytes ? (int32_t*)(w + list) : nullptr, (float*)(w + parts),
                  (float2*)(w + stats), d->scale == 0.0f ? kLog2e : std::fabs(d->scale) * kLog2e, d->scale < 0.0f ? (d->type == REEF_TYPE_F32 ? 0x80000000u : 0x80008000u) : 0u,
-                 d->scale == 0.0f, group, p.tile_rows, p.at_once, p.join, p.budget, (int32_t)p.items, (int32_t)p.slots, (int32_t*)(w + jobs), (int4*)(w + jobs) + 1,
+                 d->scale == 0.0f, group, p.tile_rows, p.at_once, p.looked, p.join, p.budget, (int32_t)p.items, (int32_t)p.slots, (int32_t*)(w + jobs), (int4*)(w + jobs) + 1,
                  divider((uint32_t)d->cache.block_size), divider((uint32_t)group)};
     switch (d->type * 4 + d->cache.type) {
         case REEF_TYPE_F32 * 4 + REEF_TYPE_F32: return run<float, float>(what, a, p, stream);
