@@ -498,7 +498,7 @@ struct Shape {
 // that are not rounded: the output is off by no more than the mean |value| times that half step, as much as its own rounding where it is of values' size.  A
 // second term would double the products with the values, and products are what bounds it.
 //
-// One prompt of 8191 tokens, 32 heads over 8 of 128, bf16: 607 us, 0.91 PFLOP/s; three pieces of 509 over 40000, 64 heads over 8, fp16: 2.27 ms, 0.89.  When
+// One prompt of 8191 tokens, 32 heads over 8 of 128, bf16: 616 us, 0.89 PFLOP/s; three pieces of 509 over 40000, 64 heads over 8, fp16: 2.30 ms, 0.88.  When
 // the former took 646 us, it took 588 without loads, 541 without stores to LDS too, 503 without exponentials too, and 463 with its products alone
 // (1.19 PFLOP/s, what a large matrix product reaches here).  Heads of up to 64 leave room for two workgroups of four wavefronts a CU, which do not wait
 // for each other (four prompts of 2048, 12 heads of 64, bf16: 89 -> 79 us; two pieces of 300 over 20000: 91 -> 99); for heads of 80 and 128 eight wavefronts

@@ -1,5 +1,6 @@
 // Log probabilities of given tokens, their ranks, the entropy and the best alternatives (reef_ops_token_scores).
 #include <algorithm>
+#include <type_traits>
 
 #include "ops_common.h"
 
@@ -34,6 +35,7 @@ struct Args {
     uint32_t* maxima;       // [row][groups]
     int32_t slices, slice_units;
     Groups by;
+    int32_t loads;
 };
 // What a part of a row comes to: its maximum, the sums relative to it, values that come before the given token.
 struct Part {
@@ -139,7 +141,7 @@ enum { kWhole, kSlice, kJoin };
 // LOADS: of a wavefront in flight, 1 KiB each, a unit.
 template <class T, int WAVES, int LOADS, int STAGE>
 __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
-    constexpr int kLoads = LOADS, kThreads = WAVES * 64, kE = 16 / sizeof(T), kUnit = 64 * kE, kMine = kGroups / 64, kLoadBits = LOADS == 8 ? 3 : 2;
+    constexpr int kLoads = LOADS, kThreads = WAVES * 64, kE = 16 / sizeof(T), kUnit = 64 * kE, kMine = kGroups / 64, kLoadBits = __builtin_ctz(LOADS);
     constexpr int kShift = sizeof(T) == 4 ? 0 : __is_same(T, _Float16) ? 13 : 16;
     typedef T Raw __attribute__((ext_vector_type(kE), aligned(sizeof(T))));
     const reef_token_scores_desc& d = a.d;
@@ -516,14 +518,21 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
 
 // How a call is laid out: slices of 128 units, which sixteen wavefronts read at once, where rows are few and have more of them (a row of 150001, f32: 24 us
 // whole, 17.6 in slices; 16 of 128257, bf16: 24.3 and 22.2).
+// Units that a wavefront reads at once: as few as leave none idle (123 rows of 1270, bf16: 10.6 us, with eight 17.4; 500 of 8000: 12.8 and 16.1), eight,
+// or four where rows fill the device, for longer ones.
+int32_t loads_of(int32_t rows, int32_t units) {
+    const int32_t waves = rows <= 256 ? 16 : 8;
+    return units <= waves ? 1 : units <= 2 * waves ? 2 : rows <= 512 ? 8 : 4;
+}
 struct Plan {
     int32_t slices, slice_units;
     Groups by;
+    int32_t loads;
     int64_t parts_bytes, bytes;
 };
 Plan plan_of(const reef_token_scores_desc& d) {
-    const int32_t unit = 1024 / type_bytes(d.type), units = (d.vocab + unit - 1) / unit, loads = d.rows <= 512 ? 8 : 4;
-    Plan p{1, units, groups_of(units, loads), 0, 0};
+    const int32_t unit = 1024 / type_bytes(d.type), units = (d.vocab + unit - 1) / unit, loads = loads_of(d.rows, units);
+    Plan p{1, units, groups_of(units, loads), loads, 0, 0};
     if (d.rows > 128 || units <= 192) return p;
     const int32_t most = std::min(256 / d.rows, (units + 127) / 128);
     const int32_t step = p.by.per * loads;        // no group and no batch reaches into the next slice
@@ -543,9 +552,15 @@ int run(const char* what, const Args& a, const Plan& p, void* stream) {
         if (int rc = launch(what, token_scores<T, 16, 8, kSlice>, dim3((unsigned)(a.d.rows * p.slices)), dim3(16 * 64), a, stream)) return rc;
         return launch(what, token_scores<T, 16, 8, kJoin>, rows, dim3(16 * 64), a, stream);
     }
-    if (a.d.rows <= 256) return launch(what, token_scores<T, 16, 8, kWhole>, rows, dim3(16 * 64), a, stream);
-    if (a.d.rows <= 512) return launch(what, token_scores<T, 8, 8, kWhole>, rows, dim3(8 * 64), a, stream);
-    return launch(what, token_scores<T, 4, 4, kWhole>, rows, dim3(4 * 64), a, stream);
+    auto go = [&](auto loads) {
+        constexpr int kLoads = decltype(loads)::value;
+        if (a.d.rows <= 256) return launch(what, token_scores<T, 16, kLoads, kWhole>, rows, dim3(16 * 64), a, stream);
+        if (a.d.rows <= 512) return launch(what, token_scores<T, 8, kLoads, kWhole>, rows, dim3(8 * 64), a, stream);
+        return launch(what, token_scores<T, 4, kLoads == 8 ? 4 : kLoads, kWhole>, rows, dim3(4 * 64), a, stream);
+    };
+    if (a.loads == 1) return go(std::integral_constant<int, 1>());
+    if (a.loads == 2) return go(std::integral_constant<int, 2>());
+    return go(std::integral_constant<int, 8>());
 }
 
 int check(const char* what, const reef_token_scores_desc* d) {
@@ -580,7 +595,7 @@ extern "C" int reef_ops_token_scores(const reef_token_scores_desc* d, const void
     const Span in[] = {{logits, ((n - 1) * d->logits_stride + d->vocab) * type_bytes(d->type)}, {tokens, 4 * n}};
     if (overlap(out, in)) return refuse(what, "an output overlaps an input");
     const Plan p = plan_of(*d);
-    const Args a{*d, logits, tokens, scores, ranks, entropy, top_tokens, top_scores, (Part*)workspace, (uint32_t*)((char*)workspace + p.parts_bytes), p.slices, p.slice_units, p.by};
+    const Args a{*d, logits, tokens, scores, ranks, entropy, top_tokens, top_scores, (Part*)workspace, (uint32_t*)((char*)workspace + p.parts_bytes), p.slices, p.slice_units, p.by, p.loads};
     switch (d->type) {
         case REEF_TYPE_F32: return run<float>(what, a, p, stream);
         case REEF_TYPE_F16: return run<_Float16>(what, a, p, stream);

@@ -569,6 +569,17 @@ def test_scores_sizes(kind, rows, vocab):
 
 
 @pytest.mark.parametrize("kind", [F32, F16, BF16])
+@pytest.mark.parametrize("rows", [200, 400, 600])
+@pytest.mark.parametrize("vocab", [130, 1999, 6001, 20011])
+def test_scores_many_rows(kind, rows, vocab):
+    """Rows of few and of many units, taken by many wavefronts and by few; some of them masked in front, behind, all over."""
+    rng = np.random.default_rng(rows + vocab)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32) * 3
+    x[1, :vocab // 2], x[2, vocab // 3:], x[3], x[4, 5:] = -np.inf, -np.inf, -np.inf, np.finfo(np.float16).min
+    run_scores(kind, x, rng.integers(-1, vocab + 1, rows), 33, pad=int(vocab % 2))
+
+
+@pytest.mark.parametrize("kind", [F32, F16, BF16])
 @pytest.mark.parametrize("vocab", [300, 9001, 66000])
 def test_scores_odd_values(kind, vocab):
     rng = np.random.default_rng(vocab)
