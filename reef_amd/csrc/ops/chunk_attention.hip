@@ -756,15 +756,21 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
             for (int i = 0; i < 16; ++i) s[u][i] = yes >> i & 1 ? s[u][i] : -INFINITY;
         }
     };
+    // Products as scores but for `scale`: once a tile.
+    auto shrunk = [&](auto& s) __attribute__((always_inline)) {
+        if constexpr (kHalf && kTermsQ > 1) {
+#pragma unroll
+            for (int u = 0; u < (int)(sizeof(s) / sizeof(s[0])); ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[u][i] *= shrink;
+        }
+    };
     auto largest = [&](auto& s) __attribute__((always_inline)) {
         float top = -INFINITY;
 #pragma unroll
         for (int u = 0; u < (int)(sizeof(s) / sizeof(s[0])); ++u)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                if constexpr (kHalf && kTermsQ > 1) s[u][i] *= shrink;
-                top = fmaxf(top, s[u][i]);
-            }
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
         return other_max(top) * scale;
     };
     auto refer = [&](float top, auto slabs) __attribute__((always_inline)) {
@@ -954,6 +960,7 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            shrunk(s);
             const bool by_all = t0 >= all_lo && t0 + 32 <= all_hi;
             if (!by_all || there_now != ~0u) hide(s, t0, there_now);
             refer(largest(s), kAcc);
@@ -1157,6 +1164,7 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
                 multiply_keys(next, k_near + kNow * kBuffer);
                 weigh(s);
                 multiply_values(v_near + (kValues == 2 ? kNow ^ 1 : 0) * kBuffer);
+                shrunk(next);
                 look(j, next, largest(next));
                 take(j, parity);
             };
@@ -1167,6 +1175,7 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
             };
             ask(0, kEvenOnes);
             multiply_keys(even, k_near);
+            shrunk(even);
             look(0, even, largest(even));
             take(0, kEvenOnes);
             uint32_t j = 1;

@@ -186,6 +186,14 @@ def test_chunk_queries_far_from_one(kind, cache):
         run_chunk(kind, cache, "thd", 16, 2, 2, 64, [300, 2000], [20, 40], grow=grow, scale=scale, seed=1)
 
 
+@pytest.mark.parametrize("kind,cache", [(F32, F16), (F32, BF16), (F32, F32)])
+@pytest.mark.parametrize("cached,added,window", [([300, 40], [20, 130], 0), ([0, 700, 5], [600, 200, 300], 0), ([1000], [90], 130), ([2000, 50], [5, 1], 0)])
+def test_chunk_large_queries_at_full_scale(kind, cache, cached, added, window):
+    """Queries of 2^14 and more whose scores are moderate, as keys are small: tiles that all rows see beside ones that some do."""
+    for grow, size, scale in ((2e4, 1e-4, 1.0), (7e4, 2e-5, 2.5), (3e4, 5e-5, -1.0)):
+        run_chunk(kind, cache, "thd", 16, 2, 2, 64, cached, added, window=window, grow=grow, size=size, scale=scale, seed=1)
+
+
 def one_request(kind, cache, keys, values, q, scale, cached, longest=0):
     """One request in one block: raw host values keys, values [tokens][dim], q [new][heads][dim] -> out, lse."""
     t, dim = keys.shape
