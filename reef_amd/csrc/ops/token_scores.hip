@@ -121,7 +121,8 @@ struct Sum {
     __device__ V operator()(V a, V b) const { return a + b; }
 };
 
-constexpr float kBehind = -0x1p18f;          // (plain)
+// What stands behind a row's end, and how far above it a lane's largest has to be for its exponential to be 0: 1000 powers of two.
+constexpr float kBehind = -0x1p18f, kAbove = 1024.0f;        // (plain)
 constexpr int kHeld = 2048;                  // candidates that are held
 
 // A row a workgroup, read once: a lane keeps its 16 bytes of a batch of units, their maximum m and sums relative to the largest so far; how many values come
@@ -235,7 +236,7 @@ __global__ void __launch_bounds__(WAVES * 64) token_scores(Args a) {
             }
         }
         const bool any = full || u0 * kUnit + lane * kE < d.vocab;           // of the lane's values are real
-        if (__builtin_amdgcn_ballot_w64(any && !((plain(base) || next == -INFINITY) && (full || all > kBehind))) == 0) {
+        if (__builtin_amdgcn_ballot_w64(any && !((plain(base) || next == -INFINITY) && (full || all > kBehind + kAbove))) == 0) {
             if (any) {
                 if (next > m) {
                     const float y = step(m, next), f = __builtin_amdgcn_exp2f(y);

@@ -651,6 +651,17 @@ def test_scores_of_large_values(vocab):
     run_scores(F32, x, [vocab - 1] * 8, 0)
 
 
+# (Places behind a row's end are filled with -2^18 at most: rows whose largest logit is not far above.)
+@pytest.mark.parametrize("rows,vocab", [(7, 5), (7, 301), (7, 1026), (7, 2050), (7, 30011), (2, 150001), (300, 1270), (300, 9001), (600, 515), (600, 7001)])
+def test_scores_just_above_what_stands_behind_the_end(rows, vocab):
+    rng = np.random.default_rng(vocab)
+    above = np.array([0.5, 1.0, 10.0, 30.0, 100.0, 740.0, 2000.0])[np.arange(rows) % 7]
+    flat = np.repeat((above - 2.0 ** 18)[:, None], vocab, 1)
+    for x in (flat, flat - rng.integers(0, 64, (rows, vocab)) / 8, np.where(rng.random((rows, vocab)) < 0.5, flat, -np.inf)):
+        x[:, 0] = flat[:, 0]
+        run_scores(F32, x, np.where(np.arange(rows) % 3 == 2, rng.integers(0, vocab, rows), 0), min(vocab, 5))
+
+
 # ---- blocks ---------------------------------------------------------------------------------------
 def run_sweep(table, lengths, blocks, bs, max_blocks):
     rows, stride = table.shape
