@@ -400,15 +400,17 @@ __device__ inline f32x16 product(u32x4 a, u32x4 b, f32x16 c, __bf16) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Two values as N terms of a 16-bit type, whose sums they are but for what the last rounds off.  The first of three is cut, so that it is
+// Two values as N terms of a 16-bit type, whose sums they are but for what the last rounds off.  The first of several is cut, so that it is
 // finite where the value is.
 template <int N>
 __device__ inline void terms(float a, float b, uint32_t (&t)[N], __bf16) {
     typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    if constexpr (N == 3) {
+    if constexpr (N > 1) {
         t[0] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
         a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
         b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+    }
+    if constexpr (N == 3) {
         const bf16x2 x = {(__bf16)a, (__bf16)b};
         t[1] = __builtin_bit_cast(uint32_t, x);
         a -= __uint_as_float(t[1] << 16);
@@ -472,11 +474,12 @@ template <class Q, class C, int DP>
 struct Shape {
     static constexpr bool kHalf = __is_same(C, _Float16);
     static constexpr int kTermsC = sizeof(C) == 4 ? 3 : 1, kTermsQ = sizeof(Q) == 2 ? 1 : kHalf ? 2 : 3;
+    static constexpr int kTermsFew = sizeof(Q) == 2 ? 2 : kTermsQ;           // of weights in tiles of 32 rows in all; in others kTermsQ
     static constexpr bool kPair = DP <= 64;
     static constexpr int kWaves = DP <= 128 && !kPair ? 8 : 4, kTile = kTermsQ == 1 && DP <= 128 ? 64 : 32;
     // Tiles of 32 rows in all: registers of what a wavefront holds (keys, values, queries, output, weights), and so how many wavefronts; 0: too many for any.
     static constexpr int kFewV = DP <= 64 ? 2 : DP <= 128 ? 4 : 8;            // values of a row of V a lane
-    static constexpr int kFewHeld = DP * (int)sizeof(C) / 8 + 16 * kFewV * (int)sizeof(C) / 4 + kTermsQ * DP / 4 + kFewV * 16 + 16 + 8 * kTermsQ;
+    static constexpr int kFewHeld = DP * (int)sizeof(C) / 8 + 16 * kFewV * (int)sizeof(C) / 4 + kTermsQ * DP / 4 + kFewV * 16 + 16 + 8 * kTermsFew;
     static constexpr int kFewWaves = kFewHeld <= 220 ? 8 : kFewHeld <= 440 ? 4 : 0;
 };
 
@@ -494,9 +497,11 @@ struct Shape {
 // by 2^(R - R') is exact and rare.  For fp16, whose weights want room below, they are 2^kGrow times larger.
 //
 // 32-bit queries over 16-bit caches are two terms of fp16 or three of bf16 each, and so are their weights; 32-bit caches are three terms of bf16 on
-// both sides, six products (the others are below 2^-22).  Weights of 16-bit types are rounded to the type once, half a step of each at most, and their sum is of those
-// that are not rounded: the output is off by no more than the mean |value| times that half step, as much as its own rounding where it is of values' size.  A
-// second term would double the products with the values, and products are what bounds it.
+// both sides, six products (the others are below 2^-22).  Weights of 16-bit types are two terms in tiles of 32 rows in all, which memory or latency
+// bounds (64 single tokens over 4000, 32 heads over 8 of 128, bf16: 199 us with one term, 204 with two).  In larger tiles they are rounded to the type once, half a
+// step of each at most, and their sum is of those that are not rounded: the output is off by no more than the mean |value| times that half step, as much as its
+// own rounding where it is of values' size.  Products bound these, and a second term would double those with the values: 600 -> 771 us for the prompt
+// below, 2225 -> 2948 for the three pieces, 164 -> 205 for two prompts of 2797 (heads of 80, fp16).
 //
 // One prompt of 8191 tokens, 32 heads over 8 of 128, bf16: 616 us, 0.89 PFLOP/s; three pieces of 509 over 40000, 64 heads over 8, fp16: 2.30 ms, 0.88.  When
 // the former took 646 us, it took 588 without loads, 541 without stores to LDS too, 503 without exponentials too, and 463 with its products alone
@@ -508,7 +513,8 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
     using E = std::conditional_t<sizeof(C) == 4, __bf16, C>;                  // what is multiplied
     using Sh = Shape<Q, C, DP>;
     constexpr bool kHalf = Sh::kHalf;
-    constexpr int kTermsC = Sh::kTermsC, kTermsQ = Sh::kTermsQ, kTile = Sh::kTile, kSub = kTile / 32, kWaves = FEW ? Sh::kFewWaves : Sh::kWaves, kThreads = kWaves * 64;
+    constexpr int kTermsC = Sh::kTermsC, kTermsQ = Sh::kTermsQ, kTermsP = FEW ? Sh::kTermsFew : kTermsQ;
+    constexpr int kTile = Sh::kTile, kSub = kTile / 32, kWaves = FEW ? Sh::kFewWaves : Sh::kWaves, kThreads = kWaves * 64;
     constexpr float kGrow = kHalf ? 6.0f : 0.0f;                              // 2^(6 + 8 + 1/2) < 65504
     constexpr int kSteps = DP / 16, kSlabs = DP / 32, kTileRows = FEW ? kRows : kWaves * kRows;
     using N = Near<DP>;
@@ -806,7 +812,7 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
         }
     };
     // Weights of a tile, as operands.
-    u32x4 p[kTile / 16][kTermsQ];
+    u32x4 p[kTile / 16][kTermsP];
     auto weigh = [&](auto& s) __attribute__((always_inline)) {
         float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -816,10 +822,10 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
                 const int i = (c & 1) * 8 + 2 * w;
                 const float x = __builtin_amdgcn_exp2f(fmaf(s[c >> 1][i], times, plus)), y = __builtin_amdgcn_exp2f(fmaf(s[c >> 1][i + 1], times, plus));
                 sum[w] += x + y;
-                uint32_t t[kTermsQ];
+                uint32_t t[kTermsP];
                 terms(x, y, t, E());
 #pragma unroll
-                for (int k = 0; k < kTermsQ; ++k) p[c][k][w] = t[k];
+                for (int k = 0; k < kTermsP; ++k) p[c][k][w] = t[k];
             }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
     };
@@ -837,7 +843,7 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
     auto multiply_by = [&](u32x4 (&v)[kTermsC], int c, int m) __attribute__((always_inline)) {
         if constexpr (kTermsC == 1) {
 #pragma unroll
-            for (int x = kTermsQ - 1; x >= 0; --x) o[m] = product(v[0], p[c][x], o[m], E());
+            for (int x = kTermsP - 1; x >= 0; --x) o[m] = product(v[0], p[c][x], o[m], E());
         } else {
 #pragma unroll
             for (int both = 2; both >= 0; --both)
@@ -1008,7 +1014,7 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
                     }
                     if constexpr (kTermsC == 1) {
 #pragma unroll
-                        for (int i = kTermsQ - 1; i >= 0; --i) o[e] = product(x[0], p[c][i], o[e], E());
+                        for (int i = kTermsP - 1; i >= 0; --i) o[e] = product(x[0], p[c][i], o[e], E());
                     } else {
 #pragma unroll
                         for (int both = 2; both >= 0; --both)

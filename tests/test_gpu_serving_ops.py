@@ -511,6 +511,24 @@ def test_chunk_of_single_tokens_is_paged_attention():
     assert np.abs(ls[0].to_array() - ls[1].to_array()).max() <= 2.0 ** -15
 
 
+@pytest.mark.parametrize("kind", [BF16, F16])
+@pytest.mark.parametrize("cached,new,group,dim", [(20, 1, 2, 64), (30, 1, 4, 128), (60, 3, 2, 32), (45, 5, 1, 72), (40, 3, 8, 256), (25, 2, 3, 192), (9000, 2, 3, 192)])
+def test_chunk_of_few_rows_keeps_its_weights(kind, cached, new, group, dim):
+    """Up to 32 rows a request a weight is two numbers of the 16-bit type, which leave out 2^-16 (bf16) or 2^-22 (fp16) of it at most, as in the operator for single
+    tokens: the output is off by that times the mean |value|, by fp16's smallest numbers (2^-25 where the largest weight is 2^5), by what 32 bits
+    round, and by half its own step."""
+    rng = np.random.default_rng(dim)
+    n = cached + new
+    keys, values, q = (R.decode(R.encode(rng.standard_normal(s).astype(np.float32), kind), kind) for s in ((n, dim), (n, dim), (new, group, dim)))
+    scale = 0.1 * dim ** -0.5
+    got, lse = one_request(kind, kind, keys.astype(np.float32), values.astype(np.float32), q.astype(np.float32), scale, cached)
+    want, want_lse, tol, tol_lse = S.chunk(q, keys[None], values[None], cached, n, scale, 0, kind, kind)
+    mean = S.chunk(q, keys[None], np.abs(values)[None], cached, n, scale, 0, kind, kind)[0]
+    lim = tol - HALF[kind] * mean + (2.0 ** -16 if kind == BF16 else 2.0 ** -21) * mean + HALF[kind] * np.abs(want) + (2.0 ** -25 if kind == F16 else 0)
+    assert (np.abs(got - want) <= lim).all(), float((np.abs(got - want) / lim).max())
+    assert (np.abs(lse - want_lse) <= tol_lse).all()
+
+
 def test_chunk_starts_that_do_not_ascend_stay_inside():
     """Nothing is read or written behind the tensors, whatever starts, cached and lengths hold."""
     rng = np.random.default_rng(1)
