@@ -26,7 +26,7 @@ struct Args {
     float* lse;
     int2* info;             // [request], where there are many: first item, first slot
     int32_t* list;          // numbers of all (kListHead), then the request of each item
-    float* parts;           // [slot][cache head][row of the tile][head_dim], sums that are not divided yet
+    float* parts;           // [slot (a share of a tile that is cut)][cache head][row of the tile][head_dim], sums that are not divided yet
     float2* stats;          // [slot][cache head][row of the tile]: power of two that they are to be multiplied by, sum of the weights
     float scale;            // |scale| log2 e, or log2 e where it is 0
     uint32_t flip;          // of the queries' sign where scale is negative
@@ -51,7 +51,7 @@ struct Request {
 // An item: a tile of rows over a share of the tokens that they see.
 struct Item {
     Request r;
-    int32_t request, tile, share, shares, slot;   // tile < 0: there is no such item; slot of the tile's first share, -1: none of the request's has one
+    int32_t request, tile, share, shares, slot;   // tile < 0: there is no such item; slot of the tile's first share where there are several
     int32_t slots;                           // of all
 };
 
@@ -105,7 +105,7 @@ __device__ inline Sizes size_up(const Args& a, const Request& r) {
 // without that; the one of 2348 would take 91).
 // Where there are fewer workgroups than the budget, and tiles of a request are much alike (not as a prompt's, of which long ones and short ones make up for
 // each other), they are cut into the number n that takes the least rounds, ceil(n N / at once) (1 / n + c / tokens).
-// Where all that makes more items than there are workgroups for, shares are made longer, up to four times; then (lengths that were not expected) none is cut.
+// Where all that makes more items than there are workgroups for, or shares than there are slots, shares are made longer, up to four times; then (lengths that were not expected) none is cut.
 struct Cut {
     float whole, tokens, alike;              // tiles of up to `whole` tokens are not cut, others into shares of `tokens`; alike: of tiles much alike; 0: as others
 };
@@ -141,7 +141,7 @@ __device__ inline Cut cut_of(const Args& a, float all, float tiles) {
 // Into how many shares the tiles of each part are cut.
 struct Shares {
     int32_t n[kParts];
-    bool any, first;        // shares that are longer than half a round come first, so that none of them begins when the others are nearly done
+    bool first;             // shares that are longer than half a round come first, so that none of them begins when the others are nearly done
 };
 __device__ inline Shares shares_of(const Args& a, const Cut& c, const Sizes& s, int32_t tiles) {
 #pragma clang fp contract(off)
@@ -150,11 +150,10 @@ __device__ inline Shares shares_of(const Args& a, const Cut& c, const Sizes& s, 
     const float each = fmaxf(least, alike ? c.alike : c.tokens), whole = fmaxf(1.5f * least, 1.3f * (alike ? c.alike : c.tokens));
     const bool cut = s.top > fmaxf(looked, alike ? c.alike : c.whole);
     Shares x;
-    x.any = x.first = false;
+    x.first = false;
 #pragma unroll
     for (int q = 0; q < kParts; ++q) {
         x.n[q] = !cut || s.most[q] <= whole ? 1 : (int32_t)ceilf(s.most[q] / each);
-        x.any |= x.n[q] > 1;
         x.first |= s.most[q] > 0.5f * c.tokens * (float)x.n[q];
     }
     return x;
@@ -163,7 +162,6 @@ __device__ inline Shares not_cut() {
     Shares x;
 #pragma unroll
     for (int q = 0; q < kParts; ++q) x.n[q] = 1;
-    x.any = false;
     x.first = true;
     return x;
 }
@@ -181,6 +179,13 @@ __device__ inline uint32_t items_of(const Request& r, const Shares& x) {
     uint32_t n = 0;
 #pragma unroll
     for (int q = 0; q < kParts; ++q) n = plus(n, product(part_of(r, q + 1) - part_of(r, q), x.n[q]));
+    return n;
+}
+// Those of tiles that are cut, which have a slot each.
+__device__ inline uint32_t slots_of(const Request& r, const Shares& x) {
+    uint32_t n = 0;
+#pragma unroll
+    for (int q = 0; q < kParts; ++q) n = plus(n, x.n[q] > 1 ? product(part_of(r, q + 1) - part_of(r, q), x.n[q]) : 0);
     return n;
 }
 // Prefix sums over the wavefront without the lane's own value; *all: with all of them.
@@ -222,17 +227,19 @@ __device__ inline Item find_item(const Args& a, int32_t id) {
     } else if (a.d.requests == 1) {
         it.request = 0;
         it.r = request_of(a, 0);
-        uint32_t items = (uint32_t)it.r.tiles;
+        uint32_t items = (uint32_t)it.r.tiles, slots = 0;
         if (a.budget) {
             const Sizes sizes = size_up(a, it.r);
             Cut cut = cut_of(a, sizes.all, (float)it.r.tiles);
             for (int tries = 1;; ++tries) {
                 shares = shares_of(a, cut, sizes, it.r.tiles);
                 items = items_of(it.r, shares);
-                if (items <= (uint32_t)a.most_items) break;
+                slots = slots_of(it.r, shares);
+                if (items <= (uint32_t)a.most_items && slots <= (uint32_t)a.most_slots) break;
                 if (tries == kTries) {
                     shares = not_cut();
                     items = (uint32_t)it.r.tiles;
+                    slots = 0;
                     break;
                 }
                 cut_less(cut);
@@ -240,7 +247,7 @@ __device__ inline Item find_item(const Args& a, int32_t id) {
         }
         if ((uint32_t)id >= items) return it;
         it.slot = 0;
-        it.slots = shares.any ? (int32_t)min(items, 1u << 30) : 0;
+        it.slots = (int32_t)slots;
         local = id;
     } else {
         const int lane = threadIdx.x & 63;
@@ -256,16 +263,17 @@ __device__ inline Item find_item(const Args& a, int32_t id) {
                 at = before_me(shares.first ? mine : 0, &firsts);
                 const uint32_t x = before_me(shares.first ? 0 : mine, &others);
                 at = shares.first ? at : plus(firsts, x);
-                if (plus(firsts, others) <= (uint32_t)a.most_items) break;
+                slot = before_me(slots_of(r, shares), &all_slots);
+                if (plus(firsts, others) <= (uint32_t)a.most_items && all_slots <= (uint32_t)a.most_slots) break;
                 if (tries == kTries) {
                     shares = not_cut();
                     mine = (uint32_t)r.tiles;
                     at = before_me(mine, &firsts);
+                    all_slots = 0;
                     break;
                 }
                 cut_less(cut);
             }
-            slot = before_me(shares.any ? mine : 0, &all_slots);
         } else {
             at = before_me(mine, &firsts);
         }
@@ -280,13 +288,12 @@ __device__ inline Item find_item(const Args& a, int32_t id) {
         it.r.tiles = __builtin_amdgcn_readlane(r.tiles, l);
 #pragma unroll
         for (int q = 0; q < kParts; ++q) shares.n[q] = __builtin_amdgcn_readlane(shares.n[q], l);
-        shares.any = __builtin_amdgcn_readlane((int32_t)shares.any, l);
-        it.slot = (int32_t)min(__builtin_amdgcn_readlane(slot, l), 1u << 30);
-        it.slots = (int32_t)min(all_slots, 1u << 30);
+        it.slot = __builtin_amdgcn_readlane((int32_t)slot, l);
+        it.slots = (int32_t)all_slots;
         local = id - (int32_t)__builtin_amdgcn_readlane(at, l);
     }
     // the last tiles, which see most, first
-    int32_t before = 0, from = 0, to = 0;
+    int32_t before = 0, from = 0, to = 0, slots_before = 0, slots_from = 0;
     it.shares = 1;
 #pragma unroll
     for (int q = kParts - 1; q >= 0; --q) {
@@ -295,13 +302,15 @@ __device__ inline Item find_item(const Args& a, int32_t id) {
             from = before;
             to = t;
             it.shares = shares.n[q];
+            slots_from = slots_before;
         }
         before += n;
+        if (shares.n[q] > 1) slots_before += n;
     }
     const int32_t k = (local - from) / it.shares;
     it.share = local - from - k * it.shares;
     it.tile = to - 1 - k;
-    it.slot = __builtin_amdgcn_readfirstlane(shares.any ? it.slot + local - it.share : -1);
+    it.slot = __builtin_amdgcn_readfirstlane(it.slot + slots_from + k * it.shares);
     it.shares = __builtin_amdgcn_readfirstlane(it.shares);
     it.share = __builtin_amdgcn_readfirstlane(it.share);
     it.tile = __builtin_amdgcn_readfirstlane(it.tile);
@@ -335,20 +344,21 @@ __global__ void __launch_bounds__(kListThreads) list_items(Args a) {
         cut = cut_of(a, sum, tiles);
     }
     bool is_cut = a.budget != 0;
-    auto shares_and_items = [&](int32_t i, uint32_t* mine) {
+    auto shares_and_items = [&](int32_t i, uint32_t* mine, uint32_t* slots) {
         const Request r = request_of(a, i);
         const Shares x = is_cut ? shares_of(a, cut, size_up(a, r), r.tiles) : not_cut();
         *mine = items_of(r, x);
+        *slots = slots_of(r, x);
         return x;
     };
     uint32_t all, all_slots, item, later, slot;            // later: where the next request that does not come first has its items
     for (int tries = 1;; ++tries) {
-        uint32_t items = 0, others = 0, slots = 0, of_wave, others_of_wave, slots_of_wave, mine;
+        uint32_t items = 0, others = 0, slots = 0, of_wave, others_of_wave, slots_of_wave, mine, its_slots;
         for (int32_t i = lo; i < hi; ++i) {
-            const Shares x = shares_and_items(i, &mine);
+            const Shares x = shares_and_items(i, &mine, &its_slots);
             if (x.first) items = plus(items, mine);
             else others = plus(others, mine);
-            if (x.any) slots = plus(slots, mine);
+            slots = plus(slots, its_slots);
         }
         item = before_me(items, &of_wave);
         later = before_me(others, &others_of_wave);
@@ -369,22 +379,22 @@ __global__ void __launch_bounds__(kListThreads) list_items(Args a) {
             all_slots = plus(all_slots, counts[w].z);
         }
         later = plus(later, firsts);
-        if (!is_cut || all <= (uint32_t)a.most_items) break;
+        if (!is_cut || (all <= (uint32_t)a.most_items && all_slots <= (uint32_t)a.most_slots)) break;
         if (tries == kTries) is_cut = false;
         else cut_less(cut);
     }
     for (int32_t i = lo; i < hi; ++i) {
-        uint32_t mine;
-        const Shares x = shares_and_items(i, &mine);
+        uint32_t mine, its_slots;
+        const Shares x = shares_and_items(i, &mine, &its_slots);
         uint32_t& at = x.first ? item : later;
-        a.info[i] = make_int2((int32_t)min(at, 1u << 30), (int32_t)min(slot, 1u << 30));
+        a.info[i] = make_int2((int32_t)min(at, 1u << 30), (int32_t)slot);
         for (uint32_t k = at; k < min(plus(at, mine), (uint32_t)a.most_items); ++k) a.list[kListHead + k] = i;
         at = plus(at, mine);
-        if (x.any) slot = plus(slot, mine);
+        slot += its_slots;
     }
     if (tid == 0) {
         a.list[0] = (int32_t)min(all, (uint32_t)a.most_items);
-        a.list[1] = (int32_t)min(all_slots, 1u << 30);
+        a.list[1] = (int32_t)all_slots;
         a.list[2] = __float_as_int(cut.whole);
         a.list[3] = __float_as_int(cut.tokens);
         a.list[4] = __float_as_int(cut.alike);
@@ -535,10 +545,8 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
     const int32_t id = (int32_t)(blockIdx.x / (uint32_t)d.cache.kv_heads), kvh = (int32_t)(blockIdx.x - (uint32_t)id * (uint32_t)d.cache.kv_heads);
     const Item it = find_item(a, id);
     if (a.budget && kvh == 0 && threadIdx.x == 0) {
-        // (no shares: tiles that are not cut, of requests that have others that are)
-        if (it.tile >= 0 && it.slot >= 0 && it.slot + it.share < a.most_slots)
-            a.jobs[it.slot + it.share] = make_int4(it.request, it.tile, it.share, it.shares > 1 ? it.shares : 0);
-        if (id == 0) *a.used = it.tile < 0 ? 0 : min(it.slots, a.most_slots);      // (without a first item there are none)
+        if (it.tile >= 0 && it.shares > 1) a.jobs[it.slot + it.share] = make_int4(it.request, it.tile, it.share, it.shares);
+        if (id == 0) *a.used = it.tile < 0 ? 0 : it.slots;   // (without a first item there are none)
     }
     if (it.tile < 0) return;
     const Request& r = it.r;
@@ -1072,9 +1080,8 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
                 sum += weight[w] * x.y;
             }
         }
-        const int32_t slot_of = it.slot + it.share;
-        if (!valid || (it.shares > 1 && slot_of >= a.most_slots)) return;      // (the latter where starts do not ascend)
-        const int64_t at = ((int64_t)slot_of * d.cache.kv_heads + kvh) * kTileRows + n;
+        if (!valid) return;
+        const int64_t at = ((int64_t)(it.slot + it.share) * d.cache.kv_heads + kvh) * kTileRows + n;
         const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
         Q* const to = (Q*)a.out + out_row * d.out_stride + head * d.out_head_stride;
         for (int u = wave; u < kUnits; u += kWaves) {
@@ -1213,9 +1220,7 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
 
     l = other_sum(l);
     if (it.shares > 1) {
-        const int32_t slot = it.slot + it.share;
-        if (slot >= a.most_slots) return;                 // (starts that do not ascend)
-        const int64_t at = ((int64_t)slot * d.cache.kv_heads + kvh) * kTileRows + in_tile;
+        const int64_t at = ((int64_t)(it.slot + it.share) * d.cache.kv_heads + kvh) * kTileRows + in_tile;
         if (h == 0) a.stats[at] = make_float2(R == -INFINITY ? -INFINITY : R - kGrow, l);
 #pragma unroll
         for (int m = 0; m < kSlabs; ++m)
@@ -1249,11 +1254,8 @@ __global__ void __launch_bounds__(kThreads) join_shares(Args a) {
     for (uint32_t work = blockIdx.x; work < works; work += gridDim.x) {
         const int32_t id = (int32_t)(work / kv_heads), kvh = (int32_t)(work - (uint32_t)id * kv_heads);
         const int4 job = a.jobs[id];
-        // (tiles that are not cut; where starts do not ascend there may be none)
-        if ((uint32_t)job.x >= (uint32_t)d.requests || job.z < 0 || job.z >= job.w || job.z > id) continue;
         const Request r = request_of(a, job.x);
-        if ((uint32_t)job.y >= (uint32_t)r.tiles) continue;
-        const int32_t rows = min(a.tile_rows, r.added * a.group - job.y * a.tile_rows), slot = id - job.z, shares = min(job.w, a.most_slots - slot);
+        const int32_t rows = min(a.tile_rows, r.added * a.group - job.y * a.tile_rows), slot = id - job.z, shares = job.w;
         const int32_t from = (int32_t)((int64_t)rows * quads * job.z / job.w), to = (int32_t)((int64_t)rows * quads * (job.z + 1) / job.w);
         const int64_t step = (int64_t)d.cache.kv_heads * a.tile_rows;
         for (int32_t x = from + (int32_t)threadIdx.x; x < to; x += kThreads) {
@@ -1357,7 +1359,8 @@ Plan plan_of(const reef_chunk_attention_desc& d) {
         const int64_t shares = (longest + least - 1) / least, tiles = p.items;
         p.budget = p.at_once * (tiles * kv <= p.at_once / 2 ? 1 : (int32_t)std::max<int64_t>(1, std::min<int64_t>(3, most * waves.products / 1000)));
         p.items = std::min(tiles * shares, tiles + (p.budget + kv - 1) / kv);
-        p.slots = p.items;
+        // (a tile that is cut has two shares at least, so that these are what tiles may be cut into beside one each, twice: a slot of 256 rows, heads of 128, has 133 KB)
+        p.slots = std::min<int64_t>(p.items, 2ll * ((p.budget + kv - 1) / kv));
         p.jobs_bytes = 16 * (size_t)(1 + p.slots);
         p.stats_bytes = (size_t)p.slots * kv * p.tile_rows * 8;
     }

@@ -106,6 +106,18 @@ def test_chunk_workspace_goes_by_the_descriptor():
             assert 0 <= n < 1 << 30
 
 
+@pytest.mark.parametrize("kind,cache", [(BF16, BF16), (F16, F16), (F32, F32), (F32, F16)])
+@pytest.mark.parametrize("heads,kv,dim", [(64, 8, 128), (32, 8, 128), (128, 8, 128), (64, 64, 64), (16, 1, 256), (256, 128, 96)])
+def test_chunk_workspace_holds_shares_of_cut_tiles_alone(kind, cache, heads, kv, dim):
+    """Up to 3 workgroups for each that runs at once are cut for, 768 of 256 rows or their like, and a cut tile has two shares at least: 1536 of them, and one or two
+    a cache head by rounding, of 256 rows of 128 values and 2 numbers, 4 bytes each; lists of requests and items beside them."""
+    c = layout(type=cache, blocks=1 << 20, block_size=16, kv_heads=kv, head_dim=dim, block_stride=16 * kv * dim, slot_stride=kv * dim, head_stride=dim)
+    for requests, tokens in ((1, 1 << 15), (4, 1 << 15), (16, 1 << 15), (16, 1 << 16), (64, 1 << 12), (65, 1 << 12), (1000, 3000), (200, 1700)):
+        n = B.ops_chunk_attention_workspace(chunk(c, type=kind, requests=requests, tokens=tokens, heads=heads, max_blocks=1 << 12, table_stride=1 << 12,
+                                                  query_stride=heads * dim, query_head_stride=dim, out_stride=heads * dim, out_head_stride=dim))
+        assert 0 <= n < (1536 + 2 * kv) * 256 * 130 * 4 + (1 << 22), (requests, tokens, n)
+
+
 @pytest.mark.parametrize("change,text", [(dict(type=3), "type"), (dict(rows=-1), "sizes"), (dict(rows=1 << 24), "sizes"), (dict(vocab=0), "sizes"), (dict(vocab=1 << 24), "sizes"),
                                          (dict(top=-1), "given"), (dict(top=129), "given"), (dict(vocab=4), "given"), (dict(logits_stride=999), "overlap"),
                                          (dict(rows=1 << 20, vocab=1 << 20, logits_stride=1 << 20), "2^40")])
