@@ -545,6 +545,38 @@ def test_chunk_starts_that_do_not_ascend_stay_inside():
     behind(work, B.ops_chunk_attention_workspace(d))
 
 
+@pytest.mark.parametrize("kind,cache", [(BF16, BF16), (F32, F16)])
+@pytest.mark.parametrize("requests,tokens,dim", [(5, 50, 64), (5, 700, 64), (90, 300, 32), (90, 3000, 128), (1, 400, 64), (3, 20, 192)])
+@pytest.mark.parametrize("longest", [0, 3000])
+def test_chunk_starts_that_do_not_ascend_stay_inside_where_tiles_are_cut(kind, cache, requests, tokens, dim, longest):
+    """The same with tables of some thousand tokens, whose tiles are cut into shares, few and many requests, tiles of both sizes."""
+    rng = np.random.default_rng(tokens)
+    kv, group, width = 1, 4, 400
+    heads, size = kv * group, 4 if kind == F32 else 2
+    pools = Pools(cache, 40, 16, kv, dim)
+    q = up(R.encode(rng.standard_normal((tokens, heads, dim)).astype(np.float32), kind))
+    n = tokens * heads * dim * size // 2
+    out, ls = up(np.full(n + 64, 0x4242, np.uint16)), up(np.full(tokens * heads + 16, 77, np.float32))
+    d = B.ChunkAttentionDesc(pools.layout, kind, requests, heads, tokens, width, width, longest, 0, 0.125, heads * dim, dim, heads * dim, dim)
+    n_work = B.ops_chunk_attention_workspace(d)
+    assert n_work
+    work = work_of(n_work)
+    table = ints(rng.integers(-3, 50, (requests, width)))
+    for starts in (np.arange(requests + 1) % 2 * tokens, rng.integers(-2 ** 31, 2 ** 31, requests + 1), np.linspace(tokens, 0, requests + 1), np.zeros(requests + 1), np.full(requests + 1, tokens),
+                   np.r_[0, rng.integers(0, tokens + 1, requests)]):
+        for lengths in (np.full(requests, 6400), rng.integers(-5, 7000, requests), np.full(requests, 2 ** 31 - 1)):
+            for cached in (rng.integers(-5, 6400, requests), np.zeros(requests)):
+                ok(B.ops_chunk_attention(d, q, *pools.dev, table, ints(np.asarray(starts, np.int64)), ints(np.asarray(cached, np.int64)), ints(lengths), out, ls, work))
+    assert (out.to_array(np.uint16)[n:] == 0x4242).all() and (ls.to_array()[tokens * heads:] == 77).all()
+    behind(work, n_work)
+    # and a call as it should be in the same workspace afterwards
+    fine = np.linspace(0, tokens, requests + 1).astype(np.int64)
+    ok(B.ops_chunk_attention(d, q, *pools.dev, table, ints(fine), ints(np.zeros(requests)), ints(fine[1:] - fine[:-1]), out, ls, work))
+    got = out.to_array(np.uint16)[:n].copy()
+    ok(B.ops_chunk_attention(d, q, *pools.dev, table, ints(fine), ints(np.zeros(requests)), ints(fine[1:] - fine[:-1]), out, ls, work_of(n_work)))
+    np.testing.assert_array_equal(got, out.to_array(np.uint16)[:n])
+
+
 # ---- scores of given tokens ----------------------------------------------------------------------
 def run_scores(kind, logits, tokens, top, pad=0, raw=None):
     rows, vocab = logits.shape
