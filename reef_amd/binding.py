@@ -620,6 +620,9 @@ def ops_cache_append(desc, key, value, slots, key_cache, value_cache, stream=Non
 def _workspace(name, desc):
     f = getattr(lib(), "reef_ops_%s_workspace" % name)
     f.argtypes, f.restype = [ctypes.c_void_p], ctypes.c_int64
+    size = ctypes.sizeof(_OPS[name][0])
+    if ctypes.sizeof(desc) != size:          # (of another call: the library would read behind it)
+        raise TypeError("a descriptor of %d bytes is needed, not one of %d" % (size, ctypes.sizeof(desc)))
     n = f(ctypes.addressof(desc))
     if n < 0:
         raise ReefError("reef_ops_%s_workspace" % name, 1)

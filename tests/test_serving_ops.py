@@ -128,6 +128,20 @@ def test_scores_refusals(change, text):
         B.ops_token_scores_workspace(d)
 
 
+def test_workspaces_of_another_descriptor():
+    """Smaller ones would be read behind their end."""
+    descs = dict(chunk_attention=chunk(layout()), token_scores=scores(), block_sweep=sweep(), cache_compact=compact(layout()), cache_fork=fork(layout()))
+    for name in ("chunk_attention", "token_scores", "block_sweep", "cache_compact"):
+        f = getattr(B, "ops_%s_workspace" % name)
+        assert f(descs[name]) >= 0
+        for other, d in descs.items():
+            if ctypes.sizeof(d) != ctypes.sizeof(descs[name]):
+                with pytest.raises(TypeError):
+                    f(d)
+        with pytest.raises(TypeError):
+            f(None)
+
+
 def test_scores_pointers():
     d = scores()
     need = B.ops_token_scores_workspace(d)
