@@ -479,7 +479,7 @@ struct Near {
     static __device__ inline uint32_t at(uint32_t row, uint32_t piece) { return row * kPitch + ((piece ^ turn(row)) << 4); }
 };
 
-// How a kernel is laid out, by its types and head size.  TK: tokens of a tile of keys and values; WAVES of 32 rows each share them.
+// How a kernel is laid out, by its types and head size.  kTile: tokens of a tile of keys and values; kWaves of 32 rows each share them.
 template <class Q, class C, int DP>
 struct Shape {
     static constexpr bool kHalf = __is_same(C, _Float16);
@@ -490,6 +490,8 @@ struct Shape {
     // Tiles of 32 rows in all: registers of what a wavefront holds (keys, values, queries, output, weights), and so how many wavefronts; 0: too many for any.
     static constexpr int kFewV = DP <= 64 ? 2 : DP <= 128 ? 4 : 8;            // values of a row of V a lane
     static constexpr int kFewHeld = DP * (int)sizeof(C) / 8 + 16 * kFewV * (int)sizeof(C) / 4 + kTermsQ * DP / 4 + kFewV * 16 + 16 + 8 * kTermsFew;
+    // (Four wavefronts of heads of 192 and 256 hold 30 to 120 registers more than there are, in scratch, and are faster than the other tiles all the same: 64 single tokens over
+    // 4000, 32 heads over 8, bf16 292 us against 399 for 192 and 401 against 466 for 256, 32-bit queries over bf16 647 against 677; but 725 against 677 over fp16 for 256.)
     static constexpr int kFewWaves = kFewHeld <= 220 ? 8 : kFewHeld <= 440 ? 4 : 0;
 };
 
@@ -891,17 +893,22 @@ __global__ void __launch_bounds__((FEW ? Shape<Q, C, DP>::kFewWaves : Shape<Q, C
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             return (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0);
         };
+        // (Larger heads leave no registers for these places: held ahead of the loop they cost scratch.  64 single tokens over 4000, 32 heads over 8 of 192, bf16: 762 us, made
+        // again 292; of 256, 493 and 401; but 204 and 200 for 128, 24.5 and 26.7 for 16 tokens over 2000 of 128.)
+        auto key_lane = [&]() __attribute__((always_inline)) -> uint32_t { return DP > 128 ? again(lane) : lane; };
         auto load_k = [&](int slot) __attribute__((always_inline)) {
+            const uint32_t mine = key_lane();
 #pragma unroll
             for (int i = 0; i < kKLoads; ++i) {
-                const uint32_t x = i * 64 + lane, row = x / kRowPieces, piece = x - row * kRowPieces;
+                const uint32_t x = i * 64 + mine, row = x / kRowPieces, piece = x - row * kRowPieces;
                 k[i] = *(const u32x4*)(keys + offsets[wave][slot][row] + (piece * 16 < D * (uint32_t)sizeof(C) ? piece * (16 / (uint32_t)sizeof(C)) : 0));
             }
         };
         auto store_k = [&]() __attribute__((always_inline)) {
+            const uint32_t mine = key_lane();
 #pragma unroll
             for (int i = 0; i < kKLoads; ++i) {
-                const uint32_t x = i * 64 + lane, row = x / kRowPieces, piece = x - row * kRowPieces;
+                const uint32_t x = i * 64 + mine, row = x / kRowPieces, piece = x - row * kRowPieces;
                 *(u32x4*)(k_mine + K::at(row, piece)) = piece * 16 < D * (uint32_t)sizeof(C) ? k[i] : u32x4{0, 0, 0, 0};
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
