@@ -377,14 +377,17 @@ int reef_ops_beam_reorder(const reef_beam_reorder_desc* d, const int32_t* parent
  * lengths[i] (of a request that the plan refused) attends to nothing.  Without a token, or where all s_t are -infinity, out is 0 and lse -infinity.  Rows in front of
  * starts[0] or behind starts[requests] are left as they were; starts ascend (where they do not, rows may be left out or belong to either request).
  * Values that a row does not see (behind its place, in front of its window, behind a sequence, in no block) may be anything; an infinity
- * or a NaN among the values that it sees gives infinities or NaN in it.  Queries are finite; |scale| < 2^127.  type (of query and out): the cache's, or REEF_TYPE_F32.
+ * or a NaN among the values that it sees gives infinities or NaN in it.  Queries are finite, and so are the keys that a row sees and its scores in 32 bits (with
+ * others it may be NaN); |scale| < 2^127.  type (of query and out): the cache's, or REEF_TYPE_F32.
  * Scores, weights' sums and outputs are held in 32 bits.  Where type has 16, a weight enters its product with a value as two numbers of that type where there are up to
  * 32 rows a cache head and request on the average (tokens * heads <= 32 * kv_heads * requests; 2^-16 of it at most is left out), and as one, rounded to nearest, where
  * there are more: outputs are off by up to half a step of the type of the mean |value| then, beside their own rounding.  32-bit queries and their weights are two
- * numbers of fp16 or three of bf16 (2^-22 left out at most).
+ * numbers of fp16 or three of bf16 (2^-22 left out at most); 32-bit keys and values are three of bf16, which hold all of their bits from 2^-110 on and leave out
+ * 2^-134 at most of smaller ones.
  * query, out: [tokens][heads][head_dim], strides in elements, multiples of 16 bytes, 16-byte aligned; no two rows of out overlap.
  * lse: [tokens][heads], may be NULL.  `longest`: the largest length to expect, which sets into how many shares long sequences are
- * split (0: what a row of the table can hold); other lengths are right too. */
+ * split (0: what a row of the table can hold); other lengths are right too.  The workspace is up to some 200 MB (more than 128 cache heads: 0.3 MB each).
+ * One launch may hold all CUs for milliseconds (three pieces of 509 tokens over 40000, 64 heads of 128: 2.3 ms): where others wait for the device, pieces are cut shorter. */
 typedef struct {
     reef_cache_layout cache;
     int32_t type, requests, heads, tokens;
