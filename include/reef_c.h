@@ -386,7 +386,7 @@ int reef_ops_beam_reorder(const reef_beam_reorder_desc* d, const int32_t* parent
  * 2^-134 at most of smaller ones.
  * query, out: [tokens][heads][head_dim], strides in elements, multiples of 16 bytes, 16-byte aligned; no two rows of out overlap.
  * lse: [tokens][heads], may be NULL.  `longest`: the largest length to expect, which sets into how many shares long sequences are
- * split (0: what a row of the table can hold); other lengths are right too.  The workspace is up to some 200 MB (more than 128 cache heads: 0.3 MB each).
+ * split (0: what a row of the table can hold); other lengths are right too.  The workspace is up to 240 MB (more than 128 cache heads: 0.3 MB each).
  * One launch may hold all CUs for milliseconds (three pieces of 509 tokens over 40000, 64 heads of 128: 2.3 ms): where others wait for the device, pieces are cut shorter. */
 typedef struct {
     reef_cache_layout cache;

@@ -205,6 +205,30 @@ def one_request(kind, cache, keys, values, q, scale, cached, longest=0):
     return R.decode(out.to_array(R.np_type(kind)).reshape(new, heads, dim), kind), ls.to_array().reshape(new, heads)
 
 
+@pytest.mark.parametrize("cached,new", [(300, 2), (300, 200)])
+@pytest.mark.parametrize("size", [1e-30, 1e-33, 1e-36, 1e-38, 1e-40])
+def test_chunk_small_32_bit_keys_and_values(cached, new, size):
+    """Three numbers of bf16 leave out 2^-134 at most of a key or a value, in fewer bits than 32 below 2^-110: outputs are off by that much more, and by half of the
+    smallest 32-bit number; scores by that times the sum of |query|, weights by as much of themselves, twice."""
+    rng = np.random.default_rng(new)
+    n, dim, left = cached + new, 64, 2.0 ** -134
+    small, one = (rng.standard_normal((n, dim)).astype(np.float32) for _ in range(2))
+    small *= np.float32(size)
+    q = rng.standard_normal((new, 2, dim)).astype(np.float32)
+    wide = lambda *a: [x.astype(np.float64) for x in a]                                         # noqa: E731
+    qw, sw, ow = wide(q, small, one)
+    out, ls = one_request(F32, F32, one, small, q, 0.1, cached)
+    want, want_lse, tol, tol_lse = S.chunk(qw, ow[None], sw[None], cached, n, 0.1, 0, F32, F32)
+    assert (np.abs(out - want) <= tol + HALF[F32] * np.abs(want) + left + 2.0 ** -150).all()
+    assert (np.abs(ls - want_lse) <= tol_lse).all()
+    scale = float(np.float32(0.1 / max(size, 1e-37)))
+    out, ls = one_request(F32, F32, small, one, q, scale, cached)
+    want, want_lse, tol, tol_lse = S.chunk(qw, sw[None], ow[None], cached, n, scale, 0, F32, F32)
+    off = left * scale * np.abs(qw).sum(2)
+    assert (np.abs(out - want) <= tol + HALF[F32] * np.abs(want) + (2 * off * np.abs(one).max())[:, :, None]).all()
+    assert (np.abs(ls - want_lse) <= tol_lse + off).all()
+
+
 @pytest.mark.parametrize("kind,cache", PAIRS)
 @pytest.mark.parametrize("cached,new", [(0, 150), (70, 30), (3000, 140)])
 @pytest.mark.parametrize("dim", [40, 64, 128])
